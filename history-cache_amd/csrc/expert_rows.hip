@@ -1,0 +1,387 @@
+// Rows sorted by expert and back.  A row i names top_k experts; pair q = i * top_k + j is its j-th choice.
+//
+// hc_expert_order: stable counting sort of the pairs by expert.  offset[e] is the first place of expert e; pair[place] = q
+// and slot[q] = place for the pairs that name an expert, -1 for the others (whose places lie behind offset[E]).
+//   One block sorts up to OR_SMALL_PAIRS pairs in one launch.  More take three: every block counts its chunk of pairs by
+//   expert, a block per expert turns the counts of the chunks into first places, every block places its chunk.  Inside a
+//   chunk a wave owns a run of adjacent pairs and takes 64 at a time: lanes with the same expert find each other by
+//   ballots over the bits of the expert's number, so that places ascend with the pair whatever the scheduling.
+//
+// hc_rows_to_experts: rows[place] = x[pair[place] / top_k], zeros behind offset[E].  Walks the rows of x, each read once
+//   and stored at its top_k places.
+// hc_rows_from_experts: out[i] = sum_j weight[q] * y[slot[q]] in the order of j, summed in fp32 (weight NULL: 1, which is
+//   the gradient of hc_rows_to_experts).
+// hc_rows_from_experts_grad: grad_y[place] = weight[q] * g[i], zeros behind offset[E], and grad_weight[q] = <g[i], y[slot[q]]>.
+// All four are bound by the rows' way through memory.
+#include "hc_common.h"
+
+namespace {
+
+constexpr int OR_MAX_EXPERTS = 1024;
+constexpr int OR_SMALL_PAIRS = 8192;
+constexpr int OR_SMALL_BLOCK = 1024;
+constexpr int OR_CHUNK = 2048;            // pairs of a block, at least
+constexpr int OR_MAX_CHUNKS = 4096;
+
+// The expert of a pair, E ("nowhere") for any number outside [0, E).
+__device__ __forceinline__ int or_expert(const int64_t *__restrict__ expert, int64_t q, int E) {
+  const int64_t e = expert[q];
+  return e >= 0 && e < E ? (int)e : E;
+}
+
+// Places the pairs lo .. hi of a wave: `next` (LDS, E + 1 counters of this wave) holds the next place of each expert.
+__device__ __forceinline__ void or_place(const int64_t *__restrict__ expert, int64_t lo, int64_t hi, int E, int bits,
+                                         int *next, int32_t *__restrict__ slot, int32_t *__restrict__ pair) {
+  const int lane = hc_lane();
+  for (int64_t q0 = lo; q0 < hi; q0 += HC_WAVE) {
+    const int64_t q = q0 + lane;
+    const bool on = q < hi;
+    const int e = on ? or_expert(expert, q, E) : 0;
+    uint64_t same = __ballot(on);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1ull)), first = on ? __ffsll((long long)same) - 1 : lane;
+    int place = 0;
+    if (on && first == lane) place = atomicAdd(&next[e], __popcll(same));
+    place = __shfl(place, first, HC_WAVE) + rank;
+    if (on) {
+      slot[q] = e < E ? place : -1;
+      pair[place] = e < E ? (int32_t)q : -1;
+    }
+  }
+}
+
+// Exclusive prefix sums of cnt[0 .. m) in LDS by one wave; returns the total.
+__device__ __forceinline__ int or_scan(int *cnt, int m) {
+  const int lane = hc_lane();
+  int before = 0;
+  for (int i0 = 0; i0 < m; i0 += HC_WAVE) {
+    const int v = i0 + lane < m ? cnt[i0 + lane] : 0;
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < HC_WAVE; d *= 2) {
+      const int o = __shfl_up(s, d, HC_WAVE);
+      if (lane >= d) s += o;
+    }
+    if (i0 + lane < m) cnt[i0 + lane] = before + s - v;
+    before += __shfl(s, HC_WAVE - 1, HC_WAVE);
+  }
+  return before;
+}
+
+// Everything in one block: WAVES runs of pairs, a row of E + 1 counters for each and one for the sums.
+__global__ __launch_bounds__(OR_SMALL_BLOCK) void or_small(const int64_t *__restrict__ expert, int32_t *__restrict__ slot,
+                                                            int32_t *__restrict__ pair, int64_t *__restrict__ offset, int P,
+                                                            int E, int bits) {
+  extern __shared__ int s_cnt[];
+  const int waves = (int)(blockDim.x / HC_WAVE), wave = hc_wave_in_block(), bins = E + 1;
+  int *sum = s_cnt + waves * bins, *mine = s_cnt + wave * bins;
+  for (int i = (int)threadIdx.x; i < (waves + 1) * bins; i += (int)blockDim.x) s_cnt[i] = 0;
+  __syncthreads();
+  const int run = ((P + waves - 1) / waves + HC_WAVE - 1) / HC_WAVE * HC_WAVE;
+  const int lo = wave * run < P ? wave * run : P, hi = lo + run < P ? lo + run : P;
+  for (int q = lo + hc_lane(); q < hi; q += HC_WAVE) atomicAdd(&mine[or_expert(expert, q, E)], 1);
+  __syncthreads();
+  for (int e = (int)threadIdx.x; e < bins; e += (int)blockDim.x) {
+    int s = 0;
+    for (int w = 0; w < waves; ++w) {
+      const int c = s_cnt[w * bins + e];
+      s_cnt[w * bins + e] = s;
+      s += c;
+    }
+    sum[e] = s;
+  }
+  __syncthreads();
+  if (wave == 0) or_scan(sum, bins);
+  __syncthreads();
+  for (int e = (int)threadIdx.x; e < bins; e += (int)blockDim.x) {
+    offset[e] = sum[e];
+    for (int w = 0; w < waves; ++w) s_cnt[w * bins + e] += sum[e];
+  }
+  __syncthreads();
+  or_place(expert, lo, hi, E, bits, mine, slot, pair);
+}
+
+__global__ __launch_bounds__(HC_BLOCK) void or_count(const int64_t *__restrict__ expert, int *__restrict__ count, int64_t P,
+                                                     int E, int64_t chunk) {
+  extern __shared__ int s_cnt[];
+  const int bins = E + 1;
+  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) s_cnt[e] = 0;
+  __syncthreads();
+  const int64_t lo = (int64_t)blockIdx.x * chunk, hi = lo + chunk < P ? lo + chunk : P;
+  for (int64_t q = lo + threadIdx.x; q < hi; q += HC_BLOCK) atomicAdd(&s_cnt[or_expert(expert, q, E)], 1);
+  __syncthreads();
+  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) count[(int64_t)e * gridDim.x + blockIdx.x] = s_cnt[e];
+}
+
+// count[e][chunk] becomes the number of e's pairs in the chunks before; total[e] their number in all.
+__global__ __launch_bounds__(HC_WAVE) void or_prefix(int *__restrict__ count, int *__restrict__ total, int chunks) {
+  int *row = count + (int64_t)blockIdx.x * chunks;
+  const int t = or_scan(row, chunks);
+  if (hc_lane() == 0) total[blockIdx.x] = t;
+}
+
+__global__ __launch_bounds__(HC_BLOCK) void or_scatter(const int64_t *__restrict__ expert, const int *__restrict__ count,
+                                                       const int *__restrict__ total, int32_t *__restrict__ slot,
+                                                       int32_t *__restrict__ pair, int64_t *__restrict__ offset, int64_t P,
+                                                       int E, int64_t chunk, int bits) {
+  extern __shared__ int s_cnt[];
+  constexpr int W = HC_WAVES_PER_BLOCK;
+  const int wave = hc_wave_in_block(), bins = E + 1;
+  int *sum = s_cnt + W * bins, *mine = s_cnt + wave * bins;
+  for (int i = (int)threadIdx.x; i < W * bins; i += HC_BLOCK) s_cnt[i] = 0;
+  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) sum[e] = total[e];
+  __syncthreads();
+  const int64_t begin = (int64_t)blockIdx.x * chunk, end = begin + chunk < P ? begin + chunk : P;
+  const int64_t lo0 = begin + wave * (chunk / W), lo = lo0 < end ? lo0 : end, hi = lo + chunk / W < end ? lo + chunk / W : end;
+  for (int64_t q = lo + hc_lane(); q < hi; q += HC_WAVE) atomicAdd(&mine[or_expert(expert, q, E)], 1);
+  if (wave == 0) or_scan(sum, bins);
+  __syncthreads();
+  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) {
+    if (blockIdx.x == 0) offset[e] = sum[e];
+    int s = sum[e] + count[(int64_t)e * gridDim.x + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int c = s_cnt[w * bins + e];
+      s_cnt[w * bins + e] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+  or_place(expert, lo, hi, E, bits, mine, slot, pair);
+}
+
+struct OrShape {
+  int64_t chunk, chunks;
+};
+
+static OrShape or_shape(int64_t P) {
+  OrShape s;
+  s.chunk = OR_CHUNK;
+  while ((P + s.chunk - 1) / s.chunk > OR_MAX_CHUNKS) s.chunk *= 2;
+  s.chunks = (P + s.chunk - 1) / s.chunk;
+  return s;
+}
+
+// ---- rows ------------------------------------------------------------------
+// A row is D elements in pieces of VEC; a thread owns one piece of one row.
+struct MvArgs {
+  int64_t n, P;
+  int D, k, pieces, E;
+  const int32_t *slot;
+  const int64_t *offset;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void mv_zero_tail(const MvArgs &a, T *__restrict__ rows) {
+  typedef typename hc_vec<T, VEC>::raw_t raw;
+  const int64_t live = a.offset[a.E], rest = (a.P - live) * a.pieces;
+  for (int64_t i = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x; i < rest; i += (int64_t)gridDim.x * HC_BLOCK)
+    *reinterpret_cast<raw *>(rows + (live + i / a.pieces) * a.D + i % a.pieces * VEC) = raw{};
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(HC_BLOCK) void mv_to(MvArgs a, const T *__restrict__ x, T *__restrict__ rows) {
+  typedef typename hc_vec<T, VEC>::raw_t raw;
+  const int64_t item = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x;
+  const int64_t i = item / a.pieces;
+  if (i < a.n) {
+    const int c = (int)(item - i * a.pieces) * VEC;
+    const raw v = *reinterpret_cast<const raw *>(x + i * a.D + c);
+    for (int j = 0; j < a.k; ++j) {
+      const int32_t s = a.slot[i * a.k + j];
+      if (s >= 0) *reinterpret_cast<raw *>(rows + (int64_t)s * a.D + c) = v;
+    }
+  }
+  mv_zero_tail<T, VEC>(a, rows);
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restrict__ y, const float *__restrict__ weight,
+                                                    T *__restrict__ out) {
+  const int64_t item = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x;
+  const int64_t i = item / a.pieces;
+  if (i >= a.n) return;
+  const int c = (int)(item - i * a.pieces) * VEC;
+  float sum[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) sum[v] = 0.f;
+  for (int j = 0; j < a.k; ++j) {
+    const int32_t s = a.slot[i * a.k + j];
+    if (s < 0) continue;
+    float p[VEC];
+    hc_vec<T, VEC>::load(y + (int64_t)s * a.D + c, p);
+    const float w = weight != nullptr ? weight[i * a.k + j] : 1.f;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) sum[v] = fmaf(w, p[v], sum[v]);
+  }
+  hc_vec<T, VEC>::store(out + i * a.D + c, sum);
+}
+
+// L lanes a row.
+template <typename T, int VEC>
+__global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__restrict__ g, const T *__restrict__ y,
+                                                         const float *__restrict__ weight, T *__restrict__ grad_y,
+                                                         float *__restrict__ grad_weight, int L) {
+  const int lane = (int)threadIdx.x & (L - 1);
+  const int64_t i = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
+  if (i < a.n) {
+    for (int j = 0; j < a.k; ++j) {
+      const int32_t s = a.slot[i * a.k + j];
+      const float w = weight[i * a.k + j];
+      float dot = 0.f;
+      if (s >= 0)
+        for (int p = lane; p < a.pieces; p += L) {
+          float gv[VEC], yv[VEC], o[VEC];
+          hc_vec<T, VEC>::load(g + i * a.D + p * VEC, gv);
+          hc_vec<T, VEC>::load(y + (int64_t)s * a.D + p * VEC, yv);
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            dot = fmaf(gv[v], yv[v], dot);
+            o[v] = w * gv[v];
+          }
+          hc_vec<T, VEC>::store(grad_y + (int64_t)s * a.D + p * VEC, o);
+        }
+      for (int d = L / 2; d >= 1; d /= 2) dot += __shfl_xor(dot, d, HC_WAVE);
+      if (lane == 0) grad_weight[i * a.k + j] = dot;
+    }
+  }
+  mv_zero_tail<T, VEC>(a, grad_y);
+}
+
+static bool mv_args(int64_t n, int64_t top_k, int64_t E, int64_t D, const int32_t *slot, const int64_t *offset, MvArgs *a) {
+  if (n < 0 || top_k < 1 || E < 1 || D < 1) return false;
+  a->n = n;
+  a->P = n * top_k;
+  a->D = (int)D;
+  a->k = (int)top_k;
+  a->E = (int)E;
+  a->slot = slot;
+  a->offset = offset;
+  return true;
+}
+
+// Elements of T in a piece: 16 bytes, or as many as the row length and the matrices' alignment allow.
+template <typename T, typename F>
+static int mv_with_piece(uintptr_t at, int64_t D, F &&f) {
+  const uint64_t a = (uint64_t)at | (uint64_t)D * sizeof(T);
+  if (a % 16 == 0) return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
+  if (a % 8 == 0) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{});
+  if (a % 4 == 0) return f(std::integral_constant<int, 4 / (int)sizeof(T)>{});
+  return f(std::integral_constant<int, 1>{});
+}
+
+template <typename F>
+static int mv_with_type(int dtype, F &&f) {
+  if (dtype == HC_F32) return f(float{});
+  if (dtype == HC_F16) return f(__half{});
+  if (dtype == HC_BF16) return f(__hip_bfloat16{});
+  return HC_EDTYPE;
+}
+
+static bool or_sizes_ok(int64_t pairs, int64_t E) { return pairs < (1ll << 31) && E <= OR_MAX_EXPERTS; }
+
+}  // namespace
+
+extern "C" size_t hc_expert_order_workspace_bytes(int64_t pairs, int64_t E) {
+  if (pairs < 0 || E < 1 || !or_sizes_ok(pairs, E) || pairs <= OR_SMALL_PAIRS) return 0;
+  return hc_align_up((size_t)(E + 1) * (size_t)(or_shape(pairs).chunks + 1) * sizeof(int), 256);
+}
+
+extern "C" int hc_expert_order(const int64_t *expert, int64_t pairs, int64_t E, int32_t *slot, int32_t *pair,
+                               int64_t *offset, void *workspace, size_t workspace_bytes, void *stream) {
+  HC_REQUIRE(pairs >= 0 && E >= 1);
+  if (!or_sizes_ok(pairs, E)) return HC_EUNSUPPORTED;
+  HC_REQUIRE(offset && (pairs == 0 || (expert && slot && pair)));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int bits = 1;
+  while ((1 << bits) < E + 1) ++bits;
+  const size_t bins = (size_t)E + 1;
+  if (pairs <= OR_SMALL_PAIRS) {
+    // a wave for every 64 pairs, up to sixteen
+    int waves = (int)((pairs + HC_WAVE - 1) / HC_WAVE);
+    waves = waves < 1 ? 1 : waves > OR_SMALL_BLOCK / HC_WAVE ? OR_SMALL_BLOCK / HC_WAVE : waves;
+    while ((waves + 1) * bins * sizeof(int) > 64 * 1024) waves /= 2;
+    or_small<<<dim3(1), dim3((unsigned)waves * HC_WAVE), (waves + 1) * bins * sizeof(int), st>>>(expert, slot, pair, offset,
+                                                                                                (int)pairs, (int)E, bits);
+    return hc_launch_status();
+  }
+  const OrShape s = or_shape(pairs);
+  if (!workspace || workspace_bytes < hc_expert_order_workspace_bytes(pairs, E) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return HC_EWORKSPACE;
+  int *count = static_cast<int *>(workspace), *total = count + bins * s.chunks;
+  or_count<<<dim3((unsigned)s.chunks), dim3(HC_BLOCK), bins * sizeof(int), st>>>(expert, count, pairs, (int)E, s.chunk);
+  or_prefix<<<dim3((unsigned)bins), dim3(HC_WAVE), 0, st>>>(count, total, (int)s.chunks);
+  or_scatter<<<dim3((unsigned)s.chunks), dim3(HC_BLOCK), (HC_WAVES_PER_BLOCK + 1) * bins * sizeof(int), st>>>(
+      expert, count, total, slot, pair, offset, pairs, (int)E, s.chunk, bits);
+  return hc_launch_status();
+}
+
+extern "C" int hc_rows_to_experts(const void *x, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
+                                  const int32_t *slot, const int64_t *offset, void *rows, void *stream) {
+  MvArgs a;
+  HC_REQUIRE(mv_args(n, top_k, E, D, slot, offset, &a));
+  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
+  HC_REQUIRE(x && slot && offset && rows);
+  return mv_with_type(dtype, [&](auto type) {
+    typedef decltype(type) T;
+    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows), D, [&](auto piece) {
+      constexpr int VEC = decltype(piece)::value;
+      a.pieces = (int)(D / VEC);
+      const int64_t blocks = (n * a.pieces + HC_BLOCK - 1) / HC_BLOCK;
+      if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
+      mv_to<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+          a, static_cast<const T *>(x), static_cast<T *>(rows));
+      return hc_launch_status();
+    });
+  });
+}
+
+extern "C" int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
+                                    const int32_t *slot, const float *weight, void *out, void *stream) {
+  MvArgs a;
+  HC_REQUIRE(mv_args(n, top_k, E, D, slot, nullptr, &a));
+  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
+  HC_REQUIRE(y && slot && out);
+  return mv_with_type(dtype, [&](auto type) {
+    typedef decltype(type) T;
+    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out), D, [&](auto piece) {
+      constexpr int VEC = decltype(piece)::value;
+      a.pieces = (int)(D / VEC);
+      const int64_t blocks = (n * a.pieces + HC_BLOCK - 1) / HC_BLOCK;
+      if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
+      mv_from<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+          a, static_cast<const T *>(y), weight, static_cast<T *>(out));
+      return hc_launch_status();
+    });
+  });
+}
+
+extern "C" int hc_rows_from_experts_grad(const void *g, const void *y, int dtype, int64_t n, int64_t top_k, int64_t E,
+                                         int64_t D, const int32_t *slot, const int64_t *offset, const float *weight,
+                                         void *grad_y, float *grad_weight, void *stream) {
+  MvArgs a;
+  HC_REQUIRE(mv_args(n, top_k, E, D, slot, offset, &a));
+  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
+  HC_REQUIRE(g && y && slot && offset && weight && grad_y && grad_weight);
+  return mv_with_type(dtype, [&](auto type) {
+    typedef decltype(type) T;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(grad_y);
+    return mv_with_piece<T>(at, D, [&](auto piece) {
+      constexpr int VEC = decltype(piece)::value;
+      a.pieces = (int)(D / VEC);
+      int L = 1;
+      while (L < HC_WAVE && L < a.pieces) L *= 2;
+      const int64_t blocks = (n * L + HC_BLOCK - 1) / HC_BLOCK;
+      if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
+      mv_from_grad<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+          a, static_cast<const T *>(g), static_cast<const T *>(y), weight, static_cast<T *>(grad_y), grad_weight, L);
+      return hc_launch_status();
+    });
+  });
+}

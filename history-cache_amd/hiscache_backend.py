@@ -24,6 +24,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # HISCACHE_HIP_LIB overrides the location of the built library (default: next to this file)
@@ -149,6 +150,22 @@ _SIGNATURES = {
     "hc_edge_types_by_ranges": (_c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_int, _c_p, _c_p, _c_i64, _c_i64, _c_p]),
     "hc_typed_csr": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p,
                               _c_p, _c_p, _c_sz, _c_p, _c_p]),
+    "hc_route_rows": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p]),
+    "hc_route_rows_grad": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "hc_expert_order_workspace_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "hc_expert_order": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "hc_rows_to_experts": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p]),
+    "hc_rows_from_experts": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p]),
+    "hc_rows_from_experts_grad": (_c_int, [_c_p, _c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p,
+                                           _c_p, _c_p]),
+    "hc_expert_linear": (_c_int, [_c_p, _c_int, _c_p, _c_int, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p]),
+    "hc_expert_linear_grad_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "hc_expert_linear_grad": (_c_int, [_c_p, _c_p, _c_int, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_sz,
+                                       _c_p]),
+    "hc_pack_rows": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
+    "hc_unpack_rows": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_int, _c_p]),
+    "hc_gated_pack": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p]),
+    "hc_gated_grad": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
 }
 
 _lib_handle = None
@@ -1576,6 +1593,337 @@ def bias_bn_relu_eval(x, bias, gamma, beta, running_mean, running_var, eps):
     _check(lib.hc_bn_relu_eval(_ptr(x), _ptr(bias), _ptr(gamma), _ptr(beta), _ptr(running_mean), _ptr(running_var),
                                float(eps), _ptr(y), x.shape[0], x.shape[1], _stream()), "hc_bn_relu_eval")
     return y
+
+
+# ----------------------------------------------------------------------------- rows and their experts
+def _together(t, *others):
+    """Do these tensors lie on one device, the current one (whose stream the launch goes to)?"""
+    index = t.device.index
+    if index != torch.cuda.current_device() or any(o is not None and o.device.index != index for o in others):
+        raise ValueError("the tensors must lie on one device, and it must be the current one")
+
+
+def _arriving(g):
+    """A gradient as the kernels read it: packed, with its own sign."""
+    return g.contiguous().resolve_neg()
+
+
+class _RouteRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, normalize):
+        n, E = logits.shape
+        expert = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
+        weight = torch.empty((n, top_k), dtype=torch.float32, device=logits.device)
+        _check(load_library().hc_route_rows(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
+                                            expert.data_ptr(), weight.data_ptr(), _stream()), "hc_route_rows")
+        ctx.mark_non_differentiable(expert)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, expert, weight)
+        ctx.hc = (top_k, normalize)
+        return expert, weight
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _g_expert, g):
+        if g is None:
+            return None, None, None
+        logits, expert, weight = ctx.saved_tensors
+        top_k, normalize = ctx.hc
+        n, E = logits.shape
+        g = _arriving(g)
+        grad = torch.empty_like(logits)
+        _check(load_library().hc_route_rows_grad(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
+                                                 expert.data_ptr(), weight.data_ptr(), g.data_ptr(), grad.data_ptr(),
+                                                 _stream()), "hc_route_rows_grad")
+        return grad, None, None
+
+
+def route_rows(logits, top_k, normalize=True):
+    """The ``top_k`` experts of every row and their weights: softmax of ``logits`` [n, E] (fp32, fp16 or bf16, E <= 1024),
+    its largest entries in falling order, of equal ones the lowest index first.  Returns (expert int64 [n, top_k],
+    weight fp32 [n, top_k]); ``normalize``: the weights of a row are divided by their sum.  A logit of -inf closes an
+    expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
+    weights.  The gradient of the weights reaches ``logits``.  top_k <= 32."""
+    _dev(logits, "logits")
+    _float_dtype(logits, "logits")
+    top_k = int(top_k)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [n, E]")
+    if not 1 <= top_k <= logits.shape[1]:
+        raise ValueError(f"top_k must be between 1 and the {logits.shape[1]} experts, got {top_k}")
+    _together(logits)
+    return _RouteRows.apply(logits, top_k, int(bool(normalize)))
+
+
+class ExpertOrder:
+    """The (row, choice) pairs of a batch in expert order (:func:`expert_order`).  Pair q = i * top_k + j is row i's j-th
+    choice.  ``offset`` int64 [E + 1]: expert e has the places offset[e] to offset[e + 1]; ``pair`` int32 [rows * top_k]: the
+    pair at every place; ``slot`` int32 [rows * top_k]: every pair's place; -1 where there is none (choices that name
+    no expert, and the places behind offset[E])."""
+    __slots__ = ("slot", "pair", "offset", "rows", "top_k", "experts")
+
+    def __init__(self, slot, pair, offset, rows, top_k, experts):
+        self.slot, self.pair, self.offset = slot, pair, offset
+        self.rows, self.top_k, self.experts = int(rows), int(top_k), int(experts)
+
+    @property
+    def places(self):
+        return self.rows * self.top_k
+
+
+def expert_order(expert, num_expert):
+    """Sort the choices ``expert`` (int64 [n, top_k] or [n]) by expert: an :class:`ExpertOrder`.  Stable: an expert's pairs
+    are in ascending order.  Numbers outside [0, num_expert) name no expert.  Nothing is read back: the sizes stay on the
+    device.  num_expert <= 1024, n * top_k < 2^31."""
+    lib = load_library()
+    _dev(expert, "expert", torch.int64)
+    if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
+        raise ValueError("expert must be [n] or [n, top_k]")
+    _together(expert)
+    E, P, dev = int(num_expert), expert.numel(), expert.device
+    if E < 1:
+        raise ValueError("num_expert must be positive")
+    at = torch.empty((2, P), dtype=torch.int32, device=dev)
+    offset = torch.empty(E + 1, dtype=torch.int64, device=dev)
+    slot, pair = at.unbind(0)
+    nbytes = int(lib.hc_expert_order_workspace_bytes(P, E))
+    ws = _workspace(nbytes, dev) if nbytes else None
+    _check(lib.hc_expert_order(expert.data_ptr(), P, E, slot.data_ptr(), pair.data_ptr(), offset.data_ptr(), _ptr(ws),
+                               nbytes, _stream()), "hc_expert_order")
+    return ExpertOrder(slot, pair, offset, expert.shape[0], 1 if expert.dim() == 1 else expert.shape[1], E)
+
+
+def _to_experts(x, order):
+    rows = torch.empty((order.places, x.shape[1]), dtype=x.dtype, device=x.device)
+    _check(load_library().hc_rows_to_experts(x.data_ptr(), _DTYPES[x.dtype], order.rows, order.top_k, order.experts,
+                                             x.shape[1], order.slot.data_ptr(), order.offset.data_ptr(), rows.data_ptr(),
+                                             _stream()), "hc_rows_to_experts")
+    return rows
+
+
+def _from_experts(y, order, weight):
+    out = torch.empty((order.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+    _check(load_library().hc_rows_from_experts(y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts,
+                                               y.shape[1], order.slot.data_ptr(), _ptr(weight), out.data_ptr(), _stream()),
+           "hc_rows_from_experts")
+    return out
+
+
+class _RowsToExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.hc = order
+        return _to_experts(x, order)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return _from_experts(_arriving(g), ctx.hc, None), None
+
+
+class _RowsFromExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, order, weight):
+        ctx.hc = order
+        ctx.save_for_backward(y if weight is not None else None, weight)
+        return _from_experts(y, order, weight)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        y, weight = ctx.saved_tensors
+        order, g = ctx.hc, _arriving(g)
+        if weight is None:
+            return _to_experts(g, order), None, None
+        return _from_experts_grads(g, y, order, weight)
+
+
+def _from_experts_grads(g, y, order, weight):
+    grad_y, grad_weight = torch.empty_like(y), torch.empty_like(weight)
+    _check(load_library().hc_rows_from_experts_grad(
+        g.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts, y.shape[1],
+        order.slot.data_ptr(), order.offset.data_ptr(), weight.data_ptr(), grad_y.data_ptr(), grad_weight.data_ptr(),
+        _stream()), "hc_rows_from_experts_grad")
+    return grad_y, None, grad_weight
+
+
+def _expert_rows(t, name, order, a_choice):
+    """Is ``t`` a matrix with a row for every row of the order, or (``a_choice``) for every choice of one?"""
+    _dev(t, name)
+    _float_dtype(t, name)
+    if not isinstance(order, ExpertOrder):
+        raise TypeError("order must be an ExpertOrder")
+    rows = order.places if a_choice else order.rows
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+        raise ValueError(f"{name} must be [{rows}, D], got {tuple(t.shape)}")
+    _together(t, order.slot)
+
+
+def rows_to_experts(x, order):
+    """The rows of x [n, D] in expert order, [n * top_k, D]: place p holds row ``order.pair[p] // top_k``, zeros where there is
+    no pair.  The gradient of a row is the sum over its places."""
+    _expert_rows(x, "x", order, False)
+    return _RowsToExperts.apply(x, order)
+
+
+def rows_from_experts(y, order, weight=None):
+    """``out[i] = sum_j weight[i, j] * y[slot of (i, j)]`` for the experts' results y [n * top_k, D], summed in fp32 in the
+    order of j; choices that name no expert add nothing.  ``weight`` fp32 [n, top_k] (None: ones).  Gradients for y and
+    weight."""
+    _expert_rows(y, "y", order, True)
+    if weight is not None:
+        _dev(weight, "weight", torch.float32)
+        if weight.numel() != order.places:
+            raise ValueError(f"weight must hold {order.places} values")
+        _together(y, weight)
+    return _RowsFromExperts.apply(y, order, weight)
+
+
+class _ExpertLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offset):
+        ctx.save_for_backward(x, w, offset)
+        return _expert_product(x, w, offset, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, offset = ctx.saved_tensors
+        g = _arriving(g)
+        return (_expert_product(g, w, offset, True) if ctx.needs_input_grad[0] else None,
+                expert_linear_grad(g, x, offset) if ctx.needs_input_grad[1] else None, None)
+
+
+def _expert_product(x, w, offset, transposed):
+    S, (E, N, K) = x.shape[0], w.shape
+    if transposed:
+        N, K = K, N
+    out = torch.empty((S, N), dtype=x.dtype, device=x.device)
+    _check(load_library().hc_expert_linear(x.data_ptr(), _DTYPES[x.dtype], w.data_ptr(), int(transposed), offset.data_ptr(),
+                                           S, E, N, K, out.data_ptr(), _stream()), "hc_expert_linear")
+    return out
+
+
+def _expert_offset(offset):
+    _dev(offset, "offset", torch.int64)
+    if offset.dim() != 1 or offset.numel() < 2:
+        raise ValueError("offset must be [E + 1]")
+
+
+def expert_linear(x, w, offset):
+    """``x[s] @ w[e].t()`` for the rows s = offset[e] .. offset[e + 1] of x [S, K], w [E, N, K] of x's type; rows behind
+    offset[E] are zeros.  ``offset`` int64 [E + 1] stays on the device.  Sums in fp32 (fp32 rows: fp32 products), one
+    rounding to the type of x.  Gradients for x and w."""
+    _dev(x, "x")
+    _float_dtype(x, "x")
+    _dev(w, "w", x.dtype)
+    _expert_offset(offset)
+    if x.dim() != 2 or w.dim() != 3 or w.shape[2] != x.shape[1] or offset.numel() != w.shape[0] + 1:
+        raise ValueError(f"x [S, K], w [E, N, K] and offset [E + 1] do not fit: {tuple(x.shape)}, {tuple(w.shape)}, "
+                         f"{tuple(offset.shape)}")
+    _together(x, w, offset)
+    return _ExpertLinear.apply(x, w, offset)
+
+
+def expert_linear_grad(g, x, offset):
+    """``g[rows of e].t() @ x[rows of e]`` for every expert e: [E, N, K] of x's type from g [S, N] and x [S, K]."""
+    lib = load_library()
+    _dev(x, "x")
+    _dev(g, "g", x.dtype)
+    _expert_offset(offset)
+    if g.dim() != 2 or x.dim() != 2 or g.shape[0] != x.shape[0]:
+        raise ValueError("g [S, N] and x [S, K] must have the same number of rows")
+    _together(x, g, offset)
+    (S, N), K, E, dtype = g.shape, x.shape[1], offset.numel() - 1, _float_dtype(x, "x")
+    gw = torch.empty((E, N, K), dtype=x.dtype, device=x.device)
+    nbytes = int(lib.hc_expert_linear_grad_workspace_bytes(S, E, N, K, dtype))
+    ws = _workspace(nbytes, x.device) if nbytes else None
+    _check(lib.hc_expert_linear_grad(g.data_ptr(), x.data_ptr(), dtype, offset.data_ptr(), S, E, N, K, gw.data_ptr(),
+                                     _ptr(ws), nbytes, _stream()), "hc_expert_linear_grad")
+    return gw
+
+
+# ----------------------------------------------------------------------------- activations kept in 8 bits
+class PackedRows:
+    """A matrix kept in 8 bits (:func:`pack_rows`, :func:`gated_pack`): ``codes`` int8 [n, columns] and ``scale`` fp32
+    [n, groups], ``dtype`` the type it had."""
+    __slots__ = ("codes", "scale", "group", "dtype")
+
+    def __init__(self, codes, scale, group, dtype):
+        self.codes, self.scale, self.group, self.dtype = codes, scale, int(group), dtype
+
+
+def _packed_like(x, halves, group):
+    n, F = x.shape[0], x.shape[1] // halves
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty((n, halves * -(-F // group)), dtype=torch.float32, device=x.device)
+    return codes, scale
+
+
+def _pack_arguments(x, name, group):
+    _dev(x, name)
+    _float_dtype(x, name)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{name} must be [n, F]")
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
+    _together(x)
+
+
+def pack_rows(x, group=64):
+    """x [n, F] in 8 bits: every ``group`` adjacent columns of a row share an fp32 scale m * (1 / 127) (m their largest
+    magnitude) and keep rint(x * (1 / m * 127)).  Half a scale is the most that a value is off.  Groups whose m is below 2^-120 are kept as
+    zeros; one that holds an infinity or a NaN reads back as NaN."""
+    _pack_arguments(x, "x", group)
+    codes, scale = _packed_like(x, 1, group)
+    _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], group, codes.data_ptr(),
+                                       scale.data_ptr(), _stream()), "hc_pack_rows")
+    return PackedRows(codes, scale, group, x.dtype)
+
+
+def unpack_rows(kept, dtype=None):
+    """What :func:`pack_rows` kept, [n, F] in ``dtype`` (default: the type it had)."""
+    dtype = kept.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    codes, scale = kept.codes, kept.scale
+    n, F = codes.shape
+    if scale.shape[1] != -(-F // kept.group):
+        raise ValueError("these rows were kept by gated_pack")
+    _together(codes)
+    x = torch.empty((n, F), dtype=dtype, device=codes.device)
+    _check(load_library().hc_unpack_rows(codes.data_ptr(), scale.data_ptr(), n, F, kept.group, x.data_ptr(),
+                                         _DTYPES[dtype], _stream()), "hc_unpack_rows")
+    return x
+
+
+def gated_pack(x, group=64, keep=True):
+    """``silu(a) * b`` for rows [a | b] of x [n, 2 F], and x in 8 bits for :func:`gated_grad`: (h [n, F], PackedRows), the
+    second one None without ``keep``."""
+    _pack_arguments(x, "x", group)
+    if x.shape[1] % 2 != 0:
+        raise ValueError("x must hold two halves of the same width")
+    n, F = x.shape[0], x.shape[1] // 2
+    h = torch.empty((n, F), dtype=x.dtype, device=x.device)
+    codes, scale = _packed_like(x, 2, group) if keep else (None, None)
+    _check(load_library().hc_gated_pack(x.data_ptr(), _DTYPES[x.dtype], n, F, group, h.data_ptr(), _ptr(codes), _ptr(scale),
+                                        _stream()), "hc_gated_pack")
+    return h, PackedRows(codes, scale, group, x.dtype) if keep else None
+
+
+def gated_grad(kept, g):
+    """From what :func:`gated_pack` kept and the gradient g [n, F] of h: the gradient of x [n, 2 F], and h [n, F] again."""
+    codes, scale = kept.codes, kept.scale
+    n, F = codes.shape[0], codes.shape[1] // 2
+    _dev(g, "g", kept.dtype)
+    if codes.shape[1] % 2 or scale.shape[1] != 2 * -(-F // kept.group) or g.shape != (n, F):
+        raise ValueError("g must be [n, F] for rows [n, 2 F] that gated_pack kept")
+    _together(g, codes)
+    gx = torch.empty((n, 2 * F), dtype=kept.dtype, device=g.device)
+    h = torch.empty((n, F), dtype=kept.dtype, device=g.device)
+    _check(load_library().hc_gated_grad(codes.data_ptr(), scale.data_ptr(), g.data_ptr(), _DTYPES[kept.dtype], n, F,
+                                        kept.group, gx.data_ptr(), h.data_ptr(), _stream()), "hc_gated_grad")
+    return gx, h
 
 
 def evict(checkin, slot2full, full2slot, stale_iter, sub2slot=None, score=None, thres=None):

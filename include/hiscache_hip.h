@@ -789,6 +789,82 @@ int hc_bn_relu_bwd_dev(const float *dy, const float *x, const float *gamma, cons
                        float *dbeta, float *dbias, int64_t n, int64_t C, const int64_t *n_dev,
                        void *workspace, size_t workspace_bytes, unsigned *ticket, void *stream);
 
+/* ---------------------------------------------------------------- rows and their experts
+ * Operators of a layer that sends every row to a few of E dense maps.  No
+ * reference counterpart.
+ *
+ * hc_route_rows: softmax of logits [n, E] (dtype), its top_k largest entries in
+ * falling order, of equal ones the lowest index first: expert [n, top_k],
+ * weight [n, top_k].  normalize != 0: a row's weights are divided by their sum.
+ * A logit of -inf closes an expert to the row; where fewer than top_k are open
+ * the rest are -1 with weight 0.  A row with a NaN or +inf has NaN weights.
+ * E <= 1024, top_k <= 32 and <= E.
+ * hc_route_rows_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and
+ * the outputs of hc_route_rows (logits may be NULL with normalize). */
+int hc_route_rows(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int normalize,
+                  int64_t *expert, float *weight, void *stream);
+int hc_route_rows_grad(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int normalize,
+                       const int64_t *expert, const float *weight, const float *grad_weight, void *grad_logits,
+                       void *stream);
+
+/* hc_expert_order: stable sort of the pairs (row, choice) by expert, for
+ * expert [pairs]; numbers outside [0, E) name no expert.  offset[E + 1]: the
+ * places of expert e are offset[e] .. offset[e + 1]; pair[place] and
+ * slot[pair]: -1 where there is none.  E <= 1024, pairs < 2^31.  Kernels only, nothing is read back.
+ * workspace: hc_expert_order_workspace_bytes(pairs, E) (0: none), 16-byte aligned. */
+size_t hc_expert_order_workspace_bytes(int64_t pairs, int64_t E);
+int hc_expert_order(const int64_t *expert, int64_t pairs, int64_t E, int32_t *slot, int32_t *pair,
+                    int64_t *offset, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The rows of x [n, D] (dtype) on their way to the experts and back; slot and
+ * offset from hc_expert_order with pairs = n * top_k, row i owning the pairs
+ * i * top_k ...:
+ *   hc_rows_to_experts         rows[place] = x[row of the place's pair]; 0 behind offset[E]
+ *   hc_rows_from_experts       out[i] = sum_j weight[i, j] y[slot], in fp32 in the order of j
+ *                              (weight NULL: 1, the gradient of hc_rows_to_experts)
+ *   hc_rows_from_experts_grad  grad_y[place] = weight g[row], 0 behind offset[E];
+ *                              grad_weight[i, j] = <g[i], y[slot]>
+ * rows, y, grad_y are [n * top_k, D]. */
+int hc_rows_to_experts(const void *x, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
+                       const int32_t *slot, const int64_t *offset, void *rows, void *stream);
+int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
+                         const int32_t *slot, const float *weight, void *out, void *stream);
+int hc_rows_from_experts_grad(const void *g, const void *y, int dtype, int64_t n, int64_t top_k, int64_t E,
+                              int64_t D, const int32_t *slot, const int64_t *offset, const float *weight,
+                              void *grad_y, float *grad_weight, void *stream);
+
+/* hc_expert_linear: rows offset[e] .. offset[e + 1] of x [S, K] times w[e]
+ * ([E, N, K]; w_is_kn: [E, K, N]), out [S, N], all of one dtype; rows behind
+ * offset[E] are zeros.  Sums in fp32, one rounding.  hc_expert_linear_grad:
+ * grad_w [E, N, K] = g^T x over each expert's rows.  E <= 1024, N and K <= 2^20,
+ * N * K < 2^31, S < 2^31 - 1.  The offsets are read on the device and clamped to
+ * [0, S].  workspace: hc_expert_linear_grad_workspace_bytes (0: none), 16-byte
+ * aligned. */
+int hc_expert_linear(const void *x, int dtype, const void *w, int w_is_kn, const int64_t *offset, int64_t S,
+                     int64_t E, int64_t N, int64_t K, void *out, void *stream);
+size_t hc_expert_linear_grad_workspace_bytes(int64_t S, int64_t E, int64_t N, int64_t K, int dtype);
+int hc_expert_linear_grad(const void *g, const void *x, int dtype, const int64_t *offset, int64_t S, int64_t E,
+                          int64_t N, int64_t K, void *grad_w, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
+/* ---------------------------------------------------------------- activations kept in 8 bits
+ * hc_pack_rows: x [n, F] (dtype) as codes [n, F] and scale [n, ceil(F / group)]:
+ * m the largest magnitude of a group of columns (32, 64 or 128), scale = m * (1 / 127),
+ * code = rint(x * (1 / m * 127)) in fp32; groups with m < 2^-120 are zeros, groups with an
+ * infinity or a NaN read back as NaN.  hc_unpack_rows: x = code * scale.
+ * hc_gated_pack: h [n, F] = silu(a) b for rows [a | b] of x [n, 2 F]; codes
+ * [n, 2 F] and scale [n, 2 ceil(F / group)] (both NULL: not kept), groups of a
+ * and of b apart.  hc_gated_grad: from those, the gradient of x [n, 2 F] and
+ * (h not NULL) h again, for grad_h [n, F]. */
+int hc_pack_rows(const void *x, int dtype, int64_t n, int64_t F, int64_t group, int8_t *codes, float *scale,
+                 void *stream);
+int hc_unpack_rows(const int8_t *codes, const float *scale, int64_t n, int64_t F, int64_t group, void *x,
+                   int dtype, void *stream);
+int hc_gated_pack(const void *x, int dtype, int64_t n, int64_t F, int64_t group, void *h, int8_t *codes,
+                  float *scale, void *stream);
+int hc_gated_grad(const int8_t *codes, const float *scale, const void *grad_h, int dtype, int64_t n, int64_t F,
+                  int64_t group, void *grad_x, void *h, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
