@@ -1,0 +1,85 @@
+// Which rows a block of an expert product works on, found from the offsets in device memory.
+#pragma once
+
+#include "hc_common.h"
+
+// Part `part` of the `parts` that expert `expert`'s rows are cut into.  Every wave of the block calls el_find and gets the same.
+struct ElPart {
+  int expert;            // E: the rows behind the last expert; E + 1: there is no such part
+  int part, parts;
+  int place;             // parts before it, counting experts of several parts only (where its partial sums lie)
+  int64_t lo, hi;        // its rows
+};
+
+// Rows offset[e] .. offset[e + 1] (offsets out of order or range describe no rows, but never ones outside x).
+__device__ __forceinline__ void el_rows_of(const int64_t *__restrict__ offset, int E, int64_t S, int e, int64_t *lo, int64_t *hi) {
+  int64_t a = 0, b = 0;
+  if (e <= E) {
+    a = offset[e];
+    a = a < 0 ? 0 : a > S ? S : a;
+    b = e < E ? offset[e + 1] : S;
+    b = b < a ? a : b > S ? S : b;
+  }
+  *lo = a;
+  *hi = b;
+}
+
+__device__ __forceinline__ int el_scan(int v) {
+  const int lane = hc_lane();
+#pragma unroll
+  for (int d = 1; d < HC_WAVE; d *= 2) {
+    const int o = __shfl_up(v, d, HC_WAVE);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// Part `t` of the experts' rows in parts of `rows`.  REST: the rows behind the last expert follow as expert E; else an expert
+// without rows has one part of none (whose gradient is zeros).
+template <bool REST>
+__device__ __forceinline__ ElPart el_find(const int64_t *__restrict__ offset, int E, int64_t S, int64_t rows, int t) {
+  const int lane = hc_lane();
+  int before = 0, several = 0;
+  for (int e0 = 0; e0 < E + (REST ? 1 : 0); e0 += HC_WAVE) {
+    const int e = e0 + lane;
+    int64_t lo, hi;
+    el_rows_of(offset, E, S, e, &lo, &hi);
+    int parts = (int)((hi - lo + rows - 1) / rows);
+    if (!REST) parts = e >= E ? 0 : parts < 1 ? 1 : parts;
+    const int upto = el_scan(parts), more = parts > 1 ? parts : 0, more_upto = REST ? 0 : el_scan(more);
+    const uint64_t in = __ballot(t < before + upto);
+    if (in != 0) {
+      const int l = __ffsll((long long)in) - 1;
+      ElPart r;
+      r.expert = e0 + l;
+      r.parts = __builtin_amdgcn_readlane(parts, l);
+      r.part = t - (before + __builtin_amdgcn_readlane(upto, l) - r.parts);
+      r.place = several + __builtin_amdgcn_readlane(more_upto - more, l) + r.part;
+      r.lo = hc_readlane64(lo, l) + r.part * rows;
+      const int64_t end = hc_readlane64(hi, l);
+      r.hi = r.lo + rows < end ? r.lo + rows : end;
+      return r;
+    }
+    before += __builtin_amdgcn_readlane(upto, HC_WAVE - 1);
+    if (!REST) several += __builtin_amdgcn_readlane(more_upto, HC_WAVE - 1);
+  }
+  ElPart r = {};
+  r.expert = E + 1;
+  return r;
+}
+
+// expert_half.hip: the products of 16-bit rows (arguments are checked by the callers).
+struct ElProduct {
+  const void *p, *q;            // rows of the result come from p, columns from q
+  void *out;
+  const int64_t *offset;
+  int64_t S;
+  int E, rows, cols, inner;     // rows: of one expert's gradient (by rows of the batch: unused)
+  int tiles_p, tiles_q;
+  int64_t slab;                 // rows of the batch in one part of a gradient
+  float *part;                  // their partial sums
+  bool whole;                   // the result is stored in pieces of 16 bytes
+};
+__attribute__((visibility("hidden"))) int el_half_rows(int dtype, bool w_is_kn, ElProduct a, hipStream_t st);
+__attribute__((visibility("hidden"))) size_t el_half_grad_bytes(int64_t S, int64_t E, int64_t N, int64_t K);
+__attribute__((visibility("hidden"))) int el_half_grad(int dtype, ElProduct a, void *workspace, size_t workspace_bytes, hipStream_t st);

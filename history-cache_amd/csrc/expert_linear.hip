@@ -6,61 +6,13 @@
 //
 // The offsets stay on the device.  A launch has as many tiles of rows as S rows in E groups can need at most; a block finds
 // its expert by a prefix sum over the groups' tiles, and one whose number is behind the last tile ends.
-#include "hc_common.h"
+#include "expert_find.h"
 
 namespace {
 
 constexpr int EL_MAX_EXPERTS = 1024;
 
 typedef float el_acc __attribute__((ext_vector_type(4)));
-
-// Tile `t` of `rows` rows each over the groups, the rows behind the last one being group E.
-struct ElTile {
-  int expert;            // E + 1: there is no such tile
-  int part, parts;       // the tile's number in its group, the group's tiles
-  int before;            // tiles of the groups in front
-  int64_t lo, hi;        // its rows
-};
-
-__device__ __forceinline__ ElTile el_find(const int64_t *__restrict__ offset, int E, int64_t S, int rows, int t) {
-  const int lane = hc_lane();
-  int before = 0;
-  for (int e0 = 0; e0 <= E; e0 += HC_WAVE) {
-    const int e = e0 + lane;
-    int64_t lo = 0, hi = 0;
-    if (e <= E) {
-      // (offsets that are out of order or range describe no rows, but never ones outside x)
-      lo = offset[e];
-      lo = lo < 0 ? 0 : lo > S ? S : lo;
-      hi = e < E ? offset[e + 1] : S;
-      hi = hi < lo ? lo : hi > S ? S : hi;
-    }
-    const int tiles = (int)((hi - lo + rows - 1) / rows);
-    int s = tiles;
-#pragma unroll
-    for (int d = 1; d < HC_WAVE; d *= 2) {
-      const int o = __shfl_up(s, d, HC_WAVE);
-      if (lane >= d) s += o;
-    }
-    const uint64_t in = __ballot(t < before + s);
-    if (in != 0) {
-      const int l = __ffsll((long long)in) - 1;
-      ElTile r;
-      r.expert = e0 + l;
-      r.parts = __builtin_amdgcn_readlane(tiles, l);
-      r.before = before + __builtin_amdgcn_readlane(s, l) - r.parts;
-      r.part = t - r.before;
-      r.lo = hc_readlane64(lo, l) + (int64_t)r.part * rows;
-      const int64_t end = hc_readlane64(hi, l);
-      r.hi = r.lo + rows < end ? r.lo + rows : end;
-      return r;
-    }
-    before += __builtin_amdgcn_readlane(s, HC_WAVE - 1);
-  }
-  ElTile r = {};
-  r.expert = E + 1;
-  return r;
-}
 
 struct ElArgs {
   const void *a, *w;
@@ -90,7 +42,7 @@ __global__ __launch_bounds__(HC_BLOCK) void el_rows(ElArgs a, bool whole_a, bool
   constexpr int LDA = EL_BK + 2, LDW = KN ? EL_B + 16 : EL_BK + 2;
   __shared__ __attribute__((aligned(16))) float sa[EL_B * LDA], sw[KN ? EL_BK * LDW : EL_B * LDW];
   const int b = (int)blockIdx.x, n0 = b % a.tiles_n * EL_B;
-  const ElTile tile = el_find(a.offset, a.E, a.S, EL_B, b / a.tiles_n);
+  const ElPart tile = el_find<true>(a.offset, a.E, a.S, EL_B, b / a.tiles_n);
   if (tile.expert > a.E) return;
   const int t = (int)threadIdx.x, lane = hc_lane(), wave = hc_wave_in_block();
   const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32, l16 = lane & 15, g4 = lane >> 4;
@@ -222,8 +174,6 @@ __global__ __launch_bounds__(HC_BLOCK) void el_wgrad(ElGradArgs a, bool whole_g,
 template <typename F>
 static int el_with_type(int dtype, F &&f) {
   if (dtype == HC_F32) return f(float{});
-  if (dtype == HC_F16) return f(__half{});
-  if (dtype == HC_BF16) return f(__hip_bfloat16{});
   return HC_EDTYPE;
 }
 
@@ -244,6 +194,12 @@ extern "C" int hc_expert_linear(const void *x, int dtype, const void *w, int w_i
   if (!el_sizes_ok(S, E, N, K)) return HC_EUNSUPPORTED;
   if (S == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
   HC_REQUIRE(x && w && offset && out);
+  if (dtype == HC_F16 || dtype == HC_BF16) {
+    ElProduct p = {};
+    p.p = x, p.q = w, p.out = out, p.offset = offset, p.S = S;
+    p.E = (int)E, p.cols = (int)N, p.inner = (int)K;
+    return el_half_rows(dtype, w_is_kn != 0, p, static_cast<hipStream_t>(stream));
+  }
   return el_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
     ElArgs a = {x, w, out, offset, S, (int)E, (int)N, (int)K, (int)((N + EL_B - 1) / EL_B)};
@@ -257,7 +213,8 @@ extern "C" int hc_expert_linear(const void *x, int dtype, const void *w, int w_i
 }
 
 extern "C" size_t hc_expert_linear_grad_workspace_bytes(int64_t S, int64_t E, int64_t N, int64_t K, int dtype) {
-  return 0;
+  if (S < 0 || E < 1 || N < 1 || K < 1 || !el_sizes_ok(S, E, N, K)) return 0;
+  return dtype == HC_F32 ? 0 : el_half_grad_bytes(S, E, N, K);
 }
 
 extern "C" int hc_expert_linear_grad(const void *g, const void *x, int dtype, const int64_t *offset, int64_t S, int64_t E,
@@ -266,6 +223,12 @@ extern "C" int hc_expert_linear_grad(const void *g, const void *x, int dtype, co
   HC_REQUIRE(S >= 0 && E >= 1 && N >= 1 && K >= 1);
   if (!el_sizes_ok(S, E, N, K)) return HC_EUNSUPPORTED;
   HC_REQUIRE(offset && grad_w && (S == 0 || (g && x)));
+  if (dtype == HC_F16 || dtype == HC_BF16) {
+    ElProduct p = {};
+    p.p = g, p.q = x, p.out = grad_w, p.offset = offset, p.S = S;
+    p.E = (int)E, p.rows = (int)N, p.cols = (int)K;
+    return el_half_grad(dtype, p, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  }
   return el_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
     ElGradArgs a = {g, x, grad_w, offset, S, (int)E, (int)N, (int)K, (int)((N + EL_B - 1) / EL_B), (int)((K + EL_B - 1) / EL_B)};
