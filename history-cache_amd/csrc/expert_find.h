@@ -68,7 +68,7 @@ __device__ __forceinline__ ElPart el_find(const int64_t *__restrict__ offset, in
   return r;
 }
 
-// expert_half.hip: the products of 16-bit rows (arguments are checked by the callers).
+// A product for the kernels of expert_tile.h.
 struct ElProduct {
   const void *p, *q;            // rows of the result come from p, columns from q
   void *out;
@@ -80,6 +80,12 @@ struct ElProduct {
   float *part;                  // their partial sums
   bool whole;                   // the result is stored in pieces of 16 bytes
 };
-__attribute__((visibility("hidden"))) int el_half_rows(int dtype, bool w_is_kn, ElProduct a, hipStream_t st);
-__attribute__((visibility("hidden"))) size_t el_half_grad_bytes(int64_t S, int64_t E, int64_t N, int64_t K);
-__attribute__((visibility("hidden"))) int el_half_grad(int dtype, ElProduct a, void *workspace, size_t workspace_bytes, hipStream_t st);
+
+// expert_f32.hip, expert_f16.hip, expert_bf16.hip (arguments are checked by the callers).
+#define EL_DECLARE(name)                                                                                              \
+  __attribute__((visibility("hidden"))) int el_rows_##name(bool w_is_kn, const ElProduct &a, hipStream_t st);        \
+  __attribute__((visibility("hidden"))) size_t el_grad_bytes_##name(int64_t S, int64_t E, int64_t N, int64_t K);     \
+  __attribute__((visibility("hidden"))) int el_grad_##name(const ElProduct &a, void *workspace, size_t workspace_bytes, hipStream_t st)
+EL_DECLARE(f32);
+EL_DECLARE(f16);
+EL_DECLARE(bf16);

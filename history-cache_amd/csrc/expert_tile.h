@@ -1,0 +1,401 @@
+// A tile of an expert product on the matrix cores: the kernels behind hc_expert_linear and hc_expert_linear_grad, a template
+// that expert_f32.hip, expert_f16.hip and expert_bf16.hip fill in for their type.
+//
+//   result[P, Q] = sum over the inner index of p[P, inner] * q[Q, inner]
+//     forward            P: rows of the batch, Q: rows of w[e],    inner: columns of both
+//     gradient of x      P: rows of the batch, Q: columns of w[e], inner: rows of w[e]           (KN)
+//     gradient of w      P: columns of g,      Q: columns of x,    inner: rows of the batch      (GRAD)
+#pragma once
+
+#include "expert_find.h"
+
+namespace {
+
+typedef float el_acc __attribute__((ext_vector_type(16)));
+typedef float el_four __attribute__((ext_vector_type(4)));
+typedef short el_eight __attribute__((ext_vector_type(8)));
+typedef short el_quad __attribute__((ext_vector_type(4)));
+typedef uint32_t el_piece __attribute__((ext_vector_type(4)));
+
+constexpr int EL_ROW = 128;                     // bytes of inner index in a piece: 64 elements of 16 bits, 32 of fp32
+constexpr uint32_t EL_NOWHERE = 0xfffffff0u;    // behind every buffer: reads as zero
+#define EL_LDS __attribute__((address_space(3)))
+
+// 16 bytes of the inner index for 32 rows by each half of the wave; both operands go by the same order, so that which of the
+// instruction's inner indices a value takes does not matter.
+template <typename T>
+struct el_type {
+  typedef el_eight frag;
+  __device__ __forceinline__ static el_acc mfma(frag a, frag b, el_acc c) {
+    if constexpr (std::is_same<T, __half>::value) {
+      typedef _Float16 f16 __attribute__((ext_vector_type(8)));
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16, a), __builtin_bit_cast(f16, b), c, 0, 0, 0);
+    } else {
+      typedef __bf16 b16 __attribute__((ext_vector_type(8)));
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16, a), __builtin_bit_cast(b16, b), c, 0, 0, 0);
+    }
+  }
+};
+template <>
+struct el_type<float> {
+  typedef el_four frag;
+  __device__ __forceinline__ static el_acc mfma(frag a, frag b, el_acc c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// A piece of an operand in LDS: W rows (columns) of the result by 128 bytes of inner index, in chunks of 16 bytes.
+//   TR = false: inner index along memory, [W][128 bytes]; chunk c of row r lies at c ^ (r & 7), so that eight rows read at a time
+//               lie in different banks
+//   TR = true:  inner index outside.  16 bits: read by ds_read_b64_tr_b16, 4 rows x 16 columns by 16 lanes; columns 16 c .. of
+//               inner row r lie at c ^ (r & 7).  fp32: read by columns, in order
+// PIECE = 16 bytes: chunks go straight into LDS, which takes rows that start on 16 bytes; else they are loaded in pieces of
+// PIECE bytes, which may end inside a chunk, and pass through registers.
+template <typename T, int W, bool TR, int THREADS, int PIECE>
+struct el_operand {
+  static constexpr int PER = 16 / (int)sizeof(T), INNER = EL_ROW / (int)sizeof(T);
+  static constexpr int CHUNKS = W * 8, EACH = CHUNKS / THREADS;
+  static_assert(CHUNKS % THREADS == 0, "whole chunks per thread");
+  uint32_t at[EACH];        // byte offset of this thread's chunks in the operand's first piece
+  int first[EACH];          // first inner index (TR = false) or column of each
+  el_piece held[PIECE == 16 ? 1 : EACH];
+  int width;
+
+  // stride: of the operand's rows in elements; wide: rows (TR = false) or columns (TR = true) that exist from the tile's first on
+  __device__ __forceinline__ void init(int t, uint32_t stride, int wide) {
+    width = wide;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int q = i * THREADS + t;
+      int r, c;
+      if constexpr (!TR) {
+        r = q / 8;
+        c = (q % 8) ^ (r & 7);
+      } else {
+        r = q / (W / PER);
+        c = q % (W / PER);
+        if constexpr (sizeof(T) == 2) c = ((c / 2) ^ (r & 7)) * 2 + c % 2;
+      }
+      first[i] = c * PER;
+      at[i] = (TR ? first[i] : r) < wide ? ((uint32_t)r * stride + (uint32_t)first[i]) * (uint32_t)sizeof(T) : EL_NOWHERE;
+    }
+  }
+  // left: inner indices from the piece's first on
+  __device__ __forceinline__ void fetch(hc_buffer b, EL_LDS char *lds, int wave, int left) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if constexpr (PIECE == 16) {
+        const uint32_t o = TR || first[i] < left ? at[i] : EL_NOWHERE;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (EL_LDS void *)(lds + (i * THREADS + wave * HC_WAVE) * 16), 16, o, 0, 0, 0);
+      } else {
+        const int end = TR ? width : left;
+#pragma unroll
+        for (int p = 0; p < 16; p += PIECE) {
+          const uint32_t o = first[i] + p / (int)sizeof(T) < end && at[i] != EL_NOWHERE ? at[i] + p : EL_NOWHERE;
+          if constexpr (PIECE == 8) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b64(b, o, 0, 0);
+            held[i][p / 4] = v[0];
+            held[i][p / 4 + 1] = v[1];
+          } else if constexpr (PIECE == 4) {
+            held[i][p / 4] = __builtin_amdgcn_raw_buffer_load_b32(b, o, 0, 0);
+          } else {
+            const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(b, o, 0, 0);
+            held[i][p / 4] = p % 4 == 0 ? v : held[i][p / 4] | v << 16;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(EL_LDS char *lds, int t) const {
+    if constexpr (PIECE != 16)
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) *(EL_LDS el_piece *)(lds + (i * THREADS + t) * 16) = held[i];
+  }
+  // The fragment of 32 rows (columns) from `from` on in the k-th quarter of the piece: lane l has row from + l % 32 and of the
+  // quarter's 32 bytes of inner index the half l / 32.
+  __device__ __forceinline__ static typename el_type<T>::frag read(const EL_LDS char *lds, int from, int k) {
+    const int lane = hc_lane();
+    if constexpr (!TR) {
+      const int r = from + (lane & 31), c = k * 2 + (lane >> 5);
+      return *(const EL_LDS typename el_type<T>::frag *)(lds + r * EL_ROW + ((c ^ (lane & 7)) * 16));
+    } else if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, g = lane >> 4;
+      const int r = k * 16 + (g >> 1) * 8 + (i >> 2), c = from / 16 + (g & 1);
+      const EL_LDS char *p = lds + r * (W * 2) + (i & 3) * 8;
+      const el_quad a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + ((c ^ (i >> 2)) * 32)));
+      const el_quad b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + 4 * (W * 2) + ((c ^ ((i >> 2) + 4)) * 32)));
+      return el_eight{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+      const EL_LDS float *p = (const EL_LDS float *)lds + (k * 8 + (lane >> 5) * 4) * W + from + (lane & 31);
+      return el_four{p[0], p[W], p[2 * W], p[3 * W]};
+    }
+  }
+};
+
+// A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of 128 bytes of inner index through two
+// stages in LDS, the next piece on its way while one is multiplied.
+template <typename T, int BP, int BQ, int WP, int WQ, bool GRAD, bool KN, int PIECE>
+__global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
+  constexpr int THREADS = WP * WQ * HC_WAVE, TP = BP / WP / 32, TQ = BQ / WQ / 32, PER = 16 / (int)sizeof(T);
+  constexpr bool PT = GRAD, QT = GRAD || KN;
+  typedef el_operand<T, BP, PT, THREADS, PIECE> op_p;
+  typedef el_operand<T, BQ, QT, THREADS, PIECE> op_q;
+  typedef typename el_type<T>::frag frag;
+  constexpr int BK = op_p::INNER, BYTES_P = BP * EL_ROW, STAGE = (BP + BQ) * EL_ROW;
+  constexpr uint32_t SIZE = sizeof(T);
+  __shared__ __attribute__((aligned(16))) char s_mem[2 * STAGE];
+  EL_LDS char *lds = (EL_LDS char *)s_mem;
+  const int64_t b = hc_xcd_block<32>(blockIdx.x, gridDim.x);
+  const int t = (int)threadIdx.x, lane = hc_lane(), wave = hc_wave_in_block();
+  const int wp = wave % WP * (BP / WP), wq = wave / WP * (BQ / WQ);
+  const int per = GRAD ? a.tiles_p * a.tiles_q : a.tiles_q, in = (int)(b % per);
+  const ElPart part = el_find<!GRAD>(a.offset, a.E, a.S, GRAD ? a.slab : BP, (int)(b / per));
+  if (part.expert > a.E) return;
+  const int q0 = in % a.tiles_q * BQ, p0 = GRAD ? in / a.tiles_q * BP : 0;
+  const int64_t e = part.expert < a.E ? part.expert : 0;
+  const int batch = (int)(part.hi - part.lo);                           // rows of the batch
+  const int rows_out = GRAD ? (a.rows - p0 < BP ? a.rows - p0 : BP) : batch, cols_out = a.cols - q0 < BQ ? a.cols - q0 : BQ;
+  const int inner = GRAD ? batch : part.expert < a.E ? a.inner : 0;     // (rows behind the last expert: zeros)
+  const uint32_t ld_p = GRAD ? a.rows : a.inner, ld_q = QT ? a.cols : a.inner;
+  const T *pp = static_cast<const T *>(a.p) + (GRAD ? part.lo * a.rows + p0 : part.lo * a.inner);
+  const T *pq = static_cast<const T *>(a.q) +
+                (GRAD ? part.lo * a.cols + q0 : e * a.inner * a.cols + (KN ? (int64_t)q0 : (int64_t)q0 * a.inner));
+  op_p fp;
+  op_q fq;
+  fp.init(t, ld_p, rows_out);
+  fq.init(t, ld_q, cols_out);
+  const auto fetch = [&](int s, int k0) {
+    const int left = inner - k0, n = left < BK ? left : BK;
+    // a buffer with the inner index outside ends with the last row that exists
+    const hc_buffer bp = hc_make_buffer(PT ? pp + (int64_t)k0 * ld_p : pp + k0, PT ? ((uint32_t)(n - 1) * ld_p + (uint32_t)rows_out) * SIZE : 0xffffff00u);
+    const hc_buffer bq = hc_make_buffer(QT ? pq + (int64_t)k0 * ld_q : pq + k0, QT ? ((uint32_t)(n - 1) * ld_q + (uint32_t)cols_out) * SIZE : 0xffffff00u);
+    fp.fetch(bp, lds + s * STAGE, wave, left);
+    fq.fetch(bq, lds + s * STAGE + BYTES_P, wave, left);
+  };
+  const auto put = [&](int s) {
+    fp.put(lds + s * STAGE, t);
+    fq.put(lds + s * STAGE + BYTES_P, t);
+  };
+  el_acc acc[TP][TQ];
+#pragma unroll
+  for (int i = 0; i < TP; ++i)
+#pragma unroll
+    for (int j = 0; j < TQ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  const auto compute = [&](int s) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      frag u[TP], v[TQ];
+#pragma unroll
+      for (int i = 0; i < TP; ++i) u[i] = op_p::read(lds + s * STAGE, wp + i * 32, k);
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) v[j] = op_q::read(lds + s * STAGE + BYTES_P, wq + j * 32, k);
+#pragma unroll
+      for (int i = 0; i < TP; ++i)
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) acc[i][j] = el_type<T>::mfma(v[j], u[i], acc[i][j]);
+    }
+  };
+  if (inner > 0) {
+    fetch(0, 0);
+    put(0);
+  }
+  int s = 0;
+  for (int k0 = 0; k0 < inner; k0 += BK) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt 0: what this wave has fetched is in LDS
+    __syncthreads();
+    const bool more = k0 + BK < inner;
+    if (more) fetch(s ^ 1, k0 + BK);
+    __builtin_amdgcn_sched_barrier(0);
+    compute(s);
+    s ^= 1;
+    if (more) put(s);
+  }
+  // lane l has row l % 32 of a tile of 32 x 32 and of every eight columns the four from 4 (l / 32) on
+  const int l32 = lane & 31, h = lane >> 5;
+  if (GRAD && part.parts > 1) {
+    float *o = a.part + (int64_t)part.place * a.rows * a.cols + (int64_t)p0 * a.cols + q0;
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+#pragma unroll
+      for (int j = 0; j < TQ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = wp + i * 32 + l32, col = wq + j * 32 + r / 4 * 8 + h * 4 + r % 4;
+          if (row < rows_out && col < cols_out) o[(int64_t)row * a.cols + col] = acc[i][j][r];
+        }
+    return;
+  }
+  T *out = static_cast<T *>(a.out) + (GRAD ? (e * a.rows + p0) * a.cols + q0 : part.lo * a.cols + q0);
+  // a wave's 32 rows at a time through its own piece of LDS, so that a row leaves in pieces of 16 bytes
+  constexpr int ROW = TQ * 32 + PER;
+  static_assert(WP * WQ * 32 * ROW * (int)sizeof(T) <= 2 * STAGE, "the way out fits the stages");
+  __syncthreads();
+  T *own = reinterpret_cast<T *>(s_mem) + wave * 32 * ROW;
+#pragma unroll
+  for (int i = 0; i < TP; ++i) {
+#pragma unroll
+    for (int j = 0; j < TQ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float v[4] = {acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+        hc_vec<T, 4>::store(own + l32 * ROW + j * 32 + r * 2 + h * 4, v);
+      }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PIECES = TQ * 32 / PER;                  // of a row
+#pragma unroll
+    for (int q = 0; q < 32 * PIECES / HC_WAVE; ++q) {
+      const int f = q * HC_WAVE + lane, row = f / PIECES, c = f % PIECES * PER;
+      const int orow = wp + i * 32 + row, ocol = wq + c;
+      if (orow < rows_out && ocol < cols_out) {
+        T *o = out + (int64_t)orow * a.cols + ocol;
+        if (a.whole) {
+          *reinterpret_cast<el_piece *>(o) = *reinterpret_cast<const el_piece *>(own + row * ROW + c);
+        } else {
+#pragma unroll
+          for (int x = 0; x < PER; ++x)
+            if (ocol + x < cols_out) o[x] = own[row * ROW + c + x];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The gradients of experts of several parts: their partial sums added in the order of the parts.
+template <typename T>
+__global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, int64_t pieces) {
+  const int lane = hc_lane();
+  int before = 0;
+  for (int e0 = 0; e0 < a.E; e0 += HC_WAVE) {
+    int64_t lo, hi;
+    el_rows_of(a.offset, a.E, a.S, e0 + lane < a.E ? e0 + lane : a.E + 1, &lo, &hi);
+    int parts = (int)((hi - lo + a.slab - 1) / a.slab);
+    parts = parts > 1 ? parts : 0;
+    const int first = before + el_scan(parts) - parts;
+    uint64_t several = __ballot(parts > 0);
+    while (several != 0) {
+      const int l = __ffsll((long long)several) - 1;
+      several &= several - 1;
+      const int n = __builtin_amdgcn_readlane(parts, l);
+      const float *p = a.part + (int64_t)__builtin_amdgcn_readlane(first, l) * size;
+      T *o = static_cast<T *>(a.out) + (e0 + l) * size;
+      for (int64_t i = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * HC_BLOCK) {
+        const int64_t at = i * 4;
+        if (size % 4 == 0 && a.whole) {
+          float4 s = *reinterpret_cast<const float4 *>(p + at);
+          for (int q = 1; q < n; ++q) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + q * size + at);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+          }
+          const float v[4] = {s.x, s.y, s.z, s.w};
+          hc_vec<T, 4>::store(o + at, v);
+        } else {
+          for (int x = 0; x < 4 && at + x < size; ++x) {
+            float s = p[at + x];
+            for (int q = 1; q < n; ++q) s += p[q * size + at + x];
+            o[at + x] = hc_from_f32<T>(s);
+          }
+        }
+      }
+    }
+    before = __builtin_amdgcn_readlane(first + parts, HC_WAVE - 1);
+  }
+}
+
+template <typename T, int BP, int BQ, int WP, int WQ, bool GRAD, bool KN, int PIECE>
+static int el_launch(ElProduct a, int64_t parts, hipStream_t st) {
+  a.tiles_p = GRAD ? (a.rows + BP - 1) / BP : 1;
+  a.tiles_q = (a.cols + BQ - 1) / BQ;
+  const int64_t blocks = parts * a.tiles_p * a.tiles_q;
+  if (!hc_grid_ok(blocks)) return HC_EUNSUPPORTED;
+  el_tile<T, BP, BQ, WP, WQ, GRAD, KN, PIECE><<<dim3((unsigned)blocks), dim3(WP * WQ * HC_WAVE), 0, st>>>(a);
+  return hc_launch_status();
+}
+
+// Bytes in a piece that rows of these widths at these addresses allow.
+static int el_piece_of(const void *p, const void *q, int64_t w0, int64_t w1, int size) {
+  const uint64_t a = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | (uint64_t)(w0 * size) | (uint64_t)(w1 * size);
+  return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : a % 4 == 0 ? 4 : 2;
+}
+
+#ifndef EL_BIG
+#define EL_BIG(tiles) ((tiles) >= 192)
+#endif
+
+template <typename T, bool KN>
+static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
+  const int piece = el_piece_of(a.p, a.q, a.inner, KN ? a.cols : a.inner, (int)sizeof(T));
+  if constexpr (sizeof(T) == 2) {
+    const int64_t big = (a.S + 255) / 256 * ((a.cols + 255) / 256);
+    if (piece == 16 && EL_BIG(big)) return el_launch<T, 256, 256, 2, 4, false, KN, 16>(a, a.S / 256 + a.E + 1, st);
+    if (piece == 2) return el_launch<T, 128, 128, 2, 2, false, KN, 2>(a, a.S / 128 + a.E + 1, st);
+  }
+  const int64_t parts = a.S / 128 + a.E + 1;
+  if (piece == 16) return el_launch<T, 128, 128, 2, 2, false, KN, 16>(a, parts, st);
+  if (piece == 8) return el_launch<T, 128, 128, 2, 2, false, KN, 8>(a, parts, st);
+  return el_launch<T, 128, 128, 2, 2, false, KN, 4>(a, parts, st);
+}
+
+struct ElGradShape {
+  bool big;
+  int64_t slab, several;        // rows of a part; parts of experts with several of them, at most
+};
+
+static ElGradShape el_grad_shape(int64_t S, int64_t E, int64_t N, int64_t K, int size, bool wide) {
+  ElGradShape g;
+  const int64_t tiles = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
+  g.big = wide && size == 2 && EL_BIG(tiles * E);
+  const int64_t want = g.big ? 256 : 1024, have = g.big ? tiles : small;
+  g.slab = (S * have / want + 63) / 64 * 64;
+  if (g.slab < 512) g.slab = 512;
+  // an expert of p > 1 parts has more than (p - 1) slab >= p / 2 slab rows
+  g.several = S <= g.slab ? 0 : 2 * (S / g.slab);
+  return g;
+}
+
+template <typename T>
+static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  const int piece = el_piece_of(a.p, a.q, a.rows, a.cols, (int)sizeof(T));
+  const ElGradShape g = el_grad_shape(a.S, a.E, a.rows, a.cols, (int)sizeof(T), piece == 16);
+  const int64_t size = (int64_t)a.rows * a.cols;
+  if ((size_t)(g.several * size) * sizeof(float) > workspace_bytes ||
+      (g.several && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+    return HC_EWORKSPACE;
+  a.part = static_cast<float *>(workspace);
+  a.slab = g.slab;
+  const int64_t parts = a.S / g.slab + a.E;
+  int rc = HC_EUNSUPPORTED;
+  if constexpr (sizeof(T) == 2) {
+    if (g.big) rc = el_launch<T, 256, 256, 2, 4, true, false, 16>(a, parts, st);
+    else if (piece == 2) rc = el_launch<T, 128, 128, 2, 2, true, false, 2>(a, parts, st);
+  }
+  if (!g.big && piece == 16) rc = el_launch<T, 128, 128, 2, 2, true, false, 16>(a, parts, st);
+  else if (!g.big && piece == 8) rc = el_launch<T, 128, 128, 2, 2, true, false, 8>(a, parts, st);
+  else if (!g.big && piece == 4) rc = el_launch<T, 128, 128, 2, 2, true, false, 4>(a, parts, st);
+  if (rc != HC_OK || g.several == 0) return rc;
+  const int64_t pieces = (size + 3) / 4;
+  int64_t blocks = (pieces + HC_BLOCK - 1) / HC_BLOCK;
+  blocks = blocks > 2048 ? 2048 : blocks;
+  a.whole = reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0;
+  el_join<T><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, st>>>(a, size, pieces);
+  return hc_launch_status();
+}
+
+}  // namespace
+
+#define EL_FOR_TYPE(T, name)                                                                                       \
+  int el_rows_##name(bool w_is_kn, const ElProduct &a, hipStream_t st) {                                           \
+    return w_is_kn ? el_rows_of_type<T, true>(a, st) : el_rows_of_type<T, false>(a, st);                           \
+  }                                                                                                                \
+  int el_grad_##name(const ElProduct &a, void *workspace, size_t workspace_bytes, hipStream_t st) {                \
+    return el_grad_of_type<T>(a, workspace, workspace_bytes, st);                                                  \
+  }                                                                                                                \
+  size_t el_grad_bytes_##name(int64_t S, int64_t E, int64_t N, int64_t K) {                                        \
+    const int64_t wide = el_grad_shape(S, E, N, K, (int)sizeof(T), true).several;                                  \
+    const int64_t other = el_grad_shape(S, E, N, K, (int)sizeof(T), false).several;                                \
+    return (size_t)(wide > other ? wide : other) * (size_t)N * (size_t)K * sizeof(float);                          \
+  }
