@@ -3,7 +3,7 @@
 
 #include "hc_common.h"
 
-// Part `part` of the `parts` that expert `expert`'s rows are cut into.  Every wave of the block calls el_find and gets the same.
+// Part `part` of the `parts` that expert `expert`'s rows are cut into.  Every wave of a block looks for it and finds the same.
 struct ElPart {
   int expert;            // E: the rows behind the last expert; E + 1: there is no such part
   int part, parts;
@@ -34,34 +34,74 @@ __device__ __forceinline__ int el_scan(int v) {
   return v;
 }
 
-// Part `t` of the experts' rows in parts of `rows`.  REST: the rows behind the last expert follow as expert E; else an expert
-// without rows has one part of none (whose gradient is zeros).
-template <bool REST>
-__device__ __forceinline__ ElPart el_find(const int64_t *__restrict__ offset, int E, int64_t S, int64_t rows, int t) {
+// The t-th piece of up to `rows` rows, expert by expert; the rows behind the last expert follow as expert E.
+__device__ __forceinline__ ElPart el_find_rows(const int64_t *__restrict__ offset, int E, int64_t S, int rows, int t) {
   const int lane = hc_lane();
-  int before = 0, several = 0;
-  for (int e0 = 0; e0 < E + (REST ? 1 : 0); e0 += HC_WAVE) {
-    const int e = e0 + lane;
+  int before = 0;
+  for (int e0 = 0; e0 <= E; e0 += HC_WAVE) {
     int64_t lo, hi;
-    el_rows_of(offset, E, S, e, &lo, &hi);
-    int parts = (int)((hi - lo + rows - 1) / rows);
-    if (!REST) parts = e >= E ? 0 : parts < 1 ? 1 : parts;
-    const int upto = el_scan(parts), more = parts > 1 ? parts : 0, more_upto = REST ? 0 : el_scan(more);
+    el_rows_of(offset, E, S, e0 + lane, &lo, &hi);
+    const int parts = (int)((hi - lo + rows - 1) / rows), upto = el_scan(parts);
     const uint64_t in = __ballot(t < before + upto);
     if (in != 0) {
       const int l = __ffsll((long long)in) - 1;
-      ElPart r;
+      ElPart r = {};
       r.expert = e0 + l;
       r.parts = __builtin_amdgcn_readlane(parts, l);
       r.part = t - (before + __builtin_amdgcn_readlane(upto, l) - r.parts);
-      r.place = several + __builtin_amdgcn_readlane(more_upto - more, l) + r.part;
-      r.lo = hc_readlane64(lo, l) + r.part * rows;
+      r.lo = hc_readlane64(lo, l) + (int64_t)r.part * rows;
       const int64_t end = hc_readlane64(hi, l);
       r.hi = r.lo + rows < end ? r.lo + rows : end;
       return r;
     }
     before += __builtin_amdgcn_readlane(upto, HC_WAVE - 1);
-    if (!REST) several += __builtin_amdgcn_readlane(more_upto, HC_WAVE - 1);
+  }
+  ElPart r = {};
+  r.expert = E + 1;
+  return r;
+}
+
+// The t-th part of up to `rows` rows for the experts' gradients; an expert without rows has one of none (its gradient is zeros).
+// The parts of `rows` rows come first, then the experts' last, shorter ones, of up to 64 experts the longest first: what is
+// started last is short.  The order changes no result.
+__device__ __forceinline__ ElPart el_find_part(const int64_t *__restrict__ offset, int E, int64_t S, int64_t rows, int t) {
+  const int lane = hc_lane();
+  for (int last = 0; last < 2; ++last) {
+    int before = 0, several = 0;
+    for (int e0 = 0; e0 < E; e0 += HC_WAVE) {
+      int64_t lo, hi;
+      el_rows_of(offset, E, S, e0 + lane < E ? e0 + lane : E + 1, &lo, &hi);
+      const int full = (int)((hi - lo) / rows), rest = (int)(hi - lo - full * rows);
+      const bool short_one = e0 + lane < E && (rest > 0 || full == 0);
+      const int parts = full + (short_one ? 1 : 0), many = parts > 1 ? parts : 0, place = several + el_scan(many) - many;
+      const int mine = last ? (short_one ? 1 : 0) : full, upto = before + el_scan(mine);
+      uint64_t in;
+      if (last && E <= HC_WAVE) {
+        int rank = 0;
+        for (int l = 0; l < E; ++l) {
+          const int other = __builtin_amdgcn_readlane(short_one ? rest : -1, l);
+          rank += other > rest || (other == rest && l < lane) ? 1 : 0;
+        }
+        in = __ballot(short_one && rank == t);
+      } else {
+        in = __ballot(t < upto);
+      }
+      if (in != 0) {
+        const int l = __ffsll((long long)in) - 1;
+        ElPart r;
+        r.expert = e0 + l;
+        r.parts = __builtin_amdgcn_readlane(parts, l);
+        r.part = last ? __builtin_amdgcn_readlane(full, l) : t - __builtin_amdgcn_readlane(upto - mine, l);
+        r.place = __builtin_amdgcn_readlane(place, l) + r.part;
+        r.lo = hc_readlane64(lo, l) + r.part * rows;
+        const int64_t end = hc_readlane64(hi, l);
+        r.hi = r.lo + rows < end ? r.lo + rows : end;
+        return r;
+      }
+      before = __builtin_amdgcn_readlane(upto, HC_WAVE - 1);
+      several = __builtin_amdgcn_readlane(place + many, HC_WAVE - 1);
+    }
+    t -= before;
   }
   ElPart r = {};
   r.expert = E + 1;

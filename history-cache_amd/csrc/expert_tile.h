@@ -8,6 +8,15 @@
 #pragma once
 
 #include "expert_find.h"
+#ifndef EL_MINW
+#define EL_MINW 2
+#endif
+#ifndef EL_XG
+#define EL_XG 4
+#endif
+#ifndef EL_XF
+#define EL_XF 8
+#endif
 
 namespace {
 
@@ -17,7 +26,6 @@ typedef short el_eight __attribute__((ext_vector_type(8)));
 typedef short el_quad __attribute__((ext_vector_type(4)));
 typedef uint32_t el_piece __attribute__((ext_vector_type(4)));
 
-constexpr int EL_ROW = 128;                     // bytes of inner index in a piece: 64 elements of 16 bits, 32 of fp32
 constexpr uint32_t EL_NOWHERE = 0xfffffff0u;    // behind every buffer: reads as zero
 #define EL_LDS __attribute__((address_space(3)))
 
@@ -47,22 +55,27 @@ struct el_type<float> {
 };
 
 // A piece of an operand in LDS: W rows (columns) of the result by 128 bytes of inner index, in chunks of 16 bytes.
-//   TR = false: inner index along memory, [W][128 bytes]; chunk c of row r lies at c ^ (r & 7), so that eight rows read at a time
-//               lie in different banks
-//   TR = true:  inner index outside.  16 bits: read by ds_read_b64_tr_b16, 4 rows x 16 columns by 16 lanes; columns 16 c .. of
-//               inner row r lie at c ^ (r & 7).  fp32: read by columns, in order
+//   TR = false: inner index along memory, [W][ROWB]
+//   TR = true:  inner index outside, [ROWB / size][W].  16 bits: read by ds_read_b64_tr_b16, 4 rows x 16 columns by 16 lanes; fp32:
+//               read by columns
+// Chunk c of row r lies at c ^ turn(r), so that the lanes that are served at a time find their values in different banks.
 // PIECE = 16 bytes: chunks go straight into LDS, which takes rows that start on 16 bytes; else they are loaded in pieces of
 // PIECE bytes, which may end inside a chunk, and pass through registers.
-template <typename T, int W, bool TR, int THREADS, int PIECE>
+template <typename T, int W, int ROWB, bool TR, int THREADS, int PIECE>
 struct el_operand {
-  static constexpr int PER = 16 / (int)sizeof(T), INNER = EL_ROW / (int)sizeof(T);
-  static constexpr int CHUNKS = W * 8, EACH = CHUNKS / THREADS;
+  static constexpr int PER = 16 / (int)sizeof(T), INNER = ROWB / (int)sizeof(T);
+  static constexpr int CHUNKS = W * ROWB / 16, EACH = CHUNKS / THREADS;
   static_assert(CHUNKS % THREADS == 0, "whole chunks per thread");
   uint32_t at[EACH];        // byte offset of this thread's chunks in the operand's first piece
   int first[EACH];          // first inner index (TR = false) or column of each
   el_piece held[PIECE == 16 ? 1 : EACH];
   int width;
 
+  // what is added, bit by bit, to the numbers of a row's chunks (TR: of its 32 bytes, of its 128 bytes where T is fp32)
+  __device__ __forceinline__ static int turn(int r) {
+    if constexpr (TR) return sizeof(T) == 2 ? (r & 3) * 2 + ((r >> 3) & 1) : (r >> 2) & 1;
+    else return ROWB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+  }
   // stride: of the operand's rows in elements; wide: rows (TR = false) or columns (TR = true) that exist from the tile's first on
   __device__ __forceinline__ void init(int t, uint32_t stride, int wide) {
     width = wide;
@@ -71,12 +84,11 @@ struct el_operand {
       const int q = i * THREADS + t;
       int r, c;
       if constexpr (!TR) {
-        r = q / 8;
-        c = (q % 8) ^ (r & 7);
+        r = q / (ROWB / 16);
+        c = q % (ROWB / 16) ^ turn(r);
       } else {
         r = q / (W / PER);
-        c = q % (W / PER);
-        if constexpr (sizeof(T) == 2) c = ((c / 2) ^ (r & 7)) * 2 + c % 2;
+        c = q % (W / PER) ^ turn(r) * (sizeof(T) == 2 ? 2 : 8);
       }
       first[i] = c * PER;
       at[i] = (TR ? first[i] : r) < wide ? ((uint32_t)r * stride + (uint32_t)first[i]) * (uint32_t)sizeof(T) : EL_NOWHERE;
@@ -119,39 +131,66 @@ struct el_operand {
     const int lane = hc_lane();
     if constexpr (!TR) {
       const int r = from + (lane & 31), c = k * 2 + (lane >> 5);
-      return *(const EL_LDS typename el_type<T>::frag *)(lds + r * EL_ROW + ((c ^ (lane & 7)) * 16));
+      return *(const EL_LDS typename el_type<T>::frag *)(lds + r * ROWB + ((c ^ turn(lane)) * 16));
     } else if constexpr (sizeof(T) == 2) {
       const int i = lane & 15, g = lane >> 4;
       const int r = k * 16 + (g >> 1) * 8 + (i >> 2), c = from / 16 + (g & 1);
       const EL_LDS char *p = lds + r * (W * 2) + (i & 3) * 8;
-      const el_quad a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + ((c ^ (i >> 2)) * 32)));
-      const el_quad b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + 4 * (W * 2) + ((c ^ ((i >> 2) + 4)) * 32)));
+      const el_quad a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + ((c ^ turn(r)) * 32)));
+      const el_quad b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EL_LDS el_quad *)(p + 4 * (W * 2) + ((c ^ turn(r)) * 32)));
       return el_eight{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     } else {
-      const EL_LDS float *p = (const EL_LDS float *)lds + (k * 8 + (lane >> 5) * 4) * W + from + (lane & 31);
+      const EL_LDS float *p = (const EL_LDS float *)lds + (k * 8 + (lane >> 5) * 4) * W + ((from + (lane & 31)) ^ (lane >> 5) * 32);
       return el_four{p[0], p[W], p[2 * W], p[3 * W]};
     }
   }
 };
 
+// One step: the piece in `from` is multiplied while a later one is on its way to `to`.  A function of its own for the sake of the
+// two restricted pointers: they tell the compiler that what is on its way is not what is read, without which it waits for
+// all of it in front of every transposing read.
+template <typename OP_P, typename OP_Q, int TP, int TQ, int BYTES_P, int QUARTERS, typename T>
+__device__ __forceinline__ void el_step(const EL_LDS char *__restrict__ from, EL_LDS char *__restrict__ to, OP_P &fp, OP_Q &fq,
+                                        hc_buffer bp, hc_buffer bq, bool more, int left, int wave, int wp, int wq,
+                                        el_acc (&acc)[TP][TQ]) {
+  typedef typename el_type<T>::frag frag;
+  if (more) {
+    fp.fetch(bp, to, wave, left);
+    fq.fetch(bq, to + BYTES_P, wave, left);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int k = 0; k < QUARTERS; ++k) {
+    frag u[TP], v[TQ];
+#pragma unroll
+    for (int i = 0; i < TP; ++i) u[i] = OP_P::read(from, wp + i * 32, k);
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) v[j] = OP_Q::read(from + BYTES_P, wq + j * 32, k);
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) acc[i][j] = el_type<T>::mfma(v[j], u[i], acc[i][j]);
+  }
+}
+
 // A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of 128 bytes of inner index through two
 // stages in LDS, the next piece on its way while one is multiplied.
-template <typename T, int BP, int BQ, int WP, int WQ, bool GRAD, bool KN, int PIECE>
-__global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
+template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, int STAGES, bool GRAD, bool KN, int PIECE>
+__global__ __launch_bounds__(WP *WQ *HC_WAVE, EL_MINW) void el_tile(ElProduct a) {
   constexpr int THREADS = WP * WQ * HC_WAVE, TP = BP / WP / 32, TQ = BQ / WQ / 32, PER = 16 / (int)sizeof(T);
   constexpr bool PT = GRAD, QT = GRAD || KN;
-  typedef el_operand<T, BP, PT, THREADS, PIECE> op_p;
-  typedef el_operand<T, BQ, QT, THREADS, PIECE> op_q;
-  typedef typename el_type<T>::frag frag;
-  constexpr int BK = op_p::INNER, BYTES_P = BP * EL_ROW, STAGE = (BP + BQ) * EL_ROW;
+  typedef el_operand<T, BP, ROWB, PT, THREADS, PIECE> op_p;
+  typedef el_operand<T, BQ, ROWB, QT, THREADS, PIECE> op_q;
+  constexpr int BK = op_p::INNER, BYTES_P = BP * ROWB, STAGE = (BP + BQ) * ROWB;
   constexpr uint32_t SIZE = sizeof(T);
-  __shared__ __attribute__((aligned(16))) char s_mem[2 * STAGE];
+  constexpr int OUT = WP * WQ * 32 * (TQ * 32 + PER) * (int)sizeof(T), MEM = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  __shared__ __attribute__((aligned(16))) char s_mem[MEM];
   EL_LDS char *lds = (EL_LDS char *)s_mem;
-  const int64_t b = hc_xcd_block<32>(blockIdx.x, gridDim.x);
+  const int64_t b = hc_xcd_block<GRAD ? EL_XG : EL_XF>(blockIdx.x, gridDim.x);
   const int t = (int)threadIdx.x, lane = hc_lane(), wave = hc_wave_in_block();
   const int wp = wave % WP * (BP / WP), wq = wave / WP * (BQ / WQ);
   const int per = GRAD ? a.tiles_p * a.tiles_q : a.tiles_q, in = (int)(b % per);
-  const ElPart part = el_find<!GRAD>(a.offset, a.E, a.S, GRAD ? a.slab : BP, (int)(b / per));
+  const ElPart part = GRAD ? el_find_part(a.offset, a.E, a.S, a.slab, (int)(b / per)) : el_find_rows(a.offset, a.E, a.S, BP, (int)(b / per));
   if (part.expert > a.E) return;
   const int q0 = in % a.tiles_q * BQ, p0 = GRAD ? in / a.tiles_q * BP : 0;
   const int64_t e = part.expert < a.E ? part.expert : 0;
@@ -166,17 +205,15 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   op_q fq;
   fp.init(t, ld_p, rows_out);
   fq.init(t, ld_q, cols_out);
-  const auto fetch = [&](int s, int k0) {
+  // the operands from inner index k0 on; with the inner index outside a buffer ends with the last row that exists
+  const auto buffer = [&](const T *p, bool outside, uint32_t ld, int wide, int k0) {
     const int left = inner - k0, n = left < BK ? left : BK;
-    // a buffer with the inner index outside ends with the last row that exists
-    const hc_buffer bp = hc_make_buffer(PT ? pp + (int64_t)k0 * ld_p : pp + k0, PT ? ((uint32_t)(n - 1) * ld_p + (uint32_t)rows_out) * SIZE : 0xffffff00u);
-    const hc_buffer bq = hc_make_buffer(QT ? pq + (int64_t)k0 * ld_q : pq + k0, QT ? ((uint32_t)(n - 1) * ld_q + (uint32_t)cols_out) * SIZE : 0xffffff00u);
-    fp.fetch(bp, lds + s * STAGE, wave, left);
-    fq.fetch(bq, lds + s * STAGE + BYTES_P, wave, left);
+    return hc_make_buffer(outside ? p + (int64_t)k0 * ld : p + k0,
+                          left < 1 ? 0u : outside ? ((uint32_t)(n - 1) * ld + (uint32_t)wide) * SIZE : 0xffffff00u);
   };
-  const auto put = [&](int s) {
-    fp.put(lds + s * STAGE, t);
-    fq.put(lds + s * STAGE + BYTES_P, t);
+  const auto fetch = [&](int s, int k0) {
+    fp.fetch(buffer(pp, PT, ld_p, rows_out, k0), lds + s * STAGE, wave, inner - k0);
+    fq.fetch(buffer(pq, QT, ld_q, cols_out, k0), lds + s * STAGE + BYTES_P, wave, inner - k0);
   };
   el_acc acc[TP][TQ];
 #pragma unroll
@@ -185,34 +222,48 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
     for (int j = 0; j < TQ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  const auto compute = [&](int s) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      frag u[TP], v[TQ];
-#pragma unroll
-      for (int i = 0; i < TP; ++i) u[i] = op_p::read(lds + s * STAGE, wp + i * 32, k);
-#pragma unroll
-      for (int j = 0; j < TQ; ++j) v[j] = op_q::read(lds + s * STAGE + BYTES_P, wq + j * 32, k);
-#pragma unroll
-      for (int i = 0; i < TP; ++i)
-#pragma unroll
-        for (int j = 0; j < TQ; ++j) acc[i][j] = el_type<T>::mfma(v[j], u[i], acc[i][j]);
-    }
+  const auto step = [&](int from, int to, int k0, bool more) {
+    el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq, buffer(pp, PT, ld_p, rows_out, k0),
+                                                       buffer(pq, QT, ld_q, cols_out, k0), more, inner - k0, wave, wp, wq, acc);
   };
-  if (inner > 0) {
-    fetch(0, 0);
-    put(0);
-  }
-  int s = 0;
-  for (int k0 = 0; k0 < inner; k0 += BK) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);                                // vmcnt 0: what this wave has fetched is in LDS
-    __syncthreads();
-    const bool more = k0 + BK < inner;
-    if (more) fetch(s ^ 1, k0 + BK);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(s);
-    s ^= 1;
-    if (more) put(s);
+  const auto put = [&](int s) {
+    fp.put(lds + s * STAGE, t);
+    fq.put(lds + s * STAGE + BYTES_P, t);
+  };
+  if constexpr (PIECE == 16) {
+    // the pieces of the next STAGES - 1 steps are on their way; fetches behind the last piece read nothing and store zeros, so
+    // that the number outstanding is always the same
+    constexpr int LOADS = op_p::EACH + op_q::EACH, AHEAD = (STAGES - 2) * LOADS;
+    static_assert(AHEAD < 64, "the counter of outstanding loads");
+    if (inner > 0)
+      for (int i = 0; i < STAGES - 1; ++i) fetch(i, i * BK);
+    int s = 0, f = STAGES - 1;
+    for (int k0 = 0; k0 < inner; k0 += BK) {
+      // what this wave has fetched for this step is in LDS, and so, behind the barrier, is what the others have
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt((AHEAD & 15) | (AHEAD >> 4) << 14 | 0x70);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      step(s, f, k0 + (STAGES - 1) * BK, true);
+      s = s == STAGES - 1 ? 0 : s + 1;
+      f = f == STAGES - 1 ? 0 : f + 1;
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);
+  } else {
+    if (inner > 0) {
+      fetch(0, 0);
+      put(0);
+    }
+    int s = 0;
+    for (int k0 = 0; k0 < inner; k0 += BK) {
+      __syncthreads();
+      const bool more = k0 + BK < inner;
+      step(s, s ^ 1, k0 + BK, more);
+      s ^= 1;
+      if (more) put(s);
+    }
   }
   // lane l has row l % 32 of a tile of 32 x 32 and of every eight columns the four from 4 (l / 32) on
   const int l32 = lane & 31, h = lane >> 5;
@@ -232,7 +283,7 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   T *out = static_cast<T *>(a.out) + (GRAD ? (e * a.rows + p0) * a.cols + q0 : part.lo * a.cols + q0);
   // a wave's 32 rows at a time through its own piece of LDS, so that a row leaves in pieces of 16 bytes
   constexpr int ROW = TQ * 32 + PER;
-  static_assert(WP * WQ * 32 * ROW * (int)sizeof(T) <= 2 * STAGE, "the way out fits the stages");
+  static_assert(WP * WQ * 32 * ROW * (int)sizeof(T) <= MEM, "the way out fits the stages");
   __syncthreads();
   T *own = reinterpret_cast<T *>(s_mem) + wave * 32 * ROW;
 #pragma unroll
@@ -306,13 +357,13 @@ __global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, i
   }
 }
 
-template <typename T, int BP, int BQ, int WP, int WQ, bool GRAD, bool KN, int PIECE>
+template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, int STAGES, bool GRAD, bool KN, int PIECE>
 static int el_launch(ElProduct a, int64_t parts, hipStream_t st) {
   a.tiles_p = GRAD ? (a.rows + BP - 1) / BP : 1;
   a.tiles_q = (a.cols + BQ - 1) / BQ;
   const int64_t blocks = parts * a.tiles_p * a.tiles_q;
   if (!hc_grid_ok(blocks)) return HC_EUNSUPPORTED;
-  el_tile<T, BP, BQ, WP, WQ, GRAD, KN, PIECE><<<dim3((unsigned)blocks), dim3(WP * WQ * HC_WAVE), 0, st>>>(a);
+  el_tile<T, BP, BQ, WP, WQ, ROWB, STAGES, GRAD, KN, PIECE><<<dim3((unsigned)blocks), dim3(WP * WQ * HC_WAVE), 0, st>>>(a);
   return hc_launch_status();
 }
 
@@ -322,6 +373,23 @@ static int el_piece_of(const void *p, const void *q, int64_t w0, int64_t w1, int
   return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : a % 4 == 0 ? 4 : 2;
 }
 
+#ifndef EL_CFG
+#define EL_CFG 256, 256, 2, 4, 128, 2
+#define EL_BP 256
+#endif
+#ifndef EL_RB
+#define EL_RB 128
+#endif
+#ifndef EL_ST
+#define EL_ST 2
+#endif
+#ifndef EL_XG
+#define EL_XG 8
+#define EL_XF 8
+#endif
+#ifndef EL_MINW
+#define EL_MINW 2
+#endif
 #ifndef EL_BIG
 #define EL_BIG(tiles) ((tiles) >= 192)
 #endif
@@ -331,13 +399,13 @@ static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
   const int piece = el_piece_of(a.p, a.q, a.inner, KN ? a.cols : a.inner, (int)sizeof(T));
   if constexpr (sizeof(T) == 2) {
     const int64_t big = (a.S + 255) / 256 * ((a.cols + 255) / 256);
-    if (piece == 16 && EL_BIG(big)) return el_launch<T, 256, 256, 2, 4, false, KN, 16>(a, a.S / 256 + a.E + 1, st);
-    if (piece == 2) return el_launch<T, 128, 128, 2, 2, false, KN, 2>(a, a.S / 128 + a.E + 1, st);
+    if (piece == 16 && EL_BIG(big)) return el_launch<T, EL_CFG, false, KN, 16>(a, a.S / EL_BP + a.E + 1, st);
+    if (piece == 2) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 2>(a, a.S / 128 + a.E + 1, st);
   }
   const int64_t parts = a.S / 128 + a.E + 1;
-  if (piece == 16) return el_launch<T, 128, 128, 2, 2, false, KN, 16>(a, parts, st);
-  if (piece == 8) return el_launch<T, 128, 128, 2, 2, false, KN, 8>(a, parts, st);
-  return el_launch<T, 128, 128, 2, 2, false, KN, 4>(a, parts, st);
+  if (piece == 16) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 16>(a, parts, st);
+  if (piece == 8) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 8>(a, parts, st);
+  return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 4>(a, parts, st);
 }
 
 struct ElGradShape {
@@ -370,12 +438,12 @@ static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes,
   const int64_t parts = a.S / g.slab + a.E;
   int rc = HC_EUNSUPPORTED;
   if constexpr (sizeof(T) == 2) {
-    if (g.big) rc = el_launch<T, 256, 256, 2, 4, true, false, 16>(a, parts, st);
-    else if (piece == 2) rc = el_launch<T, 128, 128, 2, 2, true, false, 2>(a, parts, st);
+    if (g.big) rc = el_launch<T, EL_CFG, true, false, 16>(a, parts, st);
+    else if (piece == 2) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 2>(a, parts, st);
   }
-  if (!g.big && piece == 16) rc = el_launch<T, 128, 128, 2, 2, true, false, 16>(a, parts, st);
-  else if (!g.big && piece == 8) rc = el_launch<T, 128, 128, 2, 2, true, false, 8>(a, parts, st);
-  else if (!g.big && piece == 4) rc = el_launch<T, 128, 128, 2, 2, true, false, 4>(a, parts, st);
+  if (!g.big && piece == 16) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 16>(a, parts, st);
+  else if (!g.big && piece == 8) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 8>(a, parts, st);
+  else if (!g.big && piece == 4) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 4>(a, parts, st);
   if (rc != HC_OK || g.several == 0) return rc;
   const int64_t pieces = (size + 3) / 4;
   int64_t blocks = (pieces + HC_BLOCK - 1) / HC_BLOCK;
