@@ -8,15 +8,6 @@
 #pragma once
 
 #include "expert_find.h"
-#ifndef EL_MINW
-#define EL_MINW 2
-#endif
-#ifndef EL_XG
-#define EL_XG 4
-#endif
-#ifndef EL_XF
-#define EL_XF 8
-#endif
 
 namespace {
 
@@ -176,7 +167,7 @@ __device__ __forceinline__ void el_step(const EL_LDS char *__restrict__ from, EL
 // A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of 128 bytes of inner index through two
 // stages in LDS, the next piece on its way while one is multiplied.
 template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, int STAGES, bool GRAD, bool KN, int PIECE>
-__global__ __launch_bounds__(WP *WQ *HC_WAVE, EL_MINW) void el_tile(ElProduct a) {
+__global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   constexpr int THREADS = WP * WQ * HC_WAVE, TP = BP / WP / 32, TQ = BQ / WQ / 32, PER = 16 / (int)sizeof(T);
   constexpr bool PT = GRAD, QT = GRAD || KN;
   typedef el_operand<T, BP, ROWB, PT, THREADS, PIECE> op_p;
@@ -186,7 +177,7 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, EL_MINW) void el_tile(ElProduct a)
   constexpr int OUT = WP * WQ * 32 * (TQ * 32 + PER) * (int)sizeof(T), MEM = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
   __shared__ __attribute__((aligned(16))) char s_mem[MEM];
   EL_LDS char *lds = (EL_LDS char *)s_mem;
-  const int64_t b = hc_xcd_block<GRAD ? EL_XG : EL_XF>(blockIdx.x, gridDim.x);
+  const int64_t b = hc_xcd_block<GRAD ? 4 : 8>(blockIdx.x, gridDim.x);
   const int t = (int)threadIdx.x, lane = hc_lane(), wave = hc_wave_in_block();
   const int wp = wave % WP * (BP / WP), wq = wave / WP * (BQ / WQ);
   const int per = GRAD ? a.tiles_p * a.tiles_q : a.tiles_q, in = (int)(b % per);
@@ -269,14 +260,25 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, EL_MINW) void el_tile(ElProduct a)
   const int l32 = lane & 31, h = lane >> 5;
   if (GRAD && part.parts > 1) {
     float *o = a.part + (int64_t)part.place * a.rows * a.cols + (int64_t)p0 * a.cols + q0;
+    const bool four = a.cols % 4 == 0;
 #pragma unroll
     for (int i = 0; i < TP; ++i)
 #pragma unroll
       for (int j = 0; j < TQ; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = wp + i * 32 + l32, col = wq + j * 32 + r / 4 * 8 + h * 4 + r % 4;
-          if (row < rows_out && col < cols_out) o[(int64_t)row * a.cols + col] = acc[i][j][r];
+        for (int r = 0; r < 16; r += 4) {
+          const int row = wp + i * 32 + l32, col = wq + j * 32 + r * 2 + h * 4;
+          if (row < rows_out && col < cols_out) {
+            float *at = o + (int64_t)row * a.cols + col;
+            const float v[4] = {acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+            if (four) {
+              hc_vec<float, 4>::store(at, v);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (col + x < cols_out) at[x] = v[x];
+            }
+          }
         }
     return;
   }
@@ -316,44 +318,65 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, EL_MINW) void el_tile(ElProduct a)
   }
 }
 
-// The gradients of experts of several parts: their partial sums added in the order of the parts.
-template <typename T>
-__global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, int64_t pieces) {
-  const int lane = hc_lane();
+// The gradients of experts of several parts: their partial sums added up, a quarter of the parts by each wave in their order,
+// then the quarters in order.  A lane has four adjacent values (one where VEC is 1), a block 64 lanes' of one expert at a time.
+template <typename T, int VEC>
+__global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, int chunks) {
+  __shared__ float s_part[3][VEC][HC_WAVE];
+  const int lane = hc_lane(), wave = hc_wave_in_block();
+  int64_t item = blockIdx.x;                    // chunk of an expert of several parts, expert by expert
   int before = 0;
   for (int e0 = 0; e0 < a.E; e0 += HC_WAVE) {
     int64_t lo, hi;
     el_rows_of(a.offset, a.E, a.S, e0 + lane < a.E ? e0 + lane : a.E + 1, &lo, &hi);
     int parts = (int)((hi - lo + a.slab - 1) / a.slab);
     parts = parts > 1 ? parts : 0;
-    const int first = before + el_scan(parts) - parts;
+    const int place = before + el_scan(parts) - parts;
     uint64_t several = __ballot(parts > 0);
-    while (several != 0) {
-      const int l = __ffsll((long long)several) - 1;
-      several &= several - 1;
-      const int n = __builtin_amdgcn_readlane(parts, l);
-      const float *p = a.part + (int64_t)__builtin_amdgcn_readlane(first, l) * size;
+    for (; several != 0; several &= several - 1, item -= chunks) {
+      const int l = __ffsll((long long)several) - 1, n = __builtin_amdgcn_readlane(parts, l);
+      const float *p = a.part + (int64_t)__builtin_amdgcn_readlane(place, l) * size;
       T *o = static_cast<T *>(a.out) + (e0 + l) * size;
-      for (int64_t i = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * HC_BLOCK) {
-        const int64_t at = i * 4;
-        if (size % 4 == 0 && a.whole) {
-          float4 s = *reinterpret_cast<const float4 *>(p + at);
-          for (int q = 1; q < n; ++q) {
-            const float4 v = *reinterpret_cast<const float4 *>(p + q * size + at);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      for (; item < chunks; item += gridDim.x) {
+        const int64_t at = (item * HC_WAVE + lane) * VEC;
+        float s[VEC];
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) s[x] = 0.f;
+        if (at < size) {
+          int q = n * wave / 4;
+          const int end = n * (wave + 1) / 4;
+          constexpr int FLIGHT = 4;
+          for (; q + FLIGHT <= end; q += FLIGHT) {
+            float v[FLIGHT][VEC];
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f) hc_vec<float, VEC>::load(p + (q + f) * size + at, v[f]);
+#pragma unroll
+            for (int f = 0; f < FLIGHT; ++f)
+#pragma unroll
+              for (int x = 0; x < VEC; ++x) s[x] += v[f][x];
           }
-          const float v[4] = {s.x, s.y, s.z, s.w};
-          hc_vec<T, 4>::store(o + at, v);
-        } else {
-          for (int x = 0; x < 4 && at + x < size; ++x) {
-            float s = p[at + x];
-            for (int q = 1; q < n; ++q) s += p[q * size + at + x];
-            o[at + x] = hc_from_f32<T>(s);
+          for (; q < end; ++q) {
+            float v[VEC];
+            hc_vec<float, VEC>::load(p + q * size + at, v);
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) s[x] += v[x];
           }
         }
+        if (wave > 0)
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) s_part[wave - 1][x][lane] = s[x];
+        __syncthreads();
+        if (wave == 0 && at < size) {
+#pragma unroll
+          for (int w = 0; w < 3; ++w)
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) s[x] += s_part[w][x][lane];
+          hc_vec<T, VEC>::store(o + at, s);
+        }
+        __syncthreads();
       }
     }
-    before = __builtin_amdgcn_readlane(first + parts, HC_WAVE - 1);
+    before = __builtin_amdgcn_readlane(place + parts, HC_WAVE - 1);
   }
 }
 
@@ -373,52 +396,53 @@ static int el_piece_of(const void *p, const void *q, int64_t w0, int64_t w1, int
   return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : a % 4 == 0 ? 4 : 2;
 }
 
-#ifndef EL_CFG
-#define EL_CFG 256, 256, 2, 4, 128, 2
-#define EL_BP 256
-#endif
-#ifndef EL_RB
-#define EL_RB 128
-#endif
-#ifndef EL_ST
-#define EL_ST 2
-#endif
-#ifndef EL_XG
-#define EL_XG 8
-#define EL_XF 8
-#endif
-#ifndef EL_MINW
-#define EL_MINW 2
-#endif
-#ifndef EL_BIG
-#define EL_BIG(tiles) ((tiles) >= 192)
-#endif
+// Tiles of 256 x 256 on eight waves, one block per compute unit, or of 128 x 128 on four, several blocks per unit; pieces of 128
+// bytes of inner index, or of 64, which leaves room for four small blocks on a unit.
+#define EL_LARGE 256, 256, 2, 4, 128, 2
+#define EL_SMALL 128, 128, 2, 2, 128, 2
+#define EL_SHORT 128, 128, 2, 2, 64, 2
+
+constexpr int EL_SHORT_INNER = 512;               // longest inner size that goes in pieces of 64 bytes where both would do
+constexpr int64_t EL_SHORT_GROUP = 640;           // rows of an expert, on average, up to which its gradient does
+constexpr int64_t EL_LARGE_GRAD = 256 * 5120;     // rows of the batch that a unit would take through a large tile
+
+// Is the product of S rows in E groups by `cols` columns done sooner in large tiles?  Rounds over the 256 compute units, the
+// groups' last tiles half empty; a small tile, two at a time on a unit, takes EL_SMALL_COST of a large one's time and a
+// quarter of its work.
+constexpr float EL_SMALL_COST = 0.575f;
+static bool el_large_rows(int64_t S, int64_t E, int64_t cols) {
+  const int64_t large = ((S + 255) / 256 + E / 2) * ((cols + 255) / 256), small = ((S + 127) / 128 + E / 2) * ((cols + 127) / 128);
+  return (float)((large + 255) / 256) <= EL_SMALL_COST * (float)((small + 511) / 512);
+}
 
 template <typename T, bool KN>
 static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
   const int piece = el_piece_of(a.p, a.q, a.inner, KN ? a.cols : a.inner, (int)sizeof(T));
-  if constexpr (sizeof(T) == 2) {
-    const int64_t big = (a.S + 255) / 256 * ((a.cols + 255) / 256);
-    if (piece == 16 && EL_BIG(big)) return el_launch<T, EL_CFG, false, KN, 16>(a, a.S / EL_BP + a.E + 1, st);
-    if (piece == 2) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 2>(a, a.S / 128 + a.E + 1, st);
-  }
   const int64_t parts = a.S / 128 + a.E + 1;
-  if (piece == 16) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 16>(a, parts, st);
-  if (piece == 8) return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 8>(a, parts, st);
-  return el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, false, KN, 4>(a, parts, st);
+  if constexpr (sizeof(T) == 2) {
+    if (piece == 16 && el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, 16>(a, a.S / 256 + a.E + 1, st);
+    if (piece == 16 && a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, 16>(a, parts, st);
+    if (piece == 2) return el_launch<T, EL_SHORT, false, KN, 2>(a, parts, st);
+  }
+  if (piece == 16) return el_launch<T, EL_SHORT, false, KN, 16>(a, parts, st);
+  if (piece == 8) return el_launch<T, EL_SHORT, false, KN, 8>(a, parts, st);
+  return el_launch<T, EL_SHORT, false, KN, 4>(a, parts, st);
 }
 
+constexpr int EL_JOIN_BLOCKS = 2048;
+
 struct ElGradShape {
-  bool big;
+  bool large;
   int64_t slab, several;        // rows of a part; parts of experts with several of them, at most
 };
 
-static ElGradShape el_grad_shape(int64_t S, int64_t E, int64_t N, int64_t K, int size, bool wide) {
+// Parts: as few as give every compute unit a large tile or two small ones, had one expert all rows.
+static ElGradShape el_grad_shape(int64_t S, int64_t N, int64_t K, int size, bool wide) {
   ElGradShape g;
-  const int64_t tiles = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
-  g.big = wide && size == 2 && EL_BIG(tiles * E);
-  const int64_t want = g.big ? 256 : 1024, have = g.big ? tiles : small;
-  g.slab = (S * have / want + 63) / 64 * 64;
+  const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
+  g.large = wide && size == 2 && S * large >= EL_LARGE_GRAD;
+  const int64_t parts = g.large ? 256 / large : 512 / small;
+  g.slab = (S / (parts < 1 ? 1 : parts) + 64) / 64 * 64;
   if (g.slab < 512) g.slab = 512;
   // an expert of p > 1 parts has more than (p - 1) slab >= p / 2 slab rows
   g.several = S <= g.slab ? 0 : 2 * (S / g.slab);
@@ -428,7 +452,7 @@ static ElGradShape el_grad_shape(int64_t S, int64_t E, int64_t N, int64_t K, int
 template <typename T>
 static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes, hipStream_t st) {
   const int piece = el_piece_of(a.p, a.q, a.rows, a.cols, (int)sizeof(T));
-  const ElGradShape g = el_grad_shape(a.S, a.E, a.rows, a.cols, (int)sizeof(T), piece == 16);
+  const ElGradShape g = el_grad_shape(a.S, a.rows, a.cols, (int)sizeof(T), piece == 16);
   const int64_t size = (int64_t)a.rows * a.cols;
   if ((size_t)(g.several * size) * sizeof(float) > workspace_bytes ||
       (g.several && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
@@ -436,20 +460,24 @@ static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes,
   a.part = static_cast<float *>(workspace);
   a.slab = g.slab;
   const int64_t parts = a.S / g.slab + a.E;
-  int rc = HC_EUNSUPPORTED;
-  if constexpr (sizeof(T) == 2) {
-    if (g.big) rc = el_launch<T, EL_CFG, true, false, 16>(a, parts, st);
-    else if (piece == 2) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 2>(a, parts, st);
-  }
-  if (!g.big && piece == 16) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 16>(a, parts, st);
-  else if (!g.big && piece == 8) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 8>(a, parts, st);
-  else if (!g.big && piece == 4) rc = el_launch<T, 128, 128, 2, 2, EL_RB, EL_ST, true, false, 4>(a, parts, st);
+  const auto run = [&]() -> int {
+    if constexpr (sizeof(T) == 2) {
+      if (g.large) return el_launch<T, EL_LARGE, true, false, 16>(a, parts, st);
+      if (piece == 2) return el_launch<T, EL_SMALL, true, false, 2>(a, parts, st);
+    }
+    if (piece == 16 && a.S <= EL_SHORT_GROUP * a.E) return el_launch<T, EL_SHORT, true, false, 16>(a, parts, st);
+    if (piece == 16) return el_launch<T, EL_SMALL, true, false, 16>(a, parts, st);
+    if (piece == 8) return el_launch<T, EL_SMALL, true, false, 8>(a, parts, st);
+    return el_launch<T, EL_SMALL, true, false, 4>(a, parts, st);
+  };
+  const int rc = run();
   if (rc != HC_OK || g.several == 0) return rc;
-  const int64_t pieces = (size + 3) / 4;
-  int64_t blocks = (pieces + HC_BLOCK - 1) / HC_BLOCK;
-  blocks = blocks > 2048 ? 2048 : blocks;
-  a.whole = reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0;
-  el_join<T><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, st>>>(a, size, pieces);
+  const bool four = size % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(T)) == 0;
+  const int64_t chunks = (size + HC_WAVE * (four ? 4 : 1) - 1) / (HC_WAVE * (four ? 4 : 1));
+  const int64_t most = chunks * (a.E < g.several / 2 ? a.E : g.several / 2);
+  const dim3 blocks((unsigned)(most < EL_JOIN_BLOCKS ? most : EL_JOIN_BLOCKS));
+  if (four) el_join<T, 4><<<blocks, dim3(HC_BLOCK), 0, st>>>(a, size, (int)chunks);
+  else el_join<T, 1><<<blocks, dim3(HC_BLOCK), 0, st>>>(a, size, (int)chunks);
   return hc_launch_status();
 }
 
@@ -463,7 +491,7 @@ static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes,
     return el_grad_of_type<T>(a, workspace, workspace_bytes, st);                                                  \
   }                                                                                                                \
   size_t el_grad_bytes_##name(int64_t S, int64_t E, int64_t N, int64_t K) {                                        \
-    const int64_t wide = el_grad_shape(S, E, N, K, (int)sizeof(T), true).several;                                  \
-    const int64_t other = el_grad_shape(S, E, N, K, (int)sizeof(T), false).several;                                \
+    const int64_t wide = el_grad_shape(S, N, K, (int)sizeof(T), true).several;                                  \
+    const int64_t other = el_grad_shape(S, N, K, (int)sizeof(T), false).several;                                \
     return (size_t)(wide > other ? wide : other) * (size_t)N * (size_t)K * sizeof(float);                          \
   }
