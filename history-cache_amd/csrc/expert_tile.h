@@ -50,26 +50,27 @@ struct el_type<float> {
 //   TR = true:  inner index outside, [ROWB / size][W].  16 bits: read by ds_read_b64_tr_b16, 4 rows x 16 columns by 16 lanes; fp32:
 //               read by columns
 // Chunk c of row r lies at c ^ turn(r), so that the lanes that are served at a time find their values in different banks.
-// PIECE = 16 bytes: chunks go straight into LDS, which takes rows that start on 16 bytes; else they are loaded in pieces of
-// PIECE bytes, which may end inside a chunk, and pass through registers.
-template <typename T, int W, int ROWB, bool TR, int THREADS, int PIECE>
+// DIRECT: chunks go straight into LDS, for operands whose rows start on 4 bytes; a step that ends inside a row goes there by
+// words.  Else (16 bits, an odd width or address) elements pass through registers one by one.
+template <typename T, int W, int ROWB, bool TR, int THREADS, bool DIRECT>
 struct el_operand {
   static constexpr int PER = 16 / (int)sizeof(T), INNER = ROWB / (int)sizeof(T);
   static constexpr int CHUNKS = W * ROWB / 16, EACH = CHUNKS / THREADS;
   static_assert(CHUNKS % THREADS == 0, "whole chunks per thread");
   uint32_t at[EACH];        // byte offset of this thread's chunks in the operand's first piece
   int first[EACH];          // first inner index (TR = false) or column of each
-  el_piece held[PIECE == 16 ? 1 : EACH];
-  int width;
+  el_piece held[DIRECT ? 1 : EACH];
+  uint32_t stride;          // of the operand's rows in elements
+  int wide;                 // rows (TR = false) or columns (TR = true) that exist from the tile's first on
 
   // what is added, bit by bit, to the numbers of a row's chunks (TR: of its 32 bytes, of its 128 bytes where T is fp32)
   __device__ __forceinline__ static int turn(int r) {
     if constexpr (TR) return sizeof(T) == 2 ? (r & 3) * 2 + ((r >> 3) & 1) : (r >> 2) & 1;
     else return ROWB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
-  // stride: of the operand's rows in elements; wide: rows (TR = false) or columns (TR = true) that exist from the tile's first on
-  __device__ __forceinline__ void init(int t, uint32_t stride, int wide) {
-    width = wide;
+  __device__ __forceinline__ void init(int t, uint32_t stride_, int wide_) {
+    stride = stride_;
+    wide = wide_;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int q = i * THREADS + t;
@@ -85,34 +86,39 @@ struct el_operand {
       at[i] = (TR ? first[i] : r) < wide ? ((uint32_t)r * stride + (uint32_t)first[i]) * (uint32_t)sizeof(T) : EL_NOWHERE;
     }
   }
-  // left: inner indices from the piece's first on
-  __device__ __forceinline__ void fetch(hc_buffer b, EL_LDS char *lds, int wave, int left) {
+  // left: inner indices from the piece's first on.  Columns behind the last one may hold what lies there (they are not part of
+  // the result), inner indices behind the last one are zeros.
+  __device__ __forceinline__ void fetch(hc_buffer b, EL_LDS char *lds, int t, int wave, int left) {
+    if constexpr (DIRECT) {
+      if (TR || left >= INNER || left % PER == 0) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      if constexpr (PIECE == 16) {
-        const uint32_t o = TR || first[i] < left ? at[i] : EL_NOWHERE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (EL_LDS void *)(lds + (i * THREADS + wave * HC_WAVE) * 16), 16, o, 0, 0, 0);
+        for (int i = 0; i < EACH; ++i) {
+          const uint32_t o = TR || first[i] < left ? at[i] : EL_NOWHERE;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (EL_LDS void *)(lds + (i * THREADS + wave * HC_WAVE) * 16), 16, o, 0, 0, 0);
+        }
       } else {
-        const int end = TR ? width : left;
-#pragma unroll
-        for (int p = 0; p < 16; p += PIECE) {
-          const uint32_t o = first[i] + p / (int)sizeof(T) < end && at[i] != EL_NOWHERE ? at[i] + p : EL_NOWHERE;
-          if constexpr (PIECE == 8) {
-            const auto v = __builtin_amdgcn_raw_buffer_load_b64(b, o, 0, 0);
-            held[i][p / 4] = v[0];
-            held[i][p / 4 + 1] = v[1];
-          } else if constexpr (PIECE == 4) {
-            held[i][p / 4] = __builtin_amdgcn_raw_buffer_load_b32(b, o, 0, 0);
-          } else {
-            const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(b, o, 0, 0);
-            held[i][p / 4] = p % 4 == 0 ? v : held[i][p / 4] | v << 16;
-          }
+#pragma unroll 4
+        for (int i = 0; i < EACH * 4; ++i) {
+          const int q = i * THREADS + t, r = q / (ROWB / 4), c = (q % (ROWB / 4) / 4) ^ turn(r);
+          const int k = (c * 4 + q % 4) * (4 / (int)sizeof(T));
+          const uint32_t o = r < wide && k < left ? ((uint32_t)r * stride + (uint32_t)k) * (uint32_t)sizeof(T) : EL_NOWHERE;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (EL_LDS void *)(lds + (i * THREADS + wave * HC_WAVE) * 4), 4, o, 0, 0, 0);
         }
       }
+    } else {
+      const int end = TR ? wide : left;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const uint32_t o = first[i] + p < end && at[i] != EL_NOWHERE ? at[i] + 2u * p : EL_NOWHERE;
+          const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(b, o, 0, 0);
+          held[i][p / 2] = p % 2 == 0 ? v : held[i][p / 2] | v << 16;
+        }
     }
   }
   __device__ __forceinline__ void put(EL_LDS char *lds, int t) const {
-    if constexpr (PIECE != 16)
+    if constexpr (!DIRECT)
 #pragma unroll
       for (int i = 0; i < EACH; ++i) *(EL_LDS el_piece *)(lds + (i * THREADS + t) * 16) = held[i];
   }
@@ -142,12 +148,12 @@ struct el_operand {
 // all of it in front of every transposing read.
 template <typename OP_P, typename OP_Q, int TP, int TQ, int BYTES_P, int QUARTERS, typename T>
 __device__ __forceinline__ void el_step(const EL_LDS char *__restrict__ from, EL_LDS char *__restrict__ to, OP_P &fp, OP_Q &fq,
-                                        hc_buffer bp, hc_buffer bq, bool more, int left, int wave, int wp, int wq,
+                                        hc_buffer bp, hc_buffer bq, bool more, int left, int t, int wave, int wp, int wq,
                                         el_acc (&acc)[TP][TQ]) {
   typedef typename el_type<T>::frag frag;
   if (more) {
-    fp.fetch(bp, to, wave, left);
-    fq.fetch(bq, to + BYTES_P, wave, left);
+    fp.fetch(bp, to, t, wave, left);
+    fq.fetch(bq, to + BYTES_P, t, wave, left);
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -166,15 +172,15 @@ __device__ __forceinline__ void el_step(const EL_LDS char *__restrict__ from, EL
 
 // A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of 128 bytes of inner index through two
 // stages in LDS, the next piece on its way while one is multiplied.
-template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, int STAGES, bool GRAD, bool KN, int PIECE>
+template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, bool GRAD, bool KN, bool DIRECT>
 __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   constexpr int THREADS = WP * WQ * HC_WAVE, TP = BP / WP / 32, TQ = BQ / WQ / 32, PER = 16 / (int)sizeof(T);
   constexpr bool PT = GRAD, QT = GRAD || KN;
-  typedef el_operand<T, BP, ROWB, PT, THREADS, PIECE> op_p;
-  typedef el_operand<T, BQ, ROWB, QT, THREADS, PIECE> op_q;
+  typedef el_operand<T, BP, ROWB, PT, THREADS, DIRECT> op_p;
+  typedef el_operand<T, BQ, ROWB, QT, THREADS, DIRECT> op_q;
   constexpr int BK = op_p::INNER, BYTES_P = BP * ROWB, STAGE = (BP + BQ) * ROWB;
   constexpr uint32_t SIZE = sizeof(T);
-  constexpr int OUT = WP * WQ * 32 * (TQ * 32 + PER) * (int)sizeof(T), MEM = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  constexpr int OUT = WP * WQ * 32 * (TQ * 32 + PER) * (int)sizeof(T), MEM = 2 * STAGE > OUT ? 2 * STAGE : OUT;
   __shared__ __attribute__((aligned(16))) char s_mem[MEM];
   EL_LDS char *lds = (EL_LDS char *)s_mem;
   const int64_t b = hc_xcd_block<GRAD ? 4 : 8>(blockIdx.x, gridDim.x);
@@ -203,8 +209,8 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
                           left < 1 ? 0u : outside ? ((uint32_t)(n - 1) * ld + (uint32_t)wide) * SIZE : 0xffffff00u);
   };
   const auto fetch = [&](int s, int k0) {
-    fp.fetch(buffer(pp, PT, ld_p, rows_out, k0), lds + s * STAGE, wave, inner - k0);
-    fq.fetch(buffer(pq, QT, ld_q, cols_out, k0), lds + s * STAGE + BYTES_P, wave, inner - k0);
+    fp.fetch(buffer(pp, PT, ld_p, rows_out, k0), lds + s * STAGE, t, wave, inner - k0);
+    fq.fetch(buffer(pq, QT, ld_q, cols_out, k0), lds + s * STAGE + BYTES_P, t, wave, inner - k0);
   };
   el_acc acc[TP][TQ];
 #pragma unroll
@@ -215,46 +221,25 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   const auto step = [&](int from, int to, int k0, bool more) {
     el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq, buffer(pp, PT, ld_p, rows_out, k0),
-                                                       buffer(pq, QT, ld_q, cols_out, k0), more, inner - k0, wave, wp, wq, acc);
+                                                       buffer(pq, QT, ld_q, cols_out, k0), more, inner - k0, t, wave, wp, wq, acc);
   };
   const auto put = [&](int s) {
     fp.put(lds + s * STAGE, t);
     fq.put(lds + s * STAGE + BYTES_P, t);
   };
-  if constexpr (PIECE == 16) {
-    // the pieces of the next STAGES - 1 steps are on their way; fetches behind the last piece read nothing and store zeros, so
-    // that the number outstanding is always the same
-    constexpr int LOADS = op_p::EACH + op_q::EACH, AHEAD = (STAGES - 2) * LOADS;
-    static_assert(AHEAD < 64, "the counter of outstanding loads");
-    if (inner > 0)
-      for (int i = 0; i < STAGES - 1; ++i) fetch(i, i * BK);
-    int s = 0, f = STAGES - 1;
-    for (int k0 = 0; k0 < inner; k0 += BK) {
-      // what this wave has fetched for this step is in LDS, and so, behind the barrier, is what the others have
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt((AHEAD & 15) | (AHEAD >> 4) << 14 | 0x70);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      step(s, f, k0 + (STAGES - 1) * BK, true);
-      s = s == STAGES - 1 ? 0 : s + 1;
-      f = f == STAGES - 1 ? 0 : f + 1;
-    }
+  if (inner > 0) {
+    fetch(0, 0);
+    put(0);
+  }
+  int s = 0;
+  for (int k0 = 0; k0 < inner; k0 += BK) {
+    // what this wave has fetched for this step is in LDS, and so, behind the barrier, is what the others have
     __builtin_amdgcn_s_waitcnt(0x0070);
-  } else {
-    if (inner > 0) {
-      fetch(0, 0);
-      put(0);
-    }
-    int s = 0;
-    for (int k0 = 0; k0 < inner; k0 += BK) {
-      __syncthreads();
-      const bool more = k0 + BK < inner;
-      step(s, s ^ 1, k0 + BK, more);
-      s ^= 1;
-      if (more) put(s);
-    }
+    __syncthreads();
+    const bool more = k0 + BK < inner;
+    step(s, s ^ 1, k0 + BK, more);
+    s ^= 1;
+    if (more) put(s);
   }
   // lane l has row l % 32 of a tile of 32 x 32 and of every eight columns the four from 4 (l / 32) on
   const int l32 = lane & 31, h = lane >> 5;
@@ -380,27 +365,26 @@ __global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, i
   }
 }
 
-template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, int STAGES, bool GRAD, bool KN, int PIECE>
+template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, bool GRAD, bool KN, bool DIRECT>
 static int el_launch(ElProduct a, int64_t parts, hipStream_t st) {
   a.tiles_p = GRAD ? (a.rows + BP - 1) / BP : 1;
   a.tiles_q = (a.cols + BQ - 1) / BQ;
   const int64_t blocks = parts * a.tiles_p * a.tiles_q;
   if (!hc_grid_ok(blocks)) return HC_EUNSUPPORTED;
-  el_tile<T, BP, BQ, WP, WQ, ROWB, STAGES, GRAD, KN, PIECE><<<dim3((unsigned)blocks), dim3(WP * WQ * HC_WAVE), 0, st>>>(a);
+  el_tile<T, BP, BQ, WP, WQ, ROWB, GRAD, KN, DIRECT><<<dim3((unsigned)blocks), dim3(WP * WQ * HC_WAVE), 0, st>>>(a);
   return hc_launch_status();
 }
 
-// Bytes in a piece that rows of these widths at these addresses allow.
-static int el_piece_of(const void *p, const void *q, int64_t w0, int64_t w1, int size) {
-  const uint64_t a = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | (uint64_t)(w0 * size) | (uint64_t)(w1 * size);
-  return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : a % 4 == 0 ? 4 : 2;
+// Do rows of these widths at these addresses start on 4 bytes?
+static bool el_direct(const void *p, const void *q, int64_t w0, int64_t w1, int size) {
+  return ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | (uint64_t)(w0 * size) | (uint64_t)(w1 * size)) & 3) == 0;
 }
 
 // Tiles of 256 x 256 on eight waves, one block per compute unit, or of 128 x 128 on four, several blocks per unit; pieces of 128
 // bytes of inner index, or of 64, which leaves room for four small blocks on a unit.
-#define EL_LARGE 256, 256, 2, 4, 128, 2
-#define EL_SMALL 128, 128, 2, 2, 128, 2
-#define EL_SHORT 128, 128, 2, 2, 64, 2
+#define EL_LARGE 256, 256, 2, 4, 128
+#define EL_SMALL 128, 128, 2, 2, 128
+#define EL_SHORT 128, 128, 2, 2, 64
 
 constexpr int EL_SHORT_INNER = 512;               // longest inner size that goes in pieces of 64 bytes where both would do
 constexpr int64_t EL_SHORT_GROUP = 640;           // rows of an expert, on average, up to which its gradient does
@@ -417,16 +401,13 @@ static bool el_large_rows(int64_t S, int64_t E, int64_t cols) {
 
 template <typename T, bool KN>
 static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
-  const int piece = el_piece_of(a.p, a.q, a.inner, KN ? a.cols : a.inner, (int)sizeof(T));
   const int64_t parts = a.S / 128 + a.E + 1;
   if constexpr (sizeof(T) == 2) {
-    if (piece == 16 && el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, 16>(a, a.S / 256 + a.E + 1, st);
-    if (piece == 16 && a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, 16>(a, parts, st);
-    if (piece == 2) return el_launch<T, EL_SHORT, false, KN, 2>(a, parts, st);
+    if (!el_direct(a.p, a.q, a.inner, KN ? a.cols : a.inner, 2)) return el_launch<T, EL_SHORT, false, KN, false>(a, parts, st);
+    if (el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, true>(a, a.S / 256 + a.E + 1, st);
+    if (a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, true>(a, parts, st);
   }
-  if (piece == 16) return el_launch<T, EL_SHORT, false, KN, 16>(a, parts, st);
-  if (piece == 8) return el_launch<T, EL_SHORT, false, KN, 8>(a, parts, st);
-  return el_launch<T, EL_SHORT, false, KN, 4>(a, parts, st);
+  return el_launch<T, EL_SHORT, false, KN, true>(a, parts, st);
 }
 
 constexpr int EL_JOIN_BLOCKS = 2048;
@@ -451,8 +432,8 @@ static ElGradShape el_grad_shape(int64_t S, int64_t N, int64_t K, int size, bool
 
 template <typename T>
 static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes, hipStream_t st) {
-  const int piece = el_piece_of(a.p, a.q, a.rows, a.cols, (int)sizeof(T));
-  const ElGradShape g = el_grad_shape(a.S, a.rows, a.cols, (int)sizeof(T), piece == 16);
+  const bool direct = el_direct(a.p, a.q, a.rows, a.cols, (int)sizeof(T));
+  const ElGradShape g = el_grad_shape(a.S, a.rows, a.cols, (int)sizeof(T), direct);
   const int64_t size = (int64_t)a.rows * a.cols;
   if ((size_t)(g.several * size) * sizeof(float) > workspace_bytes ||
       (g.several && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
@@ -462,13 +443,11 @@ static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes,
   const int64_t parts = a.S / g.slab + a.E;
   const auto run = [&]() -> int {
     if constexpr (sizeof(T) == 2) {
-      if (g.large) return el_launch<T, EL_LARGE, true, false, 16>(a, parts, st);
-      if (piece == 2) return el_launch<T, EL_SMALL, true, false, 2>(a, parts, st);
+      if (!direct) return el_launch<T, EL_SMALL, true, false, false>(a, parts, st);
+      if (g.large) return el_launch<T, EL_LARGE, true, false, true>(a, parts, st);
     }
-    if (piece == 16 && a.S <= EL_SHORT_GROUP * a.E) return el_launch<T, EL_SHORT, true, false, 16>(a, parts, st);
-    if (piece == 16) return el_launch<T, EL_SMALL, true, false, 16>(a, parts, st);
-    if (piece == 8) return el_launch<T, EL_SMALL, true, false, 8>(a, parts, st);
-    return el_launch<T, EL_SMALL, true, false, 4>(a, parts, st);
+    if (a.S <= EL_SHORT_GROUP * a.E) return el_launch<T, EL_SHORT, true, false, true>(a, parts, st);
+    return el_launch<T, EL_SMALL, true, false, true>(a, parts, st);
   };
   const int rc = run();
   if (rc != HC_OK || g.several == 0) return rc;
