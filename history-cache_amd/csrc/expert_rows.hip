@@ -20,7 +20,9 @@ namespace {
 constexpr int OR_MAX_EXPERTS = 1024;
 constexpr int OR_SMALL_PAIRS = 8192;
 constexpr int OR_SMALL_BLOCK = 1024;
-constexpr int OR_CHUNK = 2048;            // pairs of a block, at least
+constexpr int OR_ROUNDS = 4;              // pairs of a lane that are held in registers
+constexpr int OR_RUN = OR_ROUNDS * HC_WAVE;
+constexpr int OR_CHUNK = OR_RUN * HC_WAVES_PER_BLOCK;
 constexpr int OR_MAX_CHUNKS = 4096;
 
 // The expert of a pair, E ("nowhere") for any number outside [0, E).
@@ -29,27 +31,23 @@ __device__ __forceinline__ int or_expert(const int64_t *__restrict__ expert, int
   return e >= 0 && e < E ? (int)e : E;
 }
 
-// Places the pairs lo .. hi of a wave: `next` (LDS, E + 1 counters of this wave) holds the next place of each expert.
-__device__ __forceinline__ void or_place(const int64_t *__restrict__ expert, int64_t lo, int64_t hi, int E, int bits,
-                                         int *next, int32_t *__restrict__ slot, int32_t *__restrict__ pair) {
+// Places 64 pairs, one a lane (`on`: there is one): `next` (LDS, E + 1 counters of this wave) holds the next place of each
+// expert.  Lanes with the same expert find each other by ballots over the bits of its number; the first of them moves the counter.
+__device__ __forceinline__ void or_place(int64_t q, bool on, int e, int E, int bits, int *next, int32_t *__restrict__ slot,
+                                         int32_t *__restrict__ pair) {
   const int lane = hc_lane();
-  for (int64_t q0 = lo; q0 < hi; q0 += HC_WAVE) {
-    const int64_t q = q0 + lane;
-    const bool on = q < hi;
-    const int e = on ? or_expert(expert, q, E) : 0;
-    uint64_t same = __ballot(on);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((e >> b) & 1);
-      same &= (e >> b) & 1 ? set : ~set;
-    }
-    const int rank = __popcll(same & ((1ull << lane) - 1ull)), first = on ? __ffsll((long long)same) - 1 : lane;
-    int place = 0;
-    if (on && first == lane) place = atomicAdd(&next[e], __popcll(same));
-    place = __shfl(place, first, HC_WAVE) + rank;
-    if (on) {
-      slot[q] = e < E ? place : -1;
-      pair[place] = e < E ? (int32_t)q : -1;
-    }
+  uint64_t same = __ballot(on);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot((e >> b) & 1);
+    same &= (e >> b) & 1 ? set : ~set;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1ull)), first = on ? __ffsll((long long)same) - 1 : lane;
+  int place = 0;
+  if (on && first == lane) place = atomicAdd(&next[e], __popcll(same));
+  place = __shfl(place, first, HC_WAVE) + rank;
+  if (on) {
+    slot[q] = e < E ? place : -1;
+    pair[place] = e < E ? (int32_t)q : -1;
   }
 }
 
@@ -71,37 +69,52 @@ __device__ __forceinline__ int or_scan(int *cnt, int m) {
   return before;
 }
 
-// Everything in one block: WAVES runs of pairs, a row of E + 1 counters for each and one for the sums.
+// A wave's run of ROUNDS * 64 adjacent pairs from `lo` on: their experts (0 behind `hi`, where no pair is).
+template <int ROUNDS>
+__device__ __forceinline__ void or_load(const int64_t *__restrict__ expert, int64_t lo, int64_t hi, int E, int (&e)[ROUNDS]) {
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int64_t q = lo + r * HC_WAVE + hc_lane();
+    e[r] = q < hi ? or_expert(expert, q, E) : 0;
+  }
+}
+
+// Everything in one block of 64 pairs a wave and round: a row of E + 1 counters for each wave, one for the sums.
+template <int ROUNDS>
 __global__ __launch_bounds__(OR_SMALL_BLOCK) void or_small(const int64_t *__restrict__ expert, int32_t *__restrict__ slot,
                                                             int32_t *__restrict__ pair, int64_t *__restrict__ offset, int P,
                                                             int E, int bits) {
   extern __shared__ int s_cnt[];
-  const int waves = (int)(blockDim.x / HC_WAVE), wave = hc_wave_in_block(), bins = E + 1;
-  int *sum = s_cnt + waves * bins, *mine = s_cnt + wave * bins;
+  const int waves = (int)(blockDim.x / HC_WAVE), wave = hc_wave_in_block(), lane = hc_lane(), bins = E + 1;
+  int *sum = s_cnt + waves * bins, *mine = s_cnt + wave * bins, e[ROUNDS];
+  const int lo = wave * ROUNDS * HC_WAVE;
+  or_load<ROUNDS>(expert, lo, P, E, e);
   for (int i = (int)threadIdx.x; i < (waves + 1) * bins; i += (int)blockDim.x) s_cnt[i] = 0;
   __syncthreads();
-  const int run = ((P + waves - 1) / waves + HC_WAVE - 1) / HC_WAVE * HC_WAVE;
-  const int lo = wave * run < P ? wave * run : P, hi = lo + run < P ? lo + run : P;
-  for (int q = lo + hc_lane(); q < hi; q += HC_WAVE) atomicAdd(&mine[or_expert(expert, q, E)], 1);
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (lo + r * HC_WAVE + lane < P) atomicAdd(&mine[e[r]], 1);
   __syncthreads();
-  for (int e = (int)threadIdx.x; e < bins; e += (int)blockDim.x) {
+  for (int b = (int)threadIdx.x; b < bins; b += (int)blockDim.x) {
     int s = 0;
     for (int w = 0; w < waves; ++w) {
-      const int c = s_cnt[w * bins + e];
-      s_cnt[w * bins + e] = s;
+      const int c = s_cnt[w * bins + b];
+      s_cnt[w * bins + b] = s;
       s += c;
     }
-    sum[e] = s;
+    sum[b] = s;
   }
   __syncthreads();
   if (wave == 0) or_scan(sum, bins);
   __syncthreads();
-  for (int e = (int)threadIdx.x; e < bins; e += (int)blockDim.x) {
-    offset[e] = sum[e];
-    for (int w = 0; w < waves; ++w) s_cnt[w * bins + e] += sum[e];
+  for (int b = (int)threadIdx.x; b < bins; b += (int)blockDim.x) {
+    offset[b] = sum[b];
+    for (int w = 0; w < waves; ++w) s_cnt[w * bins + b] += sum[b];
   }
   __syncthreads();
-  or_place(expert, lo, hi, E, bits, mine, slot, pair);
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (lo + r * HC_WAVE < P) or_place(lo + r * HC_WAVE + lane, lo + r * HC_WAVE + lane < P, e[r], E, bits, mine, slot, pair);
 }
 
 __global__ __launch_bounds__(HC_BLOCK) void or_count(const int64_t *__restrict__ expert, int *__restrict__ count, int64_t P,
@@ -111,7 +124,13 @@ __global__ __launch_bounds__(HC_BLOCK) void or_count(const int64_t *__restrict__
   for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) s_cnt[e] = 0;
   __syncthreads();
   const int64_t lo = (int64_t)blockIdx.x * chunk, hi = lo + chunk < P ? lo + chunk : P;
-  for (int64_t q = lo + threadIdx.x; q < hi; q += HC_BLOCK) atomicAdd(&s_cnt[or_expert(expert, q, E)], 1);
+  for (int64_t q0 = lo + hc_wave_in_block() * OR_RUN; q0 < hi; q0 += OR_CHUNK) {
+    int e[OR_ROUNDS];
+    or_load<OR_ROUNDS>(expert, q0, hi, E, e);
+#pragma unroll
+    for (int r = 0; r < OR_ROUNDS; ++r)
+      if (q0 + r * HC_WAVE + hc_lane() < hi) atomicAdd(&s_cnt[e[r]], 1);
+  }
   __syncthreads();
   for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) count[(int64_t)e * gridDim.x + blockIdx.x] = s_cnt[e];
 }
@@ -123,34 +142,50 @@ __global__ __launch_bounds__(HC_WAVE) void or_prefix(int *__restrict__ count, in
   if (hc_lane() == 0) total[blockIdx.x] = t;
 }
 
+// The chunk's pairs in pieces of OR_CHUNK, a run of each by every wave.
 __global__ __launch_bounds__(HC_BLOCK) void or_scatter(const int64_t *__restrict__ expert, const int *__restrict__ count,
                                                        const int *__restrict__ total, int32_t *__restrict__ slot,
                                                        int32_t *__restrict__ pair, int64_t *__restrict__ offset, int64_t P,
                                                        int E, int64_t chunk, int bits) {
   extern __shared__ int s_cnt[];
   constexpr int W = HC_WAVES_PER_BLOCK;
-  const int wave = hc_wave_in_block(), bins = E + 1;
-  int *sum = s_cnt + W * bins, *mine = s_cnt + wave * bins;
-  for (int i = (int)threadIdx.x; i < W * bins; i += HC_BLOCK) s_cnt[i] = 0;
-  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) sum[e] = total[e];
+  const int wave = hc_wave_in_block(), lane = hc_lane(), bins = E + 1;
+  int *sum = s_cnt + W * bins, *mine = s_cnt + wave * bins, e[OR_ROUNDS];
+  const int64_t lo = (int64_t)blockIdx.x * chunk, hi = lo + chunk < P ? lo + chunk : P;
+  or_load<OR_ROUNDS>(expert, lo + wave * OR_RUN, hi, E, e);
+  for (int b = (int)threadIdx.x; b < bins; b += HC_BLOCK) sum[b] = total[b];
   __syncthreads();
-  const int64_t begin = (int64_t)blockIdx.x * chunk, end = begin + chunk < P ? begin + chunk : P;
-  const int64_t lo0 = begin + wave * (chunk / W), lo = lo0 < end ? lo0 : end, hi = lo + chunk / W < end ? lo + chunk / W : end;
-  for (int64_t q = lo + hc_lane(); q < hi; q += HC_WAVE) atomicAdd(&mine[or_expert(expert, q, E)], 1);
   if (wave == 0) or_scan(sum, bins);
   __syncthreads();
-  for (int e = (int)threadIdx.x; e < bins; e += HC_BLOCK) {
-    if (blockIdx.x == 0) offset[e] = sum[e];
-    int s = sum[e] + count[(int64_t)e * gridDim.x + blockIdx.x];
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int c = s_cnt[w * bins + e];
-      s_cnt[w * bins + e] = s;
-      s += c;
-    }
+  for (int b = (int)threadIdx.x; b < bins; b += HC_BLOCK) {
+    if (blockIdx.x == 0) offset[b] = sum[b];
+    sum[b] += count[(int64_t)b * gridDim.x + blockIdx.x];
   }
-  __syncthreads();
-  or_place(expert, lo, hi, E, bits, mine, slot, pair);
+  for (int64_t piece = lo; piece < hi; piece += OR_CHUNK) {
+    const int64_t q0 = piece + wave * OR_RUN;
+    if (piece > lo) or_load<OR_ROUNDS>(expert, q0, hi, E, e);
+    for (int i = (int)threadIdx.x; i < W * bins; i += HC_BLOCK) s_cnt[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < OR_ROUNDS; ++r)
+      if (q0 + r * HC_WAVE + lane < hi) atomicAdd(&mine[e[r]], 1);
+    __syncthreads();
+    for (int b = (int)threadIdx.x; b < bins; b += HC_BLOCK) {
+      int s = sum[b];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int c = s_cnt[w * bins + b];
+        s_cnt[w * bins + b] = s;
+        s += c;
+      }
+      sum[b] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < OR_ROUNDS; ++r)
+      if (q0 + r * HC_WAVE < hi) or_place(q0 + r * HC_WAVE + lane, q0 + r * HC_WAVE + lane < hi, e[r], E, bits, mine, slot, pair);
+    __syncthreads();
+  }
 }
 
 struct OrShape {
@@ -185,10 +220,10 @@ __device__ __forceinline__ void mv_zero_tail(const MvArgs &a, T *__restrict__ ro
 template <typename T, int VEC>
 __global__ __launch_bounds__(HC_BLOCK) void mv_to(MvArgs a, const T *__restrict__ x, T *__restrict__ rows) {
   typedef typename hc_vec<T, VEC>::raw_t raw;
-  const int64_t item = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x;
-  const int64_t i = item / a.pieces;
+  const uint32_t item = blockIdx.x * HC_BLOCK + threadIdx.x;       // (a launch has less than 2^32 threads)
+  const int64_t i = item / (uint32_t)a.pieces;
   if (i < a.n) {
-    const int c = (int)(item - i * a.pieces) * VEC;
+    const int c = (int)(item - (uint32_t)i * (uint32_t)a.pieces) * VEC;
     const raw v = *reinterpret_cast<const raw *>(x + i * a.D + c);
     for (int j = 0; j < a.k; ++j) {
       const int32_t s = a.slot[i * a.k + j];
@@ -198,57 +233,93 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_to(MvArgs a, const T *__restrict_
   mv_zero_tail<T, VEC>(a, rows);
 }
 
-template <typename T, int VEC>
+// K: the choices of a row that are read at a time.
+template <typename T, int VEC, int K>
 __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restrict__ y, const float *__restrict__ weight,
                                                     T *__restrict__ out) {
-  const int64_t item = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x;
-  const int64_t i = item / a.pieces;
+  const uint32_t item = blockIdx.x * HC_BLOCK + threadIdx.x;       // (a launch has less than 2^32 threads)
+  const int64_t i = item / (uint32_t)a.pieces;
   if (i >= a.n) return;
-  const int c = (int)(item - i * a.pieces) * VEC;
+  const int c = (int)(item - (uint32_t)i * (uint32_t)a.pieces) * VEC;
   float sum[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) sum[v] = 0.f;
-  for (int j = 0; j < a.k; ++j) {
-    const int32_t s = a.slot[i * a.k + j];
-    if (s < 0) continue;
-    float p[VEC];
-    hc_vec<T, VEC>::load(y + (int64_t)s * a.D + c, p);
-    const float w = weight != nullptr ? weight[i * a.k + j] : 1.f;
+  for (int j0 = 0; j0 < a.k; j0 += K) {
+    int32_t s[K];
+    float w[K], p[K][VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) sum[v] = fmaf(w, p[v], sum[v]);
+    for (int j = 0; j < K; ++j) s[j] = j0 + j < a.k ? a.slot[i * a.k + j0 + j] : -1;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      w[j] = weight != nullptr && s[j] >= 0 ? weight[i * a.k + j0 + j] : 1.f;
+      if (s[j] >= 0 && weight != nullptr) {
+        hc_vec<T, VEC>::load(y + (int64_t)s[j] * a.D + c, p[j]);
+      } else if (s[j] >= 0) {
+        hc_vec<T, VEC>::load_nt(y + (int64_t)s[j] * a.D + c, p[j]);    // gradients: nothing reads them after this
+      } else {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p[j][v] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) sum[v] = fmaf(w[j], p[j][v], sum[v]);
   }
   hc_vec<T, VEC>::store(out + i * a.D + c, sum);
 }
 
-// L lanes a row.
-template <typename T, int VEC>
+// L lanes a row; K as above.
+template <typename T, int VEC, int K>
 __global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__restrict__ g, const T *__restrict__ y,
                                                          const float *__restrict__ weight, T *__restrict__ grad_y,
                                                          float *__restrict__ grad_weight, int L) {
   const int lane = (int)threadIdx.x & (L - 1);
   const int64_t i = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
   if (i < a.n) {
-    for (int j = 0; j < a.k; ++j) {
-      const int32_t s = a.slot[i * a.k + j];
-      const float w = weight[i * a.k + j];
-      float dot = 0.f;
-      if (s >= 0)
-        for (int p = lane; p < a.pieces; p += L) {
-          float gv[VEC], yv[VEC], o[VEC];
-          hc_vec<T, VEC>::load(g + i * a.D + p * VEC, gv);
-          hc_vec<T, VEC>::load(y + (int64_t)s * a.D + p * VEC, yv);
+    for (int j0 = 0; j0 < a.k; j0 += K) {
+      int32_t s[K];
+      float w[K], dot[K];
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            dot = fmaf(gv[v], yv[v], dot);
-            o[v] = w * gv[v];
+      for (int j = 0; j < K; ++j) {
+        s[j] = j0 + j < a.k ? a.slot[i * a.k + j0 + j] : -1;
+        w[j] = s[j] >= 0 ? weight[i * a.k + j0 + j] : 0.f;
+        dot[j] = 0.f;
+      }
+      for (int p = lane; p < a.pieces; p += L) {
+        float gv[VEC], yv[K][VEC];
+        hc_vec<T, VEC>::load(g + i * a.D + p * VEC, gv);
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (s[j] >= 0) hc_vec<T, VEC>::load(y + (int64_t)s[j] * a.D + p * VEC, yv[j]);
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (s[j] >= 0) {
+            float o[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+              dot[j] = fmaf(gv[v], yv[j][v], dot[j]);
+              o[v] = w[j] * gv[v];
+            }
+            hc_vec<T, VEC>::store(grad_y + (int64_t)s[j] * a.D + p * VEC, o);
           }
-          hc_vec<T, VEC>::store(grad_y + (int64_t)s * a.D + p * VEC, o);
-        }
-      for (int d = L / 2; d >= 1; d /= 2) dot += __shfl_xor(dot, d, HC_WAVE);
-      if (lane == 0) grad_weight[i * a.k + j] = dot;
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        for (int d = L / 2; d >= 1; d /= 2) dot[j] += __shfl_xor(dot[j], d, HC_WAVE);
+        if (lane == 0 && j0 + j < a.k) grad_weight[i * a.k + j0 + j] = dot[j];
+      }
     }
   }
   mv_zero_tail<T, VEC>(a, grad_y);
+}
+
+// As many choices at a time as a row has, up to four.
+template <typename F>
+static int mv_with_choices(int64_t k, F &&f) {
+  if (k == 1) return f(std::integral_constant<int, 1>{});
+  if (k == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 4>{});
 }
 
 static bool mv_args(int64_t n, int64_t top_k, int64_t E, int64_t D, const int32_t *slot, const int64_t *offset, MvArgs *a) {
@@ -300,12 +371,13 @@ extern "C" int hc_expert_order(const int64_t *expert, int64_t pairs, int64_t E, 
   while ((1 << bits) < E + 1) ++bits;
   const size_t bins = (size_t)E + 1;
   if (pairs <= OR_SMALL_PAIRS) {
-    // a wave for every 64 pairs, up to sixteen
-    int waves = (int)((pairs + HC_WAVE - 1) / HC_WAVE);
-    waves = waves < 1 ? 1 : waves > OR_SMALL_BLOCK / HC_WAVE ? OR_SMALL_BLOCK / HC_WAVE : waves;
-    while ((waves + 1) * bins * sizeof(int) > 64 * 1024) waves /= 2;
-    or_small<<<dim3(1), dim3((unsigned)waves * HC_WAVE), (waves + 1) * bins * sizeof(int), st>>>(expert, slot, pair, offset,
-                                                                                                (int)pairs, (int)E, bits);
+    // as many waves as sixteen rounds of two or eight need
+    const int rounds = pairs <= 2 * OR_SMALL_BLOCK ? 2 : OR_SMALL_PAIRS / OR_SMALL_BLOCK;
+    int waves = (int)((pairs + rounds * HC_WAVE - 1) / (rounds * HC_WAVE));
+    waves = waves < 1 ? 1 : waves;
+    const auto kernel = rounds == 2 ? or_small<2> : or_small<OR_SMALL_PAIRS / OR_SMALL_BLOCK>;
+    kernel<<<dim3(1), dim3((unsigned)waves * HC_WAVE), (waves + 1) * bins * sizeof(int), st>>>(expert, slot, pair, offset, (int)pairs,
+                                                                                              (int)E, bits);
     return hc_launch_status();
   }
   const OrShape s = or_shape(pairs);
@@ -354,9 +426,11 @@ extern "C" int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t
       a.pieces = (int)(D / VEC);
       const int64_t blocks = (n * a.pieces + HC_BLOCK - 1) / HC_BLOCK;
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
-      mv_from<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
-          a, static_cast<const T *>(y), weight, static_cast<T *>(out));
-      return hc_launch_status();
+      return mv_with_choices(top_k, [&](auto choices) {
+        mv_from<T, VEC, decltype(choices)::value><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+            a, static_cast<const T *>(y), weight, static_cast<T *>(out));
+        return hc_launch_status();
+      });
     });
   });
 }
@@ -379,9 +453,12 @@ extern "C" int hc_rows_from_experts_grad(const void *g, const void *y, int dtype
       while (L < HC_WAVE && L < a.pieces) L *= 2;
       const int64_t blocks = (n * L + HC_BLOCK - 1) / HC_BLOCK;
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
-      mv_from_grad<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
-          a, static_cast<const T *>(g), static_cast<const T *>(y), weight, static_cast<T *>(grad_y), grad_weight, L);
-      return hc_launch_status();
+      return mv_with_choices(top_k, [&](auto choices) {
+        mv_from_grad<T, VEC, decltype(choices)::value>
+            <<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+                a, static_cast<const T *>(g), static_cast<const T *>(y), weight, static_cast<T *>(grad_y), grad_weight, L);
+        return hc_launch_status();
+      });
     });
   });
 }
