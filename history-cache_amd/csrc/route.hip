@@ -4,57 +4,114 @@
 //   weight[j] = p[chosen j] / (normalize ? sum of the chosen p : 1); a logit of -inf is never chosen (-1, weight 0)
 //   t = sum_j w[j] g[j];  dl[chosen j] = w[j] (g[j] - t), 0 elsewhere (normalize);  dl[e] = p[e] ((e chosen ? g : 0) - t)
 //
-// A row lies in L lanes, V adjacent logits each (L = 8 for up to 64 experts), 64 / L rows per wave; the k winners are
-// found one after the other by a maximum over the lane's keys and then over the row's lanes.  A key orders
+// A row lies in L lanes, V adjacent logits each (L = 8 for up to 64 experts), 64 / L rows per wave.  A key orders
 // by value and, among equal values, by the lower index: 16-bit logits and an index fit one 32-bit key, whose maximum is
-// one instruction; fp32 takes 64 bits.  With `normalize` the sum runs over the winners alone, no other exponential is taken.
+// one instruction; fp32 takes 64 bits.  A lane sorts its keys once; the winners then are, one after the other, the largest of the
+// row's first keys, and the lane that had it moves up.  With `normalize` the sum runs over the winners alone, and each lane
+// takes the exponential of the winner that it keeps.
 #include "hc_common.h"
 
 namespace {
 
 constexpr int RT_MAX_EXPERTS = 1024;
-constexpr int RT_MAX_CHOICES = 32;      // four winners a lane where a row lies in eight
+constexpr int RT_MAX_CHOICES = 32;
 
-// ---- ordering keys: NaN above everything, -0 equal to 0, 0 is below every key
+// Another lane's value: D = 1, 2: lane ^ D; 4, 8: the lane's mirror image among 8 or 16, which after the smaller steps holds what
+// lane ^ D does; 16, 32: lane ^ D.
+template <int D>
+__device__ __forceinline__ uint32_t rt_other(uint32_t v) {
+  if constexpr (D >= 16) return (uint32_t)__shfl_xor((int)v, D, HC_WAVE);
+  constexpr int CTRL = D == 1 ? 0xb1 : D == 2 ? 0x4e : D == 4 ? 0x141 : 0x140;
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int D>
+__device__ __forceinline__ int32_t rt_other(int32_t v) { return (int32_t)rt_other<D>((uint32_t)v); }
+template <int D>
+__device__ __forceinline__ int64_t rt_other(int64_t v) {
+  return (int64_t)((uint64_t)rt_other<D>((uint32_t)((uint64_t)v >> 32)) << 32 | rt_other<D>((uint32_t)v));
+}
+template <int D>
+__device__ __forceinline__ float rt_other(float v) { return __uint_as_float(rt_other<D>(__float_as_uint(v))); }
+
+// `v` of the L lanes joined by `f`, in every one of them.
+template <int L, int D = 1, typename V, typename F>
+__device__ __forceinline__ V rt_join(V v, F &&f) {
+  if constexpr (D < L) return rt_join<L, 2 * D>(f(v, rt_other<D>(v)), f);
+  else return v;
+}
+
+// ---- ordering keys
+// A signed number whose upper half (16 bits; fp32: 32) orders like the logit -- a positive one as it is, of a negative one all but the
+// sign turned over, NaN above everything, -0 as 0 -- and whose lower half falls with the index: 8 bits for the place in
+// the lane, above them, put in when lanes are compared, the lane.  NONE is below every key.
 template <typename T>
 struct rt_key {
-  typedef uint32_t type;
-  __device__ __forceinline__ static type make(float v, int index) {
-    const float f = v + 0.0f;
-    const uint16_t b = __builtin_bit_cast(uint16_t, hc_from_f32<T>(f));      // exact: f came from a T
-    const uint16_t o = f != f ? 0xffffu : (b & 0x8000u) ? (uint16_t)~b : (uint16_t)(b | 0x8000u);
-    return (uint32_t)o << 16 | (uint32_t)(0xffff - index);
+  typedef int32_t type;
+  static constexpr type NONE = (type)0x80000000;
+  static constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  __device__ __forceinline__ static type order(uint32_t upper) {
+    return (type)(upper ^ ((uint32_t)((int32_t)upper >> 31) & 0x7fff0000u));
   }
-  __device__ __forceinline__ static int index(type k) { return 0xffff - (int)(k & 0xffffu); }
+  template <int V>
+  __device__ __forceinline__ static void make(const T (&v)[V], type (&key)[V]) {
+    uint32_t odd = 0;                      // is there a NaN or a -0 anywhere?
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t b = __builtin_bit_cast(uint16_t, v[i]);
+      key[i] = order(b << 16 | (uint32_t)(V - 1 - i));
+      odd |= (b & 0x7fffu) > INF || b == 0x8000u ? 1u : 0u;
+    }
+    if (__ballot(odd != 0) == 0) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t b = __builtin_bit_cast(uint16_t, v[i]);
+      if ((b & 0x7fffu) > INF) key[i] = (type)(0x7fff0000u | (uint32_t)(V - 1 - i));
+      else if (b == 0x8000u) key[i] = (type)(V - 1 - i);
+    }
+  }
+  __device__ __forceinline__ static uint32_t lower(type k) { return (uint32_t)k & 0xffffu; }
   __device__ __forceinline__ static float value(type k) {
-    const uint16_t o = (uint16_t)(k >> 16);
-    if (o == 0xffffu) return __builtin_nanf("");
-    const uint16_t b = (o & 0x8000u) ? (uint16_t)(o ^ 0x8000u) : (uint16_t)~o;
-    return hc_to_f32<T>(__builtin_bit_cast(T, b));
+    const uint32_t o = (uint32_t)k & 0xffff0000u;
+    if (o == 0x7fff0000u) return __builtin_nanf("");
+    return hc_to_f32<T>(__builtin_bit_cast(T, (uint16_t)((uint32_t)order(o) >> 16)));
   }
-  __device__ __forceinline__ static type other(type k, int d) { return (type)__shfl_xor((int)k, d, HC_WAVE); }
 };
 template <>
 struct rt_key<float> {
-  typedef uint64_t type;
-  __device__ __forceinline__ static type make(float v, int index) {
-    const float f = v + 0.0f;
-    const uint32_t b = __float_as_uint(f);
-    const uint32_t o = f != f ? 0xffffffffu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return (uint64_t)o << 32 | (uint32_t)(0xffff - index);
+  typedef int64_t type;
+  static constexpr type NONE = (type)0x8000000000000000ull;
+  __device__ __forceinline__ static uint32_t order(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) & 0x7fffffffu); }
+  template <int V>
+  __device__ __forceinline__ static void make(const float (&v)[V], type (&key)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float f = v[i] + 0.0f;
+      key[i] = (type)((uint64_t)(f != f ? 0x7fffffffu : order(__float_as_uint(f))) << 32 | (uint32_t)(V - 1 - i));
+    }
   }
-  __device__ __forceinline__ static int index(type k) { return 0xffff - (int)(uint32_t)k; }
+  __device__ __forceinline__ static uint32_t lower(type k) { return (uint32_t)k; }
   __device__ __forceinline__ static float value(type k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    if (o == 0xffffffffu) return __builtin_nanf("");
-    return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
-  }
-  __device__ __forceinline__ static type other(type k, int d) {
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)k, d, HC_WAVE);
-    const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(k >> 32), d, HC_WAVE);
-    return (uint64_t)hi << 32 | lo;
+    return __uint_as_float(order((uint32_t)((uint64_t)k >> 32)));            // (0x7fffffff is a NaN)
   }
 };
+
+// Sorts V keys, the largest first (Batcher's odd-even merge sort).
+template <int V, typename K>
+__device__ __forceinline__ void rt_sort(K (&a)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const K x = a[i + j], y = a[i + j + k];
+            a[i + j] = x > y ? x : y;
+            a[i + j + k] = x > y ? y : x;
+          }
+}
 
 __device__ __forceinline__ bool rt_masked(float v) { return v == -__builtin_inff(); }
 
@@ -67,18 +124,18 @@ struct rt_row {
     return E % PIECE == 0 && reinterpret_cast<uintptr_t>(p) % (sizeof(T) * PIECE) == 0;
   }
   // columns at, at + 1, ...; behind the row's end: -inf
-  __device__ __forceinline__ static void load(const T *__restrict__ row, int at, int E, bool whole, float (&v)[V]) {
+  __device__ __forceinline__ static void load(const T *__restrict__ row, int at, int E, bool whole, T (&v)[V]) {
     if (whole && at + V <= E) {
 #pragma unroll
       for (int q = 0; q < V; q += PIECE) {
-        float part[PIECE];
-        hc_vec<T, PIECE>::load(row + at + q, part);
+        typename hc_vec<T, PIECE>::U u;
+        u.raw = *reinterpret_cast<const typename hc_vec<T, PIECE>::raw_t *>(row + at + q);
 #pragma unroll
-        for (int i = 0; i < PIECE; ++i) v[q + i] = part[i];
+        for (int i = 0; i < PIECE; ++i) v[q + i] = u.e[i];
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = at + i < E ? hc_to_f32<T>(row[at + i]) : -__builtin_inff();
+      for (int i = 0; i < V; ++i) v[i] = at + i < E ? row[at + i] : hc_from_f32<T>(-__builtin_inff());
     }
   }
   __device__ __forceinline__ static void store(T *__restrict__ row, int at, int E, bool whole, const float (&v)[V]) {
@@ -98,63 +155,64 @@ struct rt_row {
   }
 };
 
-template <typename T, int L, int V>
+// KEPT: winners a lane keeps, top_k <= KEPT * L.
+template <typename T, int L, int V, int KEPT>
 __global__ __launch_bounds__(HC_BLOCK) void rt_forward(const T *__restrict__ logits, int64_t *__restrict__ expert,
                                                         float *__restrict__ weight, int64_t n, int E, int k, bool normalize,
                                                         bool whole) {
   typedef rt_key<T> key;
   typedef typename key::type key_t;
-  constexpr int KEPT = L >= RT_MAX_CHOICES ? 1 : RT_MAX_CHOICES / L;
   const int lane = (int)threadIdx.x & (L - 1);
   const int64_t r = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
   const bool live = r < n;
-  key_t have[V];
-  float v[V], sum = 0.f;
+  const auto larger = [](key_t a, key_t b) { return a > b ? a : b; };
+  const auto plus = [](float a, float b) { return a + b; };
+  T v[V];
+  key_t have[V], mine[KEPT], top = key::NONE;
+  const key_t place = (key_t)(L - 1 - lane) << 8;
   rt_row<T, V>::load(logits + (live ? r : 0) * E, lane * V, E, whole, v);
+  key::make(v, have);
 #pragma unroll
-  for (int i = 0; i < V; ++i) have[i] = lane * V + i < E ? key::make(v[i], lane * V + i) : 0;
-  int mine[KEPT];
-  float mine_e[KEPT], top = 0.f;
+  for (int i = 0; i < V; ++i)
+    if (lane * V + i >= E) have[i] = key::NONE;
+  rt_sort(have);
 #pragma unroll
-  for (int q = 0; q < KEPT; ++q) {
-    mine[q] = -1;
-    mine_e[q] = 0.f;
-  }
+  for (int q = 0; q < KEPT; ++q) mine[q] = key::NONE;
   for (int j = 0; j < k; ++j) {
-    key_t best = have[0];
+    const key_t own = have[0] | place, best = rt_join<L>(own, larger);
+    if (j == 0) top = best;
+    // (by bits: a choice between neighbours becomes a search for the chosen index)
+    const key_t won = own == best ? -1 : 0;
 #pragma unroll
-    for (int i = 1; i < V; ++i) best = have[i] > best ? have[i] : best;
-#pragma unroll
-    for (int d = L / 2; d >= 1; d /= 2) {
-      const key_t o = key::other(best, d);
-      best = o > best ? o : best;
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) have[i] = have[i] == best ? 0 : have[i];
-    const float f = key::value(best);
-    if (j == 0) top = f;
-    const bool none = rt_masked(f);
-    const float e = none ? 0.f : expf(f - top);
-    if (normalize) sum += e;
+    for (int i = 0; i < V; ++i) have[i] = (have[i] & ~won) | ((i + 1 < V ? have[i + 1] : key::NONE) & won);
 #pragma unroll
     for (int q = 0; q < KEPT; ++q)
-      if (j == q * L + lane) {
-        mine[q] = none ? -1 : key::index(best);
-        mine_e[q] = e;
-      }
+      if (j == q * L + lane) mine[q] = best;
+  }
+  const float largest = key::value(top);
+  float e[KEPT], sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < KEPT; ++q) {
+    const float f = key::value(mine[q]);
+    e[q] = q * L + lane >= k || rt_masked(f) ? 0.f : expf(f - largest);
+    sum += e[q];
   }
   if (!normalize) {
+    sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (!rt_masked(v[i])) sum += expf(v[i] - top);
-#pragma unroll
-    for (int d = L / 2; d >= 1; d /= 2) sum += __shfl_xor(sum, d, HC_WAVE);
+    for (int i = 0; i < V; ++i) {
+      const float f = hc_to_f32<T>(v[i]);
+      if (!rt_masked(f)) sum += expf(f - largest);
+    }
   }
+  sum = rt_join<L>(sum, plus);
 #pragma unroll
   for (int q = 0; q < KEPT; ++q)
     if (live && q * L + lane < k) {
-      expert[r * k + q * L + lane] = mine[q];
-      weight[r * k + q * L + lane] = mine[q] < 0 ? 0.f : mine_e[q] / sum;
+      const bool none = rt_masked(key::value(mine[q]));
+      const int from = L - 1 - (int)(key::lower(mine[q]) >> 8), at = V - 1 - (int)(key::lower(mine[q]) & 0xffu);
+      expert[r * k + q * L + lane] = none ? -1 : from * V + at;
+      weight[r * k + q * L + lane] = none ? 0.f : e[q] / sum;
     }
 }
 
@@ -167,26 +225,27 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ lo
   const int64_t r = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
   const bool live = r < n;
   const int64_t at = (live ? r : 0) * k;
+  const auto plus = [](float a, float b) { return a + b; };
+  const auto larger = [](float a, float b) { return fmaxf(a, b); };
   float t = 0.f;
   for (int j = lane; j < k; j += L)
     if (expert[at + j] >= 0) t += weight[at + j] * g[at + j];
-#pragma unroll
-  for (int d = L / 2; d >= 1; d /= 2) t += __shfl_xor(t, d, HC_WAVE);
+  t = rt_join<L>(t, plus);
   float p[V], out[V];
   if (!normalize) {
-    float v[V], top = -__builtin_inff(), sum = 0.f;
+    T v[V];
+    float top = -__builtin_inff(), sum = 0.f;
     rt_row<T, V>::load(logits + (live ? r : 0) * E, lane * V, E, whole, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = fmaxf(top, v[i]);
-#pragma unroll
-    for (int d = L / 2; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, HC_WAVE));
+    for (int i = 0; i < V; ++i) top = fmaxf(top, hc_to_f32<T>(v[i]));
+    top = rt_join<L>(top, larger);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      p[i] = rt_masked(v[i]) ? 0.f : expf(v[i] - top);
+      const float f = hc_to_f32<T>(v[i]);
+      p[i] = rt_masked(f) ? 0.f : expf(f - top);
       sum += p[i];
     }
-#pragma unroll
-    for (int d = L / 2; d >= 1; d /= 2) sum += __shfl_xor(sum, d, HC_WAVE);
+    sum = rt_join<L>(sum, plus);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       p[i] = sum == 0.f ? 0.f : p[i] / sum;
@@ -197,14 +256,13 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ lo
     for (int i = 0; i < V; ++i) out[i] = 0.f;
   }
   for (int j = 0; j < k; ++j) {
-    const int64_t e = expert[at + j];
-    const float w = weight[at + j], gj = g[at + j];
+    const int e = (int)expert[at + j] - lane * V;
+    const float w = weight[at + j], d = g[at + j] - t;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (e == lane * V + i) out[i] = (normalize ? w : p[i]) * (gj - t);
+      if (e == i) out[i] = (normalize ? w : p[i]) * d;
   }
-  if (!live) return;
-  rt_row<T, V>::store(grad + r * E, lane * V, E, whole, out);
+  if (live) rt_row<T, V>::store(grad + r * E, lane * V, E, whole, out);
 }
 
 // L lanes of V logits for E experts, in the first pair that holds them: a row of few experts is spread over eight lanes.
@@ -252,7 +310,8 @@ extern "C" int hc_route_rows(const void *logits, int dtype, int64_t n, int64_t E
       constexpr int L = decltype(lanes)::value, V = decltype(each)::value;
       const int64_t blocks = (n + HC_BLOCK / L - 1) / (HC_BLOCK / L);
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
-      rt_forward<T, L, V><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+      const auto kernel = top_k <= L ? rt_forward<T, L, V, 1> : rt_forward<T, L, V, L >= RT_MAX_CHOICES ? 1 : RT_MAX_CHOICES / L>;
+      kernel<<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
           static_cast<const T *>(logits), expert, weight, n, (int)E, (int)top_k, normalize != 0,
           rt_row<T, V>::whole(logits, E));
       return hc_launch_status();
