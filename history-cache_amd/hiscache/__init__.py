@@ -8,6 +8,7 @@ part of this package.
 from hiscache_backend import count_history_reconstruct, get_graph_structure_score, record_history
 
 from .dataset import ProcessedDataset, write_processed
+from .experts import ExpertMLP, packed_activations
 from .feature_store import PinnedFeatureStore
 from .history_cache import HistoryCache
 from .history_model import (HistoryRGCN, HistorySAGE, MyRGCNConvHistory2, MySageConvHistory, get_model,
@@ -21,7 +22,7 @@ from .sampler import NeighborSampler
 from .util import Config, backward_on_this_thread, make_config, quantile_threshold
 
 __all__ = [
-    "HistoryCache", "HistoryTable", "HistoryTrainer", "hotness", "RingHistoryCache", "RecordedIteration", "HistorySAGE", "HistoryRGCN", "MySageConvHistory", "MyRGCNConvHistory2", "typed_csr", "get_model", "prefer_low_latency_gemm",
+    "HistoryCache", "HistoryTable", "HistoryTrainer", "hotness", "RingHistoryCache", "RecordedIteration", "HistorySAGE", "HistoryRGCN", "MySageConvHistory", "MyRGCNConvHistory2", "typed_csr", "get_model", "prefer_low_latency_gemm", "ExpertMLP", "packed_activations",
     "PinnedFeatureStore", "NeighborSampler", "ProcessedDataset", "write_processed", "Config", "make_config", "quantile_threshold", "backward_on_this_thread",
     "count_history_reconstruct", "get_graph_structure_score", "record_history",
 ]

@@ -1,0 +1,79 @@
+"""A layer of experts over the nodes of a batch, and activations kept in 8 bits for the backward pass.
+
+``ExpertMLP`` stands behind (or in place of) the dense half of a layer: every node goes through a few of E gated maps, chosen by
+a learned router or given, for instance by the node's type.  ``packed_activations`` is a context in which autograd keeps
+what operators save in 8 bits.  Both run on ``hiscache_backend``'s kernels.
+"""
+import math
+
+import torch
+import torch.nn.functional as F
+
+import hiscache_backend
+
+
+class ExpertMLP(torch.nn.Module):
+    """``sum_j weight[i, j] * expert[i, j](x[i])`` with ``expert_e(x) = (silu(x A_e) * (x B_e)) C_e``.
+
+    channels: width of the rows in and out; hidden: width inside an expert; num_expert: E; top_k: experts a row;
+    normalize: a row's weights add up to one.  In training [x A | x B] is kept in 8 bits, a scale for every ``group`` columns."""
+
+    def __init__(self, channels, hidden, num_expert, top_k=2, normalize=True, group=64, device=None, dtype=None):
+        super().__init__()
+        if not 1 <= top_k <= num_expert:
+            raise ValueError(f"top_k must be between 1 and the {num_expert} experts, got {top_k}")
+        self.channels, self.hidden, self.num_expert = channels, hidden, num_expert
+        self.top_k, self.normalize, self.group = top_k, normalize, group
+        # the router's logits are fp32 whatever the rows are: near-ties decide where a row goes
+        self.router = torch.nn.Parameter(torch.empty(num_expert, channels, device=device, dtype=torch.float32))
+        self.w_in = torch.nn.Parameter(torch.empty(num_expert, 2 * hidden, channels, device=device, dtype=dtype))
+        self.w_out = torch.nn.Parameter(torch.empty(num_expert, channels, hidden, device=device, dtype=dtype))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            for w, fan in ((self.router, self.channels), (self.w_in, self.channels), (self.w_out, self.hidden)):
+                w.uniform_(-1 / math.sqrt(fan), 1 / math.sqrt(fan))
+
+    def route(self, x, allowed=None):
+        """The router's choice for the rows of x: (expert int64 [n, top_k], weight fp32 [n, top_k]).  ``allowed`` (bool
+        [n, E] or [E], optional): experts that a row may go to; a row that may go nowhere gets -1 and weight 0."""
+        logits = F.linear(x.float(), self.router)
+        if allowed is not None:
+            logits = logits.masked_fill(~allowed, -math.inf)
+        return hiscache_backend.route_rows(logits, self.top_k, normalize=self.normalize)
+
+    def forward(self, x, expert=None, weight=None, allowed=None):
+        """x [n, channels] through its experts.  ``expert`` (int64 [n] or [n, k]) and ``weight`` (fp32, default ones) replace
+        the router's choice; -1 sends a row nowhere (zeros, if it has no other)."""
+        be = hiscache_backend
+        if expert is None:
+            expert, weight = self.route(x, allowed)
+        order = be.expert_order(expert, self.num_expert)
+        y = be.gated_experts(be.rows_to_experts(x, order), self.w_in, self.w_out, order.offset, self.group)
+        return be.rows_from_experts(y, order, weight)
+
+    def extra_repr(self):
+        return (f"{self.channels}, hidden={self.hidden}, num_expert={self.num_expert}, top_k={self.top_k}, "
+                f"normalize={self.normalize}, group={self.group}")
+
+
+def packed_activations(group=64, min_elements=1 << 16):
+    """Context in which what autograd saves for backward is kept in 8 bits, a scale for every ``group`` columns
+    (``hiscache_backend.pack_rows``): the gradients are those at activations that are off by up to half a scale.
+
+    Kept as they are: parameters and other leaves that need a gradient, whole numbers, tensors of fewer than ``min_elements``
+    values or without a last dimension of their own, and anything not packed in the current GPU's memory.  Put it around the
+    layers whose activations may be rounded; a loss, a softmax or the router's weights are better left outside."""
+    be = hiscache_backend
+
+    def pack(t):
+        if (not t.is_cuda or t.dtype not in be._DTYPES or t.dim() < 2 or t.numel() < min_elements or not t.is_contiguous()
+                or (t.is_leaf and t.requires_grad) or t.device.index != torch.cuda.current_device()):
+            return t
+        return be.pack_rows(t.detach().view(-1, t.shape[-1]), group), t.shape
+
+    def unpack(kept):
+        return kept if isinstance(kept, torch.Tensor) else be.unpack_rows(kept[0]).view(kept[1])
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)

@@ -1,0 +1,131 @@
+"""The argument checks of the expert layer's entry points and of the Python calls in front of them (no kernel is launched here)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+OK, EINVAL, EDTYPE, EWORKSPACE, EUNSUPPORTED = 0, 1, 2, 4, 5
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import hiscache_backend as be
+    return be.load_library()
+
+
+@pytest.fixture(scope="module")
+def p():
+    buf = np.zeros(1 << 10, np.int64)
+    p = ctypes.c_void_p(buf.ctypes.data)
+    p.keep = buf
+    return p
+
+
+def test_route(lib, p):
+    assert lib.hc_route_rows(p, 0, -1, 8, 2, 1, p, p, None) == EINVAL
+    assert lib.hc_route_rows(p, 0, 4, 0, 1, 1, p, p, None) == EINVAL
+    assert lib.hc_route_rows(p, 0, 4, 8, 9, 1, p, p, None) == EINVAL
+    assert lib.hc_route_rows(p, 0, 4, 8, 0, 1, p, p, None) == EINVAL
+    assert lib.hc_route_rows(p, 0, 4, 1025, 2, 1, p, p, None) == EUNSUPPORTED
+    assert lib.hc_route_rows(p, 0, 4, 64, 33, 1, p, p, None) == EUNSUPPORTED
+    assert lib.hc_route_rows(p, 7, 4, 8, 2, 1, p, p, None) == EDTYPE
+    assert lib.hc_route_rows(None, 0, 4, 8, 2, 1, p, p, None) == EINVAL
+    assert lib.hc_route_rows(p, 0, 1 << 40, 8, 2, 1, p, p, None) == EUNSUPPORTED
+    assert lib.hc_route_rows(None, 0, 0, 8, 2, 1, None, None, None) == OK
+    assert lib.hc_route_rows(None, 9, 0, 8, 2, 1, None, None, None) == EDTYPE
+    assert lib.hc_route_rows_grad(None, 0, 4, 8, 2, 0, p, p, p, p, None) == EINVAL          # logits are needed unless normalised
+    assert lib.hc_route_rows_grad(p, 0, 4, 8, 2, 1, p, p, None, p, None) == EINVAL
+    assert lib.hc_route_rows_grad(p, 3, 4, 8, 2, 1, p, p, p, p, None) == EDTYPE
+    assert lib.hc_route_rows_grad(None, 0, 0, 8, 2, 1, None, None, None, None, None) == OK
+
+
+def test_order(lib, p):
+    assert lib.hc_expert_order(p, -1, 4, p, p, p, None, 0, None) == EINVAL
+    assert lib.hc_expert_order(p, 8, 0, p, p, p, None, 0, None) == EINVAL
+    assert lib.hc_expert_order(None, 8, 4, p, p, p, None, 0, None) == EINVAL
+    assert lib.hc_expert_order(p, 8, 4, p, p, None, None, 0, None) == EINVAL
+    assert lib.hc_expert_order(p, 8, 1025, p, p, p, None, 0, None) == EUNSUPPORTED
+    assert lib.hc_expert_order(p, 1 << 31, 4, p, p, p, None, 0, None) == EUNSUPPORTED
+    assert lib.hc_expert_order_workspace_bytes(8192, 1024) == 0 and lib.hc_expert_order_workspace_bytes(-1, 4) == 0
+    need = lib.hc_expert_order_workspace_bytes(1_000_000, 64)
+    assert need >= 65 * 4 * (1_000_000 // 1024) and lib.hc_expert_order_workspace_bytes((1 << 31) - 1, 1024) < 32 << 20
+    assert lib.hc_expert_order(p, 1_000_000, 64, p, p, p, None, 0, None) == EWORKSPACE
+    assert lib.hc_expert_order(p, 1_000_000, 64, p, p, p, p, need - 1, None) == EWORKSPACE
+
+
+def test_rows(lib, p):
+    for call in (lambda **k: lib.hc_rows_to_experts(k["x"], k["dt"], k["n"], k["k"], k["E"], k["D"], p, k["off"], p, None),
+                 lambda **k: lib.hc_rows_from_experts_grad(p, k["x"], k["dt"], k["n"], k["k"], k["E"], k["D"], p, k["off"], p, p, p, None)):
+        good = dict(x=p, dt=0, n=4, k=2, E=3, D=8, off=p)
+        for bad, code in ((dict(n=-1), EINVAL), (dict(k=0), EINVAL), (dict(E=0), EINVAL), (dict(D=0), EINVAL), (dict(x=None), EINVAL),
+                          (dict(off=None), EINVAL), (dict(dt=5), EDTYPE), (dict(n=1 << 31), EUNSUPPORTED), (dict(E=2000), EUNSUPPORTED),
+                          (dict(D=1 << 30), EUNSUPPORTED)):
+            assert call(**{**good, **bad}) == code, bad
+        assert call(**{**good, "n": 0, "x": None, "off": None}) == OK
+    assert lib.hc_rows_from_experts(None, 0, 4, 2, 3, 8, p, None, p, None) == EINVAL
+    assert lib.hc_rows_from_experts(p, 4, 4, 2, 3, 8, p, None, p, None) == EDTYPE
+    assert lib.hc_rows_from_experts(None, 1, 0, 2, 3, 8, None, None, None, None) == OK
+
+
+def test_products(lib, p):
+    assert lib.hc_expert_linear(p, 0, p, 0, p, -1, 2, 4, 4, p, None) == EINVAL
+    assert lib.hc_expert_linear(p, 0, p, 0, p, 4, 0, 4, 4, p, None) == EINVAL
+    assert lib.hc_expert_linear(p, 0, p, 0, None, 4, 2, 4, 4, p, None) == EINVAL
+    assert lib.hc_expert_linear(p, 3, p, 0, p, 4, 2, 4, 4, p, None) == EDTYPE
+    assert lib.hc_expert_linear(p, 0, p, 0, p, 4, 1025, 4, 4, p, None) == EUNSUPPORTED
+    assert lib.hc_expert_linear(p, 0, p, 0, p, 4, 2, (1 << 20) + 1, 4, p, None) == EUNSUPPORTED
+    assert lib.hc_expert_linear(p, 0, p, 0, p, 4, 2, 1 << 20, 1 << 20, p, None) == EUNSUPPORTED
+    assert lib.hc_expert_linear(p, 0, p, 0, p, (1 << 31) - 1, 2, 4, 4, p, None) == EUNSUPPORTED
+    assert lib.hc_expert_linear(None, 0, None, 0, None, 0, 2, 4, 4, None, None) == OK
+    need = lib.hc_expert_linear_grad_workspace_bytes(60_000, 5, 256, 256, 0)
+    assert need > 0 and lib.hc_expert_linear_grad_workspace_bytes(100, 5, 256, 256, 0) == 0
+    assert lib.hc_expert_linear_grad_workspace_bytes(60_000, 5, 256, 256, 9) == 0
+    assert lib.hc_expert_linear_grad(p, p, 0, p, 60_000, 5, 256, 256, p, None, 0, None) == EWORKSPACE
+    assert lib.hc_expert_linear_grad(p, p, 0, p, 60_000, 5, 256, 256, p, p, need - 1, None) == EWORKSPACE
+    assert lib.hc_expert_linear_grad(p, None, 0, p, 4, 5, 4, 4, p, None, 0, None) == EINVAL
+    assert lib.hc_expert_linear_grad(p, p, 8, p, 4, 5, 4, 4, p, None, 0, None) == EDTYPE
+
+
+def test_the_parts_of_a_gradient_fit_the_workspace(lib):
+    # experts of p > 1 parts hold fewer parts than twice the rows over a part's rows
+    for S in (513, 4096, 100_000, 5_000_000):
+        for N, K in ((64, 64), (300, 172), (2048, 1024)):
+            for dtype in (0, 1, 2):
+                need = lib.hc_expert_linear_grad_workspace_bytes(S, 16, N, K, dtype)
+                assert need % (N * K * 4) == 0 and need // (N * K * 4) <= 2 * (S // 512)
+
+
+def test_packed(lib, p):
+    assert lib.hc_pack_rows(p, 0, -1, 8, 64, p, p, None) == EINVAL
+    assert lib.hc_pack_rows(p, 0, 4, 0, 64, p, p, None) == EINVAL
+    assert lib.hc_pack_rows(p, 0, 4, 8, 48, p, p, None) == EUNSUPPORTED
+    assert lib.hc_pack_rows(p, 0, 1 << 40, 64, 64, p, p, None) == EUNSUPPORTED
+    assert lib.hc_pack_rows(p, 6, 4, 8, 64, p, p, None) == EDTYPE
+    assert lib.hc_pack_rows(None, 0, 4, 8, 64, p, p, None) == EINVAL
+    assert lib.hc_unpack_rows(p, None, 4, 8, 64, p, 0, None) == EINVAL
+    assert lib.hc_gated_pack(p, 0, 4, 8, 64, p, p, None, None) == EINVAL
+    assert lib.hc_gated_grad(p, p, p, 0, 4, 8, 64, None, p, None) == EINVAL
+    assert lib.hc_pack_rows(None, 0, 0, 8, 64, None, None, None) == OK
+    assert lib.hc_gated_grad(None, None, None, 2, 0, 8, 32, None, None, None) == OK
+
+
+def test_the_module_checks_its_arguments_without_a_gpu():
+    import hiscache
+    import hiscache_backend as be
+    layer = hiscache.ExpertMLP(8, 16, 4, 2)
+    assert {k: tuple(v.shape) for k, v in layer.state_dict().items()} == {"router": (4, 8), "w_in": (4, 32, 8), "w_out": (4, 8, 16)}
+    assert "num_expert=4" in repr(layer)
+    for bad in (0, 5):
+        with pytest.raises(ValueError):
+            hiscache.ExpertMLP(8, 16, 4, bad)
+    with pytest.raises(RuntimeError):                              # there is no path on the CPU
+        layer(torch.zeros(3, 8))
+    with pytest.raises(RuntimeError):
+        be.pack_rows(torch.zeros(3, 8))
+    # tensors on the CPU pass through the hooks as they are
+    with hiscache.packed_activations(min_elements=1):
+        x = torch.randn(5, 6, requires_grad=True)
+        y = (x * x).sum()
+    y.backward()
+    assert torch.equal(x.grad, 2 * x)
