@@ -18,10 +18,9 @@ static bool el_sizes_ok(int64_t S, int64_t E, int64_t N, int64_t K) {
 
 static bool el_dtype_ok(int dtype) { return dtype == HC_F32 || dtype == HC_F16 || dtype == HC_BF16; }
 
-// The result is stored in pieces of 16 bytes where its rows start on them.
+// The result is stored in pieces of 16 bytes where its rows start on 4.
 static bool el_whole(const void *out, int64_t cols, int dtype) {
-  const int64_t size = dtype == HC_F32 ? 4 : 2;
-  return cols * size % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  return cols * (dtype == HC_F32 ? 4 : 2) % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0;
 }
 
 }  // namespace

@@ -16,6 +16,7 @@ typedef float el_four __attribute__((ext_vector_type(4)));
 typedef short el_eight __attribute__((ext_vector_type(8)));
 typedef short el_quad __attribute__((ext_vector_type(4)));
 typedef uint32_t el_piece __attribute__((ext_vector_type(4)));
+typedef uint32_t el_words __attribute__((ext_vector_type(4), aligned(4)));      // 16 bytes that start on 4
 
 constexpr uint32_t EL_NOWHERE = 0xfffffff0u;    // behind every buffer: reads as zero
 #define EL_LDS __attribute__((address_space(3)))
@@ -290,8 +291,8 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
       const int orow = wp + i * 32 + row, ocol = wq + c;
       if (orow < rows_out && ocol < cols_out) {
         T *o = out + (int64_t)orow * a.cols + ocol;
-        if (a.whole) {
-          *reinterpret_cast<el_piece *>(o) = *reinterpret_cast<const el_piece *>(own + row * ROW + c);
+        if (a.whole && ocol + PER <= cols_out) {
+          *reinterpret_cast<el_words *>(o) = *reinterpret_cast<const el_piece *>(own + row * ROW + c);
         } else {
 #pragma unroll
           for (int x = 0; x < PER; ++x)

@@ -1599,8 +1599,8 @@ def bias_bn_relu_eval(x, bias, gamma, beta, running_mean, running_var, eps):
 # ----------------------------------------------------------------------------- rows and their experts
 def _together(t, *others):
     """Do these tensors lie on one device, the current one (whose stream the launch goes to)?"""
-    index = t.device.index
-    if index != torch.cuda.current_device() or any(o is not None and o.device.index != index for o in others):
+    index = t.get_device()
+    if index != torch.cuda.current_device() or any(o.get_device() != index for o in others):
         raise ValueError("the tensors must lie on one device, and it must be the current one")
 
 
@@ -1609,14 +1609,25 @@ def _arriving(g):
     return g.contiguous().resolve_neg()
 
 
+# The operators below are autograd nodes where a gradient may be asked for; without one the node itself, which costs the
+# host more than the launch, is left out.
+def _watched(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _route(logits, top_k, normalize):
+    n, E = logits.shape
+    expert = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
+    weight = torch.empty((n, top_k), dtype=torch.float32, device=logits.device)
+    _check(load_library().hc_route_rows(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
+                                        expert.data_ptr(), weight.data_ptr(), _stream()), "hc_route_rows")
+    return expert, weight
+
+
 class _RouteRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, normalize):
-        n, E = logits.shape
-        expert = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
-        weight = torch.empty((n, top_k), dtype=torch.float32, device=logits.device)
-        _check(load_library().hc_route_rows(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
-                                            expert.data_ptr(), weight.data_ptr(), _stream()), "hc_route_rows")
+        expert, weight = _route(logits, top_k, normalize)
         ctx.mark_non_differentiable(expert)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, expert, weight)
@@ -1653,7 +1664,7 @@ def route_rows(logits, top_k, normalize=True):
     if not 1 <= top_k <= logits.shape[1]:
         raise ValueError(f"top_k must be between 1 and the {logits.shape[1]} experts, got {top_k}")
     _together(logits)
-    return _RouteRows.apply(logits, top_k, int(bool(normalize)))
+    return (_RouteRows.apply if _watched(logits) else _route)(logits, top_k, int(bool(normalize)))
 
 
 class ExpertOrder:
@@ -1764,7 +1775,7 @@ def rows_to_experts(x, order):
     """The rows of x [n, D] in expert order, [n * top_k, D]: place p holds row ``order.pair[p] // top_k``, zeros where there is
     no pair.  The gradient of a row is the sum over its places."""
     _expert_rows(x, "x", order, False)
-    return _RowsToExperts.apply(x, order)
+    return (_RowsToExperts.apply if _watched(x) else _to_experts)(x, order)
 
 
 def rows_from_experts(y, order, weight=None):
@@ -1777,7 +1788,7 @@ def rows_from_experts(y, order, weight=None):
         if weight.numel() != order.places:
             raise ValueError(f"weight must hold {order.places} values")
         _together(y, weight)
-    return _RowsFromExperts.apply(y, order, weight)
+    return (_RowsFromExperts.apply if _watched(y, weight) else _from_experts)(y, order, weight)
 
 
 class _ExpertLinear(torch.autograd.Function):
@@ -1823,7 +1834,7 @@ def expert_linear(x, w, offset):
         raise ValueError(f"x [S, K], w [E, N, K] and offset [E + 1] do not fit: {tuple(x.shape)}, {tuple(w.shape)}, "
                          f"{tuple(offset.shape)}")
     _together(x, w, offset)
-    return _ExpertLinear.apply(x, w, offset)
+    return _ExpertLinear.apply(x, w, offset) if _watched(x, w) else _expert_product(x, w, offset, False)
 
 
 def expert_linear_grad(g, x, offset):
@@ -1930,12 +1941,9 @@ def gated_grad(kept, g):
 class _GatedExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w_in, w_out, offset, group):
-        # nothing is kept where no backward pass can come
-        keep = any(ctx.needs_input_grad)
-        h, kept = gated_pack(_expert_product(rows, w_in, offset, False), group, keep=keep)
-        if keep:
-            ctx.save_for_backward(rows, w_in, w_out, offset, kept.codes, kept.scale)
-            ctx.hc = (group, rows.dtype)
+        h, kept = gated_pack(_expert_product(rows, w_in, offset, False), group)
+        ctx.save_for_backward(rows, w_in, w_out, offset, kept.codes, kept.scale)
+        ctx.hc = (group, rows.dtype)
         return _expert_product(h, w_out, offset, False)
 
     @staticmethod
@@ -1965,7 +1973,9 @@ def gated_experts(rows, w_in, w_out, offset, group=64):
         raise ValueError(f"rows [S, C], w_in [E, 2 H, C], w_out [E, D, H] and offset [E + 1] do not fit: {tuple(rows.shape)}, "
                          f"{tuple(w_in.shape)}, {tuple(w_out.shape)}, {tuple(offset.shape)}")
     _together(rows, w_in, w_out, offset)
-    return _GatedExperts.apply(rows, w_in, w_out, offset, group)
+    if _watched(rows, w_in, w_out):
+        return _GatedExperts.apply(rows, w_in, w_out, offset, group)
+    return _expert_product(gated_pack(_expert_product(rows, w_in, offset, False), group, keep=False)[0], w_out, offset, False)
 
 
 def evict(checkin, slot2full, full2slot, stale_iter, sub2slot=None, score=None, thres=None):
