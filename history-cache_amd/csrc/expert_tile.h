@@ -18,7 +18,7 @@ typedef short el_quad __attribute__((ext_vector_type(4)));
 typedef uint32_t el_piece __attribute__((ext_vector_type(4)));
 typedef uint32_t el_words __attribute__((ext_vector_type(4), aligned(4)));      // 16 bytes that start on 4
 
-constexpr uint32_t EL_NOWHERE = 0xfffffff0u;    // behind every buffer: reads as zero
+constexpr uint32_t EL_NOWHERE = 0xffffff00u;    // behind every buffer, as are the bytes that follow it: reads as zero
 #define EL_LDS __attribute__((address_space(3)))
 
 // 16 bytes of the inner index for 32 rows by each half of the wave; both operands go by the same order, so that which of the
@@ -52,15 +52,17 @@ struct el_type<float> {
 //               read by columns
 // Chunk c of row r lies at c ^ turn(r), so that the lanes that are served at a time find their values in different banks.
 // DIRECT: chunks go straight into LDS, for operands whose rows start on 4 bytes; a step that ends inside a row goes there by
-// words.  Else (16 bits, an odd width or address) elements pass through registers one by one.
+// words.  Else (16 bits, an odd width or address) the five words that hold a chunk's eight elements pass through registers, in
+// which they are moved into place; of the words only the tensor's first and last can hold two bytes that are not its own.
 template <typename T, int W, int ROWB, bool TR, int THREADS, bool DIRECT>
 struct el_operand {
   static constexpr int PER = 16 / (int)sizeof(T), INNER = ROWB / (int)sizeof(T);
   static constexpr int CHUNKS = W * ROWB / 16, EACH = CHUNKS / THREADS;
   static_assert(CHUNKS % THREADS == 0, "whole chunks per thread");
-  uint32_t at[EACH];        // byte offset of this thread's chunks in the operand's first piece
+  uint32_t at[EACH];        // byte offset of this thread's chunks in the operand's first piece (not DIRECT: of their first words)
   int first[EACH];          // first inner index (TR = false) or column of each
   el_piece held[DIRECT ? 1 : EACH];
+  uint32_t last[DIRECT ? 1 : EACH], shift[DIRECT ? 1 : EACH];           // the fifth words; bytes in front of the first element
   uint32_t stride;          // of the operand's rows in elements
   int wide;                 // rows (TR = false) or columns (TR = true) that exist from the tile's first on
 
@@ -69,7 +71,7 @@ struct el_operand {
     if constexpr (TR) return sizeof(T) == 2 ? (r & 3) * 2 + ((r >> 3) & 1) : (r >> 2) & 1;
     else return ROWB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
-  __device__ __forceinline__ void init(int t, uint32_t stride_, int wide_) {
+  __device__ __forceinline__ void init(int t, uint32_t stride_, int wide_, uint32_t skip) {
     stride = stride_;
     wide = wide_;
 #pragma unroll
@@ -84,7 +86,12 @@ struct el_operand {
         c = q % (W / PER) ^ turn(r) * (sizeof(T) == 2 ? 2 : 8);
       }
       first[i] = c * PER;
-      at[i] = (TR ? first[i] : r) < wide ? ((uint32_t)r * stride + (uint32_t)first[i]) * (uint32_t)sizeof(T) : EL_NOWHERE;
+      at[i] = ((uint32_t)r * stride + (uint32_t)first[i]) * (uint32_t)sizeof(T);
+      if constexpr (!DIRECT) {
+        shift[i] = (at[i] + skip) & 2;
+        at[i] = (at[i] + skip) & ~3u;
+      }
+      if ((TR ? first[i] : r) >= wide) at[i] = EL_NOWHERE;
     }
   }
   // left: inner indices from the piece's first on.  Columns behind the last one may hold what lies there (they are not part of
@@ -107,21 +114,26 @@ struct el_operand {
         }
       }
     } else {
-      const int end = TR ? wide : left;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i)
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const uint32_t o = first[i] + p < end && at[i] != EL_NOWHERE ? at[i] + 2u * p : EL_NOWHERE;
-          const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(b, o, 0, 0);
-          held[i][p / 2] = p % 2 == 0 ? v : held[i][p / 2] | v << 16;
-        }
+      for (int i = 0; i < EACH; ++i) {
+        const uint32_t o = (TR ? (i * THREADS + t) / (W / PER) : first[i]) < left ? at[i] : EL_NOWHERE;
+        held[i] = __builtin_amdgcn_raw_buffer_load_b128(b, o, 0, 0);
+        last[i] = __builtin_amdgcn_raw_buffer_load_b32(b, o + 16, 0, 0);
+      }
     }
   }
-  __device__ __forceinline__ void put(EL_LDS char *lds, int t) const {
+  __device__ __forceinline__ void put(EL_LDS char *lds, int t, int left) const {
     if constexpr (!DIRECT)
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) *(EL_LDS el_piece *)(lds + (i * THREADS + t) * 16) = held[i];
+      for (int i = 0; i < EACH; ++i) {
+        el_piece v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          v[x] = __builtin_amdgcn_alignbyte(x < 3 ? held[i][x < 3 ? x + 1 : 3] : last[i], held[i][x], shift[i]);
+          if (!TR) v[x] &= left >= first[i] + 2 * x + 2 ? ~0u : left > first[i] + 2 * x ? 0xffffu : 0u;
+        }
+        *(EL_LDS el_piece *)(lds + (i * THREADS + t) * 16) = v;
+      }
   }
   // The fragment of 32 rows (columns) from `from` on in the k-th quarter of the piece: lane l has row from + l % 32 and of the
   // quarter's 32 bytes of inner index the half l / 32.
@@ -201,17 +213,20 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
                 (GRAD ? part.lo * a.cols + q0 : e * a.inner * a.cols + (KN ? (int64_t)q0 : (int64_t)q0 * a.inner));
   op_p fp;
   op_q fq;
-  fp.init(t, ld_p, rows_out);
-  fq.init(t, ld_q, cols_out);
-  // the operands from inner index k0 on; with the inner index outside a buffer ends with the last row that exists
-  const auto buffer = [&](const T *p, bool outside, uint32_t ld, int wide, int k0) {
+  // bytes of a word that lie in front of the operands' first elements; every piece begins as many bytes into one
+  const uint32_t skip_p = DIRECT ? 0u : reinterpret_cast<uintptr_t>(pp) & 3, skip_q = DIRECT ? 0u : reinterpret_cast<uintptr_t>(pq) & 3;
+  fp.init(t, ld_p, rows_out, skip_p);
+  fq.init(t, ld_q, cols_out, skip_q);
+  // the operands from inner index k0 on, up to their last element (not DIRECT: in whole words)
+  const auto buffer = [&](const T *p, bool outside, uint32_t ld, int wide, int k0, uint32_t skip) {
     const int left = inner - k0, n = left < BK ? left : BK;
-    return hc_make_buffer(outside ? p + (int64_t)k0 * ld : p + k0,
-                          left < 1 ? 0u : outside ? ((uint32_t)(n - 1) * ld + (uint32_t)wide) * SIZE : 0xffffff00u);
+    const uint32_t bytes = left < 1 ? 0u : (outside ? (uint32_t)(n - 1) * ld + (uint32_t)wide : (uint32_t)(wide - 1) * ld + (uint32_t)left) * SIZE;
+    return hc_make_buffer(reinterpret_cast<const char *>(outside ? p + (int64_t)k0 * ld : p + k0) - skip,
+                          DIRECT ? bytes : (bytes + skip + 3) & ~3u);
   };
   const auto fetch = [&](int s, int k0) {
-    fp.fetch(buffer(pp, PT, ld_p, rows_out, k0), lds + s * STAGE, t, wave, inner - k0);
-    fq.fetch(buffer(pq, QT, ld_q, cols_out, k0), lds + s * STAGE + BYTES_P, t, wave, inner - k0);
+    fp.fetch(buffer(pp, PT, ld_p, rows_out, k0, skip_p), lds + s * STAGE, t, wave, inner - k0);
+    fq.fetch(buffer(pq, QT, ld_q, cols_out, k0, skip_q), lds + s * STAGE + BYTES_P, t, wave, inner - k0);
   };
   el_acc acc[TP][TQ];
 #pragma unroll
@@ -221,16 +236,16 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   const auto step = [&](int from, int to, int k0, bool more) {
-    el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq, buffer(pp, PT, ld_p, rows_out, k0),
-                                                       buffer(pq, QT, ld_q, cols_out, k0), more, inner - k0, t, wave, wp, wq, acc);
+    el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq, buffer(pp, PT, ld_p, rows_out, k0, skip_p),
+                                                       buffer(pq, QT, ld_q, cols_out, k0, skip_q), more, inner - k0, t, wave, wp, wq, acc);
   };
-  const auto put = [&](int s) {
-    fp.put(lds + s * STAGE, t);
-    fq.put(lds + s * STAGE + BYTES_P, t);
+  const auto put = [&](int s, int k0) {
+    fp.put(lds + s * STAGE, t, inner - k0);
+    fq.put(lds + s * STAGE + BYTES_P, t, inner - k0);
   };
   if (inner > 0) {
     fetch(0, 0);
-    put(0);
+    put(0, 0);
   }
   int s = 0;
   for (int k0 = 0; k0 < inner; k0 += BK) {
@@ -240,7 +255,7 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
     const bool more = k0 + BK < inner;
     step(s, s ^ 1, k0 + BK, more);
     s ^= 1;
-    if (more) put(s);
+    if (more) put(s, k0 + BK);
   }
   // lane l has row l % 32 of a tile of 32 x 32 and of every eight columns the four from 4 (l / 32) on
   const int l32 = lane & 31, h = lane >> 5;

@@ -3,6 +3,8 @@ over, every type, widths and addresses off the wide loads.
 
 A sum of K products in fp32 is off by at most K units of 2^-23 of the sum of the magnitudes, whatever the order (the matrix
 instructions may cut off where they add, hence a whole unit); a narrow result by half a unit of its type besides."""
+import math
+
 import pytest
 import torch
 
@@ -101,6 +103,28 @@ def test_what_one_group_holds_does_not_reach_another(dtype):
     assert bool((rest == 64).all()) and not y[280:].any()
     assert bool((torch.cat([gx[:100], gx[150:280]]) == 64).all()) and not gx[280:].any()
     assert bool((gw[0] == 100).all()) and bool((gw[2] == 130).all()) and bool(torch.isnan(gw[1]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,K,first", ((47, 47, 101), (33, 64, 101), (64, 33, 100), (1, 1, 7), (129, 65, 33)))
+def test_what_one_group_holds_does_not_reach_another_at_odd_widths(dtype, N, K, first):
+    """Where rows of 16-bit elements share a word with their neighbours, in tensors whose neighbours in memory are not finite."""
+    def inside(*shape):
+        whole = torch.full((math.prod(shape) + 66,), float("nan"), device=DEV, dtype=dtype)
+        return whole[33:-33].view(shape).fill_(1)
+
+    x, w, g = inside(300, K), inside(3, N, K), inside(300, N)
+    offset, second = offsets((first, 50, 150 - first % 2)), first + 50
+    end = int(offset[-1])
+    x[first:second] = w[1] = float("nan")
+    g[first:second] = x[end:] = float("inf")
+    g[end:] = float("nan")
+    a, b = x.requires_grad_(True), w.requires_grad_(True)
+    y = be.expert_linear(a, b, offset)
+    gx, gw = torch.autograd.grad(y, (a, b), g)
+    for rows, n in ((y, K), (gx, N)):
+        assert bool((torch.cat([rows[:first], rows[second:end]]) == n).all()) and not rows[end:].any()
+    assert bool((gw[0] == first).all()) and bool((gw[2] == end - second).all())
 
 
 @pytest.mark.parametrize("dtype", TYPES)
