@@ -196,13 +196,18 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   constexpr int OUT = WP * WQ * 32 * (TQ * 32 + PER) * (int)sizeof(T), MEM = 2 * STAGE > OUT ? 2 * STAGE : OUT;
   __shared__ __attribute__((aligned(16))) char s_mem[MEM];
   EL_LDS char *lds = (EL_LDS char *)s_mem;
-  const int64_t b = hc_xcd_block<GRAD ? 4 : 8>(blockIdx.x, gridDim.x);
+  const int64_t b = hc_xcd_block<!GRAD ? 8 : sizeof(T) == 2 ? 16 : 4>(blockIdx.x, gridDim.x);
   const int t = (int)threadIdx.x, lane = hc_lane(), wave = hc_wave_in_block();
   const int wp = wave % WP * (BP / WP), wq = wave / WP * (BQ / WQ);
-  const int per = GRAD ? a.tiles_p * a.tiles_q : a.tiles_q, in = (int)(b % per);
-  const ElPart part = GRAD ? el_find_part(a.offset, a.E, a.S, a.slab, (int)(b / per)) : el_find_rows(a.offset, a.E, a.S, BP, (int)(b / per));
+  const uint32_t per = (uint32_t)(GRAD ? a.tiles_p * a.tiles_q : a.tiles_q), which = (uint32_t)b / per, in = (uint32_t)b % per;
+  const ElPart part = GRAD ? el_find_part(a.offset, a.E, a.S, a.slab, (int)which) : el_find_rows(a.offset, a.E, a.S, BP, (int)which);
   if (part.expert > a.E) return;
-  const int q0 = in % a.tiles_q * BQ, p0 = GRAD ? in / a.tiles_q * BP : 0;
+  // a part's tiles go by strips of four along P, column by column: sixteen that follow one another take from four rows of tiles
+  // and four columns
+  constexpr uint32_t HIGH = !GRAD ? 1 : sizeof(T) == 2 ? 4 : 2;
+  const uint32_t strip = HIGH * (uint32_t)a.tiles_q, top = in / strip * HIGH;
+  const uint32_t high = !GRAD ? 1 : (uint32_t)a.tiles_p - top < HIGH ? (uint32_t)a.tiles_p - top : HIGH;
+  const int q0 = (int)(in % strip / high) * BQ, p0 = GRAD ? (int)(top + in % strip % high) * BP : 0;
   const int64_t e = part.expert < a.E ? part.expert : 0;
   const int batch = (int)(part.hi - part.lo);                           // rows of the batch
   const int rows_out = GRAD ? (a.rows - p0 < BP ? a.rows - p0 : BP) : batch, cols_out = a.cols - q0 < BQ ? a.cols - q0 : BQ;
