@@ -68,7 +68,8 @@ struct el_operand {
 
   // what is added, bit by bit, to the numbers of a row's chunks (TR: of its 32 bytes, of its 128 bytes where T is fp32)
   __device__ __forceinline__ static int turn(int r) {
-    if constexpr (TR) return sizeof(T) == 2 ? (r & 3) * 2 + ((r >> 3) & 1) : (r >> 2) & 1;
+    // (a row of 64 columns has four such pieces and takes half of the banks, those of wider tiles have eight and take them all)
+    if constexpr (TR) return sizeof(T) == 4 ? (r >> 2) & 1 : W == 64 ? r & 2 : (r & 3) * 2 + ((r >> 3) & 1);
     else return ROWB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
   __device__ __forceinline__ void init(int t, uint32_t stride_, int wide_, uint32_t skip) {
@@ -406,28 +407,54 @@ static bool el_direct(const void *p, const void *q, int64_t w0, int64_t w1, int 
 #define EL_LARGE 256, 256, 2, 4, 128
 #define EL_SMALL 128, 128, 2, 2, 128
 #define EL_SHORT 128, 128, 2, 2, 64
+#define EL_TINY 64, 64, 2, 2, 128
+#define EL_TINY_GRAD 64, 64, 2, 2, 64
 
 constexpr int EL_SHORT_INNER = 512;               // longest inner size that goes in pieces of 64 bytes where both would do
+// 128-wide tiles of half precision up to which tiles of 64 x 64 are taken: no unit would have two (us, small / tiny: 1 000 rows, 8
+// experts, 768 x 768: 10.4 / 7.7; 3 000, 16, 512 x 512: 10 / 7; 10 000, 1, 256 x 602 (158): 11.4 / 10.5; 602 x 256 (395): 10.8 / 11.5)
+constexpr int64_t EL_TINY_ROWS = 256;
 constexpr int64_t EL_SHORT_GROUP = 640;           // rows of an expert, on average, up to which its gradient does
 constexpr int64_t EL_LARGE_GRAD = 256 * 5120;     // rows of the batch that a unit would take through a large tile
+// The same of a small tile in fp32, below which its gradient goes by tiny ones (us, small / tiny: 500 rows, 4 experts, 256 x 256:
+// 18 / 13; 20 000, 7, 300 x 172: 47 / 36; 40 000, 1, 256 x 602: 123 / 123; 30 000, 4, 768 x 768: 274 / 289)
+constexpr int64_t EL_SMALL_GRAD_F32 = 256 * 2048;
 
 // Is the product of S rows in E groups by `cols` columns done sooner in large tiles?  Rounds over the 256 compute units, the
 // groups' last tiles half empty; a small tile, two at a time on a unit, takes EL_SMALL_COST of a large one's time and a
 // quarter of its work.
 constexpr float EL_SMALL_COST = 0.575f;
+static int64_t el_tiles_of_rows(int64_t S, int64_t E, int64_t cols, int64_t tile) {
+  return ((S + tile - 1) / tile + E / 2) * ((cols + tile - 1) / tile);
+}
 static bool el_large_rows(int64_t S, int64_t E, int64_t cols) {
-  const int64_t large = ((S + 255) / 256 + E / 2) * ((cols + 255) / 256), small = ((S + 127) / 128 + E / 2) * ((cols + 127) / 128);
+  const int64_t large = el_tiles_of_rows(S, E, cols, 256), small = el_tiles_of_rows(S, E, cols, 128);
   return (float)((large + 255) / 256) <= EL_SMALL_COST * (float)((small + 511) / 512);
+}
+
+// The same for fp32, tiles of 128 x 128 and of 64 x 64.  Matrix instructions of fp32 fill a unit with one tile of either kind, so
+// that what counts is the rounds alone; a tiny tile takes EL_TINY_COST of a small one's time.  (us for the result, small / tiny:
+// 500 rows, 4 experts, 256 x 256: 22 / 9; 9 000, 3, 1 024 x 512: 133 / 91; 20 000, 1, 602 x 256: 86 / 60; 60 007, 5, 256 x 256:
+// 82 / 88; 30 000, 4, 768 x 768: 290 / 304.)
+constexpr float EL_TINY_COST = 0.28f;
+static bool el_small_rows_f32(int64_t S, int64_t E, int64_t cols) {
+  const int64_t small = el_tiles_of_rows(S, E, cols, 128), tiny = el_tiles_of_rows(S, E, cols, 64);
+  return (float)((small + 255) / 256) <= EL_TINY_COST * (float)((tiny + 255) / 256);
 }
 
 template <typename T, bool KN>
 static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
   const int64_t parts = a.S / 128 + a.E + 1;
+  bool tiny;
   if constexpr (sizeof(T) == 2) {
     if (!el_direct(a.p, a.q, a.inner, KN ? a.cols : a.inner, 2)) return el_launch<T, EL_SHORT, false, KN, false>(a, parts, st);
     if (el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, true>(a, a.S / 256 + a.E + 1, st);
-    if (a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, true>(a, parts, st);
+    tiny = el_tiles_of_rows(a.S, a.E, a.cols, 128) <= EL_TINY_ROWS;
+    if (!tiny && a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, true>(a, parts, st);
+  } else {
+    tiny = !el_small_rows_f32(a.S, a.E, a.cols);
   }
+  if (tiny) return el_launch<T, EL_TINY, false, KN, true>(a, a.S / 64 + a.E + 1, st);
   return el_launch<T, EL_SHORT, false, KN, true>(a, parts, st);
 }
 
@@ -445,7 +472,8 @@ static ElGradShape el_grad_shape(int64_t S, int64_t N, int64_t K, int size, bool
   g.large = wide && size == 2 && S * large >= EL_LARGE_GRAD;
   const int64_t parts = g.large ? 256 / large : 512 / small;
   g.slab = (S / (parts < 1 ? 1 : parts) + 64) / 64 * 64;
-  if (g.slab < 512) g.slab = 512;
+  const int64_t least = size == 2 ? 512 : 128;
+  if (g.slab < least) g.slab = least;
   // an expert of p > 1 parts has more than (p - 1) slab >= p / 2 slab rows
   g.several = S <= g.slab ? 0 : 2 * (S / g.slab);
   return g;
@@ -467,7 +495,12 @@ static int el_grad_of_type(ElProduct a, void *workspace, size_t workspace_bytes,
       if (!direct) return el_launch<T, EL_SMALL, true, false, false>(a, parts, st);
       if (g.large) return el_launch<T, EL_LARGE, true, false, true>(a, parts, st);
     }
-    if (a.S <= EL_SHORT_GROUP * a.E) return el_launch<T, EL_SHORT, true, false, true>(a, parts, st);
+    const int64_t small = (int64_t)((a.rows + 127) / 128) * ((a.cols + 127) / 128);
+    if constexpr (sizeof(T) == 4) {
+      if (a.S * small < EL_SMALL_GRAD_F32) return el_launch<T, EL_TINY_GRAD, true, false, true>(a, parts, st);
+    } else {
+      if (a.S <= EL_SHORT_GROUP * a.E) return el_launch<T, EL_SHORT, true, false, true>(a, parts, st);
+    }
     return el_launch<T, EL_SMALL, true, false, true>(a, parts, st);
   };
   const int rc = run();

@@ -69,6 +69,15 @@ def test_larger_products(dtype, sizes, S, N, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,S,N,K", (((9000, 20, 0, 3000, 4000), 16_030, 640, 70), ((9000, 20, 0, 3000, 4000), 16_030, 330, 602),
+                                         ((7000, 33, 7900), 15_000, 1000, 72), ((7000, 33, 7900), 15_000, 90, 998),
+                                         ((30_000, 1, 14_000), 44_010, 1000, 2006)))
+def test_products_of_every_tile(dtype, sizes, S, N, K):
+    """Enough tiles for the wider ones, with widths that end inside a tile and inside a step."""
+    check(sizes, S, N, K, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,K", ((64, 64), (256, 128), (100, 72)))
 def test_operands_off_the_alignment_of_wide_loads(dtype, N, K):
     gen = torch.Generator(device=DEV).manual_seed(N)
