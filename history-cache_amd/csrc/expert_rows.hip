@@ -201,7 +201,48 @@ static OrShape or_shape(int64_t P) {
 }
 
 // ---- rows ------------------------------------------------------------------
-// A row is D elements in pieces of VEC; a thread owns one piece of one row.
+// A row is D elements in pieces of VEC; a thread owns one piece of one row.  ANY: pieces of 16 bytes at the alignment of one
+// element, the last one moved back to the row's end: what it shares with the one before it is computed and stored by both, with
+// the same bits.  Else rows are whole pieces at their own alignment.  (To two experts / back, us, by the pieces that the
+// alignment allows and by ANY: 100 000 rows of 602 bf16 115 / 137 and 71 / 65; 200 000 of 601 379 / 480 and 150 / 134; 100 000 of 602
+// fp32 139 / 206 and 153 / 129.)
+typedef uint32_t mv_words_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t mv_words_4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T, int VEC, bool ANY>
+struct mv_row {
+  typedef typename std::conditional<sizeof(T) == 2, mv_words_2, mv_words_4>::type any_t;
+  typedef typename std::conditional<ANY, any_t, typename hc_vec<T, VEC>::raw_t>::type raw;
+  union U {
+    raw whole;
+    T e[VEC];
+    __device__ U() {}
+  };
+  __device__ __forceinline__ static int column(int piece, int D) {
+    const int c = piece * VEC;
+    return ANY && c > D - VEC ? D - VEC : c;
+  }
+  __device__ __forceinline__ static raw get(const T *p) { return *reinterpret_cast<const raw *>(p); }
+  __device__ __forceinline__ static void set(T *p, raw v) { *reinterpret_cast<raw *>(p) = v; }
+  template <bool NT = false>
+  __device__ __forceinline__ static void load(const T *p, float (&out)[VEC]) {
+    if constexpr (NT && !ANY) {
+      hc_vec<T, VEC>::load_nt(p, out);
+    } else {
+      U u;
+      if constexpr (NT) u.whole = __builtin_nontemporal_load(reinterpret_cast<const raw *>(p));
+      else u.whole = get(p);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[i] = hc_to_f32<T>(u.e[i]);
+    }
+  }
+  __device__ __forceinline__ static void store(T *p, const float (&in)[VEC]) {
+    U u;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u.e[i] = hc_from_f32<T>(in[i]);
+    set(p, u.whole);
+  }
+};
+
 struct MvArgs {
   int64_t n, P;
   int D, k, pieces, E;
@@ -209,38 +250,39 @@ struct MvArgs {
   const int64_t *offset;
 };
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ANY>
 __device__ __forceinline__ void mv_zero_tail(const MvArgs &a, T *__restrict__ rows) {
-  typedef typename hc_vec<T, VEC>::raw_t raw;
+  typedef mv_row<T, VEC, ANY> row;
   const int64_t live = a.offset[a.E], rest = (a.P - live) * a.pieces;
   for (int64_t i = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x; i < rest; i += (int64_t)gridDim.x * HC_BLOCK)
-    *reinterpret_cast<raw *>(rows + (live + i / a.pieces) * a.D + i % a.pieces * VEC) = raw{};
+    row::set(rows + (live + i / a.pieces) * a.D + row::column((int)(i % a.pieces), a.D), typename row::raw{});
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ANY>
 __global__ __launch_bounds__(HC_BLOCK) void mv_to(MvArgs a, const T *__restrict__ x, T *__restrict__ rows) {
-  typedef typename hc_vec<T, VEC>::raw_t raw;
+  typedef mv_row<T, VEC, ANY> row;
   const uint32_t item = blockIdx.x * HC_BLOCK + threadIdx.x;       // (a launch has less than 2^32 threads)
   const int64_t i = item / (uint32_t)a.pieces;
   if (i < a.n) {
-    const int c = (int)(item - (uint32_t)i * (uint32_t)a.pieces) * VEC;
-    const raw v = *reinterpret_cast<const raw *>(x + i * a.D + c);
+    const int c = row::column((int)(item - (uint32_t)i * (uint32_t)a.pieces), a.D);
+    const typename row::raw v = row::get(x + i * a.D + c);
     for (int j = 0; j < a.k; ++j) {
       const int32_t s = a.slot[i * a.k + j];
-      if (s >= 0) *reinterpret_cast<raw *>(rows + (int64_t)s * a.D + c) = v;
+      if (s >= 0) row::set(rows + (int64_t)s * a.D + c, v);
     }
   }
-  mv_zero_tail<T, VEC>(a, rows);
+  mv_zero_tail<T, VEC, ANY>(a, rows);
 }
 
 // K: the choices of a row that are read at a time.
-template <typename T, int VEC, int K>
+template <typename T, int VEC, bool ANY, int K>
 __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restrict__ y, const float *__restrict__ weight,
                                                     T *__restrict__ out) {
+  typedef mv_row<T, VEC, ANY> row;
   const uint32_t item = blockIdx.x * HC_BLOCK + threadIdx.x;       // (a launch has less than 2^32 threads)
   const int64_t i = item / (uint32_t)a.pieces;
   if (i >= a.n) return;
-  const int c = (int)(item - (uint32_t)i * (uint32_t)a.pieces) * VEC;
+  const int c = row::column((int)(item - (uint32_t)i * (uint32_t)a.pieces), a.D);
   float sum[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) sum[v] = 0.f;
@@ -253,9 +295,9 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restric
     for (int j = 0; j < K; ++j) {
       w[j] = weight != nullptr && s[j] >= 0 ? weight[i * a.k + j0 + j] : 1.f;
       if (s[j] >= 0 && weight != nullptr) {
-        hc_vec<T, VEC>::load(y + (int64_t)s[j] * a.D + c, p[j]);
+        row::load(y + (int64_t)s[j] * a.D + c, p[j]);
       } else if (s[j] >= 0) {
-        hc_vec<T, VEC>::load_nt(y + (int64_t)s[j] * a.D + c, p[j]);    // gradients: nothing reads them after this
+        row::template load<true>(y + (int64_t)s[j] * a.D + c, p[j]);    // gradients: nothing reads them after this
       } else {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) p[j][v] = 0.f;
@@ -266,14 +308,15 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restric
 #pragma unroll
       for (int v = 0; v < VEC; ++v) sum[v] = fmaf(w[j], p[j][v], sum[v]);
   }
-  hc_vec<T, VEC>::store(out + i * a.D + c, sum);
+  row::store(out + i * a.D + c, sum);
 }
 
 // L lanes a row; K as above.
-template <typename T, int VEC, int K>
+template <typename T, int VEC, bool ANY, int K>
 __global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__restrict__ g, const T *__restrict__ y,
                                                          const float *__restrict__ weight, T *__restrict__ grad_y,
                                                          float *__restrict__ grad_weight, int L) {
+  typedef mv_row<T, VEC, ANY> row;
   const int lane = (int)threadIdx.x & (L - 1);
   const int64_t i = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
   if (i < a.n) {
@@ -288,20 +331,21 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__re
       }
       for (int p = lane; p < a.pieces; p += L) {
         float gv[VEC], yv[K][VEC];
-        hc_vec<T, VEC>::load(g + i * a.D + p * VEC, gv);
+        const int c = row::column(p, a.D), twice = p * VEC - c;         // elements that the piece before has counted
+        row::load(g + i * a.D + c, gv);
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (s[j] >= 0) hc_vec<T, VEC>::load(y + (int64_t)s[j] * a.D + p * VEC, yv[j]);
+          if (s[j] >= 0) row::load(y + (int64_t)s[j] * a.D + c, yv[j]);
 #pragma unroll
         for (int j = 0; j < K; ++j)
           if (s[j] >= 0) {
             float o[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-              dot[j] = fmaf(gv[v], yv[j][v], dot[j]);
+              dot[j] = !ANY || v >= twice ? fmaf(gv[v], yv[j][v], dot[j]) : dot[j];
               o[v] = w[j] * gv[v];
             }
-            hc_vec<T, VEC>::store(grad_y + (int64_t)s[j] * a.D + p * VEC, o);
+            row::store(grad_y + (int64_t)s[j] * a.D + c, o);
           }
       }
 #pragma unroll
@@ -311,7 +355,7 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__re
       }
     }
   }
-  mv_zero_tail<T, VEC>(a, grad_y);
+  mv_zero_tail<T, VEC, ANY>(a, grad_y);
 }
 
 // As many choices at a time as a row has, up to four.
@@ -334,14 +378,17 @@ static bool mv_args(int64_t n, int64_t top_k, int64_t E, int64_t D, const int32_
   return true;
 }
 
-// Elements of T in a piece: 16 bytes, or as many as the row length and the matrices' alignment allow.
+// Elements of T in a piece, and whether it may lie at any element: 16 bytes, for rows that are shorter as many as their length and
+// the matrices' alignment allow.
 template <typename T, typename F>
 static int mv_with_piece(uintptr_t at, int64_t D, F &&f) {
+  constexpr int MOST = 16 / (int)sizeof(T);
   const uint64_t a = (uint64_t)at | (uint64_t)D * sizeof(T);
-  if (a % 16 == 0) return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
-  if (a % 8 == 0) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{});
-  if (a % 4 == 0) return f(std::integral_constant<int, 4 / (int)sizeof(T)>{});
-  return f(std::integral_constant<int, 1>{});
+  if (a % 16 == 0) return f(std::integral_constant<int, MOST>{}, std::false_type{});
+  if (D >= MOST) return f(std::integral_constant<int, MOST>{}, std::true_type{});
+  if (a % 8 == 0) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{}, std::false_type{});
+  if (a % 4 == 0) return f(std::integral_constant<int, 4 / (int)sizeof(T)>{}, std::false_type{});
+  return f(std::integral_constant<int, 1>{}, std::false_type{});
 }
 
 template <typename F>
@@ -400,12 +447,13 @@ extern "C" int hc_rows_to_experts(const void *x, int dtype, int64_t n, int64_t t
   HC_REQUIRE(x && slot && offset && rows);
   return mv_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
-    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows), D, [&](auto piece) {
+    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows), D, [&](auto piece, auto any) {
       constexpr int VEC = decltype(piece)::value;
-      a.pieces = (int)(D / VEC);
+      constexpr bool ANY = decltype(any)::value;
+      a.pieces = (int)((D + VEC - 1) / VEC);
       const int64_t blocks = (n * a.pieces + HC_BLOCK - 1) / HC_BLOCK;
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
-      mv_to<T, VEC><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+      mv_to<T, VEC, ANY><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
           a, static_cast<const T *>(x), static_cast<T *>(rows));
       return hc_launch_status();
     });
@@ -421,13 +469,14 @@ extern "C" int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t
   HC_REQUIRE(y && slot && out);
   return mv_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
-    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out), D, [&](auto piece) {
+    return mv_with_piece<T>(reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out), D, [&](auto piece, auto any) {
       constexpr int VEC = decltype(piece)::value;
-      a.pieces = (int)(D / VEC);
+      constexpr bool ANY = decltype(any)::value;
+      a.pieces = (int)((D + VEC - 1) / VEC);
       const int64_t blocks = (n * a.pieces + HC_BLOCK - 1) / HC_BLOCK;
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
       return mv_with_choices(top_k, [&](auto choices) {
-        mv_from<T, VEC, decltype(choices)::value><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+        mv_from<T, VEC, ANY, decltype(choices)::value><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
             a, static_cast<const T *>(y), weight, static_cast<T *>(out));
         return hc_launch_status();
       });
@@ -446,15 +495,16 @@ extern "C" int hc_rows_from_experts_grad(const void *g, const void *y, int dtype
   return mv_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
     const uintptr_t at = reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(grad_y);
-    return mv_with_piece<T>(at, D, [&](auto piece) {
+    return mv_with_piece<T>(at, D, [&](auto piece, auto any) {
       constexpr int VEC = decltype(piece)::value;
-      a.pieces = (int)(D / VEC);
+      constexpr bool ANY = decltype(any)::value;
+      a.pieces = (int)((D + VEC - 1) / VEC);
       int L = 1;
       while (L < HC_WAVE && L < a.pieces) L *= 2;
       const int64_t blocks = (n * L + HC_BLOCK - 1) / HC_BLOCK;
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
       return mv_with_choices(top_k, [&](auto choices) {
-        mv_from_grad<T, VEC, decltype(choices)::value>
+        mv_from_grad<T, VEC, ANY, decltype(choices)::value>
             <<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
                 a, static_cast<const T *>(g), static_cast<const T *>(y), weight, static_cast<T *>(grad_y), grad_weight, L);
         return hc_launch_status();
