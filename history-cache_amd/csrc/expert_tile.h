@@ -5,6 +5,11 @@
 //     forward            P: rows of the batch, Q: rows of w[e],    inner: columns of both
 //     gradient of x      P: rows of the batch, Q: columns of w[e], inner: rows of w[e]           (KN)
 //     gradient of w      P: columns of g,      Q: columns of x,    inner: rows of the batch      (GRAD)
+//
+// Sums are held in fp32 and rounded once, to the type of the result.  Large products are bound by the matrix pipes and by what
+// their feeding leaves of them -- 8 192 x 8 192 x 8 192 bf16 905 / 880 / 860 us (forward, gradient of x, of w; 1 215 to 1 280
+// TFLOP/s), 32 771 rows of 16 experts of 2 048 x 1 024 bf16 166 / 155 / 153 (830 to 900), 8 192 x 4 096 x 4 096 fp32 1 976 / 1 927 /
+// 1 875 (139 to 147) --, few rows at many experts by reading the matrices (16 rows at 15 of 2 048 x 1 024 bf16 12 us, 63 MB).
 #pragma once
 
 #include "expert_find.h"
@@ -184,8 +189,10 @@ __device__ __forceinline__ void el_step(const EL_LDS char *__restrict__ from, EL
   }
 }
 
-// A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of 128 bytes of inner index through two
-// stages in LDS, the next piece on its way while one is multiplied.
+// A block of WP x WQ waves computes BP x BQ of the result; its operands come in pieces of ROWB bytes of inner index through two
+// stages in LDS, the next piece on its way while one is multiplied.  (Half pieces through five chunks of LDS, on their way up to
+// two and a half pieces ahead and waited for by their number: 8 192 x 8 192 x 8 192 bf16 941 us where this took 976, but 100 000 x
+// 256 x 256 30 where it took 27.)
 template <typename T, int BP, int BQ, int WP, int WQ, int ROWB, bool GRAD, bool KN, bool DIRECT>
 __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   constexpr int THREADS = WP * WQ * HC_WAVE, TP = BP / WP / 32, TQ = BQ / WQ / 32, PER = 16 / (int)sizeof(T);
@@ -203,8 +210,11 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   const uint32_t per = (uint32_t)(GRAD ? a.tiles_p * a.tiles_q : a.tiles_q), which = (uint32_t)b / per, in = (uint32_t)b % per;
   const ElPart part = GRAD ? el_find_part(a.offset, a.E, a.S, a.slab, (int)which) : el_find_rows(a.offset, a.E, a.S, BP, (int)which);
   if (part.expert > a.E) return;
-  // a part's tiles go by strips of four along P, column by column: sixteen that follow one another take from four rows of tiles
-  // and four columns
+  // A part's tiles go by strips of four along P, column by column: sixteen that follow one another, on one XCD, take from four
+  // rows of tiles and four columns.  (Gradient of w in bf16, row by row in runs of four on an XCD / so, us: 38 168 rows, 38 experts,
+  // 384 x 1 280 82 / 70; 50 000, 7, 512 x 768 76 / 68; 12 000, 8, 1 408 x 2 048 87 / 94.)  fp32 needs an eighth of the bytes in the
+  // same time and rather has its tiles spread evenly: strips of two in runs of four (30 000, 4, 768 x 768: 274 us, 325 in sixteens).
+  // Tiles of a product by rows go in runs of eight (38 168, 38 experts, 1 280 to 384 bf16: 45 us, in fours 53).
   constexpr uint32_t HIGH = !GRAD ? 1 : sizeof(T) == 2 ? 4 : 2;
   const uint32_t strip = HIGH * (uint32_t)a.tiles_q, top = in / strip * HIGH;
   const uint32_t high = !GRAD ? 1 : (uint32_t)a.tiles_p - top < HIGH ? (uint32_t)a.tiles_p - top : HIGH;
@@ -226,7 +236,8 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   // the operands from inner index k0 on, up to their last element (not DIRECT: in whole words)
   const auto buffer = [&](const T *p, bool outside, uint32_t ld, int wide, int k0, uint32_t skip) {
     const int left = inner - k0, n = left < BK ? left : BK;
-    const uint32_t bytes = left < 1 ? 0u : (outside ? (uint32_t)(n - 1) * ld + (uint32_t)wide : (uint32_t)(wide - 1) * ld + (uint32_t)left) * SIZE;
+    const uint32_t elements = outside ? (uint32_t)(n - 1) * ld + (uint32_t)wide : (uint32_t)(wide - 1) * ld + (uint32_t)left;
+    const uint32_t bytes = left < 1 ? 0u : elements * SIZE;
     return hc_make_buffer(reinterpret_cast<const char *>(outside ? p + (int64_t)k0 * ld : p + k0) - skip,
                           DIRECT ? bytes : (bytes + skip + 3) & ~3u);
   };
@@ -242,8 +253,10 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   const auto step = [&](int from, int to, int k0, bool more) {
-    el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq, buffer(pp, PT, ld_p, rows_out, k0, skip_p),
-                                                       buffer(pq, QT, ld_q, cols_out, k0, skip_q), more, inner - k0, t, wave, wp, wq, acc);
+    el_step<op_p, op_q, TP, TQ, BYTES_P, ROWB / 32, T>(lds + from * STAGE, lds + to * STAGE, fp, fq,
+                                                       buffer(pp, PT, ld_p, rows_out, k0, skip_p),
+                                                       buffer(pq, QT, ld_q, cols_out, k0, skip_q), more, inner - k0, t, wave, wp,
+                                                       wq, acc);
   };
   const auto put = [&](int s, int k0) {
     fp.put(lds + s * STAGE, t, inner - k0);
@@ -402,27 +415,35 @@ static bool el_direct(const void *p, const void *q, int64_t w0, int64_t w1, int 
   return ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) | (uint64_t)(w0 * size) | (uint64_t)(w1 * size)) & 3) == 0;
 }
 
-// Tiles of 256 x 256 on eight waves, one block per compute unit, or of 128 x 128 on four, several blocks per unit; pieces of 128
-// bytes of inner index, or of 64, which leaves room for four small blocks on a unit.
+// Tiles of 256 x 256 on eight waves, one block per compute unit, of 128 x 128 on four, two blocks per unit, or of 64 x 64 on
+// four; pieces of 128 bytes of inner index, or of 64, which leaves room for four small blocks on a unit.  (256 x 128 on four waves,
+// two blocks per unit: 65 536 x 1 280 x 1 280 bf16 256 us, 222 by the large ones.)
 #define EL_LARGE 256, 256, 2, 4, 128
 #define EL_SMALL 128, 128, 2, 2, 128
 #define EL_SHORT 128, 128, 2, 2, 64
 #define EL_TINY 64, 64, 2, 2, 128
 #define EL_TINY_GRAD 64, 64, 2, 2, 64
 
-constexpr int EL_SHORT_INNER = 512;               // longest inner size that goes in pieces of 64 bytes where both would do
+// Longest inner size that small tiles take in pieces of 64 bytes.  us, in 128 / in 64: 100 000 rows, 5 experts, 256 x 256 31 / 26;
+// 20 000, 32, 512 x 512 21.0 / 20.8; 12 000, 8, 1 408 x 2 048 86 / 104.
+constexpr int EL_SHORT_INNER = 512;
 // 128-wide tiles of half precision up to which tiles of 64 x 64 are taken: no unit would have two (us, small / tiny: 1 000 rows, 8
 // experts, 768 x 768: 10.4 / 7.7; 3 000, 16, 512 x 512: 10 / 7; 10 000, 1, 256 x 602 (158): 11.4 / 10.5; 602 x 256 (395): 10.8 / 11.5)
 constexpr int64_t EL_TINY_ROWS = 256;
-constexpr int64_t EL_SHORT_GROUP = 640;           // rows of an expert, on average, up to which its gradient does
-constexpr int64_t EL_LARGE_GRAD = 256 * 5120;     // rows of the batch that a unit would take through a large tile
+// Rows of an expert, on average, up to which its gradient goes in pieces of 64 bytes (half precision; us, in 128 / in 64: 16 384 rows,
+// 64 experts, 768 x 1 024 75 / 58; 20 000, 32, 512 x 512 39 / 37; 8 192, 8, 1 024 x 1 024 41 / 41; 12 000, 8, 1 408 x 2 048 84 / 108).
+constexpr int64_t EL_SHORT_GROUP = 640;
+// Rows of the batch that a unit would take through a large tile, times the units, from which a gradient goes by large ones (us, small /
+// large: 65 536 rows, 1 280 x 1 280 (25 tiles) 262 / 221; 32 771, 16 experts, 2 048 x 1 024 (32) 150 / 160).
+constexpr int64_t EL_LARGE_GRAD = 256 * 5120;
 // The same of a small tile in fp32, below which its gradient goes by tiny ones (us, small / tiny: 500 rows, 4 experts, 256 x 256:
 // 18 / 13; 20 000, 7, 300 x 172: 47 / 36; 40 000, 1, 256 x 602: 123 / 123; 30 000, 4, 768 x 768: 274 / 289)
 constexpr int64_t EL_SMALL_GRAD_F32 = 256 * 2048;
 
 // Is the product of S rows in E groups by `cols` columns done sooner in large tiles?  Rounds over the 256 compute units, the
-// groups' last tiles half empty; a small tile, two at a time on a unit, takes EL_SMALL_COST of a large one's time and a
-// quarter of its work.
+// groups' last tiles half empty; a small tile, two at a time on a unit, takes EL_SMALL_COST of a large one's time and does a
+// quarter of its work.  (us, large / small: 65 536 rows, 1 280 x 1 280 225 / 265; 8 192, 8 192 x 1 024 134 / 145, its gradient of x
+// 179 / 121; 38 168, 38 experts, 384 x 1 280 67 / 45.)
 constexpr float EL_SMALL_COST = 0.575f;
 static int64_t el_tiles_of_rows(int64_t S, int64_t E, int64_t cols, int64_t tile) {
   return ((S + tile - 1) / tile + E / 2) * ((cols + tile - 1) / tile);
@@ -465,7 +486,10 @@ struct ElGradShape {
   int64_t slab, several;        // rows of a part; parts of experts with several of them, at most
 };
 
-// Parts: as few as give every compute unit a large tile or two small ones, had one expert all rows.
+// Parts: as few as give every compute unit a large tile or two small ones, had one expert all rows (half as long, us: 50 000 rows, 7
+// experts, 512 x 768 bf16 68 / 80; 30 000, 4, 768 x 768 fp32 275 / 293; 60 007, 5, 256 x 256 fp32 84 / 96).  A part has 512 rows at
+// least, 128 in fp32, whose products of as many rows take eight times as long (4 000 rows, 8 experts, 256 x 256: 128 / 512 22 / 43 us;
+// bf16, 3 000, 16, 512 x 512: 24 / 18).
 static ElGradShape el_grad_shape(int64_t S, int64_t N, int64_t K, int size, bool wide) {
   ElGradShape g;
   const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);

@@ -3,16 +3,19 @@
 //
 //   m = max |x|;  scale = m * (1 / 127);  code = rint(x * (1 / m * 127));  x' = code * scale        (|x' - x| <= scale / 2)
 //
-// each operation rounded to fp32, one division per group.  A group whose m is below 2^-120, where 127 / m leaves fp32, is kept as zeros; one that holds an infinity or a NaN has that
-// as its scale and zeros as codes, so that all of it reads back as NaN.  The largest numbers take the largest scale whose
-// 127-fold is finite.
+// each operation rounded to fp32, one division per group.  Eight bits are what the caller asks for: they halve (fp32: quarter)
+// what a layer keeps between forward and backward.  A group whose m is below 2^-120, where 127 / m leaves fp32, is kept as zeros;
+// one that holds an infinity or a NaN has that as its scale and zeros as codes, so that all of it reads back as NaN.  The largest
+// numbers take the largest scale whose 127-fold is finite.
 //
 // The gate of an expert, h = silu(a) b for rows [a | b], keeps its argument this way (hc_gated_pack) and takes from it in
 // backward the gradients of a and b and h itself, which the second product's weight gradient needs (hc_gated_grad):
 //   s = sigma(a');  da = dh b' s (1 + a' (1 - s));  db = dh a' s;  h' = a' s b'
 // Groups do not reach over from a to b.
 //
-// A lane owns eight adjacent columns; group / 8 lanes share a group.  Bound by memory: one pass over each operand.
+// A lane owns eight adjacent columns; group / 8 lanes share a group, whose largest magnitude goes round by shuffles.  Bound by
+// memory, one pass over each operand: 150 001 rows of 602 fp32 93 us kept (4.9 TB/s), 101 read back (4.5); the gate of 65 537 rows
+// of 2 x 1 024 bf16 118 us forward (545 MB, 4.6 TB/s), 116 backward (680 MB, 5.9).
 #include "hc_common.h"
 
 namespace {

@@ -199,6 +199,13 @@ def test_rows_to_experts_and_back(dtype, n, k, E, D, dropped):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", (2, 3, 4, 6, 7, 8, 9, 12, 15, 17, 31, 65, 601))
+def test_rows_of_every_width(dtype, D):
+    """Rows shorter than a wide piece, of whole pieces, and with a last piece that reaches back over the one before."""
+    test_rows_to_experts_and_back(dtype, 37, 3, 5, D, 0.3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_places_of_no_pair_may_hold_anything(dtype):
     n, k, E, D = 50, 3, 4, 72
     gen = torch.Generator(device=DEV).manual_seed(3)
