@@ -93,7 +93,8 @@ def test_the_parts_of_a_gradient_fit_the_workspace(lib):
         for N, K in ((64, 64), (300, 172), (2048, 1024)):
             for dtype in (0, 1, 2):
                 need = lib.hc_expert_linear_grad_workspace_bytes(S, 16, N, K, dtype)
-                assert need % (N * K * 4) == 0 and need // (N * K * 4) <= 2 * (S // 512)
+                least = 128 if dtype == 0 else 512                # rows of the shortest part that is not an expert's last
+                assert need % (N * K * 4) == 0 and need // (N * K * 4) <= 2 * (S // least)
 
 
 def test_packed(lib, p):
