@@ -71,7 +71,8 @@ def test_larger_products(dtype, sizes, S, N, K):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("sizes,S,N,K", (((9000, 20, 0, 3000, 4000), 16_030, 640, 70), ((9000, 20, 0, 3000, 4000), 16_030, 330, 602),
                                          ((7000, 33, 7900), 15_000, 1000, 72), ((7000, 33, 7900), 15_000, 90, 998),
-                                         ((30_000, 1, 14_000), 44_010, 1000, 2006)))
+                                         ((30_000, 1, 14_000), 44_010, 1000, 2006), ((300,) * 100 + (0, 7), 30_100, 640, 602),
+                                         ((8000, 15_000, 9000), 32_020, 1024, 520), ((20_000, 14_000), 34_001, 512, 72)))
 def test_products_of_every_tile(dtype, sizes, S, N, K):
     """Enough tiles for the wider ones, with widths that end inside a tile and inside a step."""
     check(sizes, S, N, K, dtype)
