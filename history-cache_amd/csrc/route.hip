@@ -9,9 +9,10 @@
 // one instruction; fp32 takes 64 bits.  A lane sorts its keys once; the winners then are, one after the other, the largest of the
 // row's first keys, and the lane that had it moves up.  With `normalize` the sum runs over the winners alone, and each lane
 // takes the exponential of the winner that it keeps.
-// Bound: a lane's sort and the k joins of its row forward (500 009 rows of 64 bf16 logits to four of them: 29 us for 88 MB; with the
-// winners joined through LDS and the keys not sorted 42), the few short loads of a row backward (29 us for 96 MB; several rows'
-// loads issued together took as long).  Small batches are bound by the launch: eight rows 4 us.
+// Bound: a lane's sort and the k joins of its row forward (500 009 rows of 64 bf16 logits to four of them: 27 us for 88 MB; with the
+// winners joined through LDS and the keys not sorted 42).  Backward a row's choices are read once, by its first lanes, and go to
+// their places through LDS: 15 us for 96 MB, by memory (read by every lane of the row and looked for among its logits 26; 500 009
+// rows of 256, eight of them, 80 and 181).  Small batches are bound by the launch: eight rows 4 us.
 #include "hc_common.h"
 
 namespace {
@@ -219,25 +220,49 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_forward(const T *__restrict__ log
     }
 }
 
+// What the wave's lanes have written to LDS is what they read from here on (its accesses stay in order, so that only the
+// compiler has to keep it).
+__device__ __forceinline__ void rt_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <typename T, int L, int V>
 __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ logits, const int64_t *__restrict__ expert,
                                                          const float *__restrict__ weight, const float *__restrict__ g,
                                                          T *__restrict__ grad, int64_t n, int E, int k, bool normalize,
                                                          bool whole) {
+  // the row in LDS: what its choices bring, each from the lane that has read it; zeros elsewhere
+  __shared__ __attribute__((aligned(16))) float s_row[HC_BLOCK * V];
   const int lane = (int)threadIdx.x & (L - 1);
   const int64_t r = ((int64_t)blockIdx.x * HC_BLOCK + threadIdx.x) / L;
   const bool live = r < n;
   const int64_t at = (live ? r : 0) * k;
   const auto plus = [](float a, float b) { return a + b; };
   const auto larger = [](float a, float b) { return fmaxf(a, b); };
-  float t = 0.f;
-  for (int j = lane; j < k; j += L)
+  float *own = s_row + threadIdx.x * V, *row = own - lane * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i) own[i] = 0.f;
+  int64_t e = -1;
+  float w = 0.f, d = 0.f, t = 0.f;
+  if (lane < k) e = expert[at + lane], w = weight[at + lane], d = g[at + lane];
+  if (e >= 0) t = w * d;
+  for (int j = lane + L; j < k; j += L)
     if (expert[at + j] >= 0) t += weight[at + j] * g[at + j];
   t = rt_join<L>(t, plus);
-  float p[V], out[V];
+  const auto bring = [&](int64_t e, float w, float d) {
+    if (e >= 0 && e < E) row[e] = normalize ? w * (d - t) : d;
+  };
+  rt_in_order();
+  bring(e, w, d);
+  for (int j = lane + L; j < k; j += L) bring(expert[at + j], weight[at + j], g[at + j]);
+  rt_in_order();
+  float out[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = own[i];
   if (!normalize) {
     T v[V];
-    float top = -__builtin_inff(), sum = 0.f;
+    float p[V], top = -__builtin_inff(), sum = 0.f;
     rt_row<T, V>::load(logits + (live ? r : 0) * E, lane * V, E, whole, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmaxf(top, hc_to_f32<T>(v[i]));
@@ -252,18 +277,8 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ lo
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       p[i] = sum == 0.f ? 0.f : p[i] / sum;
-      out[i] = -(p[i] * t);
+      out[i] = p[i] * (out[i] - t);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = 0.f;
-  }
-  for (int j = 0; j < k; ++j) {
-    const int e = (int)expert[at + j] - lane * V;
-    const float w = weight[at + j], d = g[at + j] - t;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (e == i) out[i] = (normalize ? w : p[i]) * d;
   }
   if (live) rt_row<T, V>::store(grad + r * E, lane * V, E, whole, out);
 }
