@@ -88,6 +88,30 @@ __device__ __forceinline__ int64_t hc_xcd_block(int64_t bid, int64_t n) {
   return first + (in % HC_NUM_XCD) * CHUNK + in / HC_NUM_XCD;
 }
 
+// Another lane's value: D = 1, 2: lane ^ D; 4, 8: the lane's mirror image among 8 or 16, which after the smaller steps holds what
+// lane ^ D does; 16, 32: lane ^ D.
+template <int D>
+__device__ __forceinline__ uint32_t hc_other(uint32_t v) {
+  if constexpr (D >= 16) return (uint32_t)__shfl_xor((int)v, D, HC_WAVE);
+  constexpr int CTRL = D == 1 ? 0xb1 : D == 2 ? 0x4e : D == 4 ? 0x141 : 0x140;
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int D>
+__device__ __forceinline__ int32_t hc_other(int32_t v) { return (int32_t)hc_other<D>((uint32_t)v); }
+template <int D>
+__device__ __forceinline__ int64_t hc_other(int64_t v) {
+  return (int64_t)((uint64_t)hc_other<D>((uint32_t)((uint64_t)v >> 32)) << 32 | hc_other<D>((uint32_t)v));
+}
+template <int D>
+__device__ __forceinline__ float hc_other(float v) { return __uint_as_float(hc_other<D>(__float_as_uint(v))); }
+
+// `v` of the L lanes joined by `f`, in every one of them.
+template <int L, int D = 1, typename V, typename F>
+__device__ __forceinline__ V hc_join(V v, F &&f) {
+  if constexpr (D < L) return hc_join<L, 2 * D>(f(v, hc_other<D>(v)), f);
+  else return v;
+}
+
 // Butterfly sum over the 64 lanes, partner distance 32,16,8,4,2,1.  Every lane
 // ends with the same bits (fp add is commutative), and the order is the one
 // the oracle reproduces.

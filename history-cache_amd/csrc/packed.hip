@@ -13,9 +13,9 @@
 //   s = sigma(a');  da = dh b' s (1 + a' (1 - s));  db = dh a' s;  h' = a' s b'
 // Groups do not reach over from a to b.
 //
-// A lane owns eight adjacent columns; group / 8 lanes share a group, whose largest magnitude goes round by shuffles.  Bound by
-// memory, one pass over each operand: 150 001 rows of 602 fp32 93 us kept (4.9 TB/s), 101 read back (4.5); the gate of 65 537 rows
-// of 2 x 1 024 bf16 118 us forward (545 MB, 4.6 TB/s), 116 backward (680 MB, 5.9).
+// A lane owns eight adjacent columns; group / 8 lanes share a group, whose largest magnitude goes round from lane to lane.  Bound by
+// memory, one pass over each operand: 150 001 rows of 602 fp32 91 us kept (5.0 TB/s), 75 to 101 read back (4.5 to 6.0); the gate of
+// 65 537 rows of 2 x 1 024 bf16 118 us forward (545 MB, 4.6 TB/s), 116 backward (680 MB, 5.9).
 #include "hc_common.h"
 
 namespace {
@@ -23,6 +23,9 @@ namespace {
 constexpr float PK_SMALLEST = 0x1p-120f;
 constexpr float PK_LARGEST_SCALE = 0x1.0204060000000p+121f;      // 127 times the next one leaves fp32
 constexpr int PK_EACH = 8;
+// Eights that a lane reads before it packs the first (us, one / two / four: 150 001 rows of 608 bf16 66 / 58 / 57, of 602 fp32
+// 94 / 91 / 92; 300 000 of 172 fp32 49 / 48 / 52).
+constexpr int PK_AT_ONCE = 2;
 // Bytes of the last-level cache.  Reading back and a pass that reads the result, plain / non-temporal stores, us: 193 MB
 // 94 / 117, 361 MB 218 / 206, 722 MB 429 / 391.
 constexpr int64_t PK_CACHE = 256 << 20;
@@ -169,11 +172,7 @@ __device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__
     const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
     m = b > m ? b : m;
   }
-#pragma unroll
-  for (int d = L / 2; d >= 1; d /= 2) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)m, d, HC_WAVE);
-    m = o > m ? o : m;
-  }
+  m = hc_join<L>(m, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
   const float most = __uint_as_float(m);
   const bool zero = most < PK_SMALLEST, bad = m >= 0x7f800000u;
   const float inverse = zero || bad ? 0.f : 1.0f / most * 127.0f;
@@ -207,8 +206,8 @@ struct pk_item {
   int64_t row;
   int g, col, valid, lane;
   bool live;
-  __device__ __forceinline__ pk_item(const PkArgs &a) {
-    const uint32_t t = blockIdx.x * HC_BLOCK + threadIdx.x, i = t / L;       // (a launch has less than 2^32 threads)
+  __device__ __forceinline__ pk_item(const PkArgs &a, uint32_t block = blockIdx.x) {
+    const uint32_t t = block * HC_BLOCK + threadIdx.x, i = t / L;            // (there are less than 2^32 lanes' pieces)
     lane = (int)(t % L);
     live = i < a.items;
     const uint32_t r = live ? i / (uint32_t)a.groups : 0;
@@ -222,12 +221,18 @@ struct pk_item {
 template <typename T, int L>
 __global__ __launch_bounds__(HC_BLOCK) void pk_pack(PkArgs a, const T *__restrict__ x, int8_t *__restrict__ codes,
                                                     float *__restrict__ scale) {
-  const pk_item<L> it(a);
-  float v[PK_EACH];
-  const int64_t at = it.row * a.F + it.col;
-  pk_row<T>::load(x + at, it.valid, v);
-  const float s = pk_encode<L>(v, codes + at, it.valid);
-  if (it.live && it.lane == 0) scale[it.row * a.groups + it.g] = s;
+  float v[PK_AT_ONCE][PK_EACH];
+#pragma unroll
+  for (int u = 0; u < PK_AT_ONCE; ++u) {
+    const pk_item<L> it(a, blockIdx.x * PK_AT_ONCE + u);
+    pk_row<T>::load(x + it.row * a.F + it.col, it.valid, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < PK_AT_ONCE; ++u) {
+    const pk_item<L> it(a, blockIdx.x * PK_AT_ONCE + u);
+    const float s = pk_encode<L>(v[u], codes + it.row * a.F + it.col, it.valid);
+    if (it.live && it.lane == 0) scale[it.row * a.groups + it.g] = s;
+  }
 }
 
 // NT: for a result that the last-level cache cannot hold until it is read.
@@ -320,7 +325,7 @@ extern "C" int hc_pack_rows(const void *x, int dtype, int64_t n, int64_t F, int6
   HC_REQUIRE(n == 0 || (x && codes && scale));
   return pk_with(dtype, a, [&](auto type, auto lanes, dim3 grid) {
     typedef decltype(type) T;
-    pk_pack<T, decltype(lanes)::value><<<grid, dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
+    pk_pack<T, decltype(lanes)::value><<<dim3((grid.x + PK_AT_ONCE - 1) / PK_AT_ONCE), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(
         a, static_cast<const T *>(x), codes, scale);
   });
 }

@@ -20,30 +20,6 @@ namespace {
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_CHOICES = 32;
 
-// Another lane's value: D = 1, 2: lane ^ D; 4, 8: the lane's mirror image among 8 or 16, which after the smaller steps holds what
-// lane ^ D does; 16, 32: lane ^ D.
-template <int D>
-__device__ __forceinline__ uint32_t rt_other(uint32_t v) {
-  if constexpr (D >= 16) return (uint32_t)__shfl_xor((int)v, D, HC_WAVE);
-  constexpr int CTRL = D == 1 ? 0xb1 : D == 2 ? 0x4e : D == 4 ? 0x141 : 0x140;
-  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
-}
-template <int D>
-__device__ __forceinline__ int32_t rt_other(int32_t v) { return (int32_t)rt_other<D>((uint32_t)v); }
-template <int D>
-__device__ __forceinline__ int64_t rt_other(int64_t v) {
-  return (int64_t)((uint64_t)rt_other<D>((uint32_t)((uint64_t)v >> 32)) << 32 | rt_other<D>((uint32_t)v));
-}
-template <int D>
-__device__ __forceinline__ float rt_other(float v) { return __uint_as_float(rt_other<D>(__float_as_uint(v))); }
-
-// `v` of the L lanes joined by `f`, in every one of them.
-template <int L, int D = 1, typename V, typename F>
-__device__ __forceinline__ V rt_join(V v, F &&f) {
-  if constexpr (D < L) return rt_join<L, 2 * D>(f(v, rt_other<D>(v)), f);
-  else return v;
-}
-
 // ---- ordering keys
 // A signed number whose upper half (16 bits; fp32: 32) orders like the logit -- a positive one as it is, of a negative one all but the
 // sign turned over, NaN above everything, -0 as 0 -- and whose lower half falls with the index: 8 bits for the place in
@@ -183,7 +159,7 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_forward(const T *__restrict__ log
 #pragma unroll
   for (int q = 0; q < KEPT; ++q) mine[q] = key::NONE;
   for (int j = 0; j < k; ++j) {
-    const key_t own = have[0] | place, best = rt_join<L>(own, larger);
+    const key_t own = have[0] | place, best = hc_join<L>(own, larger);
     if (j == 0) top = best;
     // (by bits: a choice between neighbours becomes a search for the chosen index)
     const key_t won = own == best ? -1 : 0;
@@ -209,7 +185,7 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_forward(const T *__restrict__ log
       if (!rt_masked(f)) sum += expf(f - largest);
     }
   }
-  sum = rt_join<L>(sum, plus);
+  sum = hc_join<L>(sum, plus);
 #pragma unroll
   for (int q = 0; q < KEPT; ++q)
     if (live && q * L + lane < k) {
@@ -249,7 +225,7 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ lo
   if (e >= 0) t = w * d;
   for (int j = lane + L; j < k; j += L)
     if (expert[at + j] >= 0) t += weight[at + j] * g[at + j];
-  t = rt_join<L>(t, plus);
+  t = hc_join<L>(t, plus);
   const auto bring = [&](int64_t e, float w, float d) {
     if (e >= 0 && e < E) row[e] = normalize ? w * (d - t) : d;
   };
@@ -266,14 +242,14 @@ __global__ __launch_bounds__(HC_BLOCK) void rt_backward(const T *__restrict__ lo
     rt_row<T, V>::load(logits + (live ? r : 0) * E, lane * V, E, whole, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmaxf(top, hc_to_f32<T>(v[i]));
-    top = rt_join<L>(top, larger);
+    top = hc_join<L>(top, larger);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float f = hc_to_f32<T>(v[i]);
       p[i] = rt_masked(f) ? 0.f : expf(f - top);
       sum += p[i];
     }
-    sum = rt_join<L>(sum, plus);
+    sum = hc_join<L>(sum, plus);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       p[i] = sum == 0.f ? 0.f : p[i] / sum;
