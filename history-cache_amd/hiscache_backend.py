@@ -1597,11 +1597,25 @@ def bias_bn_relu_eval(x, bias, gamma, beta, running_mean, running_var, eps):
 
 
 # ----------------------------------------------------------------------------- rows and their experts
+# What a call of a few rows costs is the host's: 10 us for a launch of 3, so that these checks are spelled without generators and
+# torch's public accessors, which look first whether the GPU has been initialised (a tensor on it says that it has).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_of_device = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 def _together(t, *others):
     """Do these tensors lie on one device, the current one (whose stream the launch goes to)?"""
     index = t.get_device()
-    if index != torch.cuda.current_device() or any(o.get_device() != index for o in others):
+    together = index == _current_device()
+    for o in others:
+        together = together and o.get_device() == index
+    if not together:
         raise ValueError("the tensors must lie on one device, and it must be the current one")
+
+
+def _stream_for(t):
+    """The current stream of the device that t is on."""
+    return _stream_of_device(t.get_device())
 
 
 def _arriving(g):
@@ -1612,15 +1626,25 @@ def _arriving(g):
 # The operators below are autograd nodes where a gradient may be asked for; without one the node itself, which costs the
 # host more than the launch, is left out.
 def _watched(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _once(backward):
+    """``once_differentiable`` for a backward pass whose own graph is asked for; the others go without its wrapper (4 us)."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 def _route(logits, top_k, normalize):
     n, E = logits.shape
-    expert = torch.empty((n, top_k), dtype=torch.int64, device=logits.device)
-    weight = torch.empty((n, top_k), dtype=torch.float32, device=logits.device)
+    expert = logits.new_empty((n, top_k), dtype=torch.int64)
+    weight = logits.new_empty((n, top_k), dtype=torch.float32)
     _check(load_library().hc_route_rows(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
-                                        expert.data_ptr(), weight.data_ptr(), _stream()), "hc_route_rows")
+                                        expert.data_ptr(), weight.data_ptr(), _stream_for(logits)), "hc_route_rows")
     return expert, weight
 
 
@@ -1635,7 +1659,7 @@ class _RouteRows(torch.autograd.Function):
         return expert, weight
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, _g_expert, g):
         if g is None:
             return None, None, None
@@ -1646,7 +1670,7 @@ class _RouteRows(torch.autograd.Function):
         grad = torch.empty_like(logits)
         _check(load_library().hc_route_rows_grad(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
                                                  expert.data_ptr(), weight.data_ptr(), g.data_ptr(), grad.data_ptr(),
-                                                 _stream()), "hc_route_rows_grad")
+                                                 _stream_for(logits)), "hc_route_rows_grad")
         return grad, None, None
 
 
@@ -1695,28 +1719,28 @@ def expert_order(expert, num_expert):
     E, P, dev = int(num_expert), expert.numel(), expert.device
     if E < 1:
         raise ValueError("num_expert must be positive")
-    at = torch.empty((2, P), dtype=torch.int32, device=dev)
-    offset = torch.empty(E + 1, dtype=torch.int64, device=dev)
+    at = expert.new_empty((2, P), dtype=torch.int32)
+    offset = expert.new_empty(E + 1)
     slot, pair = at.unbind(0)
     nbytes = int(lib.hc_expert_order_workspace_bytes(P, E))
     ws = _workspace(nbytes, dev) if nbytes else None
     _check(lib.hc_expert_order(expert.data_ptr(), P, E, slot.data_ptr(), pair.data_ptr(), offset.data_ptr(), _ptr(ws),
-                               nbytes, _stream()), "hc_expert_order")
+                               nbytes, _stream_for(expert)), "hc_expert_order")
     return ExpertOrder(slot, pair, offset, expert.shape[0], 1 if expert.dim() == 1 else expert.shape[1], E)
 
 
 def _to_experts(x, order):
-    rows = torch.empty((order.places, x.shape[1]), dtype=x.dtype, device=x.device)
+    rows = x.new_empty((order.places, x.shape[1]))
     _check(load_library().hc_rows_to_experts(x.data_ptr(), _DTYPES[x.dtype], order.rows, order.top_k, order.experts,
                                              x.shape[1], order.slot.data_ptr(), order.offset.data_ptr(), rows.data_ptr(),
-                                             _stream()), "hc_rows_to_experts")
+                                             _stream_for(x)), "hc_rows_to_experts")
     return rows
 
 
 def _from_experts(y, order, weight):
-    out = torch.empty((order.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+    out = y.new_empty((order.rows, y.shape[1]))
     _check(load_library().hc_rows_from_experts(y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts,
-                                               y.shape[1], order.slot.data_ptr(), _ptr(weight), out.data_ptr(), _stream()),
+                                               y.shape[1], order.slot.data_ptr(), _ptr(weight), out.data_ptr(), _stream_for(y)),
            "hc_rows_from_experts")
     return out
 
@@ -1728,7 +1752,7 @@ class _RowsToExperts(torch.autograd.Function):
         return _to_experts(x, order)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         return _from_experts(_arriving(g), ctx.hc, None), None
 
@@ -1741,7 +1765,7 @@ class _RowsFromExperts(torch.autograd.Function):
         return _from_experts(y, order, weight)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         y, weight = ctx.saved_tensors
         order, g = ctx.hc, _arriving(g)
@@ -1755,7 +1779,7 @@ def _from_experts_grads(g, y, order, weight):
     _check(load_library().hc_rows_from_experts_grad(
         g.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts, y.shape[1],
         order.slot.data_ptr(), order.offset.data_ptr(), weight.data_ptr(), grad_y.data_ptr(), grad_weight.data_ptr(),
-        _stream()), "hc_rows_from_experts_grad")
+        _stream_for(y)), "hc_rows_from_experts_grad")
     return grad_y, None, grad_weight
 
 
@@ -1798,7 +1822,7 @@ class _ExpertLinear(torch.autograd.Function):
         return _expert_product(x, w, offset, False)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         x, w, offset = ctx.saved_tensors
         g = _arriving(g)
@@ -1810,9 +1834,9 @@ def _expert_product(x, w, offset, transposed):
     S, (E, N, K) = x.shape[0], w.shape
     if transposed:
         N, K = K, N
-    out = torch.empty((S, N), dtype=x.dtype, device=x.device)
+    out = x.new_empty((S, N))
     _check(load_library().hc_expert_linear(x.data_ptr(), _DTYPES[x.dtype], w.data_ptr(), int(transposed), offset.data_ptr(),
-                                           S, E, N, K, out.data_ptr(), _stream()), "hc_expert_linear")
+                                           S, E, N, K, out.data_ptr(), _stream_for(x)), "hc_expert_linear")
     return out
 
 
@@ -1847,11 +1871,11 @@ def expert_linear_grad(g, x, offset):
         raise ValueError("g [S, N] and x [S, K] must have the same number of rows")
     _together(x, g, offset)
     (S, N), K, E, dtype = g.shape, x.shape[1], offset.numel() - 1, _float_dtype(x, "x")
-    gw = torch.empty((E, N, K), dtype=x.dtype, device=x.device)
+    gw = x.new_empty((E, N, K))
     nbytes = int(lib.hc_expert_linear_grad_workspace_bytes(S, E, N, K, dtype))
     ws = _workspace(nbytes, x.device) if nbytes else None
     _check(lib.hc_expert_linear_grad(g.data_ptr(), x.data_ptr(), dtype, offset.data_ptr(), S, E, N, K, gw.data_ptr(),
-                                     _ptr(ws), nbytes, _stream()), "hc_expert_linear_grad")
+                                     _ptr(ws), nbytes, _stream_for(x)), "hc_expert_linear_grad")
     return gw
 
 
@@ -1867,8 +1891,8 @@ class PackedRows:
 
 def _packed_like(x, halves, group):
     n, F = x.shape[0], x.shape[1] // halves
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty((n, halves * -(-F // group)), dtype=torch.float32, device=x.device)
+    codes = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty((n, halves * -(-F // group)), dtype=torch.float32)
     return codes, scale
 
 
@@ -1889,7 +1913,7 @@ def pack_rows(x, group=64):
     _pack_arguments(x, "x", group)
     codes, scale = _packed_like(x, 1, group)
     _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], group, codes.data_ptr(),
-                                       scale.data_ptr(), _stream()), "hc_pack_rows")
+                                       scale.data_ptr(), _stream_for(x)), "hc_pack_rows")
     return PackedRows(codes, scale, group, x.dtype)
 
 
@@ -1903,9 +1927,9 @@ def unpack_rows(kept, dtype=None):
     if scale.shape[1] != -(-F // kept.group):
         raise ValueError("these rows were kept by gated_pack")
     _together(codes)
-    x = torch.empty((n, F), dtype=dtype, device=codes.device)
+    x = codes.new_empty((n, F), dtype=dtype)
     _check(load_library().hc_unpack_rows(codes.data_ptr(), scale.data_ptr(), n, F, kept.group, x.data_ptr(),
-                                         _DTYPES[dtype], _stream()), "hc_unpack_rows")
+                                         _DTYPES[dtype], _stream_for(codes)), "hc_unpack_rows")
     return x
 
 
@@ -1916,10 +1940,10 @@ def gated_pack(x, group=64, keep=True):
     if x.shape[1] % 2 != 0:
         raise ValueError("x must hold two halves of the same width")
     n, F = x.shape[0], x.shape[1] // 2
-    h = torch.empty((n, F), dtype=x.dtype, device=x.device)
+    h = x.new_empty((n, F))
     codes, scale = _packed_like(x, 2, group) if keep else (None, None)
     _check(load_library().hc_gated_pack(x.data_ptr(), _DTYPES[x.dtype], n, F, group, h.data_ptr(), _ptr(codes), _ptr(scale),
-                                        _stream()), "hc_gated_pack")
+                                        _stream_for(x)), "hc_gated_pack")
     return h, PackedRows(codes, scale, group, x.dtype) if keep else None
 
 
@@ -1931,10 +1955,9 @@ def gated_grad(kept, g):
     if codes.shape[1] % 2 or scale.shape[1] != 2 * -(-F // kept.group) or g.shape != (n, F):
         raise ValueError("g must be [n, F] for rows [n, 2 F] that gated_pack kept")
     _together(g, codes)
-    gx = torch.empty((n, 2 * F), dtype=kept.dtype, device=g.device)
-    h = torch.empty((n, F), dtype=kept.dtype, device=g.device)
+    gx, h = g.new_empty((n, 2 * F)), torch.empty_like(g)
     _check(load_library().hc_gated_grad(codes.data_ptr(), scale.data_ptr(), g.data_ptr(), _DTYPES[kept.dtype], n, F,
-                                        kept.group, gx.data_ptr(), h.data_ptr(), _stream()), "hc_gated_grad")
+                                        kept.group, gx.data_ptr(), h.data_ptr(), _stream_for(g)), "hc_gated_grad")
     return gx, h
 
 
@@ -1947,7 +1970,7 @@ class _GatedExperts(torch.autograd.Function):
         return _expert_product(h, w_out, offset, False)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         rows, w_in, w_out, offset, codes, scale = ctx.saved_tensors
         need, g = ctx.needs_input_grad, _arriving(g)
