@@ -7,7 +7,8 @@
 //     gradient of w      P: columns of g,      Q: columns of x,    inner: rows of the batch      (GRAD)
 //
 // Sums are held in fp32 and rounded once, to the type of the result.  Large products are bound by the matrix pipes and by what
-// their feeding leaves of them -- 8 192 x 8 192 x 8 192 bf16 905 / 880 / 860 us (forward, gradient of x, of w; 1 215 to 1 280
+// their feeding leaves of them: a step of a large tile reads 192 KB from LDS and writes 64, at 128 bytes a cycle as long as its
+// products take -- 8 192 x 8 192 x 8 192 bf16 905 / 880 / 860 us (forward, gradient of x, of w; 1 215 to 1 280
 // TFLOP/s), 32 771 rows of 16 experts of 2 048 x 1 024 bf16 166 / 155 / 153 (830 to 900), 8 192 x 4 096 x 4 096 fp32 1 976 / 1 927 /
 // 1 875 (139 to 147) --, few rows at many experts by reading the matrices (16 rows at 15 of 2 048 x 1 024 bf16 12 us, 63 MB).
 #pragma once
