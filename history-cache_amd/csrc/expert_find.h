@@ -5,24 +5,11 @@
 
 // Part `part` of the `parts` that expert `expert`'s rows are cut into.  Every wave of a block looks for it and finds the same.
 struct ElPart {
-  int expert;            // E: the rows behind the last expert; E + 1: there is no such part
+  int expert;            // E, E + 1: the rows behind the last expert, before the first; E + 2: there is no such part
   int part, parts;
   int place;             // parts before it, counting experts of several parts only (where its partial sums lie)
   int64_t lo, hi;        // its rows
 };
-
-// Rows offset[e] .. offset[e + 1] (offsets out of order or range describe no rows, but never ones outside x).
-__device__ __forceinline__ void el_rows_of(const int64_t *__restrict__ offset, int E, int64_t S, int e, int64_t *lo, int64_t *hi) {
-  int64_t a = 0, b = 0;
-  if (e <= E) {
-    a = offset[e];
-    a = a < 0 ? 0 : a > S ? S : a;
-    b = e < E ? offset[e + 1] : S;
-    b = b < a ? a : b > S ? S : b;
-  }
-  *lo = a;
-  *hi = b;
-}
 
 __device__ __forceinline__ int el_scan(int v) {
   const int lane = hc_lane();
@@ -34,13 +21,40 @@ __device__ __forceinline__ int el_scan(int v) {
   return v;
 }
 
-// The t-th piece of up to `rows` rows, expert by expert; the rows behind the last expert follow as expert E.
+// Rows offset[e] .. offset[e + 1] of the lane's expert e, for e = E the rows behind the last expert, none for a larger one.  An offset outside [0, S] counts as the end that it lies behind, one below an earlier one as that one: whatever the offsets
+// are, no two experts have a row in common.  most: the largest offset of the experts before the first lane's, then of all.
+__device__ __forceinline__ void el_rows_of(const int64_t *__restrict__ offset, int E, int64_t S, int e, int *most, int64_t *lo,
+                                           int64_t *hi) {
+  const auto inside = [&](int64_t a) { return (int)(a < 0 ? 0 : a > S ? S : a); };        // (S is below 2^31)
+  int a = e <= E ? inside(offset[e]) : (int)S;
+  const int b = e < E ? inside(offset[e + 1]) : (int)S;
+  if (__ballot(b < a) != 0 || __builtin_amdgcn_readfirstlane(a) < *most) {
+    const int lane = hc_lane();
+    a = a > *most ? a : *most;
+#pragma unroll
+    for (int d = 1; d < HC_WAVE; d *= 2) {
+      const int o = __shfl_up(a, d, HC_WAVE);
+      if (lane >= d && o > a) a = o;
+    }
+  }
+  *lo = a;
+  *hi = a > b ? a : b;
+  *most = __builtin_amdgcn_readlane(a > b ? a : b, HC_WAVE - 1);
+}
+
+// The t-th piece of up to `rows` rows, expert by expert; the rows behind the last expert follow as expert E, those before the
+// first as E + 1.
 __device__ __forceinline__ ElPart el_find_rows(const int64_t *__restrict__ offset, int E, int64_t S, int rows, int t) {
   const int lane = hc_lane();
-  int before = 0;
-  for (int e0 = 0; e0 <= E; e0 += HC_WAVE) {
+  int before = 0, most = 0;
+  for (int e0 = 0; e0 <= E + 1; e0 += HC_WAVE) {
     int64_t lo, hi;
-    el_rows_of(offset, E, S, e0 + lane, &lo, &hi);
+    el_rows_of(offset, E, S, e0 + lane, &most, &lo, &hi);
+    if (e0 + lane == E + 1) {
+      const int64_t first = offset[0];
+      lo = 0;
+      hi = first < 0 ? 0 : first > S ? S : first;
+    }
     const int parts = (int)((hi - lo + rows - 1) / rows), upto = el_scan(parts);
     const uint64_t in = __ballot(t < before + upto);
     if (in != 0) {
@@ -57,7 +71,7 @@ __device__ __forceinline__ ElPart el_find_rows(const int64_t *__restrict__ offse
     before += __builtin_amdgcn_readlane(upto, HC_WAVE - 1);
   }
   ElPart r = {};
-  r.expert = E + 1;
+  r.expert = E + 2;
   return r;
 }
 
@@ -67,10 +81,10 @@ __device__ __forceinline__ ElPart el_find_rows(const int64_t *__restrict__ offse
 __device__ __forceinline__ ElPart el_find_part(const int64_t *__restrict__ offset, int E, int64_t S, int64_t rows, int t) {
   const int lane = hc_lane();
   for (int last = 0; last < 2; ++last) {
-    int before = 0, several = 0;
+    int before = 0, several = 0, most = 0;
     for (int e0 = 0; e0 < E; e0 += HC_WAVE) {
       int64_t lo, hi;
-      el_rows_of(offset, E, S, e0 + lane < E ? e0 + lane : E + 1, &lo, &hi);
+      el_rows_of(offset, E, S, e0 + lane < E ? e0 + lane : E + 1, &most, &lo, &hi);
       const int full = (int)((hi - lo) / rows), rest = (int)(hi - lo - full * rows);
       const bool short_one = e0 + lane < E && (rest > 0 || full == 0);
       const int parts = full + (short_one ? 1 : 0), many = parts > 1 ? parts : 0, place = several + el_scan(many) - many;
@@ -104,7 +118,7 @@ __device__ __forceinline__ ElPart el_find_part(const int64_t *__restrict__ offse
     t -= before;
   }
   ElPart r = {};
-  r.expert = E + 1;
+  r.expert = E + 2;
   return r;
 }
 

@@ -1,6 +1,6 @@
 // Rows times their expert's matrix: rows offset[e] .. offset[e + 1] of x [S, K] belong to expert e with w[e] [N, K].
 //
-//   forward           y[s]  = x[s] w[e]^T            rows behind offset[E]: zeros
+//   forward           y[s]  = x[s] w[e]^T            rows before offset[0], behind offset[E]: zeros
 //   gradient of x     gx[s] = g[s] w[e]              likewise
 //   gradient of w     gw[e] = sum over e's rows of g[s]^T x[s]
 //

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   const int wp = wave % WP * (BP / WP), wq = wave / WP * (BQ / WQ);
   const uint32_t per = (uint32_t)(GRAD ? a.tiles_p * a.tiles_q : a.tiles_q), which = (uint32_t)b / per, in = (uint32_t)b % per;
   const ElPart part = GRAD ? el_find_part(a.offset, a.E, a.S, a.slab, (int)which) : el_find_rows(a.offset, a.E, a.S, BP, (int)which);
-  if (part.expert > a.E) return;
+  if (part.expert > a.E + 1) return;
   // A part's tiles go by strips of four along P, column by column: sixteen that follow one another, on one XCD, take from four
   // rows of tiles and four columns.  (Gradient of w in bf16, row by row in runs of four on an XCD / so, us: 38 168 rows, 38 experts,
   // 384 x 1 280 82 / 70; 50 000, 7, 512 x 768 76 / 68; 12 000, 8, 1 408 x 2 048 87 / 94.)  fp32 needs an eighth of the bytes in the
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(WP *WQ *HC_WAVE, 2) void el_tile(ElProduct a) {
   const int64_t e = part.expert < a.E ? part.expert : 0;
   const int batch = (int)(part.hi - part.lo);                           // rows of the batch
   const int rows_out = GRAD ? (a.rows - p0 < BP ? a.rows - p0 : BP) : batch, cols_out = a.cols - q0 < BQ ? a.cols - q0 : BQ;
-  const int inner = GRAD ? batch : part.expert < a.E ? a.inner : 0;     // (rows behind the last expert: zeros)
+  const int inner = GRAD ? batch : part.expert < a.E ? a.inner : 0;     // (rows of no expert: zeros)
   const uint32_t ld_p = GRAD ? a.rows : a.inner, ld_q = QT ? a.cols : a.inner;
   const T *pp = static_cast<const T *>(a.p) + (GRAD ? part.lo * a.rows + p0 : part.lo * a.inner);
   const T *pq = static_cast<const T *>(a.q) +
@@ -346,10 +346,10 @@ __global__ __launch_bounds__(HC_BLOCK) void el_join(ElProduct a, int64_t size, i
   __shared__ float s_part[3][VEC][HC_WAVE];
   const int lane = hc_lane(), wave = hc_wave_in_block();
   int64_t item = blockIdx.x;                    // chunk of an expert of several parts, expert by expert
-  int before = 0;
+  int before = 0, most = 0;
   for (int e0 = 0; e0 < a.E; e0 += HC_WAVE) {
     int64_t lo, hi;
-    el_rows_of(a.offset, a.E, a.S, e0 + lane < a.E ? e0 + lane : a.E + 1, &lo, &hi);
+    el_rows_of(a.offset, a.E, a.S, e0 + lane < a.E ? e0 + lane : a.E + 1, &most, &lo, &hi);
     int parts = (int)((hi - lo + a.slab - 1) / a.slab);
     parts = parts > 1 ? parts : 0;
     const int place = before + el_scan(parts) - parts;
@@ -466,17 +466,17 @@ static bool el_small_rows_f32(int64_t S, int64_t E, int64_t cols) {
 
 template <typename T, bool KN>
 static int el_rows_of_type(const ElProduct &a, hipStream_t st) {
-  const int64_t parts = a.S / 128 + a.E + 1;
+  const int64_t parts = a.S / 128 + a.E + 2;
   bool tiny;
   if constexpr (sizeof(T) == 2) {
     if (!el_direct(a.p, a.q, a.inner, KN ? a.cols : a.inner, 2)) return el_launch<T, EL_SHORT, false, KN, false>(a, parts, st);
-    if (el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, true>(a, a.S / 256 + a.E + 1, st);
+    if (el_large_rows(a.S, a.E, a.cols)) return el_launch<T, EL_LARGE, false, KN, true>(a, a.S / 256 + a.E + 2, st);
     tiny = el_tiles_of_rows(a.S, a.E, a.cols, 128) <= EL_TINY_ROWS;
     if (!tiny && a.inner > EL_SHORT_INNER) return el_launch<T, EL_SMALL, false, KN, true>(a, parts, st);
   } else {
     tiny = !el_small_rows_f32(a.S, a.E, a.cols);
   }
-  if (tiny) return el_launch<T, EL_TINY, false, KN, true>(a, a.S / 64 + a.E + 1, st);
+  if (tiny) return el_launch<T, EL_TINY, false, KN, true>(a, a.S / 64 + a.E + 2, st);
   return el_launch<T, EL_SHORT, false, KN, true>(a, parts, st);
 }
 

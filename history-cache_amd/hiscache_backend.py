@@ -1847,8 +1847,8 @@ def _expert_offset(offset):
 
 
 def expert_linear(x, w, offset):
-    """``x[s] @ w[e].t()`` for the rows s = offset[e] .. offset[e + 1] of x [S, K], w [E, N, K] of x's type; rows behind
-    offset[E] are zeros.  ``offset`` int64 [E + 1] stays on the device.  Sums in fp32 (fp32 rows: fp32 products), one
+    """``x[s] @ w[e].t()`` for the rows s = offset[e] .. offset[e + 1] of x [S, K], w [E, N, K] of x's type; rows before
+    offset[0] and behind offset[E] are zeros.  ``offset`` int64 [E + 1] stays on the device.  Sums in fp32 (fp32 rows: fp32 products), one
     rounding to the type of x.  Gradients for x and w."""
     _dev(x, "x")
     _float_dtype(x, "x")

@@ -834,11 +834,12 @@ int hc_rows_from_experts_grad(const void *g, const void *y, int dtype, int64_t n
                               void *grad_y, float *grad_weight, void *stream);
 
 /* hc_expert_linear: rows offset[e] .. offset[e + 1] of x [S, K] times w[e]
- * ([E, N, K]; w_is_kn: [E, K, N]), out [S, N], all of one dtype; rows behind
- * offset[E] are zeros.  Sums in fp32, one rounding.  hc_expert_linear_grad:
+ * ([E, N, K]; w_is_kn: [E, K, N]), out [S, N], all of one dtype; rows before
+ * offset[0] and behind offset[E] are zeros.  Sums in fp32, one rounding.  hc_expert_linear_grad:
  * grad_w [E, N, K] = g^T x over each expert's rows.  E <= 1024, N and K <= 2^20,
- * N * K < 2^31, S < 2^31 - 1.  The offsets are read on the device and clamped to
- * [0, S].  workspace: hc_expert_linear_grad_workspace_bytes (0: none), 16-byte
+ * N * K < 2^31, S < 2^31 - 1.  The offsets are read on the device; one outside
+ * [0, S] counts as the end that it lies behind, one below an earlier one as that
+ * one.  workspace: hc_expert_linear_grad_workspace_bytes (0: none), 16-byte
  * aligned. */
 int hc_expert_linear(const void *x, int dtype, const void *w, int w_is_kn, const int64_t *offset, int64_t S,
                      int64_t E, int64_t N, int64_t K, void *out, void *stream);

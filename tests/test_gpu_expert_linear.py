@@ -183,6 +183,49 @@ def test_offsets_out_of_order_or_range_touch_no_other_memory():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("E", (3, 64, 65, 130))
+def test_offsets_that_overlap_count_as_their_largest_so_far(E):
+    """Also: the partial sums of a gradient stay in their workspace, however many parts such offsets would make."""
+    S, N, K = 3000, 40, 64
+    gen = torch.Generator(device=DEV).manual_seed(E)
+    x, g = torch.randn(S, K, device=DEV, generator=gen), torch.randn(S, N, device=DEV, generator=gen)
+    w = torch.randn(E, N, K, device=DEV, generator=gen)
+    lib, size = be.load_library(), N * K
+    there_and_back = torch.arange(E + 1, device=DEV) % 2 * S
+    for offset in (there_and_back, torch.randint(-900, S + 900, (E + 1,), device=DEV, generator=gen)):
+        ordered = offset.clamp(0, S).cummax(0).values
+        assert torch.equal(be.expert_linear(x, w, offset), be.expert_linear(x, w, ordered))
+        nbytes = lib.hc_expert_linear_grad_workspace_bytes(S, E, N, K, 0)
+        assert nbytes > 0 and nbytes % 4 == 0
+        room = torch.full((nbytes // 4 + 70 * size,), 7.0, device=DEV)
+        gw = torch.empty(E, N, K, device=DEV)
+        assert lib.hc_expert_linear_grad(g.data_ptr(), x.data_ptr(), 0, offset.data_ptr(), S, E, N, K, gw.data_ptr(), room.data_ptr(),
+                                         nbytes, 0) == 0
+        torch.cuda.synchronize()
+        assert bool((room[nbytes // 4:] == 7).all())
+        assert torch.equal(gw, be.expert_linear_grad(g, x, ordered))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E", (2, 63, 64))
+def test_some_of_the_experts(E, dtype):
+    """A later part of a batch's offsets with its matrices: the rows of the other experts are zeros, and add nothing."""
+    gen = torch.Generator(device=DEV).manual_seed(E)
+    x, g = (torch.randn(700, d, device=DEV, generator=gen).to(dtype) for d in (72, 96))
+    w = torch.randn(E + 2, 96, 72, device=DEV, generator=gen).to(dtype)
+    offset = torch.randint(0, 700, (E + 3,), device=DEV, generator=gen).sort().values
+    offset[0] = 0
+    a, b = x.requires_grad_(True), w.requires_grad_(True)
+    y = be.expert_linear(a, b, offset)
+    gx, gw = torch.autograd.grad(y, (a, b), g)
+    some = b.detach()[1:-1].contiguous().requires_grad_(True)
+    part = be.expert_linear(a, some, offset[1:-1].contiguous())
+    hx, hw = torch.autograd.grad(part, (a, some), g)
+    mine = torch.zeros(700, 1, dtype=torch.bool, device=DEV)
+    mine[int(offset[1]):int(offset[-2])] = True
+    assert torch.equal(part, torch.where(mine, y, 0)) and torch.equal(hx, torch.where(mine, gx, 0)) and torch.equal(hw, gw[1:-1])
+
+
 def test_refusals():
     x, w, off = torch.randn(10, 8, device=DEV), torch.randn(2, 4, 8, device=DEV), offsets((4, 6))
     for call in (lambda: be.expert_linear(x, w.half(), off), lambda: be.expert_linear(x.double(), w.double(), off),
