@@ -253,10 +253,16 @@ struct MvArgs {
   const int64_t *offset;
 };
 
+// The place of a pair, -1 if it has none (or one that is not among the P).
+__device__ __forceinline__ int32_t mv_slot(const MvArgs &a, int64_t q) {
+  const int32_t s = a.slot[q];
+  return s < a.P ? s : -1;
+}
+
 template <typename T, int VEC, bool ANY>
 __device__ __forceinline__ void mv_zero_tail(const MvArgs &a, T *__restrict__ rows) {
   typedef mv_row<T, VEC, ANY> row;
-  const int64_t live = a.offset[a.E], rest = (a.P - live) * a.pieces;
+  const int64_t end = a.offset[a.E], live = end < 0 ? 0 : end, rest = (a.P - live) * a.pieces;
   for (int64_t i = (int64_t)blockIdx.x * HC_BLOCK + threadIdx.x; i < rest; i += (int64_t)gridDim.x * HC_BLOCK)
     row::set(rows + (live + i / a.pieces) * a.D + row::column((int)(i % a.pieces), a.D), typename row::raw{});
 }
@@ -270,7 +276,7 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_to(MvArgs a, const T *__restrict_
     const int c = row::column((int)(item - (uint32_t)i * (uint32_t)a.pieces), a.D);
     const typename row::raw v = row::get(x + i * a.D + c);
     for (int j = 0; j < a.k; ++j) {
-      const int32_t s = a.slot[i * a.k + j];
+      const int32_t s = mv_slot(a, i * a.k + j);
       if (s >= 0) row::set(rows + (int64_t)s * a.D + c, v);
     }
   }
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restric
     int32_t s[K];
     float w[K], p[K][VEC];
 #pragma unroll
-    for (int j = 0; j < K; ++j) s[j] = j0 + j < a.k ? a.slot[i * a.k + j0 + j] : -1;
+    for (int j = 0; j < K; ++j) s[j] = j0 + j < a.k ? mv_slot(a, i * a.k + j0 + j) : -1;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       w[j] = weight != nullptr && s[j] >= 0 ? weight[i * a.k + j0 + j] : 1.f;
@@ -329,7 +335,7 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from_grad(MvArgs a, const T *__re
       float w[K], dot[K];
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        s[j] = j0 + j < a.k ? a.slot[i * a.k + j0 + j] : -1;
+        s[j] = j0 + j < a.k ? mv_slot(a, i * a.k + j0 + j) : -1;
         w[j] = s[j] >= 0 ? weight[i * a.k + j0 + j] : 0.f;
         dot[j] = 0.f;
       }

@@ -331,3 +331,23 @@ def test_on_another_stream_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, layer())
+
+
+def test_places_that_are_not_there_count_as_none():
+    n, k, E, D = 20, 2, 3, 40
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    order = be.expert_order(choices(gen, n, k, E, 0.0), E)
+    none, far = order.slot.clone(), order.slot.clone()
+    none[5:8] = -1
+    far[5:8] = torch.tensor([n * k, 1 << 30, -7], device=DEV)
+    a, b = (be.ExpertOrder(s, order.pair, order.offset, n, k, E) for s in (none, far))
+    y, weight, g = (torch.randn(*s, device=DEV, generator=gen) for s in ((n * k, D), (n, k), (n, D)))
+    y.requires_grad_(True), weight.requires_grad_(True)
+    outs = []
+    for o in (a, b):
+        out = be.rows_from_experts(y, o, weight)
+        g_y, g_w = torch.autograd.grad(out, (y, weight), g)
+        placed = o.slot[(o.slot >= 0) & (o.slot < n * k)].long()
+        outs.append((out.detach(), g_y[placed], g_w, be.rows_to_experts(g, o)[placed]))
+    for u, v in zip(*outs):
+        assert torch.equal(u, v)
