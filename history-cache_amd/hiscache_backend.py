@@ -25,6 +25,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -1603,8 +1604,17 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 _stream_of_device = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
+def _no_tangent(*tensors):
+    """Forward-mode derivatives: the kernels have none, and a result without a tangent would count as a constant."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("this operator has no forward-mode derivative")
+
+
 def _together(t, *others):
-    """Do these tensors lie on one device, the current one (whose stream the launch goes to)?"""
+    """Do these tensors lie on one device, the current one (whose stream the launch goes to), and may a call read them?"""
+    _no_tangent(t, *others)
     index = t.get_device()
     together = index == _current_device()
     for o in others:
@@ -1620,6 +1630,7 @@ def _stream_for(t):
 
 def _arriving(g):
     """A gradient as the kernels read it: packed, with its own sign."""
+    _no_tangent(g)
     return g.contiguous().resolve_neg()
 
 

@@ -1,0 +1,65 @@
+"""The calls of the expert layer and of activations in 8 bits with operands that are not plain matrices in memory, inside
+autograd's other modes, and at the ends of their documented ranges."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import hiscache_backend as be
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def operands(seed=0):
+    """Every call of the layer by name, as a function of its floating-point operands, and those operands."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+
+    def draw(*shape):
+        return torch.randn(*shape, device=DEV, generator=gen)
+
+    order = be.expert_order(torch.randint(0, 3, (40, 2), device=DEV, generator=gen), 3)
+    offset = torch.tensor([0, 10, 20, 40], device=DEV)
+    kept = be.gated_pack(draw(40, 64))[1]
+    return {
+        "route": (lambda l: be.route_rows(l, 2)[1], [draw(40, 8)]),
+        "route, not normalised": (lambda l: be.route_rows(l, 2, normalize=False)[1], [draw(40, 8)]),
+        "to experts": (lambda x: be.rows_to_experts(x, order), [draw(40, 24)]),
+        "from experts": (lambda y, w: be.rows_from_experts(y, order, w), [draw(80, 24), draw(40, 2)]),
+        "from experts, unweighted": (lambda y: be.rows_from_experts(y, order), [draw(80, 24)]),
+        "linear": (lambda x, w: be.expert_linear(x, w, offset), [draw(40, 64), draw(3, 32, 64)]),
+        "linear_grad": (lambda g, x: be.expert_linear_grad(g, x, offset), [draw(40, 32), draw(40, 64)]),
+        "pack": (lambda x: be.unpack_rows(be.pack_rows(x)), [draw(40, 64)]),
+        "gated_pack": (lambda x: be.gated_pack(x, keep=False)[0], [draw(40, 64)]),
+        "gated_grad": (lambda g: be.gated_grad(kept, g)[0], [draw(40, 32)]),
+        "gated_experts": (lambda x, a, b: be.gated_experts(x, a, b, offset), [draw(40, 24), draw(3, 64, 24), draw(3, 16, 32)]),
+    }
+
+
+CALLS = ("route", "route, not normalised", "to experts", "from experts", "from experts, unweighted", "linear", "linear_grad", "pack",
+         "gated_pack", "gated_grad", "gated_experts")
+NODES = tuple(c for c in CALLS if c not in ("linear_grad", "pack", "gated_pack", "gated_grad"))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_tangent_is_refused(name):
+    call, args = operands()[name]
+    want = call(*args)
+    with forward_ad.dual_level():
+        assert torch.equal(call(*args), want)                     # plain operands, whatever level there is
+        for i, a in enumerate(args):
+            dual = [*args[:i], forward_ad.make_dual(a, torch.ones_like(a)), *args[i + 1:]]
+            with pytest.raises(NotImplementedError):
+                call(*dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError):     # forward mode does not go by the grad mode
+                call(*dual)
+
+
+@pytest.mark.parametrize("name", NODES)
+def test_a_tangent_of_a_gradient_is_refused(name):
+    call, args = operands()[name]
+    args = [a.requires_grad_(True) for a in args]
+    out = call(*args)
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(out, args, g)
