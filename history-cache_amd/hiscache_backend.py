@@ -1628,10 +1628,23 @@ def _stream_for(t):
     return _stream_of_device(t.get_device())
 
 
+def _stored(t):
+    """t as the kernels read it: a lazily negated tensor lies in memory with the other sign, zeros that were never written
+    nowhere."""
+    if t.is_neg():
+        return t.resolve_neg()
+    return t.clone() if t._is_zerotensor() else t
+
+
+def _operand(t, name, dtype=None):
+    """``_dev`` of a call's operand, and it as the kernels read it."""
+    return _stored(_dev(t, name, dtype))
+
+
 def _arriving(g):
-    """A gradient as the kernels read it: packed, with its own sign."""
+    """A gradient as the kernels read it, packed."""
     _no_tangent(g)
-    return g.contiguous().resolve_neg()
+    return _stored(g.contiguous())
 
 
 # The operators below are autograd nodes where a gradient may be asked for; without one the node itself, which costs the
@@ -1691,7 +1704,7 @@ def route_rows(logits, top_k, normalize=True):
     weight fp32 [n, top_k]); ``normalize``: the weights of a row are divided by their sum.  A logit of -inf closes an
     expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
     weights.  The gradient of the weights reaches ``logits``.  top_k <= 32."""
-    _dev(logits, "logits")
+    logits = _operand(logits, "logits")
     _float_dtype(logits, "logits")
     top_k = int(top_k)
     if logits.dim() != 2:
@@ -1723,7 +1736,7 @@ def expert_order(expert, num_expert):
     are in ascending order.  Numbers outside [0, num_expert) name no expert.  Nothing is read back: the sizes stay on the
     device.  num_expert <= 1024, n * top_k < 2^31."""
     lib = load_library()
-    _dev(expert, "expert", torch.int64)
+    expert = _operand(expert, "expert", torch.int64)
     if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
         raise ValueError("expert must be [n] or [n, top_k]")
     _together(expert)
@@ -1795,8 +1808,8 @@ def _from_experts_grads(g, y, order, weight):
 
 
 def _expert_rows(t, name, order, a_choice):
-    """Is ``t`` a matrix with a row for every row of the order, or (``a_choice``) for every choice of one?"""
-    _dev(t, name)
+    """``t``, if it is a matrix with a row for every row of the order, or (``a_choice``) for every choice of one."""
+    t = _operand(t, name)
     _float_dtype(t, name)
     if not isinstance(order, ExpertOrder):
         raise TypeError("order must be an ExpertOrder")
@@ -1804,12 +1817,13 @@ def _expert_rows(t, name, order, a_choice):
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
         raise ValueError(f"{name} must be [{rows}, D], got {tuple(t.shape)}")
     _together(t, order.slot)
+    return t
 
 
 def rows_to_experts(x, order):
     """The rows of x [n, D] in expert order, [n * top_k, D]: place p holds row ``order.pair[p] // top_k``, zeros where there is
     no pair.  The gradient of a row is the sum over its places."""
-    _expert_rows(x, "x", order, False)
+    x = _expert_rows(x, "x", order, False)
     return (_RowsToExperts.apply if _watched(x) else _to_experts)(x, order)
 
 
@@ -1817,9 +1831,9 @@ def rows_from_experts(y, order, weight=None):
     """``out[i] = sum_j weight[i, j] * y[slot of (i, j)]`` for the experts' results y [n * top_k, D], summed in fp32 in the
     order of j; choices that name no expert add nothing.  ``weight`` fp32 [n, top_k] (None: ones).  Gradients for y and
     weight."""
-    _expert_rows(y, "y", order, True)
+    y = _expert_rows(y, "y", order, True)
     if weight is not None:
-        _dev(weight, "weight", torch.float32)
+        weight = _operand(weight, "weight", torch.float32)
         if weight.numel() != order.places:
             raise ValueError(f"weight must hold {order.places} values")
         _together(y, weight)
@@ -1852,19 +1866,20 @@ def _expert_product(x, w, offset, transposed):
 
 
 def _expert_offset(offset):
-    _dev(offset, "offset", torch.int64)
+    offset = _operand(offset, "offset", torch.int64)
     if offset.dim() != 1 or offset.numel() < 2:
         raise ValueError("offset must be [E + 1]")
+    return offset
 
 
 def expert_linear(x, w, offset):
     """``x[s] @ w[e].t()`` for the rows s = offset[e] .. offset[e + 1] of x [S, K], w [E, N, K] of x's type; rows before
     offset[0] and behind offset[E] are zeros.  ``offset`` int64 [E + 1] stays on the device.  Sums in fp32 (fp32 rows: fp32 products), one
     rounding to the type of x.  Gradients for x and w."""
-    _dev(x, "x")
+    x = _operand(x, "x")
     _float_dtype(x, "x")
-    _dev(w, "w", x.dtype)
-    _expert_offset(offset)
+    w = _operand(w, "w", x.dtype)
+    offset = _expert_offset(offset)
     if x.dim() != 2 or w.dim() != 3 or w.shape[2] != x.shape[1] or offset.numel() != w.shape[0] + 1:
         raise ValueError(f"x [S, K], w [E, N, K] and offset [E + 1] do not fit: {tuple(x.shape)}, {tuple(w.shape)}, "
                          f"{tuple(offset.shape)}")
@@ -1875,9 +1890,9 @@ def expert_linear(x, w, offset):
 def expert_linear_grad(g, x, offset):
     """``g[rows of e].t() @ x[rows of e]`` for every expert e: [E, N, K] of x's type from g [S, N] and x [S, K]."""
     lib = load_library()
-    _dev(x, "x")
-    _dev(g, "g", x.dtype)
-    _expert_offset(offset)
+    x = _operand(x, "x")
+    g = _operand(g, "g", x.dtype)
+    offset = _expert_offset(offset)
     if g.dim() != 2 or x.dim() != 2 or g.shape[0] != x.shape[0]:
         raise ValueError("g [S, N] and x [S, K] must have the same number of rows")
     _together(x, g, offset)
@@ -1908,20 +1923,21 @@ def _packed_like(x, halves, group):
 
 
 def _pack_arguments(x, name, group):
-    _dev(x, name)
+    x = _operand(x, name)
     _float_dtype(x, name)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"{name} must be [n, F]")
     if group not in (32, 64, 128):
         raise ValueError(f"group must be 32, 64 or 128, got {group}")
     _together(x)
+    return x
 
 
 def pack_rows(x, group=64):
     """x [n, F] in 8 bits: every ``group`` adjacent columns of a row share an fp32 scale m * (1 / 127) (m their largest
     magnitude) and keep rint(x * (1 / m * 127)).  Half a scale is the most that a value is off.  Groups whose m is below 2^-120 are kept as
     zeros; one that holds an infinity or a NaN reads back as NaN."""
-    _pack_arguments(x, "x", group)
+    x = _pack_arguments(x, "x", group)
     codes, scale = _packed_like(x, 1, group)
     _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], group, codes.data_ptr(),
                                        scale.data_ptr(), _stream_for(x)), "hc_pack_rows")
@@ -1947,7 +1963,7 @@ def unpack_rows(kept, dtype=None):
 def gated_pack(x, group=64, keep=True):
     """``silu(a) * b`` for rows [a | b] of x [n, 2 F], and x in 8 bits for :func:`gated_grad`: (h [n, F], PackedRows), the
     second one None without ``keep``."""
-    _pack_arguments(x, "x", group)
+    x = _pack_arguments(x, "x", group)
     if x.shape[1] % 2 != 0:
         raise ValueError("x must hold two halves of the same width")
     n, F = x.shape[0], x.shape[1] // 2
@@ -1962,7 +1978,7 @@ def gated_grad(kept, g):
     """From what :func:`gated_pack` kept and the gradient g [n, F] of h: the gradient of x [n, 2 F], and h [n, F] again."""
     codes, scale = kept.codes, kept.scale
     n, F = codes.shape[0], codes.shape[1] // 2
-    _dev(g, "g", kept.dtype)
+    g = _operand(g, "g", kept.dtype)
     if codes.shape[1] % 2 or scale.shape[1] != 2 * -(-F // kept.group) or g.shape != (n, F):
         raise ValueError("g must be [n, F] for rows [n, 2 F] that gated_pack kept")
     _together(g, codes)
@@ -1997,10 +2013,10 @@ def gated_experts(rows, w_in, w_out, offset, group=64):
     [E, D, H], offset as in :func:`expert_linear`.  One autograd node, which keeps [a | b] in 8 bits (:func:`gated_pack`) and no
     other row of that width: 2 H bytes a row and a scale for every ``group`` columns, where operator by operator [a | b] and
     silu(a) * b are kept, 12 H bytes in fp32 and 6 H in half precision."""
-    _pack_arguments(rows, "rows", group)
-    _dev(w_in, "w_in", rows.dtype)
-    _dev(w_out, "w_out", rows.dtype)
-    _expert_offset(offset)
+    rows = _pack_arguments(rows, "rows", group)
+    w_in = _operand(w_in, "w_in", rows.dtype)
+    w_out = _operand(w_out, "w_out", rows.dtype)
+    offset = _expert_offset(offset)
     E = offset.numel() - 1
     if (w_in.dim() != 3 or w_out.dim() != 3 or w_in.shape[0] != E or w_out.shape[0] != E or w_in.shape[2] != rows.shape[1]
             or w_in.shape[1] != 2 * w_out.shape[2]):

@@ -63,3 +63,38 @@ def test_a_tangent_of_a_gradient_is_refused(name):
         g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(out, args, g)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_lazily_negated_operand_counts_with_its_sign(name):
+    call, args = operands()[name]
+    for i, a in enumerate(args):
+        lazy = torch._neg_view(-a)
+        assert lazy.is_neg() and torch.equal(call(*args[:i], lazy, *args[i + 1:]), call(*args))
+        if name in NODES:
+            leaf = (-a).requires_grad_(True)
+            grad, = torch.autograd.grad(call(*args[:i], torch._neg_view(leaf), *args[i + 1:]).sum(), leaf)
+            plain = a.clone().requires_grad_(True)
+            want, = torch.autograd.grad(call(*args[:i], plain, *args[i + 1:]).sum(), plain)
+            assert torch.equal(grad, -want)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_zeros_that_were_never_written(name):
+    call, args = operands()[name]
+    for i, a in enumerate(args):
+        lazy = torch._efficientzerotensor(a.shape, device=DEV)
+        want = call(*args[:i], torch.zeros_like(a), *args[i + 1:])
+        assert torch.equal(call(*args[:i], lazy, *args[i + 1:]), want)
+
+
+@pytest.mark.parametrize("name", NODES)
+def test_gradients_that_are_negated_or_never_written(name):
+    call, args = operands()[name]
+    args = [a.requires_grad_(True) for a in args]
+    out = call(*args)
+    g = torch.randn(out.shape, device=DEV)
+    for lazy, plain in ((torch._neg_view(-g), g), (torch._efficientzerotensor(g.shape, device=DEV), torch.zeros_like(g))):
+        got = torch.autograd.grad(out, args, lazy, retain_graph=True)
+        for a, b in zip(got, torch.autograd.grad(out, args, plain, retain_graph=True)):
+            assert torch.equal(a, b)
