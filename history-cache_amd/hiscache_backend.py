@@ -1769,30 +1769,36 @@ def _from_experts(y, order, weight):
     return out
 
 
+# (the order's tensors are saved ones, so that autograd notices a change in place between forward and backward)
+def _saved_order(ctx, slot, offset):
+    return ExpertOrder(slot, None, offset, *ctx.hc)
+
+
 class _RowsToExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
-        ctx.hc = order
+        ctx.save_for_backward(order.slot, order.offset)
+        ctx.hc = (order.rows, order.top_k, order.experts)
         return _to_experts(x, order)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        return _from_experts(_arriving(g), ctx.hc, None), None
+        return _from_experts(_arriving(g), _saved_order(ctx, *ctx.saved_tensors), None), None
 
 
 class _RowsFromExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, order, weight):
-        ctx.hc = order
-        ctx.save_for_backward(y if weight is not None else None, weight)
+        ctx.save_for_backward(y if weight is not None else None, weight, order.slot, order.offset)
+        ctx.hc = (order.rows, order.top_k, order.experts)
         return _from_experts(y, order, weight)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        y, weight = ctx.saved_tensors
-        order, g = ctx.hc, _arriving(g)
+        y, weight, slot, offset = ctx.saved_tensors
+        order, g = _saved_order(ctx, slot, offset), _arriving(g)
         if weight is None:
             return _to_experts(g, order), None, None
         return _from_experts_grads(g, y, order, weight)

@@ -98,3 +98,17 @@ def test_gradients_that_are_negated_or_never_written(name):
         got = torch.autograd.grad(out, args, lazy, retain_graph=True)
         for a, b in zip(got, torch.autograd.grad(out, args, plain, retain_graph=True)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", ("slot", "offset"))
+@pytest.mark.parametrize("weighted", (True, False))
+def test_an_order_changed_in_place_is_noticed(what, weighted):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, y = (torch.randn(n, 24, device=DEV, generator=gen).requires_grad_(True) for n in (40, 80))
+    weight = torch.rand(40, 2, device=DEV, generator=gen) if weighted else None
+    order = be.expert_order(torch.randint(0, 3, (40, 2), device=DEV, generator=gen), 3)
+    outs = be.rows_to_experts(x, order), be.rows_from_experts(y, order, weight)
+    getattr(order, what).fill_(0)
+    for out, leaf in zip(outs, (x, y)):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), leaf)
