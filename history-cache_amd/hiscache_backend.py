@@ -1813,16 +1813,26 @@ def _from_experts_grads(g, y, order, weight):
     return grad_y, None, grad_weight
 
 
+def _check_order(order):
+    """Can the kernels go by this order?  They read a place for every pair and the offset behind the last expert."""
+    if not isinstance(order, ExpertOrder):
+        raise TypeError("order must be an ExpertOrder")
+    slot, offset = order.slot, order.offset
+    if (slot.dtype != torch.int32 or offset.dtype != torch.int64 or slot.numel() != order.rows * order.top_k
+            or offset.numel() != order.experts + 1 or not slot.is_contiguous() or not offset.is_contiguous()):
+        raise ValueError(f"the order must hold {order.rows * order.top_k} places (slot, int32) and {order.experts + 1} offsets "
+                         "(int64), both contiguous")
+
+
 def _expert_rows(t, name, order, a_choice):
     """``t``, if it is a matrix with a row for every row of the order, or (``a_choice``) for every choice of one."""
     t = _operand(t, name)
     _float_dtype(t, name)
-    if not isinstance(order, ExpertOrder):
-        raise TypeError("order must be an ExpertOrder")
+    _check_order(order)
     rows = order.places if a_choice else order.rows
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
         raise ValueError(f"{name} must be [{rows}, D], got {tuple(t.shape)}")
-    _together(t, order.slot)
+    _together(t, order.slot, order.offset)
     return t
 
 

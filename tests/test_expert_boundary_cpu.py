@@ -130,3 +130,16 @@ def test_the_module_checks_its_arguments_without_a_gpu():
         y = (x * x).sum()
     y.backward()
     assert torch.equal(x.grad, 2 * x)
+
+
+def test_an_order_that_does_not_fit_its_rows_is_refused():
+    import hiscache_backend as be
+    slot, offset = torch.zeros(12, dtype=torch.int32), torch.zeros(5, dtype=torch.int64)
+    be._check_order(be.ExpertOrder(slot, slot, offset, 6, 2, 4))
+    wide = torch.zeros(12, 2, dtype=torch.int32)
+    for bad in ((slot[:11], offset, 6, 2, 4), (slot, offset, 7, 2, 4), (slot, offset, 6, 3, 4), (slot, offset[:4], 6, 2, 4),
+                (slot, offset, 6, 2, 5), (slot.long(), offset, 6, 2, 4), (slot, offset.int(), 6, 2, 4), (wide[:, 0], offset, 6, 2, 4)):
+        with pytest.raises(ValueError):
+            be._check_order(be.ExpertOrder(bad[0], slot, *bad[1:]))
+    with pytest.raises(TypeError):
+        be._check_order(slot)

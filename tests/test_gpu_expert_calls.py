@@ -112,3 +112,15 @@ def test_an_order_changed_in_place_is_noticed(what, weighted):
     for out, leaf in zip(outs, (x, y)):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(out.sum(), leaf)
+
+
+def test_an_order_that_does_not_fit_is_refused_by_the_calls():
+    x, y, weight = torch.randn(6, 8, device=DEV), torch.randn(12, 8, device=DEV), torch.ones(6, 2, device=DEV)
+    good = be.expert_order(torch.zeros(6, 2, dtype=torch.int64, device=DEV), 4)
+    for slot, offset in ((good.slot[:11], good.offset), (good.slot, good.offset[:4]), (good.slot.long(), good.offset),
+                         (good.slot.cpu(), good.offset), (good.slot, good.offset.cpu())):
+        order = be.ExpertOrder(slot, good.pair, offset, 6, 2, 4)
+        for call in (lambda: be.rows_to_experts(x, order), lambda: be.rows_from_experts(y, order),
+                     lambda: be.rows_from_experts(y, order, weight)):
+            with pytest.raises(ValueError):
+                call()
