@@ -1949,6 +1949,21 @@ def _pack_arguments(x, name, group):
     return x
 
 
+def _check_kept(kept, halves):
+    """Rows and columns of what :func:`pack_rows` (``halves`` 1) or :func:`gated_pack` (2) kept, if it is whole."""
+    codes, scale, group = kept.codes, kept.scale, kept.group
+    if codes.dim() != 2 or scale.dim() != 2 or group not in (32, 64, 128) or codes.shape[1] < 1 or codes.shape[1] % halves:
+        raise ValueError("codes must be [n, columns], scale [n, groups], a group 32, 64 or 128 columns")
+    n, F = codes.shape[0], codes.shape[1] // halves
+    if tuple(scale.shape) != (n, halves * -(-F // group)):
+        raise ValueError("the scales do not fit the codes" + (": were these rows kept by gated_pack?" if halves == 1 else
+                                                              ": rows [n, 2 F] that gated_pack kept"))
+    if (codes.dtype != torch.int8 or scale.dtype != torch.float32 or not codes.is_contiguous() or not scale.is_contiguous()
+            or kept.dtype not in _DTYPES):
+        raise ValueError("codes must be int8 and scale float32, both contiguous, dtype float32, float16 or bfloat16")
+    return n, F
+
+
 def pack_rows(x, group=64):
     """x [n, F] in 8 bits: every ``group`` adjacent columns of a row share an fp32 scale m * (1 / 127) (m their largest
     magnitude) and keep rint(x * (1 / m * 127)).  Half a scale is the most that a value is off.  Groups whose m is below 2^-120 are kept as
@@ -1966,10 +1981,8 @@ def unpack_rows(kept, dtype=None):
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     codes, scale = kept.codes, kept.scale
-    n, F = codes.shape
-    if scale.shape[1] != -(-F // kept.group):
-        raise ValueError("these rows were kept by gated_pack")
-    _together(codes)
+    n, F = _check_kept(kept, 1)
+    _together(codes, scale)
     x = codes.new_empty((n, F), dtype=dtype)
     _check(load_library().hc_unpack_rows(codes.data_ptr(), scale.data_ptr(), n, F, kept.group, x.data_ptr(),
                                          _DTYPES[dtype], _stream_for(codes)), "hc_unpack_rows")
@@ -1993,11 +2006,11 @@ def gated_pack(x, group=64, keep=True):
 def gated_grad(kept, g):
     """From what :func:`gated_pack` kept and the gradient g [n, F] of h: the gradient of x [n, 2 F], and h [n, F] again."""
     codes, scale = kept.codes, kept.scale
-    n, F = codes.shape[0], codes.shape[1] // 2
+    n, F = _check_kept(kept, 2)
     g = _operand(g, "g", kept.dtype)
-    if codes.shape[1] % 2 or scale.shape[1] != 2 * -(-F // kept.group) or g.shape != (n, F):
-        raise ValueError("g must be [n, F] for rows [n, 2 F] that gated_pack kept")
-    _together(g, codes)
+    if g.shape != (n, F):
+        raise ValueError(f"g must be [{n}, {F}], got {tuple(g.shape)}")
+    _together(g, codes, scale)
     gx, h = g.new_empty((n, 2 * F)), torch.empty_like(g)
     _check(load_library().hc_gated_grad(codes.data_ptr(), scale.data_ptr(), g.data_ptr(), _DTYPES[kept.dtype], n, F,
                                         kept.group, gx.data_ptr(), h.data_ptr(), _stream_for(g)), "hc_gated_grad")

@@ -143,3 +143,22 @@ def test_an_order_that_does_not_fit_its_rows_is_refused():
             be._check_order(be.ExpertOrder(bad[0], slot, *bad[1:]))
     with pytest.raises(TypeError):
         be._check_order(slot)
+
+
+def test_kept_rows_that_are_not_whole_are_refused():
+    import hiscache_backend as be
+    codes, scale = torch.zeros(6, 200, dtype=torch.int8), torch.zeros(6, 4)
+    assert be._check_kept(be.PackedRows(codes, scale, 64, torch.float16), 1) == (6, 200)
+    assert be._check_kept(be.PackedRows(codes, scale, 64, torch.float16), 2) == (6, 100)
+    assert be._check_kept(be.PackedRows(codes[:0], scale[:0], 64, torch.float16), 1) == (0, 200)
+    for halves in (1, 2):
+        for bad in ((codes, scale[:5], 64), (codes, scale[:, :3], 64), (codes, scale, 32), (codes, scale, 48), (codes, scale.view(-1), 64),
+                    (codes.view(-1), scale, 64), (codes.int(), scale, 64), (codes, scale.double(), 64),
+                    (torch.zeros(12, 200, dtype=torch.int8)[::2], scale, 64), (codes, torch.zeros(6, 8)[:, ::2], 64),
+                    (codes[:, :0], scale[:, :0], 64)):
+            with pytest.raises(ValueError):
+                be._check_kept(be.PackedRows(*bad, torch.float16), halves)
+        with pytest.raises(ValueError):
+            be._check_kept(be.PackedRows(codes, scale, 64, torch.float64), halves)
+    with pytest.raises(ValueError):
+        be._check_kept(be.PackedRows(torch.zeros(6, 129, dtype=torch.int8), scale, 64, torch.float16), 2)

@@ -124,3 +124,13 @@ def test_an_order_that_does_not_fit_is_refused_by_the_calls():
                      lambda: be.rows_from_experts(y, order, weight)):
             with pytest.raises(ValueError):
                 call()
+
+
+def test_kept_rows_that_are_not_whole_are_refused_by_the_calls():
+    x, g = torch.randn(6, 128, device=DEV), torch.randn(6, 64, device=DEV)
+    plain, gated = be.pack_rows(x), be.gated_pack(x)[1]
+    for kept, call in ((plain, be.unpack_rows), (gated, lambda k: be.gated_grad(k, g))):
+        for codes, scale in ((kept.codes, kept.scale[:5]), (kept.codes[:, ::2], kept.scale), (kept.codes, kept.scale.cpu()),
+                             (kept.codes, kept.scale.half()), (kept.codes.int(), kept.scale)):
+            with pytest.raises(ValueError):
+                call(be.PackedRows(codes, scale, 64, x.dtype))
