@@ -70,7 +70,8 @@ def packed_activations(group=64, min_elements=1 << 16):
     def pack(t):
         if (not t.is_cuda or t.dtype not in be._DTYPES or t.dim() < 2 or t.numel() < min_elements or not t.is_contiguous()
                 or (t.is_leaf and t.requires_grad) or t.device.index != torch.cuda.current_device()):
-            return t
+            # (a node that held its own result would be held by it in turn, out of the garbage collector's sight)
+            return t if t.is_leaf else t.detach()
         return be.pack_rows(t.detach().view(-1, t.shape[-1]), group), t.shape
 
     def unpack(kept):

@@ -1,0 +1,34 @@
+"""What ``packed_activations`` does with tensors that it keeps as they are, on the CPU, where that is all of them."""
+import gc
+import weakref
+
+import pytest
+import torch
+
+import hiscache
+
+
+@pytest.mark.parametrize("op", (torch.exp, torch.sigmoid, torch.relu, lambda x: torch.softmax(x, 1)))
+def test_a_graph_without_a_backward_pass_is_freed(op):
+    x = torch.randn(6, 8, requires_grad=True)
+    with hiscache.packed_activations(min_elements=1):
+        y = op(x * 2)
+    result = weakref.ref(y)
+    del y
+    gc.collect()
+    assert result() is None
+
+
+def test_gradients_through_what_is_kept():
+    x, w = torch.randn(6, 8, requires_grad=True), torch.randn(8, 5, requires_grad=True)
+
+    def loss():
+        return (torch.tanh(x @ w).exp() * 2).sum()
+
+    want = torch.autograd.grad(loss(), (x, w))
+    with hiscache.packed_activations(min_elements=1):
+        y = loss()
+        g, = torch.autograd.grad((w * w * w).sum(), w, create_graph=True)
+    for a, b in zip(torch.autograd.grad(y, (x, w)), want):
+        assert torch.equal(a, b)
+    assert torch.allclose(torch.autograd.grad(g.sum(), w)[0], 6 * w)          # a gradient of a gradient
