@@ -71,10 +71,18 @@ def packed_activations(group=64, min_elements=1 << 16):
         if (not t.is_cuda or t.dtype not in be._DTYPES or t.dim() < 2 or t.numel() < min_elements or not t.is_contiguous()
                 or (t.is_leaf and t.requires_grad) or t.device.index != torch.cuda.current_device()):
             # (a node that held its own result would be held by it in turn, out of the garbage collector's sight)
-            return t if t.is_leaf else t.detach()
+            t = t if t.is_leaf else t.detach()
+            return t, t._version
         return be.pack_rows(t.detach().view(-1, t.shape[-1]), group), t.shape
 
-    def unpack(kept):
-        return kept if isinstance(kept, torch.Tensor) else be.unpack_rows(kept[0]).view(kept[1])
+    def unpack(saved):
+        kept, of = saved
+        if not isinstance(kept, torch.Tensor):
+            return be.unpack_rows(kept).view(of)
+        # (autograd itself looks at versions only where there are no hooks)
+        if kept._version != of:
+            raise RuntimeError("one of the variables needed for gradient computation has been modified by an inplace operation: "
+                               f"{kept.dtype} {list(kept.shape)} is at version {kept._version}; expected version {of} instead")
+        return kept
 
     return torch.autograd.graph.saved_tensors_hooks(pack, unpack)

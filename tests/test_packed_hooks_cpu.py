@@ -32,3 +32,23 @@ def test_gradients_through_what_is_kept():
     for a, b in zip(torch.autograd.grad(y, (x, w)), want):
         assert torch.equal(a, b)
     assert torch.allclose(torch.autograd.grad(g.sum(), w)[0], 6 * w)          # a gradient of a gradient
+
+
+@pytest.mark.parametrize("which", ("parameter", "result", "view", "data"))
+def test_what_is_changed_in_place_before_the_backward_pass_is_noticed(which):
+    x, w = torch.randn(6, 8), torch.randn(8, 8, requires_grad=True)
+    with hiscache.packed_activations(min_elements=1):
+        h = (x @ w).exp()
+        y = (h.view(48) * 3).sum() + ((h @ w) ** 2).sum()
+    with torch.no_grad():
+        {"parameter": w, "result": h, "view": h[:1], "data": x}[which].mul_(100)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_operators_in_place_within_the_context():
+    a = torch.randn(6, 8, requires_grad=True)
+    with hiscache.packed_activations(min_elements=1):
+        y = ((a * 2).exp_() + 1).sigmoid_()
+    got, = torch.autograd.grad(y.sum(), a)
+    assert torch.equal(got, torch.autograd.grad(((a * 2).exp() + 1).sigmoid().sum(), a)[0])
