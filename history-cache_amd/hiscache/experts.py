@@ -58,18 +58,23 @@ class ExpertMLP(torch.nn.Module):
                 f"normalize={self.normalize}, group={self.group}")
 
 
+def _is_activation(t, min_elements):
+    """Is what autograd saves here a matrix that may be kept in 8 bits?"""
+    return (t.layout is torch.strided and t.dtype in hiscache_backend._DTYPES and t.dim() >= 2 and t.numel() >= max(min_elements, 1)
+            and t.is_contiguous() and not (t.is_leaf and t.requires_grad))
+
+
 def packed_activations(group=64, min_elements=1 << 16):
     """Context in which what autograd saves for backward is kept in 8 bits, a scale for every ``group`` columns
     (``hiscache_backend.pack_rows``): the gradients are those at activations that are off by up to half a scale.
 
     Kept as they are: parameters and other leaves that need a gradient, whole numbers, tensors of fewer than ``min_elements``
-    values or without a last dimension of their own, and anything not packed in the current GPU's memory.  Put it around the
+    values or without a last dimension of their own, sparse tensors, and anything not packed in the current GPU's memory.  Put it around the
     layers whose activations may be rounded; a loss, a softmax or the router's weights are better left outside."""
     be = hiscache_backend
 
     def pack(t):
-        if (not t.is_cuda or t.dtype not in be._DTYPES or t.dim() < 2 or t.numel() < min_elements or not t.is_contiguous()
-                or (t.is_leaf and t.requires_grad) or t.device.index != torch.cuda.current_device()):
+        if not t.is_cuda or t.device.index != torch.cuda.current_device() or not _is_activation(t, min_elements):
             # (a node that held its own result would be held by it in turn, out of the garbage collector's sight)
             t = t if t.is_leaf else t.detach()
             return t, t._version

@@ -52,3 +52,21 @@ def test_operators_in_place_within_the_context():
         y = ((a * 2).exp_() + 1).sigmoid_()
     got, = torch.autograd.grad(y.sum(), a)
     assert torch.equal(got, torch.autograd.grad(((a * 2).exp() + 1).sigmoid().sum(), a)[0])
+
+
+def test_what_counts_as_an_activation():
+    is_activation = hiscache.experts._is_activation
+    h = torch.randn(6, 8)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        assert is_activation(h.to(dtype), 1) and is_activation(h.view(2, 3, 8).to(dtype), 48)
+    for other in (h.view(-1), h.double(), h.long(), h.t(), h[:, ::2], h.clone().requires_grad_(True)):
+        assert not is_activation(other, 1)
+    assert not is_activation(h, 49)
+    for empty in (h[:0], h[:, :0], torch.empty(0, 0)):
+        assert not is_activation(empty, 0)
+
+
+@pytest.mark.parametrize("layout", (torch.sparse_coo, torch.sparse_csr, torch.sparse_csc, torch.sparse_bsr))
+def test_sparse_matrices_are_kept_as_they_are(layout):
+    blocks = dict(blocksize=(2, 2)) if layout is torch.sparse_bsr else {}
+    assert not hiscache.experts._is_activation(torch.eye(8).to_sparse(layout=layout, **blocks), 1)
