@@ -1663,6 +1663,15 @@ def _once(backward):
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
+# What the nodes keep for themselves (routing weights, logits, the scales of rows in 8 bits) is saved as the whole numbers that its
+# bits are: hooks on saved tensors that round matrices leave those alone.
+_WORD = {torch.float32: torch.int32, torch.float16: torch.int16, torch.bfloat16: torch.int16}
+
+
+def _bits(t):
+    return None if t is None else t.view(_WORD[t.dtype])
+
+
 def _route(logits, top_k, normalize):
     n, E = logits.shape
     expert = logits.new_empty((n, top_k), dtype=torch.int64)
@@ -1678,8 +1687,9 @@ class _RouteRows(torch.autograd.Function):
         expert, weight = _route(logits, top_k, normalize)
         ctx.mark_non_differentiable(expert)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, expert, weight)
-        ctx.hc = (top_k, normalize)
+        # (normalised, the gradient goes by the weights alone)
+        ctx.save_for_backward(None if normalize else _bits(logits), expert, _bits(weight))
+        ctx.hc = (top_k, normalize, logits.shape, logits.dtype)
         return expert, weight
 
     @staticmethod
@@ -1688,13 +1698,12 @@ class _RouteRows(torch.autograd.Function):
         if g is None:
             return None, None, None
         logits, expert, weight = ctx.saved_tensors
-        top_k, normalize = ctx.hc
-        n, E = logits.shape
+        top_k, normalize, (n, E), dtype = ctx.hc
         g = _arriving(g)
-        grad = torch.empty_like(logits)
-        _check(load_library().hc_route_rows_grad(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, normalize,
-                                                 expert.data_ptr(), weight.data_ptr(), g.data_ptr(), grad.data_ptr(),
-                                                 _stream_for(logits)), "hc_route_rows_grad")
+        grad = g.new_empty((n, E), dtype=dtype)
+        _check(load_library().hc_route_rows_grad(_ptr(logits), _DTYPES[dtype], n, E, top_k, normalize, expert.data_ptr(),
+                                                 weight.data_ptr(), g.data_ptr(), grad.data_ptr(), _stream_for(g)),
+               "hc_route_rows_grad")
         return grad, None, None
 
 
@@ -1790,7 +1799,7 @@ class _RowsToExperts(torch.autograd.Function):
 class _RowsFromExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, order, weight):
-        ctx.save_for_backward(y if weight is not None else None, weight, order.slot, order.offset)
+        ctx.save_for_backward(y if weight is not None else None, _bits(weight), order.slot, order.offset)
         ctx.hc = (order.rows, order.top_k, order.experts)
         return _from_experts(y, order, weight)
 
@@ -1801,7 +1810,7 @@ class _RowsFromExperts(torch.autograd.Function):
         order, g = _saved_order(ctx, slot, offset), _arriving(g)
         if weight is None:
             return _to_experts(g, order), None, None
-        return _from_experts_grads(g, y, order, weight)
+        return _from_experts_grads(g, y, order, weight.view(torch.float32))
 
 
 def _from_experts_grads(g, y, order, weight):
@@ -2021,7 +2030,7 @@ class _GatedExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w_in, w_out, offset, group):
         h, kept = gated_pack(_expert_product(rows, w_in, offset, False), group)
-        ctx.save_for_backward(rows, w_in, w_out, offset, kept.codes, kept.scale)
+        ctx.save_for_backward(rows, w_in, w_out, offset, kept.codes, _bits(kept.scale))
         ctx.hc = (group, rows.dtype)
         return _expert_product(h, w_out, offset, False)
 
@@ -2030,7 +2039,7 @@ class _GatedExperts(torch.autograd.Function):
     def backward(ctx, g):
         rows, w_in, w_out, offset, codes, scale = ctx.saved_tensors
         need, g = ctx.needs_input_grad, _arriving(g)
-        g_pre, h = gated_grad(PackedRows(codes, scale, *ctx.hc), _expert_product(g, w_out, offset, True))
+        g_pre, h = gated_grad(PackedRows(codes, scale.view(torch.float32), *ctx.hc), _expert_product(g, w_out, offset, True))
         g_out = expert_linear_grad(g, h, offset) if need[2] else None
         del h
         return (_expert_product(g_pre, w_in, offset, True) if need[0] else None,
