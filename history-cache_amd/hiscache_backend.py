@@ -1354,6 +1354,15 @@ def bn_relu_supported(x, channels):
     return x.is_cuda and x.dtype == torch.float32 and channels % 4 == 0 and 4 <= channels <= BN_RELU_MAX_CHANNELS
 
 
+# What the nodes keep for themselves (statistics, routing weights, logits, the scales of rows in 8 bits) is saved as the whole numbers that its
+# bits are: hooks on saved tensors that round matrices leave those alone.
+_WORD = {torch.float32: torch.int32, torch.float16: torch.int16, torch.bfloat16: torch.int16}
+
+
+def _bits(t):
+    return None if t is None else t.view(_WORD[t.dtype])
+
+
 class _BiasBnRelu(torch.autograd.Function):
     """relu(batch_norm(x + bias)) in training mode as one autograd node over ``hc_bn_relu_fwd`` /
     ``hc_bn_relu_bwd`` (/root/reference/hiscache/history_model.py:139-140).  ``x`` comes WITHOUT the
@@ -1372,7 +1381,7 @@ class _BiasBnRelu(torch.autograd.Function):
                                       _ptr(running_var), _ptr(batches_tracked), float(momentum), float(eps), _ptr(y),
                                       _c_p(sp), _c_p(sp + 4 * C), n, C, _ptr(n_dev), _ptr(ws), ws.numel(),
                                       _ptr(_ticket(x.device)), _stream()), "hc_bn_relu_fwd")
-        ctx.save_for_backward(x, stats, gamma if gamma is not None else x.new_empty(0),
+        ctx.save_for_backward(x, _bits(stats), gamma if gamma is not None else x.new_empty(0),
                               beta if beta is not None else x.new_empty(0))
         ctx.hc = (bias is not None, gamma is not None, beta is not None, n_dev)
         return y
@@ -1661,15 +1670,6 @@ def _once(backward):
     """``once_differentiable`` for a backward pass whose own graph is asked for; the others go without its wrapper (4 us)."""
     guarded = once_differentiable(backward)
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-
-# What the nodes keep for themselves (routing weights, logits, the scales of rows in 8 bits) is saved as the whole numbers that its
-# bits are: hooks on saved tensors that round matrices leave those alone.
-_WORD = {torch.float32: torch.int32, torch.float16: torch.int16, torch.bfloat16: torch.int16}
-
-
-def _bits(t):
-    return None if t is None else t.view(_WORD[t.dtype])
 
 
 def _route(logits, top_k, normalize):

@@ -76,3 +76,14 @@ def test_a_layer_of_experts_in_the_context(normalize, closed):
         assert bool(torch.isfinite(inside).all())
         # rows and results in 8 bits, a scale of 1 / 127 of 64 values' largest, half of it the most that one is off
         assert float((outside - inside).norm() / outside.norm()) <= 0.02, name
+
+
+def test_the_statistics_of_a_normalisation_are_kept_exactly():
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(700, 64, device=DEV, generator=gen) * torch.exp(2 * torch.randn(64, device=DEV, generator=gen))
+    x.requires_grad_(True)
+    bn = torch.nn.BatchNorm1d(64).to(DEV)
+    from hiscache.history_model import bn_relu
+    # (a leaf is not packed, so that all that could differ are the node's own statistics)
+    for outside, inside in both(lambda: bn_relu(x, bn), (x, bn.weight, bn.bias)):
+        assert torch.equal(outside, inside)
