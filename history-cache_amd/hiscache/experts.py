@@ -58,19 +58,68 @@ class ExpertMLP(torch.nn.Module):
                 f"normalize={self.normalize}, group={self.group}")
 
 
+# Steps back through the history of a matrix that are looked at: a cast, a slice or a normalised weight is up to six from its
+# parameter, a stack of weights with an update of low rank ten (twelve take the host about as long as packing).
+_WEIGHT_STEPS = 12
+
+
+def _result_shape(node, i):
+    """The shape of a node's i-th result."""
+    leaf = getattr(node, "variable", None)
+    return tuple(leaf.shape if leaf is not None else node._input_metadata[i].shape)
+
+
+def _is_weight(t):
+    """Is t a parameter or a leaf that needs a gradient, a view of one, or computed from parameters alone?  The last is told by t's
+    history: it ends at parameters within a few steps, and no data took part in it -- an index, or an operand that needs no
+    gradient in a step whose result has another shape than the other operand (rows of a batch; a number has none) --, or t has
+    as many elements as one of the parameters all the same."""
+    base = t if t._base is None else t._base
+    if isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad):
+        return True
+    if t.grad_fn is None:
+        return False
+    nodes, data, alike = [(t.grad_fn, 0)], False, False
+    for _ in range(_WEIGHT_STEPS):
+        if not nodes:
+            break
+        node, i = nodes.pop()
+        if isinstance(node, torch.autograd.function.BackwardCFunction):
+            return False                                  # an operator of its own, whatever it takes
+        leaf = getattr(node, "variable", None)
+        if leaf is not None:
+            if not isinstance(leaf, torch.nn.Parameter):
+                return False
+            alike = alike or leaf.numel() == t.numel()
+            continue
+        before = [edge for edge in node.next_functions if edge[0] is not None]
+        if node.name().startswith(("Embedding", "Index", "Gather")):
+            data = True
+        elif len(before) < len(node.next_functions):
+            if any(isinstance(n, torch.autograd.function.BackwardCFunction) for n, _ in before):
+                return False
+            data = data or _result_shape(node, i) not in [_result_shape(*edge) for edge in before]
+        nodes += before
+    return not nodes and (alike or not data)
+
+
 def _is_activation(t, min_elements):
     """Is what autograd saves here a matrix that may be kept in 8 bits?"""
     return (t.layout is torch.strided and t.dtype in hiscache_backend._DTYPES and t.dim() >= 2 and t.numel() >= max(min_elements, 1)
-            and t.is_contiguous() and not (t.is_leaf and t.requires_grad))
+            and t.is_contiguous() and not _is_weight(t))
 
 
 def packed_activations(group=64, min_elements=1 << 16):
     """Context in which what autograd saves for backward is kept in 8 bits, a scale for every ``group`` columns
     (``hiscache_backend.pack_rows``): the gradients are those at activations that are off by up to half a scale.
 
-    Kept as they are: parameters and other leaves that need a gradient, whole numbers, tensors of fewer than ``min_elements``
-    values or without a last dimension of their own, sparse tensors, and anything not packed in the current GPU's memory.  Put it around the
-    layers whose activations may be rounded; a loss, a softmax or the router's weights are better left outside."""
+    Kept as they are: parameters, views of parameters and matrices computed from parameters alone in a few steps (a cast copy,
+    a scaled or normalised weight); other leaves that need a gradient and their views; whole numbers; tensors of fewer than
+    ``min_elements`` values or without a last dimension of their own; sparse tensors; and anything not packed in the current GPU's
+    memory.  Any other matrix counts as an activation, a copy of a frozen weight among them, since nothing tells it from the rows of a
+    batch: run a product by one outside.  A matrix that several operators save is kept once for each of them, and one that the caller
+    holds on to is kept besides.  Put the context around the layers whose activations may be rounded; a loss, a softmax or the
+    router's weights are better left outside."""
     be = hiscache_backend
 
     def pack(t):

@@ -87,3 +87,24 @@ def test_the_statistics_of_a_normalisation_are_kept_exactly():
     # (a leaf is not packed, so that all that could differ are the node's own statistics)
     for outside, inside in both(lambda: bn_relu(x, bn), (x, bn.weight, bn.bias)):
         assert torch.equal(outside, inside)
+
+
+WEIGHTS = {
+    "row block": lambda x, w, frozen: x @ w[1],
+    "stack": lambda x, w, frozen: torch.matmul(x.expand(4, 64, 300), w).sum(0),
+    "frozen": lambda x, w, frozen: x @ frozen,
+    "scaled": lambda x, w, frozen: x @ (w[0] * 0.5),
+    "normalised": lambda x, w, frozen: x @ torch.nn.functional.normalize(w[2], dim=0),
+    "experts": lambda x, w, frozen: be.expert_linear(x, w * 2, torch.tensor([0, 20, 30, 50, 64], device=DEV)),
+    "experts, cast": lambda x, w, frozen: be.expert_linear(x.bfloat16(), w.bfloat16(), torch.tensor([0, 20, 30, 50, 64], device=DEV)),
+}
+
+
+@pytest.mark.parametrize("name", WEIGHTS)
+def test_a_gradient_of_rows_goes_by_the_weights_as_they_are(name):
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    w = torch.nn.Parameter(torch.randn(4, 300, 300, device=DEV, generator=gen))
+    frozen = torch.nn.Parameter(torch.randn(300, 300, device=DEV, generator=gen), requires_grad=False)
+    x = torch.randn(64, 300, device=DEV, generator=gen).requires_grad_(True)
+    for outside, inside in both(lambda: WEIGHTS[name](x, w, frozen), (x,)):
+        assert torch.equal(outside, inside)

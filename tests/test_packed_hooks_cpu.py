@@ -70,3 +70,59 @@ def test_what_counts_as_an_activation():
 def test_sparse_matrices_are_kept_as_they_are(layout):
     blocks = dict(blocksize=(2, 2)) if layout is torch.sparse_bsr else {}
     assert not hiscache.experts._is_activation(torch.eye(8).to_sparse(layout=layout, **blocks), 1)
+
+
+class Twice(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x * 2
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * 2
+
+
+P = torch.nn.Parameter
+WEIGHTS = {
+    "parameter": lambda w: w,
+    "frozen": lambda w: P(w.detach(), requires_grad=False),
+    "row block": lambda w: w[1],
+    "flattened": lambda w: w.view(-1, 8),
+    "frozen row block": lambda w: P(w.detach(), requires_grad=False)[1],
+    "cast": lambda w: w.bfloat16(),
+    "row block of a cast": lambda w: w.bfloat16()[1],
+    "scaled": lambda w: w * 0.5,
+    "scaled by a tensor": lambda w: w * torch.full((8,), 0.5),
+    "a scaled row block": lambda w: w[1] * 0.5,
+    "transposed copy": lambda w: w[0].t().contiguous(),
+    "normalised": lambda w: torch.nn.functional.normalize(w, dim=-1),
+    "sum of two": lambda w: w + P(torch.randn(3, 8, 2)) @ P(torch.randn(3, 2, 8)),
+    "leaf": lambda w: w.detach().clone().requires_grad_(True),
+    "view of a leaf": lambda w: w.detach().clone().requires_grad_(True).view(24, 8),
+}
+ACTIVATIONS = {
+    "data": lambda x, w: x,
+    "a row block of data": lambda x, w: x[:3],
+    "product": lambda x, w: x @ w[0],
+    "linear": lambda x, w: torch.nn.functional.linear(x, w[0], P(torch.zeros(8))),
+    "relu": lambda x, w: torch.relu(x @ w[0]),
+    "product by a cast": lambda x, w: x.bfloat16() @ w[0].bfloat16(),
+    "rows times a vector": lambda x, w: x * P(torch.ones(8)),
+    "embedding": lambda x, w: torch.nn.functional.embedding(torch.arange(5), P(torch.randn(9, 8))),
+    "rows of a table": lambda x, w: P(torch.randn(9, 8))[torch.tensor([1, 1, 4])],
+    "of an operator of one's own": lambda x, w: Twice.apply(w[0]),
+    "rows over a norm": lambda x, w: (x @ w[0]) / (x @ w[0]).norm(),
+    "masked": lambda x, w: (x @ w[0]) * torch.ones(7, 8),
+    "of a leaf": lambda x, w: x.clone().requires_grad_(True) * 1,
+    "deep": lambda x, w: torch.relu(torch.relu(torch.relu(x @ w[0]) @ w[1]) @ w[2]) + 1,
+}
+
+
+@pytest.mark.parametrize("name", WEIGHTS)
+def test_weights_are_not_activations(name):
+    assert not hiscache.experts._is_activation(WEIGHTS[name](P(torch.randn(3, 8, 8))), 1)
+
+
+@pytest.mark.parametrize("name", ACTIVATIONS)
+def test_activations_are(name):
+    assert hiscache.experts._is_activation(ACTIVATIONS[name](torch.randn(7, 8), P(torch.randn(3, 8, 8))), 1)
