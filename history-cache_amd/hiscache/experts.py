@@ -103,9 +103,11 @@ def _is_weight(t):
     return not nodes and (alike or not data)
 
 
-def _is_activation(t, min_elements):
-    """Is what autograd saves here a matrix that may be kept in 8 bits?"""
+def _is_activation(t, min_elements, group=64):
+    """Is what autograd saves here a matrix that may be kept in 8 bits, and does it get smaller (a narrow row's scales weigh more
+    than what its values lose)?"""
     return (t.layout is torch.strided and t.dtype in hiscache_backend._DTYPES and t.dim() >= 2 and t.numel() >= max(min_elements, 1)
+            and t.shape[-1] + 4 * -(-t.shape[-1] // group) < t.shape[-1] * t.element_size()
             and t.is_contiguous() and not _is_weight(t))
 
 
@@ -115,15 +117,15 @@ def packed_activations(group=64, min_elements=1 << 16):
 
     Kept as they are: parameters, views of parameters and matrices computed from parameters alone in a few steps (a cast copy,
     a scaled or normalised weight); other leaves that need a gradient and their views; whole numbers; tensors of fewer than
-    ``min_elements`` values or without a last dimension of their own; sparse tensors; and anything not packed in the current GPU's
-    memory.  Any other matrix counts as an activation, a copy of a frozen weight among them, since nothing tells it from the rows of a
-    batch: run a product by one outside.  A matrix that several operators save is kept once for each of them, and one that the caller
-    holds on to is kept besides.  Put the context around the layers whose activations may be rounded; a loss, a softmax or the
-    router's weights are better left outside."""
+    ``min_elements`` values, without a last dimension of their own or so narrow that codes and scales would not be smaller;
+    sparse tensors; and anything not packed in the current GPU's memory.  Any other matrix counts as an activation, a copy of a
+    frozen weight among them, since nothing tells it from the rows of a batch: run a product by one outside.  A matrix that
+    several operators save is kept once for each of them, and one that the caller holds on to is kept besides.  Put the context
+    around the layers whose activations may be rounded; a loss, a softmax or the router's weights are better left outside."""
     be = hiscache_backend
 
     def pack(t):
-        if not t.is_cuda or t.device.index != torch.cuda.current_device() or not _is_activation(t, min_elements):
+        if not t.is_cuda or t.device.index != torch.cuda.current_device() or not _is_activation(t, min_elements, group):
             # (a node that held its own result would be held by it in turn, out of the garbage collector's sight)
             t = t if t.is_leaf else t.detach()
             return t, t._version

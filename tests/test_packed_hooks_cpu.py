@@ -126,3 +126,12 @@ def test_weights_are_not_activations(name):
 @pytest.mark.parametrize("name", ACTIVATIONS)
 def test_activations_are(name):
     assert hiscache.experts._is_activation(ACTIVATIONS[name](torch.randn(7, 8), P(torch.randn(3, 8, 8))), 1)
+
+
+@pytest.mark.parametrize("dtype,least", ((torch.float32, 2), (torch.float16, 5), (torch.bfloat16, 5)))
+@pytest.mark.parametrize("group", (32, 64, 128))
+def test_rows_too_narrow_to_get_smaller_are_kept_as_they_are(dtype, least, group):
+    for width in (1, 2, 3, 4, 5, 6, 31, 33, 65, 129):
+        t = torch.randn(9, width).to(dtype)
+        smaller = width + 4 * -(-width // group) < width * t.element_size()
+        assert hiscache.experts._is_activation(t, 1, group) == smaller == (width >= least)
