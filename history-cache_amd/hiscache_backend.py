@@ -1913,7 +1913,8 @@ def expert_linear(x, w, offset):
 
 
 def expert_linear_grad(g, x, offset):
-    """``g[rows of e].t() @ x[rows of e]`` for every expert e: [E, N, K] of x's type from g [S, N] and x [S, K]."""
+    """``g[rows of e].t() @ x[rows of e]`` for every expert e: [E, N, K] of x's type from g [S, N] and x [S, K] (not an
+    autograd node)."""
     lib = load_library()
     x = _operand(x, "x")
     g = _operand(g, "g", x.dtype)
@@ -1976,7 +1977,8 @@ def _check_kept(kept, halves):
 def pack_rows(x, group=64):
     """x [n, F] in 8 bits: every ``group`` adjacent columns of a row share an fp32 scale m * (1 / 127) (m their largest
     magnitude) and keep rint(x * (1 / m * 127)).  Half a scale is the most that a value is off.  Groups whose m is below 2^-120 are kept as
-    zeros; one that holds an infinity or a NaN reads back as NaN."""
+    zeros; one that holds an infinity or a NaN reads back as NaN.  Not an autograd node: codes and what reads back pass no
+    gradient on."""
     x = _pack_arguments(x, "x", group)
     codes, scale = _packed_like(x, 1, group)
     _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], group, codes.data_ptr(),
@@ -2000,8 +2002,11 @@ def unpack_rows(kept, dtype=None):
 
 def gated_pack(x, group=64, keep=True):
     """``silu(a) * b`` for rows [a | b] of x [n, 2 F], and x in 8 bits for :func:`gated_grad`: (h [n, F], PackedRows), the
-    second one None without ``keep``."""
+    second one None without ``keep``.  Not an autograd node: where a gradient of x would be recorded it raises (that gradient is
+    :func:`gated_grad`'s, for ``gated_pack(x.detach())`` in a node of one's own)."""
     x = _pack_arguments(x, "x", group)
+    if _watched(x):
+        raise RuntimeError("gated_pack records no gradient: call it on x.detach() and take the gradient from gated_grad")
     if x.shape[1] % 2 != 0:
         raise ValueError("x must hold two halves of the same width")
     n, F = x.shape[0], x.shape[1] // 2
@@ -2013,7 +2018,8 @@ def gated_pack(x, group=64, keep=True):
 
 
 def gated_grad(kept, g):
-    """From what :func:`gated_pack` kept and the gradient g [n, F] of h: the gradient of x [n, 2 F], and h [n, F] again."""
+    """From what :func:`gated_pack` kept and the gradient g [n, F] of h: the gradient of x [n, 2 F], and h [n, F] again (not an
+    autograd node)."""
     codes, scale = kept.codes, kept.scale
     n, F = _check_kept(kept, 2)
     g = _operand(g, "g", kept.dtype)

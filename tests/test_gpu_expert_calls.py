@@ -134,3 +134,15 @@ def test_kept_rows_that_are_not_whole_are_refused_by_the_calls():
                              (kept.codes, kept.scale.half()), (kept.codes.int(), kept.scale)):
             with pytest.raises(ValueError):
                 call(be.PackedRows(codes, scale, 64, x.dtype))
+
+
+def test_a_gate_that_would_lose_its_gradient_is_refused():
+    x = torch.randn(6, 128, device=DEV, requires_grad=True)
+    for of in (x, x * 2):
+        with pytest.raises(RuntimeError, match="records no gradient"):
+            be.gated_pack(of)
+        with pytest.raises(RuntimeError, match="records no gradient"):
+            be.gated_pack(of, keep=False)
+    want, _ = be.gated_pack(x.detach())
+    with torch.no_grad():
+        assert torch.equal(be.gated_pack(x)[0], want)
