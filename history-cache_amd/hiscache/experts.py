@@ -24,7 +24,8 @@ class ExpertMLP(torch.nn.Module):
             raise ValueError(f"top_k must be between 1 and the {num_expert} experts, got {top_k}")
         self.channels, self.hidden, self.num_expert = channels, hidden, num_expert
         self.top_k, self.normalize, self.group = top_k, normalize, group
-        # the router's logits are fp32 whatever the rows are: near-ties decide where a row goes
+        # the router's logits are fp32 whatever the rows are, under autocast and in a module cast to half precision as well: near-ties
+        # decide where a row goes
         self.router = torch.nn.Parameter(torch.empty(num_expert, channels, device=device, dtype=torch.float32))
         self.w_in = torch.nn.Parameter(torch.empty(num_expert, 2 * hidden, channels, device=device, dtype=dtype))
         self.w_out = torch.nn.Parameter(torch.empty(num_expert, channels, hidden, device=device, dtype=dtype))
@@ -38,7 +39,11 @@ class ExpertMLP(torch.nn.Module):
     def route(self, x, allowed=None):
         """The router's choice for the rows of x: (expert int64 [n, top_k], weight fp32 [n, top_k]).  ``allowed`` (bool
         [n, E] or [E], optional): experts that a row may go to; a row that may go nowhere gets -1 and weight 0."""
-        logits = F.linear(x.float(), self.router)
+        if torch.is_autocast_enabled(x.device.type):
+            with torch.autocast(x.device.type, enabled=False):
+                logits = F.linear(x.float(), self.router.float())
+        else:
+            logits = F.linear(x.float(), self.router.float())
         if allowed is not None:
             logits = logits.masked_fill(~allowed, -math.inf)
         return hiscache_backend.route_rows(logits, self.top_k, normalize=self.normalize)

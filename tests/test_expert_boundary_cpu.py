@@ -162,3 +162,20 @@ def test_kept_rows_that_are_not_whole_are_refused():
             be._check_kept(be.PackedRows(codes, scale, 64, torch.float64), halves)
     with pytest.raises(ValueError):
         be._check_kept(be.PackedRows(torch.zeros(6, 129, dtype=torch.int8), scale, 64, torch.float16), 2)
+
+
+@pytest.mark.parametrize("module", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("autocast", (False, True))
+def test_the_router_s_logits_are_fp32(monkeypatch, module, autocast):
+    import hiscache
+    import hiscache_backend as be
+    seen = []
+    monkeypatch.setattr(be, "route_rows", lambda logits, top_k, normalize: seen.append(logits))
+    layer = hiscache.ExpertMLP(32, 16, 4, 2).to(module)
+    x = torch.randn(50, 32).to(module)
+    with torch.autocast("cpu", dtype=torch.bfloat16, enabled=autocast):
+        layer.route(x)
+        layer.route(x, torch.ones(4, dtype=torch.bool))
+    want = x.float() @ layer.router.float().t()
+    for logits in seen:
+        assert logits.dtype == torch.float32 and torch.allclose(logits, want, rtol=32 * 2.0 ** -24, atol=32 * 2.0 ** -23)

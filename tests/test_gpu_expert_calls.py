@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import hiscache
 import hiscache_backend as be
 
 pytestmark = pytest.mark.gpu
@@ -146,3 +147,19 @@ def test_a_gate_that_would_lose_its_gradient_is_refused():
     want, _ = be.gated_pack(x.detach())
     with torch.no_grad():
         assert torch.equal(be.gated_pack(x)[0], want)
+
+
+def test_routing_under_autocast_and_in_half_precision():
+    torch.manual_seed(2)
+    layer = hiscache.ExpertMLP(64, 32, 8, 2, device=DEV)
+    x = torch.randn(400, 64, device=DEV)
+    expert, weight = layer.route(x)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        again, weight_again = layer.route(x)
+    assert torch.equal(expert, again) and torch.equal(weight, weight_again)
+    half = layer.bfloat16()
+    rows = x.bfloat16().requires_grad_(True)
+    out = half(rows)
+    out.float().sum().backward()
+    assert out.dtype == torch.bfloat16 and all(bool(torch.isfinite(p.grad).all()) for p in (rows, *half.parameters()))
+    assert half.router.grad.dtype == torch.bfloat16
