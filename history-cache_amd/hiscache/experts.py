@@ -50,8 +50,11 @@ class ExpertMLP(torch.nn.Module):
 
     def forward(self, x, expert=None, weight=None, allowed=None):
         """x [n, channels] through its experts.  ``expert`` (int64 [n] or [n, k]) and ``weight`` (fp32, default ones) replace
-        the router's choice; -1 sends a row nowhere (zeros, if it has no other)."""
+        the router's choice; -1 sends a row nowhere (zeros, if it has no other).  ``allowed`` is for the router
+        (:meth:`route`)."""
         be = hiscache_backend
+        if (weight if expert is None else allowed) is not None:
+            raise ValueError("weight goes with expert, allowed with the router's choice")
         if expert is None:
             expert, weight = self.route(x, allowed)
         order = be.expert_order(expert, self.num_expert)

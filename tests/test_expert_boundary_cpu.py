@@ -179,3 +179,12 @@ def test_the_router_s_logits_are_fp32(monkeypatch, module, autocast):
     want = x.float() @ layer.router.float().t()
     for logits in seen:
         assert logits.dtype == torch.float32 and torch.allclose(logits, want, rtol=32 * 2.0 ** -24, atol=32 * 2.0 ** -23)
+
+
+def test_arguments_that_would_be_ignored_are_refused():
+    import hiscache
+    layer, x, expert = hiscache.ExpertMLP(8, 16, 4, 2), torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="weight goes with expert"):
+        layer(x, weight=torch.ones(3, 2))
+    with pytest.raises(ValueError, match="weight goes with expert"):
+        layer(x, expert, allowed=torch.ones(4, dtype=torch.bool))
