@@ -250,6 +250,9 @@ def _empty(t):
 # request seen (up to _WS_KEEP_BYTES; larger requests, and calls on a capturing stream, whose buffer must
 # stay alive with the graph, get a buffer of their own).  Sampled batches change every size at every
 # iteration; without this each call paid an allocator look-up, and a device allocation when it missed.
+# One thread at a time may call into a stream: a call that takes several launches runs without the interpreter's lock,
+# and another thread's launches in between would write into the same buffer.  (The expert layer's calls take a buffer of
+# their own, which goes back to the stream's pool when the launches are enqueued: see _scratch.)
 _WS_KEEP_BYTES = 64 << 20
 _ws_cache = {}
 
@@ -266,6 +269,12 @@ def _workspace(nbytes, device):
             size <<= 1
         buf = _ws_cache[key] = torch.empty(size, dtype=torch.uint8, device=device)
     return buf
+
+
+def _scratch(t, nbytes):
+    """Scratch memory of one call on t's stream, None where it needs none.  (A new tensor takes the host as long as looking
+    the shared buffer up.)"""
+    return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def release_workspaces():
@@ -1749,14 +1758,14 @@ def expert_order(expert, num_expert):
     if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
         raise ValueError("expert must be [n] or [n, top_k]")
     _together(expert)
-    E, P, dev = int(num_expert), expert.numel(), expert.device
+    E, P = int(num_expert), expert.numel()
     if E < 1:
         raise ValueError("num_expert must be positive")
     at = expert.new_empty((2, P), dtype=torch.int32)
     offset = expert.new_empty(E + 1)
     slot, pair = at.unbind(0)
     nbytes = int(lib.hc_expert_order_workspace_bytes(P, E))
-    ws = _workspace(nbytes, dev) if nbytes else None
+    ws = _scratch(expert, nbytes)
     _check(lib.hc_expert_order(expert.data_ptr(), P, E, slot.data_ptr(), pair.data_ptr(), offset.data_ptr(), _ptr(ws),
                                nbytes, _stream_for(expert)), "hc_expert_order")
     return ExpertOrder(slot, pair, offset, expert.shape[0], 1 if expert.dim() == 1 else expert.shape[1], E)
@@ -1925,7 +1934,7 @@ def expert_linear_grad(g, x, offset):
     (S, N), K, E, dtype = g.shape, x.shape[1], offset.numel() - 1, _float_dtype(x, "x")
     gw = x.new_empty((E, N, K))
     nbytes = int(lib.hc_expert_linear_grad_workspace_bytes(S, E, N, K, dtype))
-    ws = _workspace(nbytes, x.device) if nbytes else None
+    ws = _scratch(x, nbytes)
     _check(lib.hc_expert_linear_grad(g.data_ptr(), x.data_ptr(), dtype, offset.data_ptr(), S, E, N, K, gw.data_ptr(),
                                      _ptr(ws), nbytes, _stream_for(x)), "hc_expert_linear_grad")
     return gw

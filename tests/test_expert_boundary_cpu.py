@@ -188,3 +188,37 @@ def test_arguments_that_would_be_ignored_are_refused():
         layer(x, weight=torch.ones(3, 2))
     with pytest.raises(ValueError, match="weight goes with expert"):
         layer(x, expert, allowed=torch.ones(4, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("call", ("order", "grad"))
+def test_calls_of_two_threads_on_one_stream_share_no_scratch_memory(monkeypatch, call):
+    """Both calls are held inside the library at the same time, as a call without the interpreter's lock may be."""
+    import threading
+    import hiscache_backend as be
+    meet, seen = threading.Barrier(2), []
+
+    class Library:
+        def __getattr__(self, name):
+            def enqueue(*args):
+                if name.endswith("_workspace_bytes"):
+                    return 4096
+                seen.append([a for a, b in zip(args, args[1:]) if b == 4096][0])
+                meet.wait(timeout=30)
+                return 0
+            return enqueue
+
+    monkeypatch.setattr(be, "load_library", Library)
+    monkeypatch.setattr(be, "_dev", lambda t, *_: t)
+    monkeypatch.setattr(be, "_together", lambda *_: None)
+    monkeypatch.setattr(be, "_stream_for", lambda _: 0)
+    monkeypatch.setattr(be, "_raw_stream", lambda *_: 0)
+    monkeypatch.setattr(be, "_ws_cache", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    one = {"order": lambda: be.expert_order(torch.zeros(9000, dtype=torch.int64), 4),
+           "grad": lambda: be.expert_linear_grad(torch.zeros(8, 4), torch.zeros(8, 4), torch.tensor([0, 8]))}[call]
+    threads = [threading.Thread(target=one) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(seen) == 2 and seen[0] != seen[1]
