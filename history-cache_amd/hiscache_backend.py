@@ -272,8 +272,8 @@ def _workspace(nbytes, device):
 
 
 def _scratch(t, nbytes):
-    """Scratch memory of one call on t's stream, None where it needs none.  (A new tensor takes the host as long as looking
-    the shared buffer up.)"""
+    """Scratch memory of one call on t's stream, None where it needs none.  (A new tensor takes the host up to a microsecond
+    longer than looking the shared buffer up.)"""
     return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
@@ -1624,15 +1624,15 @@ _stream_of_device = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 def _no_tangent(*tensors):
     """Forward-mode derivatives: the kernels have none, and a result without a tangent would count as a constant."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("this operator has no forward-mode derivative")
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("this operator has no forward-mode derivative")
 
 
 def _together(t, *others):
     """Do these tensors lie on one device, the current one (whose stream the launch goes to), and may a call read them?"""
-    _no_tangent(t, *others)
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, *others)
     index = t.get_device()
     together = index == _current_device()
     for o in others:
@@ -1646,23 +1646,21 @@ def _stream_for(t):
     return _stream_of_device(t.get_device())
 
 
-def _stored(t):
-    """t as the kernels read it: a lazily negated tensor lies in memory with the other sign, zeros that were never written
-    nowhere."""
+def _operand(t, name, dtype=None):
+    """``_dev`` of a call's operand, and it as the kernels read it: a lazily negated tensor lies in memory with the other sign,
+    zeros that were never written nowhere."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
+        _dev(t, name, dtype)                              # says what is wrong
     if t.is_neg():
         return t.resolve_neg()
     return t.clone() if t._is_zerotensor() else t
 
 
-def _operand(t, name, dtype=None):
-    """``_dev`` of a call's operand, and it as the kernels read it."""
-    return _stored(_dev(t, name, dtype))
-
-
 def _arriving(g):
     """A gradient as the kernels read it, packed."""
-    _no_tangent(g)
-    return _stored(g.contiguous())
+    if forward_ad._current_level >= 0:
+        _no_tangent(g)
+    return _operand(g.contiguous(), "gradient")
 
 
 # The operators below are autograd nodes where a gradient may be asked for; without one the node itself, which costs the
@@ -1723,12 +1721,13 @@ def route_rows(logits, top_k, normalize=True):
     expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
     weights.  The gradient of the weights reaches ``logits``.  top_k <= 32."""
     logits = _operand(logits, "logits")
-    _float_dtype(logits, "logits")
-    top_k = int(top_k)
-    if logits.dim() != 2:
+    if logits.dtype not in _DTYPES:
+        _float_dtype(logits, "logits")
+    top_k, shape = int(top_k), logits.shape
+    if len(shape) != 2:
         raise ValueError("logits must be [n, E]")
-    if not 1 <= top_k <= logits.shape[1]:
-        raise ValueError(f"top_k must be between 1 and the {logits.shape[1]} experts, got {top_k}")
+    if not 1 <= top_k <= shape[1]:
+        raise ValueError(f"top_k must be between 1 and the {shape[1]} experts, got {top_k}")
     _together(logits)
     return (_RouteRows.apply if _watched(logits) else _route)(logits, top_k, int(bool(normalize)))
 
@@ -1738,9 +1737,10 @@ class ExpertOrder:
     choice.  ``offset`` int64 [E + 1]: expert e has the places offset[e] to offset[e + 1]; ``pair`` int32 [rows * top_k]: the
     pair at every place; ``slot`` int32 [rows * top_k]: every pair's place; -1 where there is none (choices that name
     no expert, and the places behind offset[E])."""
-    __slots__ = ("slot", "pair", "offset", "rows", "top_k", "experts")
+    __slots__ = ("slot", "pair", "offset", "rows", "top_k", "experts", "_checked")
 
     def __init__(self, slot, pair, offset, rows, top_k, experts):
+        self._checked = None
         self.slot, self.pair, self.offset = slot, pair, offset
         self.rows, self.top_k, self.experts = int(rows), int(top_k), int(experts)
 
@@ -1755,123 +1755,143 @@ def expert_order(expert, num_expert):
     device.  num_expert <= 1024, n * top_k < 2^31."""
     lib = load_library()
     expert = _operand(expert, "expert", torch.int64)
-    if expert.dim() not in (1, 2) or (expert.dim() == 2 and expert.shape[1] < 1):
+    shape = expert.shape
+    if len(shape) not in (1, 2) or (len(shape) == 2 and shape[1] < 1):
         raise ValueError("expert must be [n] or [n, top_k]")
     _together(expert)
-    E, P = int(num_expert), expert.numel()
+    n, top_k = shape if len(shape) == 2 else (shape[0], 1)
+    E, P = int(num_expert), n * top_k
     if E < 1:
         raise ValueError("num_expert must be positive")
-    at = expert.new_empty((2, P), dtype=torch.int32)
-    offset = expert.new_empty(E + 1)
-    slot, pair = at.unbind(0)
+    # (tensors of their own: two rows of one would take two microseconds longer and count a change of either as one of both)
+    slot, pair, offset = expert.new_empty(P, dtype=torch.int32), expert.new_empty(P, dtype=torch.int32), expert.new_empty(E + 1)
     nbytes = int(lib.hc_expert_order_workspace_bytes(P, E))
     ws = _scratch(expert, nbytes)
     _check(lib.hc_expert_order(expert.data_ptr(), P, E, slot.data_ptr(), pair.data_ptr(), offset.data_ptr(), _ptr(ws),
                                nbytes, _stream_for(expert)), "hc_expert_order")
-    return ExpertOrder(slot, pair, offset, expert.shape[0], 1 if expert.dim() == 1 else expert.shape[1], E)
+    return ExpertOrder(slot, pair, offset, n, top_k, E)
 
 
-def _to_experts(x, order):
-    rows = x.new_empty((order.places, x.shape[1]))
-    _check(load_library().hc_rows_to_experts(x.data_ptr(), _DTYPES[x.dtype], order.rows, order.top_k, order.experts,
-                                             x.shape[1], order.slot.data_ptr(), order.offset.data_ptr(), rows.data_ptr(),
-                                             _stream_for(x)), "hc_rows_to_experts")
+def _to_experts(x, slot, offset, n, top_k, E):
+    D = x.shape[1]
+    rows = x.new_empty((n * top_k, D))
+    _check(load_library().hc_rows_to_experts(x.data_ptr(), _DTYPES[x.dtype], n, top_k, E, D, slot.data_ptr(),
+                                             offset.data_ptr(), rows.data_ptr(), _stream_for(x)), "hc_rows_to_experts")
     return rows
 
 
-def _from_experts(y, order, weight):
-    out = y.new_empty((order.rows, y.shape[1]))
-    _check(load_library().hc_rows_from_experts(y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts,
-                                               y.shape[1], order.slot.data_ptr(), _ptr(weight), out.data_ptr(), _stream_for(y)),
-           "hc_rows_from_experts")
+def _from_experts(y, weight, slot, offset, n, top_k, E):
+    D = y.shape[1]
+    out = y.new_empty((n, D))
+    _check(load_library().hc_rows_from_experts(y.data_ptr(), _DTYPES[y.dtype], n, top_k, E, D, slot.data_ptr(),
+                                               _ptr(weight), out.data_ptr(), _stream_for(y)), "hc_rows_from_experts")
     return out
-
-
-# (the order's tensors are saved ones, so that autograd notices a change in place between forward and backward)
-def _saved_order(ctx, slot, offset):
-    return ExpertOrder(slot, None, offset, *ctx.hc)
 
 
 class _RowsToExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, order):
-        ctx.save_for_backward(order.slot, order.offset)
-        ctx.hc = (order.rows, order.top_k, order.experts)
-        return _to_experts(x, order)
+    def forward(ctx, x, places):
+        _keep_places(ctx, places)
+        return _to_experts(x, *places)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        return _from_experts(_arriving(g), _saved_order(ctx, *ctx.saved_tensors), None), None
+        return _from_experts(_arriving(g), None, *_kept_places(ctx)), None
 
 
 class _RowsFromExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, order, weight):
-        ctx.save_for_backward(y if weight is not None else None, _bits(weight), order.slot, order.offset)
-        ctx.hc = (order.rows, order.top_k, order.experts)
-        return _from_experts(y, order, weight)
+    def forward(ctx, y, weight, places):
+        if weight is not None:
+            ctx.save_for_backward(y, _bits(weight))
+        _keep_places(ctx, places)
+        return _from_experts(y, weight, *places)
 
     @staticmethod
     @_once
     def backward(ctx, g):
-        y, weight, slot, offset = ctx.saved_tensors
-        order, g = _saved_order(ctx, slot, offset), _arriving(g)
-        if weight is None:
-            return _to_experts(g, order), None, None
-        return _from_experts_grads(g, y, order, weight.view(torch.float32))
+        places, g, saved = _kept_places(ctx), _arriving(g), ctx.saved_tensors
+        if not saved:
+            return _to_experts(g, *places), None, None
+        slot, offset, n, top_k, E = places
+        y, weight = saved
+        grad_y, grad_weight = torch.empty_like(y), torch.empty_like(weight, dtype=torch.float32)
+        _check(load_library().hc_rows_from_experts_grad(
+            g.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], n, top_k, E, y.shape[1], slot.data_ptr(), offset.data_ptr(),
+            weight.data_ptr(), grad_y.data_ptr(), grad_weight.data_ptr(), _stream_for(y)), "hc_rows_from_experts_grad")
+        return grad_y, grad_weight, None
 
 
-def _from_experts_grads(g, y, order, weight):
-    grad_y, grad_weight = torch.empty_like(y), torch.empty_like(weight)
-    _check(load_library().hc_rows_from_experts_grad(
-        g.data_ptr(), y.data_ptr(), _DTYPES[y.dtype], order.rows, order.top_k, order.experts, y.shape[1],
-        order.slot.data_ptr(), order.offset.data_ptr(), weight.data_ptr(), grad_y.data_ptr(), grad_weight.data_ptr(),
-        _stream_for(y)), "hc_rows_from_experts_grad")
-    return grad_y, None, grad_weight
+# The places are whole numbers that no hook has to see and the graph may hold; what autograd does for saved tensors beyond that is
+# done here at a tenth of its host time: a change in place between forward and backward is noticed.
+def _keep_places(ctx, places):
+    slot, offset = places[:2]
+    ctx.hc = places
+    ctx.versions = slot._version, offset._version
+
+
+def _kept_places(ctx):
+    slot, offset = ctx.hc[:2]
+    if (slot._version, offset._version) != ctx.versions:
+        raise RuntimeError("one of the variables needed for gradient computation has been modified by an inplace operation: the "
+                           "places or the offsets of an ExpertOrder")
+    return ctx.hc
+
+
+def _places(order):
+    """What the kernels go by, if it fits together: they read a place for every pair and the offset behind the last expert."""
+    if not isinstance(order, ExpertOrder):
+        raise TypeError("order must be an ExpertOrder")
+    known, slot, offset, n, top_k, E = order._checked, order.slot, order.offset, order.rows, order.top_k, order.experts
+    if (known is not None and known[0] is slot and known[1] is offset and known[2] == n and known[3] == top_k and known[4] == E):
+        return known
+    if (slot.dtype != torch.int32 or offset.dtype != torch.int64 or slot.numel() != n * top_k or offset.numel() != E + 1
+            or not slot.is_contiguous() or not offset.is_contiguous()):
+        raise ValueError(f"the order must hold {n * top_k} places (slot, int32) and {E + 1} offsets (int64), both contiguous")
+    order._checked = slot, offset, n, top_k, E
+    return order._checked
 
 
 def _check_order(order):
-    """Can the kernels go by this order?  They read a place for every pair and the offset behind the last expert."""
-    if not isinstance(order, ExpertOrder):
-        raise TypeError("order must be an ExpertOrder")
-    slot, offset = order.slot, order.offset
-    if (slot.dtype != torch.int32 or offset.dtype != torch.int64 or slot.numel() != order.rows * order.top_k
-            or offset.numel() != order.experts + 1 or not slot.is_contiguous() or not offset.is_contiguous()):
-        raise ValueError(f"the order must hold {order.rows * order.top_k} places (slot, int32) and {order.experts + 1} offsets "
-                         "(int64), both contiguous")
+    """Can the kernels go by this order?"""
+    _places(order)
 
 
 def _expert_rows(t, name, order, a_choice):
-    """``t``, if it is a matrix with a row for every row of the order, or (``a_choice``) for every choice of one."""
+    """``t``, if it is a matrix with a row for every row of the order, or (``a_choice``) for every choice of one, and the places
+    that its rows go to or come from."""
     t = _operand(t, name)
-    _float_dtype(t, name)
-    _check_order(order)
-    rows = order.places if a_choice else order.rows
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+    if t.dtype not in _DTYPES:
+        _float_dtype(t, name)
+    places, shape = _places(order), t.shape
+    rows = places[2] * places[3] if a_choice else places[2]
+    if len(shape) != 2 or shape[0] != rows or shape[1] < 1:
         raise ValueError(f"{name} must be [{rows}, D], got {tuple(t.shape)}")
-    _together(t, order.slot, order.offset)
-    return t
+    return t, places
 
 
 def rows_to_experts(x, order):
     """The rows of x [n, D] in expert order, [n * top_k, D]: place p holds row ``order.pair[p] // top_k``, zeros where there is
     no pair.  The gradient of a row is the sum over its places."""
-    x = _expert_rows(x, "x", order, False)
-    return (_RowsToExperts.apply if _watched(x) else _to_experts)(x, order)
+    x, places = _expert_rows(x, "x", order, False)
+    _together(x, places[0], places[1])
+    return _RowsToExperts.apply(x, places) if _watched(x) else _to_experts(x, *places)
 
 
 def rows_from_experts(y, order, weight=None):
     """``out[i] = sum_j weight[i, j] * y[slot of (i, j)]`` for the experts' results y [n * top_k, D], summed in fp32 in the
     order of j; choices that name no expert add nothing.  ``weight`` fp32 [n, top_k] (None: ones).  Gradients for y and
     weight."""
-    y = _expert_rows(y, "y", order, True)
-    if weight is not None:
+    y, places = _expert_rows(y, "y", order, True)
+    if weight is None:
+        _together(y, places[0], places[1])
+    else:
         weight = _operand(weight, "weight", torch.float32)
-        if weight.numel() != order.places:
-            raise ValueError(f"weight must hold {order.places} values")
-        _together(y, weight)
-    return (_RowsFromExperts.apply if _watched(y, weight) else _from_experts)(y, order, weight)
+        if weight.numel() != places[2] * places[3]:
+            raise ValueError(f"weight must hold {places[2] * places[3]} values")
+        _together(y, weight, places[0], places[1])
+    return _RowsFromExperts.apply(y, weight, places) if _watched(y, weight) else _from_experts(y, weight, *places)
 
 
 class _ExpertLinear(torch.autograd.Function):
@@ -1886,7 +1906,7 @@ class _ExpertLinear(torch.autograd.Function):
         x, w, offset = ctx.saved_tensors
         g = _arriving(g)
         return (_expert_product(g, w, offset, True) if ctx.needs_input_grad[0] else None,
-                expert_linear_grad(g, x, offset) if ctx.needs_input_grad[1] else None, None)
+                _expert_grad(g, x, offset) if ctx.needs_input_grad[1] else None, None)
 
 
 def _expert_product(x, w, offset, transposed):
@@ -1911,11 +1931,13 @@ def expert_linear(x, w, offset):
     offset[0] and behind offset[E] are zeros.  ``offset`` int64 [E + 1] stays on the device.  Sums in fp32 (fp32 rows: fp32 products), one
     rounding to the type of x.  Gradients for x and w."""
     x = _operand(x, "x")
-    _float_dtype(x, "x")
+    if x.dtype not in _DTYPES:
+        _float_dtype(x, "x")
     w = _operand(w, "w", x.dtype)
     offset = _expert_offset(offset)
-    if x.dim() != 2 or w.dim() != 3 or w.shape[2] != x.shape[1] or offset.numel() != w.shape[0] + 1:
-        raise ValueError(f"x [S, K], w [E, N, K] and offset [E + 1] do not fit: {tuple(x.shape)}, {tuple(w.shape)}, "
+    of_x, of_w = x.shape, w.shape
+    if len(of_x) != 2 or len(of_w) != 3 or of_w[2] != of_x[1] or offset.numel() != of_w[0] + 1:
+        raise ValueError(f"x [S, K], w [E, N, K] and offset [E + 1] do not fit: {tuple(of_x)}, {tuple(of_w)}, "
                          f"{tuple(offset.shape)}")
     _together(x, w, offset)
     return _ExpertLinear.apply(x, w, offset) if _watched(x, w) else _expert_product(x, w, offset, False)
@@ -1924,14 +1946,20 @@ def expert_linear(x, w, offset):
 def expert_linear_grad(g, x, offset):
     """``g[rows of e].t() @ x[rows of e]`` for every expert e: [E, N, K] of x's type from g [S, N] and x [S, K] (not an
     autograd node)."""
-    lib = load_library()
     x = _operand(x, "x")
+    if x.dtype not in _DTYPES:
+        _float_dtype(x, "x")
     g = _operand(g, "g", x.dtype)
     offset = _expert_offset(offset)
-    if g.dim() != 2 or x.dim() != 2 or g.shape[0] != x.shape[0]:
+    of_g, of_x = g.shape, x.shape
+    if len(of_g) != 2 or len(of_x) != 2 or of_g[0] != of_x[0]:
         raise ValueError("g [S, N] and x [S, K] must have the same number of rows")
     _together(x, g, offset)
-    (S, N), K, E, dtype = g.shape, x.shape[1], offset.numel() - 1, _float_dtype(x, "x")
+    return _expert_grad(g, x, offset)
+
+
+def _expert_grad(g, x, offset):
+    lib, (S, N), K, E, dtype = load_library(), g.shape, x.shape[1], offset.numel() - 1, _DTYPES[x.dtype]
     gw = x.new_empty((E, N, K))
     nbytes = int(lib.hc_expert_linear_grad_workspace_bytes(S, E, N, K, dtype))
     ws = _scratch(x, nbytes)
@@ -1944,23 +1972,27 @@ def expert_linear_grad(g, x, offset):
 class PackedRows:
     """A matrix kept in 8 bits (:func:`pack_rows`, :func:`gated_pack`): ``codes`` int8 [n, columns] and ``scale`` fp32
     [n, groups], ``dtype`` the type it had."""
-    __slots__ = ("codes", "scale", "group", "dtype")
+    __slots__ = ("codes", "scale", "group", "dtype", "_checked")
 
     def __init__(self, codes, scale, group, dtype):
         self.codes, self.scale, self.group, self.dtype = codes, scale, int(group), dtype
+        self._checked = None
 
 
 def _packed_like(x, halves, group):
-    n, F = x.shape[0], x.shape[1] // halves
-    codes = x.new_empty(x.shape, dtype=torch.int8)
+    shape = x.shape
+    n, F = shape[0], shape[1] // halves
+    codes = x.new_empty(shape, dtype=torch.int8)
     scale = x.new_empty((n, halves * -(-F // group)), dtype=torch.float32)
     return codes, scale
 
 
 def _pack_arguments(x, name, group):
     x = _operand(x, name)
-    _float_dtype(x, name)
-    if x.dim() != 2 or x.shape[1] < 1:
+    if x.dtype not in _DTYPES:
+        _float_dtype(x, name)
+    shape = x.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{name} must be [n, F]")
     if group not in (32, 64, 128):
         raise ValueError(f"group must be 32, 64 or 128, got {group}")
@@ -1970,7 +2002,10 @@ def _pack_arguments(x, name, group):
 
 def _check_kept(kept, halves):
     """Rows and columns of what :func:`pack_rows` (``halves`` 1) or :func:`gated_pack` (2) kept, if it is whole."""
-    codes, scale, group = kept.codes, kept.scale, kept.group
+    codes, scale, group, dtype, known = kept.codes, kept.scale, kept.group, kept.dtype, kept._checked
+    if (known is not None and known[0] is codes and known[1] is scale and known[2] == group and known[3] is dtype
+            and known[4] == halves):
+        return known[5]
     if codes.dim() != 2 or scale.dim() != 2 or group not in (32, 64, 128) or codes.shape[1] < 1 or codes.shape[1] % halves:
         raise ValueError("codes must be [n, columns], scale [n, groups], a group 32, 64 or 128 columns")
     n, F = codes.shape[0], codes.shape[1] // halves
@@ -1978,8 +2013,9 @@ def _check_kept(kept, halves):
         raise ValueError("the scales do not fit the codes" + (": were these rows kept by gated_pack?" if halves == 1 else
                                                               ": rows [n, 2 F] that gated_pack kept"))
     if (codes.dtype != torch.int8 or scale.dtype != torch.float32 or not codes.is_contiguous() or not scale.is_contiguous()
-            or kept.dtype not in _DTYPES):
+            or dtype not in _DTYPES):
         raise ValueError("codes must be int8 and scale float32, both contiguous, dtype float32, float16 or bfloat16")
+    kept._checked = codes, scale, group, dtype, halves, (n, F)
     return n, F
 
 
@@ -1990,9 +2026,16 @@ def pack_rows(x, group=64):
     gradient on."""
     x = _pack_arguments(x, "x", group)
     codes, scale = _packed_like(x, 1, group)
-    _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], group, codes.data_ptr(),
-                                       scale.data_ptr(), _stream_for(x)), "hc_pack_rows")
-    return PackedRows(codes, scale, group, x.dtype)
+    n, F = codes.shape
+    _check(load_library().hc_pack_rows(x.data_ptr(), _DTYPES[x.dtype], n, F, group, codes.data_ptr(), scale.data_ptr(),
+                                       _stream_for(x)), "hc_pack_rows")
+    return _whole(PackedRows(codes, scale, group, x.dtype), 1, n, F)
+
+
+def _whole(kept, halves, n, F):
+    """``kept``, which has just been made: it need not be checked."""
+    kept._checked = kept.codes, kept.scale, kept.group, kept.dtype, halves, (n, F)
+    return kept
 
 
 def unpack_rows(kept, dtype=None):
@@ -2016,14 +2059,21 @@ def gated_pack(x, group=64, keep=True):
     x = _pack_arguments(x, "x", group)
     if _watched(x):
         raise RuntimeError("gated_pack records no gradient: call it on x.detach() and take the gradient from gated_grad")
-    if x.shape[1] % 2 != 0:
+    n, F = x.shape
+    if F % 2 != 0:
         raise ValueError("x must hold two halves of the same width")
-    n, F = x.shape[0], x.shape[1] // 2
+    h, codes, scale = _gate(x, group, keep)
+    return h, _whole(PackedRows(codes, scale, group, x.dtype), 2, n, F // 2) if keep else None
+
+
+def _gate(x, group, keep):
+    n, F = x.shape
+    F //= 2
     h = x.new_empty((n, F))
     codes, scale = _packed_like(x, 2, group) if keep else (None, None)
     _check(load_library().hc_gated_pack(x.data_ptr(), _DTYPES[x.dtype], n, F, group, h.data_ptr(), _ptr(codes), _ptr(scale),
                                         _stream_for(x)), "hc_gated_pack")
-    return h, PackedRows(codes, scale, group, x.dtype) if keep else None
+    return h, codes, scale
 
 
 def gated_grad(kept, g):
@@ -2035,18 +2085,23 @@ def gated_grad(kept, g):
     if g.shape != (n, F):
         raise ValueError(f"g must be [{n}, {F}], got {tuple(g.shape)}")
     _together(g, codes, scale)
+    return _gate_grad(codes, scale, kept.group, g)
+
+
+def _gate_grad(codes, scale, group, g):
+    n, F = g.shape
     gx, h = g.new_empty((n, 2 * F)), torch.empty_like(g)
-    _check(load_library().hc_gated_grad(codes.data_ptr(), scale.data_ptr(), g.data_ptr(), _DTYPES[kept.dtype], n, F,
-                                        kept.group, gx.data_ptr(), h.data_ptr(), _stream_for(g)), "hc_gated_grad")
+    _check(load_library().hc_gated_grad(codes.data_ptr(), scale.data_ptr(), g.data_ptr(), _DTYPES[g.dtype], n, F, group,
+                                        gx.data_ptr(), h.data_ptr(), _stream_for(g)), "hc_gated_grad")
     return gx, h
 
 
 class _GatedExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w_in, w_out, offset, group):
-        h, kept = gated_pack(_expert_product(rows, w_in, offset, False), group)
-        ctx.save_for_backward(rows, w_in, w_out, offset, kept.codes, _bits(kept.scale))
-        ctx.hc = (group, rows.dtype)
+        h, codes, scale = _gate(_expert_product(rows, w_in, offset, False), group, True)
+        ctx.save_for_backward(rows, w_in, w_out, offset, codes, _bits(scale))
+        ctx.hc = group
         return _expert_product(h, w_out, offset, False)
 
     @staticmethod
@@ -2054,11 +2109,11 @@ class _GatedExperts(torch.autograd.Function):
     def backward(ctx, g):
         rows, w_in, w_out, offset, codes, scale = ctx.saved_tensors
         need, g = ctx.needs_input_grad, _arriving(g)
-        g_pre, h = gated_grad(PackedRows(codes, scale.view(torch.float32), *ctx.hc), _expert_product(g, w_out, offset, True))
-        g_out = expert_linear_grad(g, h, offset) if need[2] else None
+        g_pre, h = _gate_grad(codes, scale, ctx.hc, _expert_product(g, w_out, offset, True))
+        g_out = _expert_grad(g, h, offset) if need[2] else None
         del h
         return (_expert_product(g_pre, w_in, offset, True) if need[0] else None,
-                expert_linear_grad(g_pre, rows, offset) if need[1] else None, g_out, None, None)
+                _expert_grad(g_pre, rows, offset) if need[1] else None, g_out, None, None)
 
 
 def gated_experts(rows, w_in, w_out, offset, group=64):
@@ -2078,7 +2133,7 @@ def gated_experts(rows, w_in, w_out, offset, group=64):
     _together(rows, w_in, w_out, offset)
     if _watched(rows, w_in, w_out):
         return _GatedExperts.apply(rows, w_in, w_out, offset, group)
-    return _expert_product(gated_pack(_expert_product(rows, w_in, offset, False), group, keep=False)[0], w_out, offset, False)
+    return _expert_product(_gate(_expert_product(rows, w_in, offset, False), group, False)[0], w_out, offset, False)
 
 
 def evict(checkin, slot2full, full2slot, stale_iter, sub2slot=None, score=None, thres=None):
