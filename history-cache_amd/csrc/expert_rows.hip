@@ -82,7 +82,8 @@ __device__ __forceinline__ void or_load(const int64_t *__restrict__ expert, int6
   }
 }
 
-// Everything in one block of 64 pairs a wave and round: a row of E + 1 counters for each wave, one for the sums.
+// Everything in one block of 64 pairs a wave and round: a row of E + 1 counters for each wave, one for the sums (69 700 bytes of LDS
+// with sixteen waves and 1 024 experts, of the 160 KB that a launch may ask for on this device).
 template <int ROUNDS>
 __global__ __launch_bounds__(OR_SMALL_BLOCK) void or_small(const int64_t *__restrict__ expert, int32_t *__restrict__ slot,
                                                             int32_t *__restrict__ pair, int64_t *__restrict__ offset, int P,
@@ -379,13 +380,18 @@ static int mv_with_choices(int64_t k, F &&f) {
 static bool mv_args(int64_t n, int64_t top_k, int64_t E, int64_t D, const int32_t *slot, const int64_t *offset, MvArgs *a) {
   if (n < 0 || top_k < 1 || E < 1 || D < 1) return false;
   a->n = n;
-  a->P = n * top_k;
+  a->P = (int64_t)((uint64_t)n * (uint64_t)top_k);          // (below 2^31, or the call is refused)
   a->D = (int)D;
   a->k = (int)top_k;
   a->E = (int)E;
   a->slot = slot;
   a->offset = offset;
   return true;
+}
+
+// Fewer than 2^31 pairs, as hc_expert_order sorts.
+static bool mv_sizes_ok(int64_t n, int64_t top_k, int64_t E, int64_t D) {
+  return D < (1 << 30) && n <= ((1ll << 31) - 1) / top_k && top_k < (1ll << 31) && E <= OR_MAX_EXPERTS;
 }
 
 // Elements of T in a piece, and whether it may lie at any element: 16 bytes, for rows that are shorter as many as their length and
@@ -452,7 +458,7 @@ extern "C" int hc_rows_to_experts(const void *x, int dtype, int64_t n, int64_t t
                                   const int32_t *slot, const int64_t *offset, void *rows, void *stream) {
   MvArgs a;
   HC_REQUIRE(mv_args(n, top_k, E, D, slot, offset, &a));
-  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (!mv_sizes_ok(n, top_k, E, D)) return HC_EUNSUPPORTED;
   if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
   HC_REQUIRE(x && slot && offset && rows);
   return mv_with_type(dtype, [&](auto type) {
@@ -474,7 +480,7 @@ extern "C" int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t
                                     const int32_t *slot, const float *weight, void *out, void *stream) {
   MvArgs a;
   HC_REQUIRE(mv_args(n, top_k, E, D, slot, nullptr, &a));
-  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (!mv_sizes_ok(n, top_k, E, D)) return HC_EUNSUPPORTED;
   if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
   HC_REQUIRE(y && slot && out);
   return mv_with_type(dtype, [&](auto type) {
@@ -499,7 +505,7 @@ extern "C" int hc_rows_from_experts_grad(const void *g, const void *y, int dtype
                                          void *grad_y, float *grad_weight, void *stream) {
   MvArgs a;
   HC_REQUIRE(mv_args(n, top_k, E, D, slot, offset, &a));
-  if (D >= (1 << 30) || n > (1ll << 31) / top_k || E > OR_MAX_EXPERTS) return HC_EUNSUPPORTED;
+  if (!mv_sizes_ok(n, top_k, E, D)) return HC_EUNSUPPORTED;
   if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
   HC_REQUIRE(g && y && slot && offset && weight && grad_y && grad_weight);
   return mv_with_type(dtype, [&](auto type) {

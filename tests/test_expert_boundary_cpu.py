@@ -222,3 +222,11 @@ def test_calls_of_two_threads_on_one_stream_share_no_scratch_memory(monkeypatch,
     for t in threads:
         t.join()
     assert len(seen) == 2 and seen[0] != seen[1]
+
+
+def test_more_pairs_than_an_order_holds_are_refused(lib, p):
+    for n, k in ((1, 1 << 31), (1 << 30, 2), (2, 1 << 30), (1 << 40, 1 << 40), (0, 1 << 31)):
+        for call in (lambda: lib.hc_rows_to_experts(p, 0, n, k, 4, 8, p, p, p, None),
+                     lambda: lib.hc_rows_from_experts(p, 0, n, k, 4, 8, p, p, p, None),
+                     lambda: lib.hc_rows_from_experts_grad(p, p, 0, n, k, 4, 8, p, p, p, p, p, None)):
+            assert call() == EUNSUPPORTED, (n, k)
