@@ -819,8 +819,8 @@ VsLayout vs_layout(const VsShape &S) {
   return L;
 }
 
-// A launch with more dynamic LDS than the default limit (64 KB) has to be allowed once per kernel; the
-// compute unit has 160 KB.  The largest size allowed so far is remembered per kernel (a benign race: two
+// A launch with more dynamic LDS than 64 KB is allowed once per kernel, as HIP documents for limits that are set per kernel (ROCm 7.2
+// launches up to the compute unit's 160 KB without it, as hc_expert_order's single block does).  The largest size allowed so far is remembered per kernel (a benign race: two
 // threads may both ask).
 template <auto KERNEL>
 bool vs_allow_lds(size_t bytes) {

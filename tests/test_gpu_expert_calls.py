@@ -163,3 +163,18 @@ def test_routing_under_autocast_and_in_half_precision():
     out.float().sum().backward()
     assert out.dtype == torch.bfloat16 and all(bool(torch.isfinite(p.grad).all()) for p in (rows, *half.parameters()))
     assert half.router.grad.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("n,k,E", ((1921, 1, 963), (256, 8, 1024), (2047, 1, 1024), (7681, 1, 1000), (1024, 8, 1024), (8191, 1, 1024)))
+def test_an_order_by_one_block_with_many_experts(n, k, E):
+    """Sixteen waves with a row of counters each: more than 64 KB of LDS."""
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    expert = torch.randint(-1, E, (n, k), device=DEV, generator=gen)
+    order, flat = be.expert_order(expert, E), expert.reshape(-1)
+    live = int((flat >= 0).sum())
+    pair = torch.sort(torch.where(flat < 0, E, flat), stable=True)[1]
+    place = torch.empty_like(pair)
+    place[pair] = torch.arange(n * k, device=DEV)
+    assert torch.equal(order.pair[:live].long(), pair[:live]) and bool((order.pair[live:] == -1).all())
+    assert torch.equal(order.slot.long(), torch.where(flat < 0, -1, place))
+    assert torch.equal(order.offset, torch.searchsorted(torch.sort(flat)[0], torch.arange(E + 1, device=DEV)) - (n * k - live))
