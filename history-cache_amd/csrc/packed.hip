@@ -1,9 +1,10 @@
 // Activations kept in 8 bits for the backward pass.  A row's columns are taken in groups of 32, 64 or 128 (the last one may
 // be shorter); a group keeps one fp32 scale and a signed byte per element:
 //
-//   m = max |x|;  scale = m * (1 / 127);  code = rint(x * (1 / m * 127));  x' = code * scale        (|x' - x| <= scale / 2)
+//   m = max |x|;  scale = m * (1 / 127);  code = rint(x * (1 / m * 127));  x' = code * scale
 //
-// each operation rounded to fp32, one division per group.  Eight bits are what the caller asks for: they halve (fp32: quarter)
+// |x' - x| is at most half a scale and what six fp32 operations on up to 127 scales round (0.50005 scales); x' rounded to fp16 is
+// another 0.062 scales off, to bf16 0.5 (half a unit of the type, of 127 scales).  Each operation rounded to fp32, one division per group.  Eight bits are what the caller asks for: they halve (fp32: quarter)
 // what a layer keeps between forward and backward.  A group whose m is below 2^-120, where 127 / m leaves fp32, is kept as zeros;
 // one that holds an infinity or a NaN has that as its scale and zeros as codes, so that all of it reads back as NaN.  The largest
 // numbers take the largest scale whose 127-fold is finite.

@@ -121,7 +121,8 @@ def _is_activation(t, min_elements, group=64):
 
 def packed_activations(group=64, min_elements=1 << 16):
     """Context in which what autograd saves for backward is kept in 8 bits, a scale for every ``group`` columns
-    (``hiscache_backend.pack_rows``): the gradients are those at activations that are off by up to half a scale.
+    (``hiscache_backend.pack_rows``): the gradients are those at activations that are off by up to half a scale
+    (16-bit ones by what they are rounded to their type besides: up to a whole scale in bf16).
 
     Kept as they are: parameters, views of parameters and matrices computed from parameters alone in a few steps (a cast copy,
     a scaled or normalised weight); other leaves that need a gradient and their views; whole numbers; tensors of fewer than

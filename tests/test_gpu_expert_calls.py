@@ -178,3 +178,16 @@ def test_an_order_by_one_block_with_many_experts(n, k, E):
     assert torch.equal(order.pair[:live].long(), pair[:live]) and bool((order.pair[live:] == -1).all())
     assert torch.equal(order.slot.long(), torch.where(flat < 0, -1, place))
     assert torch.equal(order.offset, torch.searchsorted(torch.sort(flat)[0], torch.arange(E + 1, device=DEV)) - (n * k - live))
+
+
+@pytest.mark.parametrize("dtype,most", ((torch.float32, 0.5001), (torch.float16, 0.57), (torch.bfloat16, 1.0)))
+@pytest.mark.parametrize("group", (32, 64, 128))
+def test_how_far_off_rows_in_8_bits_read_back(dtype, most, group):
+    """Half a scale, 127 x 6 x 2^-24 scales of rounding in fp32, and half a unit of the type on up to 127 scales: 2^-11 of them in
+    fp16 (0.0621), 2^-8 in bf16 (0.4961)."""
+    gen = torch.Generator(device=DEV).manual_seed(group)
+    x = (torch.randn(20_000, 2 * group + 7, device=DEV, generator=gen) * torch.exp(torch.randn(20_000, 1, device=DEV, generator=gen))).to(dtype)
+    kept = be.pack_rows(x, group)
+    off = (be.unpack_rows(kept).double() - x.double()).abs()
+    scale = kept.scale.double().repeat_interleave(group, 1)[:, :x.shape[1]]
+    assert bool((off <= most * scale).all())
