@@ -798,7 +798,8 @@ int hc_bn_relu_bwd_dev(const float *dy, const float *x, const float *gamma, cons
  * weight [n, top_k].  normalize != 0: a row's weights are divided by their sum.
  * A logit of -inf closes an expert to the row; where fewer than top_k are open
  * the rest are -1 with weight 0.  A row with a NaN or +inf has NaN weights.
- * E <= 1024, top_k <= 32 and <= E.
+ * E <= 1024, top_k <= 32 and <= E; n L <= 2^32 - 512 for L = 8 lanes a row up to
+ * 64 experts, 16 up to 128, 32 up to 256, 64 above.
  * hc_route_rows_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and
  * the outputs of hc_route_rows (logits may be NULL with normalize). */
 int hc_route_rows(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int normalize,
@@ -824,7 +825,8 @@ int hc_expert_order(const int64_t *expert, int64_t pairs, int64_t E, int32_t *sl
  *                              (weight NULL: 1, the gradient of hc_rows_to_experts)
  *   hc_rows_from_experts_grad  grad_y[place] = weight g[row], 0 behind offset[E];
  *                              grad_weight[i, j] = <g[i], y[slot]>
- * rows, y, grad_y are [n * top_k, D]. */
+ * rows, y, grad_y are [n * top_k, D].  n * top_k < 2^31, D < 2^30, n * ceil(D *
+ * size / 16) <= 2^32 - 512 (pieces of 16 bytes). */
 int hc_rows_to_experts(const void *x, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
                        const int32_t *slot, const int64_t *offset, void *rows, void *stream);
 int hc_rows_from_experts(const void *y, int dtype, int64_t n, int64_t top_k, int64_t E, int64_t D,
@@ -858,7 +860,8 @@ int hc_expert_linear_grad(const void *g, const void *x, int dtype, const int64_t
  * hc_gated_pack: h [n, F] = silu(a) b for rows [a | b] of x [n, 2 F]; codes
  * [n, 2 F] and scale [n, 2 ceil(F / group)] (both NULL: not kept), groups of a
  * and of b apart.  hc_gated_grad: from those, the gradient of x [n, 2 F] and
- * (h not NULL) h again, for grad_h [n, F]. */
+ * (h not NULL) h again, for grad_h [n, F].  F < 2^30; n *
+ * ceil(F / group) * group / 8 <= 2^32 - 512. */
 int hc_pack_rows(const void *x, int dtype, int64_t n, int64_t F, int64_t group, int8_t *codes, float *scale,
                  void *stream);
 int hc_unpack_rows(const int8_t *codes, const float *scale, int64_t n, int64_t F, int64_t group, void *x,

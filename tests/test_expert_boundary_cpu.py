@@ -230,3 +230,20 @@ def test_more_pairs_than_an_order_holds_are_refused(lib, p):
                      lambda: lib.hc_rows_from_experts(p, 0, n, k, 4, 8, p, p, p, None),
                      lambda: lib.hc_rows_from_experts_grad(p, p, 0, n, k, 4, 8, p, p, p, p, p, None)):
             assert call() == EUNSUPPORTED, (n, k)
+
+
+def test_the_documented_limits_of_rows(lib, p):
+    """The first size behind each limit is refused before anything is launched."""
+    for E, lanes in ((64, 8), (65, 16), (129, 32), (257, 64), (1024, 64)):
+        assert lib.hc_route_rows(p, 0, (1 << 32) // lanes, E, 1, 1, p, p, None) == EUNSUPPORTED
+        assert lib.hc_route_rows_grad(p, 0, (1 << 32) // lanes, E, 1, 1, p, p, p, p, None) == EUNSUPPORTED
+    n = (1 << 32) // 512                                           # rows of 4 096 bf16: 512 pieces
+    assert lib.hc_rows_to_experts(p, 2, n, 2, 4, 4096, p, p, p, None) == EUNSUPPORTED
+    assert lib.hc_rows_from_experts(p, 2, n, 2, 4, 4096, p, p, p, None) == EUNSUPPORTED
+    assert lib.hc_rows_from_experts_grad(p, p, 2, (1 << 32) // 64, 2, 4, 4096, p, p, p, p, p, None) == EUNSUPPORTED
+    for group in (32, 64, 128):
+        n = (1 << 35) // (2 * group)                               # rows of one group and a column
+        assert lib.hc_pack_rows(p, 0, n, group + 1, group, p, p, None) == EUNSUPPORTED
+        assert lib.hc_unpack_rows(p, p, n, group + 1, group, p, 0, None) == EUNSUPPORTED
+        assert lib.hc_gated_pack(p, 0, n, group + 1, group, p, p, p, None) == EUNSUPPORTED
+        assert lib.hc_gated_grad(p, p, p, 0, n, group + 1, group, p, p, None) == EUNSUPPORTED
