@@ -1826,14 +1826,16 @@ class _RowsFromExperts(torch.autograd.Function):
 # The places are whole numbers that no hook has to see and the graph may hold; what autograd does for saved tensors beyond that is
 # done here at a tenth of its host time: a change in place between forward and backward is noticed.
 def _keep_places(ctx, places):
-    slot, offset = places[:2]
-    ctx.hc = places
-    ctx.versions = slot._version, offset._version
+    ctx.hc, ctx.versions = places, _versions(*places[:2])
+
+
+def _versions(*tensors):
+    # (a tensor made in inference mode counts none, and may not be changed in place outside it)
+    return tuple(None if t.is_inference() else t._version for t in tensors)
 
 
 def _kept_places(ctx):
-    slot, offset = ctx.hc[:2]
-    if (slot._version, offset._version) != ctx.versions:
+    if _versions(*ctx.hc[:2]) != ctx.versions:
         raise RuntimeError("one of the variables needed for gradient computation has been modified by an inplace operation: the "
                            "places or the offsets of an ExpertOrder")
     return ctx.hc

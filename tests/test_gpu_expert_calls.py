@@ -191,3 +191,16 @@ def test_how_far_off_rows_in_8_bits_read_back(dtype, most, group):
     off = (be.unpack_rows(kept).double() - x.double()).abs()
     scale = kept.scale.double().repeat_interleave(group, 1)[:, :x.shape[1]]
     assert bool((off <= most * scale).all())
+
+
+def test_an_order_made_in_inference_mode():
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    expert = torch.randint(0, 3, (40, 2), device=DEV, generator=gen)
+    x, w = torch.randn(40, 24, device=DEV, generator=gen).requires_grad_(True), torch.rand(40, 2, device=DEV, generator=gen)
+    with torch.inference_mode():
+        made = be.expert_order(expert, 3)
+    grads = []
+    for order in (be.expert_order(expert, 3), made):
+        out = be.rows_from_experts(be.rows_to_experts(x, order), order, w)
+        grads.append(torch.autograd.grad(out.square().sum(), x)[0])
+    assert torch.equal(*grads)
