@@ -6,16 +6,18 @@
 //   expert, a block per expert turns the counts of the chunks into first places, every block places its chunk.  Inside a
 //   chunk a wave owns a run of adjacent pairs and takes 64 at a time: lanes with the same expert find each other by
 //   ballots over the bits of the expert's number, so that places ascend with the pair whatever the scheduling.
-//   Bound by its launches: 65 644 pairs of 64 experts 5 + 3 + 6 us, eight pairs 2.6.
+//   Bound by its launches: 65 644 pairs of 64 experts 5 + 3 + 6 us, 400 006 of 8 5 + 6 + 7 (the middle one walks an expert's chunks
+//   64 at a time, each behind the one before), eight pairs 2.6.
 //
 // hc_rows_to_experts: rows[place] = x[pair[place] / top_k], zeros behind offset[E].  Walks the rows of x, each read once
 //   and stored at its top_k places.
 // hc_rows_from_experts: out[i] = sum_j weight[q] * y[slot[q]] in the order of j, summed in fp32 (weight NULL: 1, which is
 //   the gradient of hc_rows_to_experts).
 // hc_rows_from_experts_grad: grad_y[place] = weight[q] * g[i], zeros behind offset[E], and grad_weight[q] = <g[i], y[slot[q]]>.
-// All are bound by the rows' way through memory (a plain copy reaches 4.7 TB/s, a fill 6.8).  16 411 rows of 1 024 bf16 to four experts /
-// back / the gradient of that: 29 / 41 / 58 us, 5.8 / 4.1 / 5.2 TB/s; 200 003 rows of 256 fp32 to two: 112 / 108 / 179, 5.5 / 5.7 / 5.7.
-// A row's choices are read side by side (one after the other: 195 us for all of the first case, 181 so).
+// All are bound by the rows' way through memory (a plain copy reaches 4.7 TB/s, a fill 6.8).  In a training pass (one kernel after
+// the other, each with its own matrices) 16 411 rows of 1 024 bf16 to four experts / back with weights / the gradient of that / of
+// the way there: 30 / 48 / 58 / 34 us, 5.7 / 3.4 / 5.2 / 4.9 TB/s; 200 003 rows of 256 fp32 to two: 111 / 125 / 178 / 91, 5.5 / 4.6 /
+// 5.5 / 6.3.  A row's choices are read side by side (one after the other: 195 us for all of the first case, 181 so).
 #include "hc_common.h"
 
 namespace {
@@ -307,7 +309,8 @@ __global__ __launch_bounds__(HC_BLOCK) void mv_from(MvArgs a, const T *__restric
       if (s[j] >= 0 && weight != nullptr) {
         row::load(y + (int64_t)s[j] * a.D + c, p[j]);
       } else if (s[j] >= 0) {
-        // gradients: nothing reads them after this (the first case above, plain / non-temporal: 42 / 33 us; the second 110 / 93)
+        // gradients: nothing reads them after this.  (In the passes above, plain / non-temporal: 43 / 34 and 101 / 91 us; what the last-level
+        // cache then holds makes the next pass's sum with weights take 42 / 48 and 116 / 125: both together 85 / 82 and 217 / 216.)
         row::template load<true>(y + (int64_t)s[j] * a.D + c, p[j]);
       } else {
 #pragma unroll

@@ -8,9 +8,10 @@
 //
 // Sums are held in fp32 and rounded once, to the type of the result.  Large products are bound by the matrix pipes and by what
 // their feeding leaves of them: a step of a large tile reads 192 KB from LDS and writes 64, at 128 bytes a cycle as long as its
-// products take -- 8 192 x 8 192 x 8 192 bf16 905 / 880 / 860 us (forward, gradient of x, of w; 1 215 to 1 280
-// TFLOP/s), 32 771 rows of 16 experts of 2 048 x 1 024 bf16 166 / 155 / 153 (830 to 900), 8 192 x 4 096 x 4 096 fp32 1 976 / 1 927 /
-// 1 875 (139 to 147) --, few rows at many experts by reading the matrices (16 rows at 15 of 2 048 x 1 024 bf16 12 us, 63 MB).
+// products take -- 8 192 x 8 192 x 8 192 bf16 910 / 896 / 877 us (forward, gradient of x, of w with its join; 1 209 to
+// 1 254 TFLOP/s), 32 771 rows of 16 experts of 2 048 x 1 024 bf16 169 / 157 / 159 (812 to 875), 8 192 x 4 096 x 4 096 fp32 1 979 / 1 948 /
+// 1 934 (139 to 142) --, few rows at many experts by reading the matrices (16 rows at 15 of 2 048 x 1 024 bf16 12 us, 63 MB).  These are
+// launches of one kind back to back; the three of a training pass take 528 us there (each by itself, under a profiler, 201 / 206 / 192).
 #pragma once
 
 #include "expert_find.h"

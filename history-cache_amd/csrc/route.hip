@@ -9,8 +9,9 @@
 // one instruction; fp32 takes 64 bits.  A lane sorts its keys once; the winners then are, one after the other, the largest of the
 // row's first keys, and the lane that had it moves up.  With `normalize` the sum runs over the winners alone, and each lane
 // takes the exponential of the winner that it keeps.
-// Bound: a lane's sort and the k joins of its row forward (500 009 rows of 64 bf16 logits to four of them: 27 us for 88 MB; with the
-// winners joined through LDS and the keys not sorted 42).  Backward a row's choices are read once, by its first lanes, and go to
+// Bound: a lane's sort and the k joins of its row forward (500 009 rows of 64 bf16 logits to four of them: 28 us for 88 MB, with
+// the winners joined through LDS and the keys not sorted 42; fp32 logits, whose keys take 64 bits, 43 for 152 MB; of 256 experts to
+// eight of them 127 for 304 and 227 for 560).  Backward a row's choices are read once, by its first lanes, and go to
 // their places through LDS: 15 us for 96 MB, by memory (read by every lane of the row and looked for among its logits 26; 500 009
 // rows of 256, eight of them, 80 and 181).  Small batches are bound by the launch: eight rows 4 us.
 #include "hc_common.h"

@@ -1829,9 +1829,9 @@ def _keep_places(ctx, places):
     ctx.hc, ctx.versions = places, _versions(*places[:2])
 
 
-def _versions(*tensors):
+def _versions(slot, offset):
     # (a tensor made in inference mode counts none, and may not be changed in place outside it)
-    return tuple(None if t.is_inference() else t._version for t in tensors)
+    return None if slot.is_inference() else slot._version, None if offset.is_inference() else offset._version
 
 
 def _kept_places(ctx):
