@@ -130,7 +130,8 @@ def packed_activations(group=64, min_elements=1 << 16):
     sparse tensors; and anything not packed in the current GPU's memory.  Any other matrix counts as an activation, a copy of a
     frozen weight among them, since nothing tells it from the rows of a batch: run a product by one outside.  A matrix that
     several operators save is kept once for each of them, and one that the caller holds on to is kept besides.  Put the context
-    around the layers whose activations may be rounded; a loss, a softmax or the router's weights are better left outside."""
+    around the layers whose activations may be rounded; a loss, a softmax, attention (whose sums of exponentials would be rounded as
+    logarithms) or the router's weights are better left outside."""
     be = hiscache_backend
 
     def pack(t):
