@@ -18,7 +18,7 @@
 //   pass 3  per tile: ballot-rank the mask, un-map old owners, map, copy rows
 // Pass 1 is the only pass that touches the gradient matrix; pass 3 only touches
 // admitted rows, so HBM traffic is the algorithmic minimum.
-#include "hc_common.h"
+#include "packed_rows.h"
 
 #include <mutex>
 
@@ -380,16 +380,40 @@ __device__ __forceinline__ void copy_rows_fast(const float *__restrict__ emb, TT
   }
 }
 
+// The same for a table in 8 bits (packed_rows.h): a lane takes eight adjacent columns of a row, L lanes share a group's scale, and
+// the block's lanes lie one after the other over the admitted rows' groups.  slot_of (held by lane j): the slot of rank j.
+template <int L>
+__device__ __forceinline__ void copy_rows_packed(const float *__restrict__ emb, int8_t *__restrict__ codes,
+                                                 float *__restrict__ scale, int64_t F, int src_lane, int64_t slot_of,
+                                                 int64_t tile0, int first_rank, int n_adm, int wave, int lane) {
+  const uint32_t groups = (uint32_t)((F + L * PK_EACH - 1) / (L * PK_EACH)), lanes = groups * L;
+  const uint64_t items = (uint64_t)(uint32_t)(n_adm - first_rank) * lanes;
+  for (uint64_t t0 = (uint64_t)wave * HC_WAVE; t0 < items; t0 += HC_BLOCK) {
+    const uint64_t t = t0 + (uint64_t)lane;
+    const bool live = t < items;
+    const uint32_t k = live ? (uint32_t)(t / lanes) : 0, in = live ? (uint32_t)(t - (uint64_t)k * lanes) : 0;
+    const int q = first_rank + (int)k;
+    const int64_t row = tile0 + __shfl(src_lane, q, HC_WAVE), slot = __shfl(slot_of, q, HC_WAVE);
+    const int64_t col = (int64_t)in * PK_EACH;
+    const int valid = !live || col >= F ? 0 : F - col >= PK_EACH ? PK_EACH : (int)(F - col);
+    float v[PK_EACH];
+    pk_row<float>::load(emb + row * F + col, valid, v);
+    const float s = pk_encode<L>(v, codes + slot * F + col, valid);
+    if (live && in % L == 0) scale[slot * groups + in / L] = s;
+  }
+}
+
 // No barrier and no LDS: every wave of the block reads the tile's 64 mask bytes and offsets itself, so
 // its first row loads are issued one memory round trip after the wave starts.
-template <bool SMALL>
+// PACKED: lanes of a group of a table in 8 bits (0: the table holds numbers of table_dtype).
+template <bool SMALL, int PACKED>
 __global__ __launch_bounds__(HC_BLOCK) void gc_pass3_ring(
     const uint8_t *__restrict__ mask, const uint8_t *__restrict__ tile_counts,
     const int64_t *__restrict__ chunk_prefix, const GcScalars *__restrict__ sc, const float *__restrict__ emb,
     const int64_t *__restrict__ sub_to_full, void *__restrict__ table, int table_dtype, int64_t capacity,
     int64_t *__restrict__ full2slot, int64_t *__restrict__ slot2full, int64_t *__restrict__ checkin,
     int64_t *__restrict__ slot_out, int64_t *__restrict__ header, int64_t glb_iter_value,
-    const int64_t *__restrict__ glb_iter_dev, int64_t M, int64_t F, int64_t n_tiles) {
+    const int64_t *__restrict__ glb_iter_dev, int64_t M, int64_t F, int64_t n_tiles, float *__restrict__ scale) {
   const int lane = hc_lane();
   const int wave = hc_wave_in_block();
   // the iteration number that admitted rows are stamped with: by value, or read from device memory by
@@ -486,6 +510,11 @@ __global__ __launch_bounds__(HC_BLOCK) void gc_pass3_ring(
   // the others to the lanes behind the admitted ones (a permutation of the 64 lanes)
   const int target = m ? rank : n_adm + (lane - rank);
   const int src_lane = __builtin_amdgcn_ds_permute(target << 2, lane);
+  if constexpr (PACKED != 0) {
+    copy_rows_packed<PACKED>(emb, static_cast<int8_t *>(table), scale, F, src_lane, (slot0 + lane) % capacity, tile0, first_rank,
+                             n_adm, wave, lane);
+    return;
+  }
   const bool fast = (F % 256 == 0) && (F / 256 <= 4) && (reinterpret_cast<uintptr_t>(emb) % 16 == 0) &&
                     (reinterpret_cast<uintptr_t>(table) % 16 == 0);
   if (fast) {
@@ -635,7 +664,7 @@ int grad_check_launch(const float *grad, const float *score_in, const float *emb
                       int64_t *slot_out, void *table, int table_dtype, int64_t capacity, int64_t *full2slot,
                       int64_t *slot2full, int64_t *checkin, int64_t *header, int64_t glb_iter,
                       const int64_t *glb_iter_dev, int64_t M, int64_t F, void *workspace, size_t workspace_bytes,
-                      void *stream) {
+                      void *stream, float *scale = nullptr, int64_t group = 0) {
   HC_REQUIRE(M >= 0 && F > 0 && capacity > 0);
   HC_REQUIRE(norm_kind == HC_NORM_L2 || norm_kind == HC_NORM_L1);
   HC_REQUIRE(cmp_kind == HC_CMP_LT || cmp_kind == HC_CMP_NOT_GT);
@@ -657,20 +686,24 @@ int grad_check_launch(const float *grad, const float *score_in, const float *emb
   int rc = launch_pass1<true>(grad, score_in, slot, age, used, thres, age_limit, norm_kind, cmp_kind,
                               mask_out, score_out, tiles_buf, M, F, st, header, small ? sc : nullptr);
   if (rc != HC_OK) return rc;
-  if (small) {
-    // two launches: every pass-3 block adds up the (at most 1 024) tile counts in front of it itself
-    gc_pass3_ring<true><<<dim3((unsigned)tiles), dim3(HC_BLOCK), 0, st>>>(
+  const auto pass3 = [&](auto small_, auto packed) {
+    gc_pass3_ring<decltype(small_)::value, decltype(packed)::value><<<dim3((unsigned)tiles), dim3(HC_BLOCK), 0, st>>>(
         mask_out, tiles_buf, chunk_prefix, sc, emb, sub_to_full, table, table_dtype, capacity, full2slot, slot2full,
-        checkin, slot_out, header, glb_iter, glb_iter_dev, M, F, tiles);
+        checkin, slot_out, header, glb_iter, glb_iter_dev, M, F, tiles, scale);
     return hc_launch_status();
-  }
+  };
+  const auto with_table = [&](auto small_) {
+    if (group == 32) return pass3(small_, std::integral_constant<int, 4>{});
+    if (group == 64) return pass3(small_, std::integral_constant<int, 8>{});
+    if (group == 128) return pass3(small_, std::integral_constant<int, 16>{});
+    return pass3(small_, std::integral_constant<int, 0>{});
+  };
+  // two launches: every pass-3 block adds up the (at most 1 024) tile counts in front of it itself
+  if (small) return with_table(std::true_type{});
   gc_pass2<<<dim3(1), dim3(GC_SCAN_THREADS), 0, st>>>(tiles_buf, tiles, chunk_prefix, sc, header, capacity, 1,
                                                       nullptr);
   if (hc_launch_status() != HC_OK) return HC_ELAUNCH;
-  gc_pass3_ring<false><<<dim3((unsigned)tiles), dim3(HC_BLOCK), 0, st>>>(
-      mask_out, tiles_buf, chunk_prefix, sc, emb, sub_to_full, table, table_dtype, capacity, full2slot, slot2full,
-      checkin, slot_out, header, glb_iter, glb_iter_dev, M, F, tiles);
-  return hc_launch_status();
+  return with_table(std::false_type{});
 }
 }  // namespace
 
@@ -699,6 +732,21 @@ extern "C" int hc_grad_check_dev(const float *grad, const float *score_in, const
   return grad_check_launch(grad, score_in, emb, slot, age, used, sub_to_full, thres, age_limit, norm_kind, cmp_kind,
                            mask_out, score_out, slot_out, table, table_dtype, capacity, full2slot, slot2full, checkin,
                            header, 0, glb_iter_dev, M, F, workspace, workspace_bytes, stream);
+}
+
+extern "C" int hc_grad_check_packed(const float *grad, const float *score_in, const float *emb,
+                                    const int64_t *slot, const int32_t *age, const uint8_t *used,
+                                    const int64_t *sub_to_full, const float *thres, int32_t age_limit,
+                                    int norm_kind, int cmp_kind, uint8_t *mask_out, float *score_out,
+                                    int64_t *slot_out, int8_t *codes, float *scale, int64_t group, int64_t capacity,
+                                    int64_t *full2slot, int64_t *slot2full, int64_t *checkin, int64_t *header,
+                                    int64_t glb_iter, const int64_t *glb_iter_dev, int64_t M, int64_t F,
+                                    void *workspace, size_t workspace_bytes, void *stream) {
+  if ((group != 32 && group != 64 && group != 128) || F >= (1 << 30)) return F < 1 ? HC_EINVAL : HC_EUNSUPPORTED;
+  HC_REQUIRE(M <= 0 || scale);
+  return grad_check_launch(grad, score_in, emb, slot, age, used, sub_to_full, thres, age_limit, norm_kind, cmp_kind,
+                           mask_out, score_out, slot_out, codes, HC_F32, capacity, full2slot, slot2full, checkin,
+                           header, glb_iter, glb_iter_dev, M, F, workspace, workspace_bytes, stream, scale, group);
 }
 
 // ---------------------------------------------------------------------------------------

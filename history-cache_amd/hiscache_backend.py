@@ -22,6 +22,7 @@ There is no CPU or PyTorch fallback: if the shared library is missing or a
 tensor is not on a GPU, the call raises.
 """
 import ctypes
+import math
 import os
 
 import torch
@@ -168,6 +169,18 @@ _SIGNATURES = {
     "hc_unpack_rows": (_c_int, [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_int, _c_p]),
     "hc_gated_pack": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p]),
     "hc_gated_grad": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
+    "hc_route_scores": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_int, ctypes.c_float, _c_p,
+                                 _c_p, _c_p, _c_p]),
+    "hc_route_scores_grad": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_int, ctypes.c_float, _c_p, _c_p, _c_p,
+                                      _c_p, _c_p, _c_p]),
+    "hc_grad_check_packed": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, ctypes.c_int32, _c_int,
+                                      _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p,
+                                      _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_sz, _c_p]),
+    "hc_ring_lookup_packed": (_c_int, [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64,
+                                       _c_p, _c_p, _c_i64, _c_p]),
+    "hc_adamw_step": (_c_int, [_c_int, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, ctypes.c_double, _c_p,
+                               ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _c_p]),
+    "hc_adamw_moments": (_c_int, [_c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_p]),
 }
 
 _lib_handle = None
@@ -848,7 +861,7 @@ def grad_check(grad, emb, slot, sub_to_full, thres, table, full2slot, slot2full,
 
     ``grad`` [M,F] fp32 (or None with ``score`` given), ``emb`` [M,F] fp32, ``slot`` [M] int64
     (-1 = not cached), ``thres`` 1-element fp32 device tensor, ``table`` [capacity,F]
-    fp32/fp16/bf16, maps int64, ``header`` 1-element int64 device tensor (advanced in place).
+    fp32/fp16/bf16, or :class:`PackedRows` of as many rows (an admitted row is packed as :func:`pack_rows` does), maps int64, ``header`` 1-element int64 device tensor (advanced in place).
     Returns (mask[bool], score[f32]) and the per-row slot when ``want_slots``."""
     lib = load_library()
     _dev(emb, "emb", torch.float32)
@@ -865,12 +878,14 @@ def grad_check(grad, emb, slot, sub_to_full, thres, table, full2slot, slot2full,
     _dev(slot, "slot", torch.int64)
     _dev(sub_to_full, "sub_to_full", torch.int64)
     thres = _dev(thres.reshape(1), "thres", torch.float32)
-    _dev(table, "table")
-    if table.dim() != 2 or table.shape[1] != F:
+    packed = isinstance(table, PackedRows)
+    shape = _packed_table(table) if packed else _dev(table, "table").shape
+    if len(shape) != 2 or shape[1] != F:
         raise ValueError("table must be [capacity, F]")
+    capacity = shape[0]
     for t, n in ((full2slot, "full2slot"), (slot2full, "slot2full"), (header, "header")):
         _dev(t, n, torch.int64)
-    if slot2full.numel() < table.shape[0]:
+    if slot2full.numel() < capacity:
         raise ValueError("slot2full is shorter than the table")
     if age is not None:
         _dev(age, "age", torch.int32)
@@ -892,10 +907,28 @@ def grad_check(grad, emb, slot, sub_to_full, thres, table, full2slot, slot2full,
         _dev(glb_iter, "glb_iter", torch.int64)
         if static_scratch:
             raise ValueError("glb_iter on the device goes with a workspace")
+    if packed:
+        if static_scratch:
+            raise ValueError("a table in 8 bits goes with a workspace")
+        for t, n in ((checkin, "checkin"), (full2slot, "full2slot")):
+            if t is not None and t.device != table.codes.device:
+                raise ValueError(f"{n} and the table must lie on one device")
+        if checkin is not None and checkin.numel() < capacity:
+            raise ValueError("checkin is shorter than the table")
+        ws = _workspace(lib.hc_grad_check_workspace_bytes(M), dev)
+        _check(lib.hc_grad_check_packed(
+            _ptr(grad), _ptr(score), _ptr(emb), _ptr(slot), _ptr(age), _ptr(used), _ptr(sub_to_full), _ptr(thres),
+            int(age_limit), int(norm_kind), int(cmp_kind), _ptr(mask), _ptr(score_out), _ptr(slot_out), _ptr(table.codes),
+            _ptr(table.scale), table.group, capacity, _ptr(full2slot), _ptr(slot2full), _ptr(checkin), _ptr(header),
+            0 if iter_on_device else int(glb_iter), _ptr(glb_iter) if iter_on_device else None, M, F, _ptr(ws), ws.numel(),
+            _stream()), "hc_grad_check_packed")
+        if want_slots:
+            return mask.view(torch.bool), score_out, slot_out
+        return mask.view(torch.bool), score_out
     args = (_ptr(grad), _ptr(score), _ptr(emb), _ptr(slot), _ptr(age), _ptr(used),
             _ptr(sub_to_full), _ptr(thres), int(age_limit), int(norm_kind), int(cmp_kind),
             _ptr(mask), _ptr(score_out), _ptr(slot_out), _ptr(table),
-            _float_dtype(table, "table"), table.shape[0], _ptr(full2slot), _ptr(slot2full),
+            _float_dtype(table, "table"), capacity, _ptr(full2slot), _ptr(slot2full),
             _ptr(checkin), _ptr(header), _ptr(glb_iter) if iter_on_device else int(glb_iter), M, F)
     if iter_on_device:
         ws = _workspace(lib.hc_grad_check_workspace_bytes(M), dev)
@@ -1228,24 +1261,50 @@ def lookup(map_tensor, ids, offset=0, n_valid=None):
     return out
 
 
+def _packed_table(table):
+    """Rows and columns of a ring table in 8 bits."""
+    capacity, F = _check_kept(table, 1)
+    if not table.codes.is_cuda or table.scale.device != table.codes.device:
+        raise RuntimeError("codes and scale of a table must live on one GPU; this module has no CPU path")
+    return capacity, F
+
+
 def ring_lookup(full2slot, ids, table, checkin=None, now=0, age_limit=1 << 62, want_rows=True, n_valid=None):
-    """Slots of ``ids`` in a ring table and the table rows of the hits, in one launch.  An entry with
+    """Slots of ``ids`` in a ring table (fp32, fp16, bf16 or :class:`PackedRows`) and the table rows of the hits, in one launch.
+    An entry with
     ``now - checkin[slot] >= age_limit`` counts as absent (-1).  Returns (slot[int64], rows[fp32] or
     None); rows of absent ids are zero.  For recorded iterations ``now`` may be a one-element int64 device
     tensor, together with ``n_valid`` (the same): ids behind the first ``n_valid`` are padding and find nothing."""
     lib = load_library()
     _dev(full2slot, "full2slot", torch.int64)
     _dev(ids, "ids", torch.int64)
-    _dev(table, "table")
-    if table.dim() != 2:
-        raise ValueError("table must be [capacity, F]")
+    packed = isinstance(table, PackedRows)
+    if packed:
+        capacity, F = _packed_table(table)
+    else:
+        _dev(table, "table")
+        if table.dim() != 2:
+            raise ValueError("table must be [capacity, F]")
+        capacity, F = table.shape
     if checkin is not None:
         _dev(checkin, "checkin", torch.int64)
-        if checkin.numel() < table.shape[0]:
+        if checkin.numel() < capacity:
             raise ValueError("checkin is shorter than the table")
     n = ids.numel()
     slot = torch.empty(n, dtype=torch.int64, device=ids.device)
-    rows = torch.empty((n, table.shape[1]), dtype=torch.float32, device=ids.device) if want_rows else None
+    rows = torch.empty((n, F), dtype=torch.float32, device=ids.device) if want_rows else None
+    if packed:
+        on_device = isinstance(now, torch.Tensor)
+        if on_device != (n_valid is not None):
+            raise ValueError("now and n_valid go together as one-element int64 device tensors")
+        if on_device:
+            _dev(now, "now", torch.int64)
+            _dev(n_valid, "n_valid", torch.int64)
+        _check(lib.hc_ring_lookup_packed(_ptr(full2slot), full2slot.numel(), _ptr(ids), _ptr(checkin),
+                                         0 if on_device else int(now), _ptr(now) if on_device else None, _ptr(n_valid),
+                                         int(age_limit), _ptr(table.codes), _ptr(table.scale), table.group, capacity, F,
+                                         _ptr(slot), _ptr(rows), n, _stream()), "hc_ring_lookup_packed")
+        return slot, rows
     if isinstance(now, torch.Tensor) or n_valid is not None:
         if not isinstance(now, torch.Tensor) or n_valid is None:
             raise ValueError("now and n_valid go together as one-element int64 device tensors")
@@ -1714,12 +1773,61 @@ class _RouteRows(torch.autograd.Function):
         return grad, None, None
 
 
-def route_rows(logits, top_k, normalize=True):
+def _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, scale, keep=False):
+    n, E = logits.shape
+    expert = logits.new_empty((n, top_k), dtype=torch.int64)
+    weight = logits.new_empty((n, top_k), dtype=torch.float32)
+    picked = torch.empty_like(weight) if keep else None
+    _check(load_library().hc_route_scores(logits.data_ptr(), _DTYPES[logits.dtype], n, E, top_k, score, _ptr(bias), num_group,
+                                          top_group, normalize, scale, expert.data_ptr(), weight.data_ptr(), _ptr(picked),
+                                          _stream_for(logits)), "hc_route_scores")
+    return (expert, weight, picked) if keep else (expert, weight)
+
+
+class _RouteScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, normalize, score, num_group, top_group, scale):
+        by_logit = score == _SCORES["sigmoid"]
+        expert, weight, *picked = _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, scale, by_logit)
+        ctx.mark_non_differentiable(expert)
+        ctx.set_materialize_grads(False)
+        # (softmax weights that add up to one go by themselves, sigmoid ones by the chosen logits)
+        kept = picked[0] if by_logit else None if normalize else logits
+        ctx.save_for_backward(_bits(kept), expert, _bits(weight))
+        ctx.hc = (top_k, normalize, score, scale, by_logit, logits.shape, logits.dtype)
+        return expert, weight
+
+    @staticmethod
+    @_once
+    def backward(ctx, _g_expert, g):
+        if g is None:
+            return (None,) * 8
+        kept, expert, weight = ctx.saved_tensors
+        top_k, normalize, score, scale, by_logit, (n, E), dtype = ctx.hc
+        g = _arriving(g)
+        grad = g.new_empty((n, E), dtype=dtype)
+        _check(load_library().hc_route_scores_grad(None if by_logit else _ptr(kept), _DTYPES[dtype], n, E, top_k, score, normalize,
+                                                   scale, expert.data_ptr(), weight.data_ptr(), _ptr(kept) if by_logit else None,
+                                                   g.data_ptr(), grad.data_ptr(), _stream_for(g)), "hc_route_scores_grad")
+        return (grad,) + (None,) * 7
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+MAX_EXPERT_GROUPS = 64
+
+
+def route_rows(logits, top_k, normalize=True, score="softmax", bias=None, num_group=1, top_group=1, scale=1.0):
     """The ``top_k`` experts of every row and their weights: softmax of ``logits`` [n, E] (fp32, fp16 or bf16, E <= 1024),
     its largest entries in falling order, of equal ones the lowest index first.  Returns (expert int64 [n, top_k],
     weight fp32 [n, top_k]); ``normalize``: the weights of a row are divided by their sum.  A logit of -inf closes an
     expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
-    weights.  The gradient of the weights reaches ``logits``.  top_k <= 32."""
+    weights.  The gradient of the weights reaches ``logits``.  top_k <= 32.
+
+    ``score`` "sigmoid": the logistic function of each logit in place of the softmax (a NaN logit is chosen first; weights whose
+    sum is 0 are 0).  ``bias`` (fp32 [E]): experts are chosen by score + bias, the larger in fp64, and weighted by the score alone; it
+    has no gradient, and -inf closes an expert.  ``top_group`` < ``num_group`` <= 64: experts lie in ``num_group`` groups of as many neighbours, of
+    which a row may take the ``top_group`` with the largest sum of two (score + bias) in them, of equal ones the lowest.
+    ``scale``: a positive factor of the weights."""
     logits = _operand(logits, "logits")
     if logits.dtype not in _DTYPES:
         _float_dtype(logits, "logits")
@@ -1728,6 +1836,28 @@ def route_rows(logits, top_k, normalize=True):
         raise ValueError("logits must be [n, E]")
     if not 1 <= top_k <= shape[1]:
         raise ValueError(f"top_k must be between 1 and the {shape[1]} experts, got {top_k}")
+    if bias is not None or score != "softmax" or num_group != 1 or top_group != 1 or scale != 1:
+        E, num_group, top_group, scale = shape[1], int(num_group), int(top_group), float(scale)
+        if score not in _SCORES:
+            raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+        if not 1 <= top_group <= num_group <= min(E, MAX_EXPERT_GROUPS) or E % num_group:
+            raise ValueError(f"num_group must divide the {E} experts and be at most {MAX_EXPERT_GROUPS}, top_group lie between 1 and "
+                             f"num_group: got {num_group}, {top_group}")
+        if top_k > E // num_group * top_group:
+            raise ValueError(f"top_k must be at most the {E // num_group * top_group} experts of {top_group} groups, got {top_k}")
+        if not 0 < scale < math.inf:
+            raise ValueError(f"scale must be positive, got {scale}")
+        if bias is None:
+            _together(logits)
+        else:
+            bias = _operand(bias, "bias", torch.float32)
+            if bias.shape != (E,):
+                raise ValueError(f"bias must be [{E}], got {list(bias.shape)}")
+            if bias.requires_grad and torch.is_grad_enabled():
+                raise ValueError("bias takes part in the choice alone and has no gradient: pass bias.detach()")
+            _together(logits, bias)
+        how = bias, top_k, int(bool(normalize)), _SCORES[score], num_group, top_group, scale
+        return _RouteScores.apply(logits, *how) if _watched(logits) else _route_scores(logits, *how)
     _together(logits)
     return (_RouteRows.apply if _watched(logits) else _route)(logits, top_k, int(bool(normalize)))
 
@@ -2137,6 +2267,169 @@ def gated_experts(rows, w_in, w_out, offset, group=64):
     if _watched(rows, w_in, w_out):
         return _GatedExperts.apply(rows, w_in, w_out, offset, group)
     return _expert_product(_gate(_expert_product(rows, w_in, offset, False), group, False)[0], w_out, offset, False)
+
+
+# ----------------------------------------------------------------------------- optimizer
+ADAMW_GROUP = 128             # adjacent elements that share an exponent where states are held in 8 bits
+
+
+class AdamWState:
+    """What :func:`adamw_step` keeps of a tensor from step to step.  ``step`` int64 [2]: the steps made, and a word that is zero
+    between calls.  States in 32 bits: ``exp_avg`` and ``exp_avg_sq`` fp32, of the tensor's shape.  In 8 bits: ``exp_avg`` and
+    ``exp_avg_sq`` uint8, of the tensor's shape, codes of the first moment and of the second one's root, and ``scale`` uint8 [2,
+    groups], the exponents that every 128 adjacent elements share (``hc_adamw_step``).  ``master``: the fp32 copy of a tensor in
+    half precision, or None."""
+    __slots__ = ("exp_avg", "exp_avg_sq", "step", "scale", "master", "_checked")
+
+    def __init__(self, exp_avg, exp_avg_sq, step, scale=None, master=None):
+        self.exp_avg, self.exp_avg_sq, self.step, self.scale, self.master = exp_avg, exp_avg_sq, step, scale, master
+        self._checked = None
+
+
+def adamw_state(param, bits=32, master=False):
+    """The state that a tensor starts with, for :func:`adamw_step`: moments of zero in ``bits`` 32 or 8; ``master``: with a copy
+    in fp32, for a tensor in half precision."""
+    if bits not in (8, 32):
+        raise ValueError(f"bits must be 8 or 32, got {bits}")
+    _float_dtype(param, "param")
+    if master and param.dtype is torch.float32:
+        raise ValueError("a tensor in fp32 has no other copy in fp32")
+    param = param.detach()
+    dtype = torch.uint8 if bits == 8 else torch.float32
+    moments = [torch.zeros(param.shape, dtype=dtype, device=param.device) for _ in range(2)]
+    scale = param.new_zeros((2, -(-param.numel() // ADAMW_GROUP)), dtype=torch.uint8) if bits == 8 else None
+    return AdamWState(*moments, param.new_zeros(2, dtype=torch.int64), scale,
+                      param.float().contiguous() if master else None)
+
+
+def _check_adamw_state(state, shape, index):
+    """Do the parts of a state fit a tensor of this shape on device ``index``?"""
+    parts = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
+    known = state._checked
+    if known is not None and known[1] == shape and known[2] == index:
+        for a, b in zip(known[0], parts):
+            if a is not b:
+                break
+        else:
+            return
+    m, v, step, scale, master = parts
+    bits8 = scale is not None
+    want = torch.uint8 if bits8 else torch.float32
+    numel = math.prod(shape)
+    if m.dtype is not want or v.dtype is not want or m.shape != shape or v.shape != shape:
+        raise ValueError(f"exp_avg and exp_avg_sq must be {want} {list(shape)}" + ("" if bits8 else " (states in 8 bits have a scale)"))
+    if bits8 and (scale.dtype is not torch.uint8 or scale.shape != (2, -(-numel // ADAMW_GROUP))):
+        raise ValueError(f"scale must be uint8 [2, {-(-numel // ADAMW_GROUP)}]")
+    if step.dtype is not torch.int64 or step.shape != (2,):
+        raise ValueError("step must be int64 [2]")
+    if master is not None and (master.dtype is not torch.float32 or master.shape != shape):
+        raise ValueError(f"master must be float32 {list(shape)}")
+    for t in parts:
+        if t is not None and (not t.is_cuda or t.get_device() != index or not t.is_contiguous() or t.is_neg()
+                              or t._is_zerotensor()):
+            raise ValueError("a state's parts must be contiguous and lie on the parameter's device")
+    state._checked = parts, shape, index
+
+
+def _pointers(tensors):
+    return (_c_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    """One AdamW step over many tensors, in place and in one launch for every 48 of a kind (element type, bits of the states, with
+    or without a copy):
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g g
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    in fp32.  ``params`` (contiguous, fp32, fp16 or bf16) and ``grads`` of the same shapes and types, ``states`` one
+    :class:`AdamWState` each (:func:`adamw_state`); t is each tensor's own count, on the device, so that a recorded step can be
+    replayed.  States in 8 bits: four bits of exponent below the largest of 128 elements, with three bits of mantissa for m and four
+    for sqrt(v), which is never rounded down to 0; the step that makes them uses them unrounded.  A group that holds an infinity
+    or a NaN is NaN from the next step on.  ``lr``: a number, or one fp32 on the device.  The tensors must not overlap: one that is
+    named twice is refused."""
+    params, grads, states = list(params), list(grads), list(states)
+    if len(grads) != len(params) or len(states) != len(params):
+        raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(states)} states")
+    b1, b2 = float(betas[0]), float(betas[1])
+    if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0):
+        raise ValueError(f"betas must lie in [0, 1) and eps must not be negative, got {betas}, {eps}")
+    if not params:
+        return
+    index = params[0].get_device()
+    kinds, seen = {}, set()
+    for p, g, state in zip(params, grads, states):
+        if not isinstance(p, torch.Tensor) or not p.is_cuda or not p.is_contiguous() or p.is_neg() or p._is_zerotensor():
+            _dev(p, "param")
+            raise ValueError("a parameter must be an ordinary tensor in memory")
+        if g.layout is not torch.strided:
+            raise ValueError("gradients must be dense")
+        dtype, shape = p.dtype, p.shape
+        if dtype not in _DTYPES:
+            _float_dtype(p, "param")
+        if g.shape != shape or g.dtype is not dtype:
+            raise ValueError(f"a gradient of {g.dtype} {list(g.shape)} for a parameter of {dtype} {list(shape)}")
+        g = _operand(g if g.is_contiguous() else g.contiguous(), "grad")
+        if g.get_device() != index or p.get_device() != index:
+            raise ValueError("the tensors must lie on one device")
+        _check_adamw_state(state, shape, index)
+        if state.master is not None and dtype is torch.float32:
+            raise ValueError("a parameter in fp32 has no other copy in fp32")
+        at = p.data_ptr()
+        if at in seen and p.numel():
+            raise ValueError("a parameter is named twice")
+        seen.add(at)
+        kind = dtype, state.scale is not None, state.master is not None
+        if kind not in kinds:
+            kinds[kind] = [], [], []
+        of = kinds[kind]
+        of[0].append(p)
+        of[1].append(g)
+        of[2].append(state)
+    _together(params[0])
+    if forward_ad._current_level >= 0:
+        _no_tangent(*params, *grads)
+    lr_dev = None
+    if isinstance(lr, torch.Tensor):
+        if lr.is_cuda:
+            lr_dev = _dev(lr, "lr", torch.float32)
+            if lr.numel() != 1 or lr.get_device() != index:
+                raise ValueError("lr must be a number or one fp32 on the parameters' device")
+            lr = 0.0
+        else:
+            lr = lr.item()
+    lib, stream = load_library(), _stream_for(params[0])
+    for (dtype, bits8, copies), (ps, gs, ss) in kinds.items():
+        n = len(ps)
+        _check(lib.hc_adamw_step(n, _pointers(ps), _pointers(gs), _DTYPES[dtype], _pointers([s.exp_avg for s in ss]),
+                                 _pointers([s.exp_avg_sq for s in ss]), _pointers([s.scale for s in ss]) if bits8 else None,
+                                 _pointers([s.master for s in ss]) if copies else None, _pointers([s.step for s in ss]),
+                                 (_c_i64 * n)(*[p.numel() for p in ps]), 8 if bits8 else 32, float(lr), _ptr(lr_dev), b1, b2,
+                                 float(eps), float(weight_decay), stream), "hc_adamw_step")
+    # the kernels wrote behind autograd's back: what was saved of a parameter is out of date
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+
+
+def adamw_moments(states, dtype=torch.float32):
+    """What states in 8 bits stand for: (first moment, root of the second moment) in ``dtype`` for each :class:`AdamWState` (fp32
+    and bf16 hold them exactly but for numbers below their own range)."""
+    states = list(states)
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    if not states:
+        return []
+    for s in states:
+        if s.scale is None:
+            raise ValueError("states in 32 bits are their own values")
+        _check_adamw_state(s, s.exp_avg.shape, states[0].exp_avg.get_device())
+    _together(states[0].exp_avg)
+    out = [(torch.empty_like(s.exp_avg, dtype=dtype), torch.empty_like(s.exp_avg, dtype=dtype)) for s in states]
+    n = len(states)
+    _check(load_library().hc_adamw_moments(
+        n, _pointers([s.exp_avg for s in states]), _pointers([s.exp_avg_sq for s in states]), _pointers([s.scale for s in states]),
+        (_c_i64 * n)(*[s.exp_avg.numel() for s in states]), _pointers([a for a, _ in out]), _pointers([b for _, b in out]),
+        _DTYPES[dtype], _stream_for(states[0].exp_avg)), "hc_adamw_moments")
+    return out
 
 
 def evict(checkin, slot2full, full2slot, stale_iter, sub2slot=None, score=None, thres=None):

@@ -808,6 +808,26 @@ int hc_route_rows_grad(const void *logits, int dtype, int64_t n, int64_t E, int6
                        const int64_t *expert, const float *weight, const float *grad_weight, void *grad_logits,
                        void *stream);
 
+/* hc_route_scores: hc_route_rows by scores s, the softmax (score 0) or the logistic
+ * function (1) of the logits, with a choice that goes by c = s + bias[e] (bias [E],
+ * NULL: by the logits themselves) and, where top_group < num_group, by groups of
+ * E / num_group adjacent experts: the top_group groups whose two largest c have the
+ * largest sum (of equal ones the lowest) stay open, in them the top_k largest c are
+ * chosen, of equal ones the lowest index first.  c and the sums are compared in fp64.
+ * weight = scale * s / (normalize ? sum of the chosen s : 1); 0 where that sum is 0.
+ * A logit or a bias of -inf closes an expert (-1, weight 0, where fewer than top_k are open).
+ * picked [n, top_k] (NULL: not kept): the chosen logits, which hc_route_scores_grad
+ * takes with score 1.  num_group <= 64 divides E, top_k <= E / num_group * top_group, scale > 0;
+ * the other limits are hc_route_rows'.
+ * hc_route_scores_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and the
+ * outputs of hc_route_scores (logits: score 0 without normalize; picked: score 1). */
+int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int score, const float *bias,
+                    int64_t num_group, int64_t top_group, int normalize, float scale, int64_t *expert,
+                    float *weight, float *picked, void *stream);
+int hc_route_scores_grad(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int score,
+                         int normalize, float scale, const int64_t *expert, const float *weight,
+                         const float *picked, const float *grad_weight, void *grad_logits, void *stream);
+
 /* hc_expert_order: stable sort of the pairs (row, choice) by expert, for
  * expert [pairs]; numbers outside [0, E) name no expert.  offset[E + 1]: the
  * places of expert e are offset[e] .. offset[e + 1]; pair[place] and
@@ -870,6 +890,54 @@ int hc_gated_pack(const void *x, int dtype, int64_t n, int64_t F, int64_t group,
                   float *scale, void *stream);
 int hc_gated_grad(const int8_t *codes, const float *scale, const void *grad_h, int dtype, int64_t n, int64_t F,
                   int64_t group, void *grad_x, void *h, void *stream);
+
+/* ---------------------------------------------------------------- a ring table in 8 bits
+ * hc_grad_check_packed / hc_ring_lookup_packed: hc_grad_check and hc_ring_lookup
+ * for a table of rows as hc_pack_rows keeps them, codes [capacity, F] and
+ * scale [capacity, ceil(F / group)]: an admitted row is packed as it is stored,
+ * a row that is found is read back in fp32, code * scale.  glb_iter_dev, now_dev
+ * and n_valid_dev (NULL: the values; every id counts) as in hc_grad_check_dev and
+ * hc_ring_lookup_dev.  group 32, 64 or 128, F < 2^30. */
+int hc_grad_check_packed(const float *grad, const float *score_in, const float *emb, const int64_t *slot,
+                         const int32_t *age, const uint8_t *used, const int64_t *sub_to_full,
+                         const float *thres, int32_t age_limit, int norm_kind, int cmp_kind,
+                         uint8_t *mask_out, float *score_out, int64_t *slot_out, int8_t *codes, float *scale,
+                         int64_t group, int64_t capacity, int64_t *full2slot, int64_t *slot2full,
+                         int64_t *checkin, int64_t *header, int64_t glb_iter, const int64_t *glb_iter_dev,
+                         int64_t M, int64_t F, void *workspace, size_t workspace_bytes, void *stream);
+int hc_ring_lookup_packed(const int64_t *full2slot, int64_t n_full, const int64_t *ids,
+                          const int64_t *checkin, int64_t now, const int64_t *now_dev,
+                          const int64_t *n_valid_dev, int64_t age_limit, const int8_t *codes,
+                          const float *scale, int64_t group, int64_t capacity, int64_t F, int64_t *slot_out,
+                          float *rows_out, int64_t n, void *stream);
+
+/* ---------------------------------------------------------------- AdamW step
+ * hc_adamw_step: one step over `count` tensors of one dtype, param[k] and
+ * grad[k] of numel[k] elements each, in place:
+ *   t += 1;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g g
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32, each operation rounded.  step[k]: two int64 on the device, t and a
+ * word that is zero between calls.  master (NULL, or for fp16 / bf16 tensors one
+ * fp32 copy each): takes the step in place of param[k], which is rounded from it.
+ * lr_dev (NULL, or one fp32 on the device) goes before lr.
+ * state_bits 32: exp_avg[k] = m and exp_avg_sq[k] = v in fp32, scale NULL.
+ * state_bits 8: exp_avg[k] holds m and exp_avg_sq[k] sqrt(v), a byte an element,
+ * and scale[k] two bytes for every 128 adjacent elements, [2, ceil(numel / 128)]:
+ * the exponent E of the m's and of the roots.  E is the biased fp32 exponent of
+ * the largest magnitude rounded to the codes' mantissa; x 2^(15 - E), rounded
+ * half to even, has as fp32 number an exponent of four bits and 3 (m, with a sign
+ * above them) or 4 bits of mantissa (sqrt(v), at least the smallest code where it
+ * is not 0): the code.  E = 0: zeros.  E = 255: a group with an infinity or a NaN,
+ * all of which reads back as NaN.
+ * No two of the tensors may overlap.  hc_adamw_moments: m and sqrt(v) of states of
+ * 8 bits as numbers of dtype. */
+int hc_adamw_step(int count, void *const *param, const void *const *grad, int dtype, void *const *exp_avg,
+                  void *const *exp_avg_sq, uint8_t *const *scale, float *const *master, int64_t *const *step,
+                  const int64_t *numel, int state_bits, double lr, const float *lr_dev, double beta1, double beta2,
+                  double eps, double weight_decay, void *stream);
+int hc_adamw_moments(int count, const void *const *exp_avg, const void *const *exp_avg_sq,
+                     const uint8_t *const *scale, const int64_t *numel, void *const *to_avg, void *const *to_root,
+                     int dtype, void *stream);
 
 #ifdef __cplusplus
 }
