@@ -57,31 +57,41 @@ __device__ __forceinline__ double aw_power(double b, int64_t t) {
 // What a tensor's elements share.
 struct AwFactors {
   float keep, size, lift;
-  __device__ __forceinline__ AwFactors(const AwArgs &a, const AwTensor &t) {
+  __device__ __forceinline__ void work_out(const AwArgs &a, int64_t count) {
     const double lr = a.lr_dev != nullptr ? (double)*a.lr_dev : a.lr;
-    const int64_t count = *t.step + 1;
     keep = (float)(1.0 - lr * a.decay);
     size = (float)(lr / (1.0 - aw_power(a.b1, count)));
     lift = (float)(1.0 / sqrt(1.0 - aw_power(a.b2, count)));
   }
 };
 
+// sqrt(x) for x >= 0, correctly rounded from 2^-96 up (below within a unit in the last place): the instruction's result or one of its
+// neighbours.
+__device__ __forceinline__ float aw_sqrt(float x) {
+  const float y = __builtin_amdgcn_sqrtf(x);
+  const float down = __uint_as_float(__float_as_uint(y) - 1u), up = __uint_as_float(__float_as_uint(y) + 1u);
+  const float r = __builtin_fmaf(-down, y, x) <= 0.f ? down : y;
+  return __builtin_fmaf(-up, y, x) > 0.f ? up : r;
+}
+
 // ---- numbers of 8 bits: MAN bits of mantissa (3: with a sign, 4: without)
+// A group of E = 255 is NaN: that comes in by the sum of its first operation (aw_poison).
+__device__ __forceinline__ float aw_poison(uint32_t E) { return E == 255u ? __builtin_nanf("") : 0.f; }
+
 template <int MAN>
 __device__ __forceinline__ void aw_decode(const uint32_t (&w)[2], uint32_t E, float (&v)[PK_EACH]) {
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
-    const uint32_t c = w[i / 4] >> (8 * (i % 4)) & 0xffu;
-    const uint32_t b = MAN == 3 ? (c & 0x80u) << 24 | (c & 0x7fu) << 20 : c << 19;
-    const float f = __builtin_amdgcn_ldexpf(__uint_as_float(b), (int)E - 15);
-    v[i] = E == 255u ? __builtin_nanf("") : f;
+    const uint32_t u = w[i / 4], at = 8 * (i % 4);
+    const uint32_t b = MAN == 3 ? (uint32_t)((int32_t)(u << (24 - at)) >> 24 << 20) & 0x87f00000u : (u >> at & 0xffu) << 19;
+    v[i] = __builtin_amdgcn_ldexpf(__uint_as_float(b), (int)E - 15);
   }
 }
 
-// Rounds fp32 bits to MAN bits of mantissa, ties to even, and takes off what lies under them.
+// Adds half a unit of MAN bits of mantissa to fp32 bits, a little less where that breaks a tie the even way.
 template <int MAN>
 __device__ __forceinline__ uint32_t aw_round(uint32_t b) {
-  return (b + (1u << (22 - MAN)) - 1u + (b >> (23 - MAN) & 1u)) >> (23 - MAN);
+  return b + (1u << (22 - MAN)) - 1u + (b >> (23 - MAN) & 1u);
 }
 
 // The E of the group that AW_LANES lanes hold, and this lane's codes.
@@ -94,18 +104,27 @@ __device__ __forceinline__ uint32_t aw_encode(const float (&v)[PK_EACH], uint32_
     most = b > most ? b : most;
   }
   most = hc_join<AW_LANES>(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-  const uint32_t top = aw_round<MAN>(most) >> MAN;
-  const uint32_t E = most >= 0x7f800000u ? 255u : top > 254u ? 254u : top;
-  constexpr uint32_t LARGEST = MAN == 3 ? 0x7fu : 0xffu;
-  w[0] = w[1] = 0;
+  const uint32_t top = aw_round<MAN>(most) >> 23, E = top > 255u ? 255u : top;
+  uint32_t c[PK_EACH];                       // the code in the upper byte
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
-    const uint32_t b = __float_as_uint(__builtin_amdgcn_ldexpf(v[i], 15 - (int)E));
-    uint32_t c = aw_round<MAN>(b & 0x7fffffffu);
-    c = c > LARGEST ? LARGEST : c;
-    if (MAN == 3) c |= c == 0 ? 0u : b >> 24 & 0x80u;
-    else c = c == 0 && v[i] > 0.f ? 1u : c;
-    w[i / 4] |= c << (8 * (i % 4));
+    uint32_t b = __float_as_uint(__builtin_amdgcn_ldexpf(v[i], 15 - (int)E));
+    if constexpr (MAN == 3) {
+      b = aw_round<3>(b);
+      c[i] = (b & 0x80000000u) | (b << 4 & 0x7fffffffu);
+    } else {
+      // (a root that is not 0 is above 2^-75)
+      const uint32_t least = __float_as_uint(v[i]) < 1u << 19 ? __float_as_uint(v[i]) : 1u << 19;
+      b = b > least ? b : least;
+      c[i] = aw_round<4>(b) << 5;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // the upper bytes of four words
+    const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x00000703u);
+    const uint32_t hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x07030000u);
+    w[i] = (lo & 0xffffu) | (hi & 0xffff0000u);
   }
   if (E == 0 || E == 255u) w[0] = w[1] = 0;
   return E;
@@ -131,12 +150,26 @@ __device__ __forceinline__ void aw_store_codes(void *p, int64_t at, int valid, c
 template <typename T, int BITS, bool MASTER>
 __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
   const float b1 = (float)a.b1, c1 = (float)(1.0 - a.b1), b2 = (float)a.b2, c2 = (float)(1.0 - a.b2);
+  __shared__ AwFactors s_factor[AW_MAX];
+  const bool counts = (int)threadIdx.x < a.count;
+  const int64_t count = counts ? *a.t[threadIdx.x].step + 1 : 0;
+  // s_factor is worked out while a block's first piece is on its way where that costs nothing: with states in 8 bits, whose pieces are
+  // bound by their operations, the loop without it is faster (50 M elements of bf16 116 us against 130; eight small tensors in 32
+  // bits 6.8 against 6.5).
+  bool known = false;
+  const auto work_out = [&] {
+    if (counts) s_factor[threadIdx.x].work_out(a, count);
+    __syncthreads();
+    known = true;
+  };
+  if constexpr (BITS == 8) work_out();
   uint32_t piece = blockIdx.x;
   const uint32_t pieces = a.first[a.count];
   for (int i = 0; piece < pieces;) {
     while (piece >= a.first[i + 1]) ++i;
     const AwTensor t = a.t[i];
-    const AwFactors f(a, t);
+    AwFactors f;
+    if (BITS == 8 || known) f = s_factor[i];
     const int64_t groups = (t.n + AW_GROUP - 1) / AW_GROUP;
     const uint32_t first = a.first[i], end = a.first[i + 1];
     for (; piece < end; piece += gridDim.x) {
@@ -154,19 +187,32 @@ __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
         if (valid > 0) Em = t.scale[at / AW_GROUP], Ev = t.scale[groups + at / AW_GROUP];
         aw_decode<3>(wm, Em, m);
         aw_decode<4>(wv, Ev, v);
+        const float nan_m = aw_poison(Em), nan_v = aw_poison(Ev);
 #pragma unroll
-        for (int k = 0; k < PK_EACH; ++k) v[k] = v[k] * v[k];
+        for (int k = 0; k < PK_EACH; ++k) {
+          m[k] = __builtin_fmaf(b1, m[k], nan_m);
+          v[k] = b2 * __builtin_fmaf(v[k], v[k], nan_v);
+        }
       } else {
         pk_row<float>::load(static_cast<const float *>(t.m) + at, valid, m);
         pk_row<float>::load(static_cast<const float *>(t.v) + at, valid, v);
+#pragma unroll
+        for (int k = 0; k < PK_EACH; ++k) m[k] = b1 * m[k], v[k] = b2 * v[k];
+      }
+      if constexpr (BITS == 32) {
+        if (!known) {
+          work_out();
+          f = s_factor[i];
+        }
       }
       float r[PK_EACH];
 #pragma unroll
       for (int k = 0; k < PK_EACH; ++k) {
-        m[k] = b1 * m[k] + c1 * g[k];
-        v[k] = b2 * v[k] + c2 * g[k] * g[k];
-        r[k] = sqrtf(v[k]);
-        p[k] = p[k] * f.keep - f.size * (m[k] / (r[k] * f.lift + a.eps));
+        m[k] = m[k] + c1 * g[k];
+        v[k] = v[k] + c2 * g[k] * g[k];
+        r[k] = aw_sqrt(v[k]);
+        // (the reciprocal is off by a unit in the last place: of a step that is some thousandth of p)
+        p[k] = p[k] * f.keep - f.size * (m[k] * __builtin_amdgcn_rcpf(r[k] * f.lift + a.eps));
       }
       if constexpr (MASTER) pk_row<float>::store(t.master + at, valid, p);
       pk_row<T>::store(static_cast<T *>(t.p) + at, valid, p);
@@ -191,7 +237,7 @@ __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
       }
     }
   }
-  // Every block has read the counts that it needs when it arrives here, so that the last one may count them up.
+  // All blocks have read the counts when the last one arrives: it counts them up.
   __syncthreads();
   if (threadIdx.x >= HC_WAVE) return;
   unsigned *arrived = reinterpret_cast<unsigned *>(a.t[0].step + 1);
@@ -226,10 +272,15 @@ __global__ __launch_bounds__(HC_BLOCK) void aw_read(AwRead a) {
     uint32_t w[2];
     float v[PK_EACH];
     aw_load_codes(a.m[i], at, valid, w);
-    aw_decode<3>(w, a.scale[i][at / AW_GROUP], v);
+    const uint32_t Em = a.scale[i][at / AW_GROUP], Ev = a.scale[i][groups + at / AW_GROUP];
+    aw_decode<3>(w, Em, v);
+#pragma unroll
+    for (int k = 0; k < PK_EACH; ++k) v[k] += aw_poison(Em);
     pk_row<T>::store(static_cast<T *>(a.to_m[i]) + at, valid, v);
     aw_load_codes(a.v[i], at, valid, w);
-    aw_decode<4>(w, a.scale[i][groups + at / AW_GROUP], v);
+    aw_decode<4>(w, Ev, v);
+#pragma unroll
+    for (int k = 0; k < PK_EACH; ++k) v[k] += aw_poison(Ev);
     pk_row<T>::store(static_cast<T *>(a.to_v[i]) + at, valid, v);
   }
 }

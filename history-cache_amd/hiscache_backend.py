@@ -2304,14 +2304,11 @@ def adamw_state(param, bits=32, master=False):
 
 def _check_adamw_state(state, shape, index):
     """Do the parts of a state fit a tensor of this shape on device ``index``?"""
-    parts = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
     known = state._checked
-    if known is not None and known[1] == shape and known[2] == index:
-        for a, b in zip(known[0], parts):
-            if a is not b:
-                break
-        else:
-            return
+    if (known is not None and known[0] is state.exp_avg and known[1] is state.exp_avg_sq and known[2] is state.step
+            and known[3] is state.scale and known[4] is state.master and known[5] == shape and known[6] == index):
+        return
+    parts = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
     m, v, step, scale, master = parts
     bits8 = scale is not None
     want = torch.uint8 if bits8 else torch.float32
@@ -2328,7 +2325,7 @@ def _check_adamw_state(state, shape, index):
         if t is not None and (not t.is_cuda or t.get_device() != index or not t.is_contiguous() or t.is_neg()
                               or t._is_zerotensor()):
             raise ValueError("a state's parts must be contiguous and lie on the parameter's device")
-    state._checked = parts, shape, index
+    state._checked = *parts, shape, index
 
 
 def _pointers(tensors):
@@ -2357,35 +2354,29 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
     if not params:
         return
     index = params[0].get_device()
-    kinds, seen = {}, set()
-    for p, g, state in zip(params, grads, states):
-        if not isinstance(p, torch.Tensor) or not p.is_cuda or not p.is_contiguous() or p.is_neg() or p._is_zerotensor():
-            _dev(p, "param")
-            raise ValueError("a parameter must be an ordinary tensor in memory")
-        if g.layout is not torch.strided:
-            raise ValueError("gradients must be dense")
-        dtype, shape = p.dtype, p.shape
-        if dtype not in _DTYPES:
-            _float_dtype(p, "param")
-        if g.shape != shape or g.dtype is not dtype:
-            raise ValueError(f"a gradient of {g.dtype} {list(g.shape)} for a parameter of {dtype} {list(shape)}")
-        g = _operand(g if g.is_contiguous() else g.contiguous(), "grad")
-        if g.get_device() != index or p.get_device() != index:
-            raise ValueError("the tensors must lie on one device")
+    # (a step of a few small tensors is the host's: what can be asked of all tensors is, in lists; a tensor of its own is looked at
+    # only where an answer is not the usual one)
+    dtypes = [p.dtype for p in params]
+    shapes = [p.shape for p in params]
+    if (index < 0 or [g.dtype for g in grads] != dtypes or [g.shape for g in grads] != shapes
+            or [p.get_device() for p in params].count(index) != len(params)
+            or [g.get_device() for g in grads].count(index) != len(params)
+            or False in [p.is_contiguous() for p in params] or True in [p.is_neg() for p in params]
+            or [g.layout for g in grads].count(torch.strided) != len(params)):
+        _adamw_refuse(params, grads)
+    if False in [g.is_contiguous() for g in grads] or True in [g.is_neg() for g in grads]:
+        grads = [_operand(g.contiguous(), "grad") for g in grads]
+    numels, at, of_g = [p.numel() for p in params], [p.data_ptr() for p in params], [g.data_ptr() for g in grads]
+    if 0 in at or 0 in of_g:                              # empty tensors, and zeros that were never written
+        if 0 in [a for a, n in zip(at, numels) if n]:
+            raise ValueError("a parameter must lie in memory")
+        grads = [g.clone() if g._is_zerotensor() else g for g in grads]
+        of_g = [g.data_ptr() for g in grads]
+    if len(set(at)) < len(at) and len({a for a, n in zip(at, numels) if n}) < len([n for n in numels if n]):
+        raise ValueError("a parameter is named twice")
+    for state, shape in zip(states, shapes):
         _check_adamw_state(state, shape, index)
-        if state.master is not None and dtype is torch.float32:
-            raise ValueError("a parameter in fp32 has no other copy in fp32")
-        at = p.data_ptr()
-        if at in seen and p.numel():
-            raise ValueError("a parameter is named twice")
-        seen.add(at)
-        kind = dtype, state.scale is not None, state.master is not None
-        if kind not in kinds:
-            kinds[kind] = [], [], []
-        of = kinds[kind]
-        of[0].append(p)
-        of[1].append(g)
-        of[2].append(state)
+    kinds = [(dtype, state.scale is not None, state.master is not None) for dtype, state in zip(dtypes, states)]
     _together(params[0])
     if forward_ad._current_level >= 0:
         _no_tangent(*params, *grads)
@@ -2398,16 +2389,51 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
             lr = 0.0
         else:
             lr = lr.item()
-    lib, stream = load_library(), _stream_for(params[0])
-    for (dtype, bits8, copies), (ps, gs, ss) in kinds.items():
-        n = len(ps)
-        _check(lib.hc_adamw_step(n, _pointers(ps), _pointers(gs), _DTYPES[dtype], _pointers([s.exp_avg for s in ss]),
-                                 _pointers([s.exp_avg_sq for s in ss]), _pointers([s.scale for s in ss]) if bits8 else None,
-                                 _pointers([s.master for s in ss]) if copies else None, _pointers([s.step for s in ss]),
-                                 (_c_i64 * n)(*[p.numel() for p in ps]), 8 if bits8 else 32, float(lr), _ptr(lr_dev), b1, b2,
-                                 float(eps), float(weight_decay), stream), "hc_adamw_step")
+    lib, stream = load_library(), _stream_of_device(index)
+    for kind in set(kinds):
+        dtype, bits8, copies = kind
+        if copies and dtype is torch.float32:
+            raise ValueError("a parameter in fp32 has no other copy in fp32")
+        if dtype not in _DTYPES:
+            _float_dtype(params[kinds.index(kind)], "param")
+    for kind in set(kinds):
+        dtype, bits8, copies = kind
+        mine = range(len(kinds)) if kinds.count(kind) == len(kinds) else [i for i, k in enumerate(kinds) if k == kind]
+        n, ss = len(mine), [states[i] for i in mine]
+        words = [at[i] for i in mine]
+        words += [of_g[i] for i in mine]
+        words += [s.exp_avg.data_ptr() for s in ss]
+        words += [s.exp_avg_sq.data_ptr() for s in ss]
+        words += [s.step.data_ptr() for s in ss]
+        words += [numels[i] for i in mine]
+        if bits8:
+            words += [s.scale.data_ptr() for s in ss]
+        if copies:
+            words += [s.master.data_ptr() for s in ss]
+        host = (_c_i64 * len(words))(*words)              # the arrays of the call one after the other
+        first = ctypes.addressof(host)
+        to = [first + 8 * n * k for k in range(8)]
+        _check(lib.hc_adamw_step(n, to[0], to[1], _DTYPES[dtype], to[2], to[3], to[6] if bits8 else None,
+                                 to[6 + bits8] if copies else None, to[4], to[5], 8 if bits8 else 32, float(lr), _ptr(lr_dev),
+                                 b1, b2, float(eps), float(weight_decay), stream), "hc_adamw_step")
     # the kernels wrote behind autograd's back: what was saved of a parameter is out of date
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+
+
+def _adamw_refuse(params, grads):
+    """Says which parameter or gradient makes no step, and why."""
+    index = params[0].get_device()
+    for p, g in zip(params, grads):
+        _dev(p, "param")
+        _float_dtype(p, "param")
+        if p.is_neg():
+            raise ValueError("a parameter must be an ordinary tensor in memory")
+        if g.layout is not torch.strided:
+            raise ValueError("gradients must be dense")
+        if g.shape != p.shape or g.dtype is not p.dtype:
+            raise ValueError(f"a gradient of {g.dtype} {list(g.shape)} for a parameter of {p.dtype} {list(p.shape)}")
+        if p.get_device() != index or g.get_device() != index:
+            raise ValueError("the tensors must lie on one device")
 
 
 def adamw_moments(states, dtype=torch.float32):
