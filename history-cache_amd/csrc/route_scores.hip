@@ -10,12 +10,13 @@
 // larger is decided in fp64: in fp32 one row in some ten thousand would go to another expert than by the formula.  Without a
 // bias experts are compared by their logits, with which the score rises.
 //
-// Forward: a wave takes 64 / L rows.  It reads them whole, puts into LDS what is compared (c, or l without a bias) as fp32, and each
-// row is then gone through by L lanes, every one with the K + 1 largest of its share in registers, sorted: a 64-bit number whose
-// upper half is c and whose lower half falls with the index orders, read as fp64, by both, so that a new one moves through the list
-// with one maximum and one minimum a place.  The lists of a row's lanes are put together at the end.  c in fp32 is off by up to 2^-21 or so:
-// where neighbours among the first K + 1, or the last open and the first closed group, are nearer than that and do not come from equal
-// numbers, the wave decides the row again in fp64, all lanes on it.
+// Forward: a wave takes 64 / L rows.  It reads them whole and puts what is compared (c, or l without a bias) into LDS as fp32; each row
+// is then gone through by L lanes, which hold the K + 1 largest of their share sorted in registers: a number's lowest bits make way for
+// the expert's index, and a new one moves into the list by one median a place.  What a lane has found gets its lost bits back, is
+// sorted by them and then the index, and put together with what the row's other lanes have.
+// Such a choice is right where nothing near stands against it.  c in fp32 is off by up to 2^-21: where neighbours in the list, or the last
+// open and the first closed group, are nearer than that and do not come from equal numbers, the wave decides the row again in fp64, all
+// lanes on it.  Where the first outside the list is near by the bits that were kept, it is counted how many are that near by all bits.
 #include "route_row.h"
 
 namespace {
@@ -32,12 +33,17 @@ struct RsArgs {
   float scale;
   int dtype, E, k, groups, per_group, top_group;
   int quads, stride, rank_stride;      // in LDS: pieces of four a row, floats from one row to the next, and from one row's ranks
+  uint32_t low;            // the bits that an index takes, and what they leave of a number's differences
+  float lost;
   bool softmax, normalize, whole;
 };
 
 __device__ __forceinline__ int64_t rs_bits(double v) { return __builtin_bit_cast(int64_t, v); }
 __device__ __forceinline__ double rs_double(int64_t v) { return __builtin_bit_cast(double, v); }
-__device__ __forceinline__ float rs_closed() { return -__builtin_inff(); }
+// What is compared lies between these as fp32, so that it stays a number when its lowest bits are an index: NaN and infinity as the
+// largest number; a closed expert below the lowest of the others.
+constexpr float RS_MOST = 0x1.fffffep+127f, RS_LEAST = -0x1.ffep+127f, RS_SHUT = -0x1.fffffep+127f;
+__device__ __forceinline__ bool rs_shut(float c) { return c < RS_LEAST; }
 
 // ---- the exact way: one row by a whole wave
 // fp64 as whole numbers that order like it: NaN above everything, CLOSED below.
@@ -140,53 +146,34 @@ __device__ __forceinline__ int rs_key_index(double k) {
   const uint64_t b = (uint64_t)rs_bits(k);
   return (int)~((uint32_t)b ^ (uint32_t)((int64_t)b >> 63));
 }
-
 __device__ __forceinline__ void rs_in_order(double &x, double &y) {
   const double low = __builtin_fmin(x, y);
   x = __builtin_fmax(x, y);
   y = low;
 }
 
-// The N largest numbers so far, sorted, and the largest of the others.
+// The N largest keys of the row's lanes, sorted, and the largest of the others.
 template <int N>
 struct rs_list {
   double t[N], out;
-  __device__ __forceinline__ rs_list() {
+  // t sorted (Batcher's odd-even merge sort)
+  __device__ __forceinline__ void sort() {
 #pragma unroll
-    for (int j = 0; j < N; ++j) t[j] = rs_key(rs_closed(), 0);
-    out = t[0];
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+      for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+        for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+          for (int i = 0; i < k; ++i)
+            if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) rs_in_order(t[i + j], t[i + j + k]);
   }
-  // M sorted numbers more: the last M here meet them the other way round, which leaves the N largest of all in two runs.
-  template <int M>
-  __device__ __forceinline__ void take(const double (&o)[M]) {
+  // `out` to its place among t
+  __device__ __forceinline__ void settle() {
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
-      const double mine = t[N - M + j], other = o[M - 1 - j];
-      t[N - M + j] = __builtin_fmax(mine, other);
-      out = __builtin_fmax(out, __builtin_fmin(mine, other));
-    }
-#pragma unroll
-    for (int d = N / 2; d >= 1; d /= 2)
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if ((i & d) == 0) rs_in_order(t[i], t[i + d]);
+    for (int j = 0; j < N; ++j) rs_in_order(t[j], out);
   }
-  __device__ __forceinline__ void take_four(float4 v, int e) {
-    double o[4] = {rs_key(v.x, e), rs_key(v.y, e + 1), rs_key(v.z, e + 2), rs_key(v.w, e + 3)};
-    rs_in_order(o[0], o[1]);
-    rs_in_order(o[2], o[3]);
-    rs_in_order(o[0], o[2]);
-    rs_in_order(o[1], o[3]);
-    rs_in_order(o[1], o[2]);
-    if constexpr (N >= 4) {
-      take(o);
-    } else {
-      const double two[2] = {o[0], o[1]};
-      out = __builtin_fmax(out, o[2]);
-      take(two);
-    }
-  }
-  // The list of the row that L lanes have, in each of them.
+  // the lists of L lanes as one, in each of them: two sorted lists that meet the other way round leave the larger half in two runs
   template <int L, int D = 1>
   __device__ __forceinline__ void join() {
     if constexpr (D < L) {
@@ -194,7 +181,17 @@ struct rs_list {
 #pragma unroll
       for (int j = 0; j < N; ++j) o[j] = rs_double(hc_other<D>(rs_bits(t[j])));
       out = __builtin_fmax(out, rs_double(hc_other<D>(rs_bits(out))));
-      take(o);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const double mine = t[j], other = o[N - 1 - j];
+        t[j] = __builtin_fmax(mine, other);
+        out = __builtin_fmax(out, __builtin_fmin(mine, other));
+      }
+#pragma unroll
+      for (int d = N / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if ((i & d) == 0) rs_in_order(t[i], t[i + d]);
       join<L, 2 * D>();
     }
   }
@@ -209,12 +206,13 @@ __device__ __forceinline__ float rs_sigma(float l) {
   return (l < 0.f ? e : 1.f) / (1.f + e);
 }
 
-// What is compared, as it lies in LDS: no -0, one NaN (another could make no number of a key).
-__device__ __forceinline__ float rs_plain(float c) { return c != c ? __uint_as_float(0x7fc00000u) : c + 0.f; }
-// c of a logit and a bias that is plain: s is not below 0.
+// What is compared, as it lies in LDS: of a logit or a bias; of a sum that cannot be too small; of a logit and a bias in LDS.
+__device__ __forceinline__ float rs_plain(float l) {
+  return rt_masked(l) ? RS_SHUT : fmaxf(fminf(l + 0.f, RS_MOST), RS_LEAST);
+}
 __device__ __forceinline__ float rs_choice(float l, float bias) {
-  const int32_t c = __builtin_bit_cast(int32_t, fabsf(rs_near_sigma(l)) + bias);
-  return rt_masked(l) ? rs_closed() : __builtin_bit_cast(float, c < 0x7fc00000 ? c : 0x7fc00000);
+  const float c = fminf(rs_near_sigma(l) + bias, RS_MOST);
+  return rt_masked(l) ? RS_SHUT : c;
 }
 
 // Rows r0 .. r0 + rows into LDS: c where the score is a logit's own and there is a bias, l otherwise.
@@ -271,25 +269,20 @@ __device__ __forceinline__ void rs_stage(const RsArgs &a, int64_t r0, int rows, 
       if (col >= a.E) col -= a.E, ++row;
     }
     for (int x = lane; x < rows * 4; x += HC_WAVE)            // the rest of a row's last four
-      if (a.E + x % 4 < 4 * a.quads) s[x / 4 * a.stride + a.E + x % 4] = rs_closed();
+      if (a.E + x % 4 < 4 * a.quads) s[x / 4 * a.stride + a.E + x % 4] = RS_SHUT;
   }
 }
 
-// Calls f(four values, index of the first) for the elements from .. to of a row in LDS that lane `sub` of L takes; behind `to`: closed.
+// Calls f(four values, index of the first) for the elements from .. to of a row in LDS that lane `sub` of L takes; behind `to`: shut.
 template <int L, typename F>
 __device__ __forceinline__ void rs_each(const float *row, int from, int to, int sub, bool by_four, F &&f) {
   if (by_four) {
     for (int e = from + 4 * sub; e < to; e += 4 * L) f(*reinterpret_cast<const float4 *>(row + e), e);
   } else {
     for (int e = from + 4 * sub; e < to; e += 4 * L)
-      f(make_float4(row[e], e + 1 < to ? row[e + 1] : rs_closed(), e + 2 < to ? row[e + 2] : rs_closed(),
-                    e + 3 < to ? row[e + 3] : rs_closed()), e);
+      f(make_float4(row[e], e + 1 < to ? row[e + 1] : RS_SHUT, e + 2 < to ? row[e + 2] : RS_SHUT, e + 3 < to ? row[e + 3] : RS_SHUT),
+        e);
   }
-}
-
-template <int L, typename F>
-__device__ __forceinline__ double rs_join(double v, F &&f) {
-  return rs_double(hc_join<L>(rs_bits(v), [&](int64_t x, int64_t y) { return rs_bits(f(rs_double(x), rs_double(y))); }));
 }
 
 // K: places for winners, k <= K; L: lanes a row.
@@ -297,14 +290,15 @@ template <int K, int L>
 __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
   // rows, the groups' ranks of each, the bias
   extern __shared__ __attribute__((aligned(16))) float s_all[];
-  constexpr int ROWS = HC_WAVE / L;
+  constexpr int ROWS = HC_WAVE / L, OWN = (K + L - 1) / L;
   const int lane = hc_lane(), sub = lane % L, mine = lane / L;
   const int64_t r0 = (int64_t)blockIdx.x * ROWS;
   const int rows = a.n - r0 < ROWS ? (int)(a.n - r0) : ROWS;
   const bool live = mine < rows;
   const int64_t r = r0 + (live ? mine : 0);
+  const bool exact = a.bias == nullptr;              // what is compared are logits
   float *bias = s_all + ROWS * (a.stride + a.rank_stride);
-  if (a.bias != nullptr) {
+  if (!exact) {
     for (int e = lane; e < a.E; e += HC_WAVE) bias[e] = rs_plain(a.bias[e]);
     rt_in_order();
   }
@@ -313,64 +307,60 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
   else rs_stage<__hip_bfloat16>(a, r0, rows, s_all, bias);
   rt_in_order();
   float *row = s_all + (live ? mine : 0) * a.stride;
-  float top = rs_closed(), all = 0.f;
+  float top = RS_SHUT, all = 0.f;
   if (a.softmax) {
     rs_each<L>(row, 0, 4 * a.quads, sub, true, [&](float4 l, int) { top = fmaxf(top, fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w))); });
     top = hc_join<L>(top, [](float x, float y) { return fmaxf(x, y); });
+    // (a closed expert lies so far below every other that its exponential is 0)
     double sum = 0.0;
-    const auto e = [&](float l) { return rt_masked(l) ? 0.f : expf(l - top); };
     rs_each<L>(row, 0, 4 * a.quads, sub, true, [&](float4 l, int) {
-      sum += ((double)e(l.x) + (double)e(l.y)) + ((double)e(l.z) + (double)e(l.w));
+      sum += ((double)expf(l.x - top) + (double)expf(l.y - top)) + ((double)expf(l.z - top) + (double)expf(l.w - top));
     });
-    sum = rs_join<L>(sum, [](double x, double y) { return x + y; });
+    sum = rs_double(hc_join<L>(rs_bits(sum), [](int64_t x, int64_t y) { return rs_bits(rs_double(x) + rs_double(y)); }));
     all = (float)sum;
-    if (a.bias != nullptr) {
+    if (!exact) {
       rt_in_order();
       if (live)
         for (int e = sub; e < a.E; e += L) {
           const float l = row[e];
-          row[e] = rt_masked(l) ? l : rs_plain(expf(l - top) / all + bias[e]);
+          row[e] = rs_shut(l) ? l : fminf(expf(l - top) / all + bias[e], RS_MOST);
         }
       rt_in_order();
     }
   }
-  const bool exact = a.bias == nullptr;              // what is compared are logits
   bool near = false;                                 // too near for fp32
   uint64_t open = ~0ull;
   const bool by_four = a.per_group % 4 == 0;
   if (a.groups > 1) {
     float *rank = s_all + ROWS * a.stride + mine * a.rank_stride;
     for (int g = 0; g < a.groups; ++g) {
-      float first = rs_closed(), second = rs_closed();
-      // (a NaN makes the sum one, whose group is decided again)
-      float nan = 0.f;
+      float first = RS_SHUT, second = RS_SHUT;
       const auto more = [&](float c) {
-        second = fmaxf(second, fminf(first, c));
+        second = __builtin_amdgcn_fmed3f(first, second, c);
         first = fmaxf(first, c);
       };
       rs_each<L>(row, g * a.per_group, (g + 1) * a.per_group, sub, by_four, [&](float4 c, int) {
-        const float x = fmaxf(c.x, c.y), y = fminf(c.x, c.y), z = fmaxf(c.z, c.w), w = fminf(c.z, c.w);
-        second = fmaxf(fmaxf(second, fmaxf(y, w)), fminf(fmaxf(x, z), fmaxf(first, fminf(x, z))));
-        first = fmaxf(first, fmaxf(x, z));
-        nan = c.x != c.x || c.y != c.y || c.z != c.z || c.w != c.w ? __builtin_nanf("") : nan;
+        more(c.x);
+        more(c.y);
+        more(c.z);
+        more(c.w);
       });
 #pragma unroll
       for (int d = 1; d < L; d *= 2) {
         const float f = __shfl_xor(first, d, HC_WAVE), s = __shfl_xor(second, d, HC_WAVE);
-        nan += __shfl_xor(nan, d, HC_WAVE);
         second = fmaxf(second, s);
         more(f);
       }
-      near = near || nan != nan;
-      if (exact && !rt_masked(first)) {
+      near = near || first >= RS_MOST;               // (infinite, or no number)
+      if (exact && !rs_shut(first)) {
         first = a.softmax ? expf(first - top) : rs_sigma(first);
-        second = a.softmax ? expf(second - top) : rs_sigma(second);
+        second = rs_shut(second) ? second : a.softmax ? expf(second - top) : rs_sigma(second);
       }
-      if (sub == 0) rank[g] = rt_masked(first) ? first : rt_masked(second) ? first : first + second;
+      if (sub == 0) rank[g] = rs_shut(second) ? first : first + second;
     }
     rt_in_order();
     // the last open group and the first closed one
-    float least = -rs_closed(), most = rs_closed();
+    float least = RS_MOST, most = RS_SHUT;
     open = 0;
     for (int g = sub; g < a.groups; g += L) {
       const float own = rank[g];
@@ -386,38 +376,94 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     least = hc_join<L>(least, [](float x, float y) { return fminf(x, y); });
     most = hc_join<L>(most, [](float x, float y) { return fmaxf(x, y); });
     const float off = exact ? 0x1p-16f * fabsf(least) : 0x1p-19f * (1.f + fabsf(least));
-    near = near || (!rt_masked(most) && !(least - most > off));
+    near = near || (!rs_shut(most) && !(least - most > off));
   }
-  rs_list<K> list;
-  if (a.groups > 1) {
-    uint64_t left = open;
-    for (int t = 0; t < a.top_group; ++t) {
-      const int g = left != 0 ? __builtin_ctzll(left) : 0;
-      left &= left - 1;
-      rs_each<L>(row, g * a.per_group, (g + 1) * a.per_group, sub, by_four, [&](float4 c, int e) { list.take_four(c, e); });
+  // f for the row's open elements that this lane takes
+  const auto each_open = [&](auto &&f) {
+    if (a.groups > 1) {
+      uint64_t left = open;
+      for (int t = 0; t < a.top_group; ++t) {
+        const int g = left != 0 ? __builtin_ctzll(left) : 0;
+        left &= left - 1;
+        rs_each<L>(row, g * a.per_group, (g + 1) * a.per_group, sub, by_four, f);
+      }
+    } else {
+      rs_each<L>(row, 0, 4 * a.quads, sub, true, f);
     }
-  } else {
-    rs_each<L>(row, 0, 4 * a.quads, sub, true, [&](float4 c, int e) { list.take_four(c, e); });
+  };
+  rs_list<K> list;
+  {
+    float t[K + 1];
+#pragma unroll
+    for (int j = 0; j <= K; ++j) t[j] = RS_SHUT;
+    const uint32_t low = a.low;
+    const auto more = [&](float c, int e) {
+      const float x = __uint_as_float((__float_as_uint(c) & ~low) | (low - (uint32_t)e));
+#pragma unroll
+      for (int j = K; j >= 1; --j) t[j] = __builtin_amdgcn_fmed3f(t[j - 1], t[j], x);
+      t[0] = __builtin_amdgcn_fmed3f(t[0], x, __builtin_inff());
+    };
+    each_open([&](float4 c, int e) {
+      more(c.x, e);
+      more(c.y, e + 1);
+      more(c.z, e + 2);
+      more(c.w, e + 3);
+    });
+    // (indexes behind the row's end are those of shut places, of which the list's first ones are some as well)
+    const auto whole = [&](float x) {
+      const int e = (int)(low - (__float_as_uint(x) & low));
+      const float c = row[e < a.stride ? e : 0];
+      return rs_shut(x) ? rs_key(RS_SHUT, 0) : rs_key(c, e);
+    };
+#pragma unroll
+    for (int j = 0; j < K; ++j) list.t[j] = whole(t[j]);
+    list.out = whole(t[K]);
   }
+  list.sort();
+  list.settle();
   list.template join<L>();
-  int won[K];
-  float p[K];
+  if (rs_key_value(list.t[1]) >= RS_MOST) near = true;                 // (two that are infinite or no numbers)
+  if (!exact || a.dtype == HC_F32) {
+    // l and bias of two experts
+    const auto equal = [&](double x, double y) {
+      const int i = rs_key_index(x), j = rs_key_index(y);
+      return rs_logit(a, r * a.E + i) == rs_logit(a, r * a.E + j) && (exact || bias[i] == bias[j]);
+    };
+    if (!exact) {
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    won[j] = j < a.k && !rt_masked(rs_key_value(list.t[j])) ? rs_key_index(list.t[j]) : -1;
-    p[j] = won[j] >= 0 ? rs_logit(a, r * a.E + won[j]) : 0.f;
-  }
-  if (!exact) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      const double next = j + 1 < K ? list.t[j + 1] : list.out;
-      const float c = rs_key_value(list.t[j]), d = rs_key_value(next);
-      if (j < a.k && !rt_masked(d) && !(c - d > 0x1p-20f * (1.f + fabsf(c)))) {
-        const int y = rs_key_index(next);
-        // (equal numbers: the lower index is the right one)
-        if (!(p[j] == rs_logit(a, r * a.E + y) && bias[won[j]] == bias[y])) near = true;
+      for (int j = 0; j + 1 < K; ++j) {
+        const float c = rs_key_value(list.t[j]), d = rs_key_value(list.t[j + 1]);
+        // (of equal numbers the lower index is the right one)
+        if (j + 1 < a.k && !rs_shut(d) && !(c - d > 0x1p-20f * (1.f + fabsf(c)))) near = near || !equal(list.t[j], list.t[j + 1]);
       }
     }
+    double last = list.t[0], next = list.out;
+#pragma unroll
+    for (int j = 1; j < K; ++j) {
+      if (j == a.k) next = list.t[j];
+      if (j < a.k) last = list.t[j];
+    }
+    const float c = rs_key_value(last), d = rs_key_value(next), off = exact ? 0.f : 0x1p-20f * (1.f + fabsf(c));
+    const bool count = !near && !rs_shut(d) && !(c - d > off + a.lost * fmaxf(fabsf(c), 0x1p-126f));
+    if (__ballot(count) != 0) {
+      int there = 0;
+      each_open([&](float4 v, int) {
+        const float from = c - off;
+        there += (v.x >= from ? 1 : 0) + (v.y >= from ? 1 : 0) + (v.z >= from ? 1 : 0) + (v.w >= from ? 1 : 0);
+      });
+      there = hc_join<L>(there, [](int x, int y) { return x + y; });
+      if (count) near = there > a.k && !(there == a.k + 1 && equal(last, next));
+    }
+  }
+  // this lane's winners
+  int won[OWN];
+#pragma unroll
+  for (int u = 0; u < OWN; ++u) {
+    double x = list.t[u * L];
+#pragma unroll
+    for (int d = 1; d < L; ++d)
+      if (u * L + d < K && sub == d) x = list.t[u * L + d];
+    won[u] = u * L + sub < a.k && !rs_shut(rs_key_value(x)) ? rs_key_index(x) : -1;
   }
   uint64_t again = __ballot(near && live && sub == 0);
   if (again != 0) {
@@ -428,30 +474,34 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
       const int row_of = __builtin_ctzll(again) / L;
       again &= again - 1;
       rs_choose_exactly(a, r0 + row_of, key, found);
-      if (mine == row_of) {
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-          won[j] = j < a.k ? found[j] : -1;
-          p[j] = won[j] >= 0 ? rs_logit(a, r * a.E + won[j]) : 0.f;
-        }
-      }
+      for (int u = 0; u < OWN; ++u)
+        if (mine == row_of && u * L + sub < a.k) won[u] = found[u * L + sub];
       rt_in_order();
     }
   }
-  float s[K], sum = 0.f;
+  float p[OWN], s[OWN], sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    s[j] = won[j] < 0 ? 0.f : a.softmax ? expf(p[j] - top) : rs_sigma(p[j]);
-    sum += s[j];
+  for (int u = 0; u < OWN; ++u) {
+    p[u] = won[u] >= 0 ? rs_logit(a, r * a.E + won[u]) : 0.f;
+    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(p[u] - top) : rs_sigma(p[u]);
+    sum += s[u];
   }
-  const float of = a.normalize ? (all != all ? all : sum) : a.softmax ? all : 1.f;
+  sum = hc_join<L>(sum, [](float x, float y) { return x + y; });
+  if (a.softmax) {
+    // a NaN or an infinity is the row's first winner
+    const float first = __shfl(p[0], lane - sub, HC_WAVE);
+    if (!(first < __builtin_inff())) all = sum = __builtin_nanf("");
+  }
+  const float of = a.normalize ? sum : a.softmax ? all : 1.f;
   if (!live) return;
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    if (j >= a.k || j % L != sub) continue;
-    a.expert[r * a.k + j] = won[j];
-    a.weight[r * a.k + j] = won[j] < 0 || of == 0.f ? 0.f : a.scale * (s[j] / of);
-    if (a.picked != nullptr) a.picked[r * a.k + j] = p[j];
+  for (int u = 0; u < OWN; ++u) {
+    const int j = u * L + sub;
+    if (j >= a.k) continue;
+    a.expert[r * a.k + j] = won[u];
+    a.weight[r * a.k + j] = won[u] < 0 || of == 0.f ? 0.f : a.scale * (s[u] / of);
+    if (a.picked != nullptr) a.picked[r * a.k + j] = p[u];
   }
 }
 
@@ -479,31 +529,38 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
   float *own = s_row + threadIdx.x * V, *row = own - lane * V;
 #pragma unroll
   for (int i = 0; i < V; ++i) own[i] = 0.f;
-  float t = 0.f, sum = 0.f;
-  for (int j = lane; j < a.k; j += L) {
-    if (a.expert[at + j] < 0) continue;
-    t += a.weight[at + j] * a.g[at + j];
+  // a choice's share of t and of S; what it brings
+  const auto first = [&](int64_t e, float w, float d, float p, float &t, float &sum) {
+    if (e < 0) return;
+    t += w * d;
+    if (by_logit) sum += rs_sigma(p);
+  };
+  const auto bring = [&](int64_t e, float w, float d, float p, float t, float sum) {
+    if (e < 0 || e >= a.E) return;
+    d *= a.scale;
     if (by_logit) {
-      const float p = a.picked[at + j], e = expf(-fabsf(p));
-      sum += (p < 0.f ? e : 1.f) / (1.f + e);
-    }
-  }
-  t = hc_join<L>(t, plus);
-  sum = hc_join<L>(sum, plus);
-  rt_in_order();
-  for (int j = lane; j < a.k; j += L) {
-    const int64_t e = a.expert[at + j];
-    if (e < 0 || e >= a.E) continue;
-    const float d = a.scale * a.g[at + j];
-    float out;
-    if (by_logit) {
-      const float x = expf(-fabsf(a.picked[at + j])), slope = x / ((1.f + x) * (1.f + x));
-      out = !a.normalize ? d * slope : sum == 0.f ? 0.f : (d - t) / sum * slope;
+      const float x = expf(-fabsf(p)), slope = x / ((1.f + x) * (1.f + x));
+      row[e] = !a.normalize ? d * slope : sum == 0.f ? 0.f : (d - t) / sum * slope;
     } else {
-      out = a.normalize ? a.weight[at + j] / a.scale * (d - t) : d;
+      row[e] = a.normalize ? w / a.scale * (d - t) : d;
     }
-    row[e] = out;
+  };
+  // (the first L choices stay in registers)
+  int64_t e = -1;
+  float w = 0.f, d = 0.f, p = 0.f, t = 0.f, sum = 0.f;
+  if (lane < a.k) {
+    e = a.expert[at + lane], w = a.weight[at + lane], d = a.g[at + lane];
+    if (by_logit) p = a.picked[at + lane];
   }
+  first(e, w, d, p, t, sum);
+  for (int j = lane + L; j < a.k; j += L)
+    first(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, t, sum);
+  t = hc_join<L>(t, plus);
+  if (by_logit) sum = hc_join<L>(sum, plus);
+  rt_in_order();
+  bring(e, w, d, p, t, sum);
+  for (int j = lane + L; j < a.k; j += L)
+    bring(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, t, sum);
   rt_in_order();
   float out[V];
 #pragma unroll
@@ -549,8 +606,11 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
   if (dtype < HC_F32 || dtype > HC_BF16) return HC_EDTYPE;
   RsArgs a{logits, bias, expert, weight, picked, n, scale, dtype, (int)E, (int)top_k,
            // (all groups open: as if there were one)
-           top_group == num_group ? 1 : (int)num_group, (int)(E / num_group), (int)top_group, 0, 0, 0, score != RS_SIGMOID,
+           top_group == num_group ? 1 : (int)num_group, (int)(E / num_group), (int)top_group, 0, 0, 0, 0, 0.f, score != RS_SIGMOID,
            normalize != 0, false};
+  a.low = 15;
+  while (a.low + 1 < (uint32_t)(E + 3) / 4 * 4) a.low = 2 * a.low + 1;
+  a.lost = (float)(a.low + 1) * 0x1p-22f;
   a.whole = dtype == HC_F32 ? rt_row<float, 4>::whole(logits, E) : rt_row<__half, 8>::whole(logits, E);
   a.quads = (int)((E + 3) / 4);
   const auto launch = [&](auto places, auto lanes) {
@@ -571,12 +631,15 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
   };
   const auto with_lanes = [&](auto places) {
     // as few lanes a row as keep its wave's rows under 18 KB of LDS (nine waves a compute unit), more where rows are few
-    const int least = E <= 64 ? 1 : E <= 256 ? 4 : 16;
+    const int least = E <= 64 ? 2 : E <= 256 ? 8 : 32;
     int lanes = least;
-    while (lanes < 64 && lanes < a.quads && n * lanes < 64 * 2048) lanes *= 4;
+    while (lanes < 64 && lanes < a.quads && n * lanes < 64 * 2048) lanes *= 2;
     if (lanes == 1) return launch(places, std::integral_constant<int, 1>{});
+    if (lanes == 2) return launch(places, std::integral_constant<int, 2>{});
     if (lanes == 4) return launch(places, std::integral_constant<int, 4>{});
+    if (lanes == 8) return launch(places, std::integral_constant<int, 8>{});
     if (lanes == 16) return launch(places, std::integral_constant<int, 16>{});
+    if (lanes == 32) return launch(places, std::integral_constant<int, 32>{});
     return launch(places, std::integral_constant<int, 64>{});
   };
   if (top_k <= 2) return with_lanes(std::integral_constant<int, 2>{});
