@@ -381,25 +381,41 @@ __device__ __forceinline__ void copy_rows_fast(const float *__restrict__ emb, TT
 }
 
 // The same for a table in 8 bits (packed_rows.h): a lane takes eight adjacent columns of a row, L lanes share a group's scale, and
-// the block's lanes lie one after the other over the admitted rows' groups.  slot_of (held by lane j): the slot of rank j.
+// the block's lanes lie one after the other over the admitted rows' groups, GC_PACK_AT_ONCE times before the first of them is packed.
+// slot_of (held by lane j): the slot of rank j.
+constexpr int GC_PACK_AT_ONCE = 4;
 template <int L>
 __device__ __forceinline__ void copy_rows_packed(const float *__restrict__ emb, int8_t *__restrict__ codes,
                                                  float *__restrict__ scale, int64_t F, int src_lane, int64_t slot_of,
                                                  int64_t tile0, int first_rank, int n_adm, int wave, int lane) {
+  constexpr int U = GC_PACK_AT_ONCE;
   const uint32_t groups = (uint32_t)((F + L * PK_EACH - 1) / (L * PK_EACH)), lanes = groups * L;
-  const uint64_t items = (uint64_t)(uint32_t)(n_adm - first_rank) * lanes;
-  for (uint64_t t0 = (uint64_t)wave * HC_WAVE; t0 < items; t0 += HC_BLOCK) {
-    const uint64_t t = t0 + (uint64_t)lane;
-    const bool live = t < items;
-    const uint32_t k = live ? (uint32_t)(t / lanes) : 0, in = live ? (uint32_t)(t - (uint64_t)k * lanes) : 0;
-    const int q = first_rank + (int)k;
-    const int64_t row = tile0 + __shfl(src_lane, q, HC_WAVE), slot = __shfl(slot_of, q, HC_WAVE);
-    const int64_t col = (int64_t)in * PK_EACH;
-    const int valid = !live || col >= F ? 0 : F - col >= PK_EACH ? PK_EACH : (int)(F - col);
-    float v[PK_EACH];
-    pk_row<float>::load(emb + row * F + col, valid, v);
-    const float s = pk_encode<L>(v, codes + slot * F + col, valid);
-    if (live && in % L == 0) scale[slot * groups + in / L] = s;
+  // one lane after the other: rank and place in the row, and how far on HC_BLOCK lanes are
+  const uint32_t down = HC_BLOCK / lanes, across = HC_BLOCK % lanes, start = (uint32_t)(wave * HC_WAVE + lane);
+  uint32_t q = (uint32_t)first_rank + start / lanes, in = start % lanes;
+  while (__any(q < (uint32_t)n_adm)) {
+    float v[U][PK_EACH];
+    int64_t to[U], of_scale[U];
+    int valid[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool live = q < (uint32_t)n_adm;
+      const int from = (int)(live ? q : 0u);
+      const int64_t row = tile0 + __shfl(src_lane, from, HC_WAVE), slot = __shfl(slot_of, from, HC_WAVE);
+      const int64_t col = (int64_t)in * PK_EACH;
+      valid[u] = !live || col >= F ? 0 : F - col >= PK_EACH ? PK_EACH : (int)(F - col);
+      pk_row<float>::load(emb + row * F + col, valid[u], v[u]);
+      to[u] = slot * F + col;
+      of_scale[u] = live && in % L == 0 ? slot * groups + in / L : -1;
+      q += down;
+      in += across;
+      if (in >= lanes) in -= lanes, ++q;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float s = pk_encode<L>(v[u], codes + to[u], valid[u]);
+      if (of_scale[u] >= 0) scale[of_scale[u]] = s;
+    }
   }
 }
 

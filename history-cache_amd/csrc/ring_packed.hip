@@ -7,6 +7,8 @@
 namespace {
 
 constexpr int RP_MOST_ROWS = 64;       // rows a block
+constexpr int RP_AT_ONCE = 4;          // pieces that a lane reads before it writes the first
+constexpr int64_t RP_CACHE = 256 << 20;          // bytes of the last-level cache
 
 struct RpArgs {
   const int64_t *full2slot, *ids, *checkin, *now_dev, *n_valid_dev;
@@ -29,8 +31,8 @@ __device__ __forceinline__ int64_t rp_find(const RpArgs &a, int64_t i) {
 }
 
 // V: adjacent columns a lane: 4 where rows are whole multiples of four columns and lie at multiples of 16 bytes, otherwise 8 at
-// any alignment.
-template <int V>
+// any alignment.  NT: for rows that the last-level cache cannot hold until they are read.
+template <int V, bool NT>
 __global__ __launch_bounds__(HC_BLOCK) void rp_lookup(RpArgs a) {
   __shared__ int64_t s_slot[RP_MOST_ROWS];
   const int64_t row0 = (int64_t)blockIdx.x * a.rows;
@@ -45,35 +47,50 @@ __global__ __launch_bounds__(HC_BLOCK) void rp_lookup(RpArgs a) {
   const uint32_t pieces = (a.F + V - 1) / V, down = HC_BLOCK / pieces, across = HC_BLOCK % pieces;
   uint32_t r = threadIdx.x / pieces, c = threadIdx.x % pieces;
   while (r < rows) {
-    const int64_t slot = s_slot[r];
-    const uint32_t col = c * V;
-    float *out = a.rows_out + (row0 + r) * a.F + col;
-    if constexpr (V == 4) {
-      uint32_t w = 0;
-      float s = 0.f;
+    uint32_t w[RP_AT_ONCE][2], row_of[RP_AT_ONCE], col_of[RP_AT_ONCE];
+    float s[RP_AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < RP_AT_ONCE; ++u) {
+      row_of[u] = r;
+      col_of[u] = c * V;
+      w[u][0] = w[u][1] = 0;
+      s[u] = 0.f;
+      const int64_t slot = r < rows ? s_slot[r] : -1;
       if (slot >= 0) {
-        w = *reinterpret_cast<const uint32_t *>(a.codes + slot * a.F + col);
-        s = a.scale[slot * a.groups + col / a.group];
+        const int8_t *from = a.codes + slot * a.F + col_of[u];
+        s[u] = a.scale[slot * a.groups + col_of[u] / a.group];
+        if constexpr (V == 4) {
+          w[u][0] = *reinterpret_cast<const uint32_t *>(from);
+        } else {
+          const int valid = a.F - col_of[u] >= (uint32_t)PK_EACH ? PK_EACH : (int)(a.F - col_of[u]);
+          if (valid >= PK_EACH) {
+            const pk_codes q = *reinterpret_cast<const pk_codes *>(from);
+            w[u][0] = q.w[0];
+            w[u][1] = q.w[1];
+          } else {
+            pk_load_tail<1>(reinterpret_cast<const char *>(from), valid, w[u]);
+          }
+        }
       }
+      r += down;
+      c += across;
+      if (c >= pieces) c -= pieces, ++r;
+    }
+#pragma unroll
+    for (int u = 0; u < RP_AT_ONCE; ++u) {
+      if (row_of[u] >= rows) break;
+      float *out = a.rows_out + (row0 + row_of[u]) * a.F + col_of[u];
       float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (float)(int8_t)(w >> (8 * i)) * s;
-      if (slot < 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = 0.f;
+      for (int i = 0; i < V; ++i) v[i] = (float)(int8_t)(w[u][i / 4] >> (8 * (i % 4))) * s[u];
+      if constexpr (V == 4) {
+        if constexpr (NT) hc_vec<float, 4>::store_nt(out, v);
+        else hc_vec<float, 4>::store(out, v);
+      } else {
+        const int valid = a.F - col_of[u] >= (uint32_t)PK_EACH ? PK_EACH : (int)(a.F - col_of[u]);
+        pk_row<float>::template store<NT>(out, valid, v);
       }
-      hc_vec<float, V>::store(out, v);
-    } else {
-      const int valid = a.F - col >= (uint32_t)PK_EACH ? PK_EACH : (int)(a.F - col);
-      float v[PK_EACH];
-#pragma unroll
-      for (int i = 0; i < PK_EACH; ++i) v[i] = 0.f;
-      if (slot >= 0) pk_load_codes(a.codes + slot * a.F + col, valid, a.scale[slot * a.groups + col / a.group], v);
-      pk_row<float>::store(out, valid, v);
     }
-    r += down;
-    c += across;
-    if (c >= pieces) c -= pieces, ++r;
   }
 }
 
@@ -90,10 +107,12 @@ extern "C" int hc_ring_lookup_packed(const int64_t *full2slot, int64_t n_full, c
   HC_REQUIRE(rows_out == nullptr || (codes && scale));
   RpArgs a{full2slot, ids, checkin, now_dev, n_valid_dev, n_full, now, age_limit, capacity, n, codes, scale, slot_out, rows_out,
            (uint32_t)F, (uint32_t)((F + group - 1) / group), (uint32_t)group, 16};
+  a.rows = n >= 2048 * RP_MOST_ROWS ? RP_MOST_ROWS : 16;
   const int64_t blocks = (n + a.rows - 1) / a.rows;
   if (!hc_grid_ok(blocks)) return HC_EUNSUPPORTED;
   const bool whole = F % 4 == 0 && reinterpret_cast<uintptr_t>(codes) % 4 == 0 && reinterpret_cast<uintptr_t>(rows_out) % 16 == 0;
-  const auto kernel = whole ? rp_lookup<4> : rp_lookup<8>;
+  const bool large = n * F * (int64_t)sizeof(float) > RP_CACHE;
+  const auto kernel = whole ? (large ? rp_lookup<4, true> : rp_lookup<4, false>) : large ? rp_lookup<8, true> : rp_lookup<8, false>;
   kernel<<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(a);
   return hc_launch_status();
 }

@@ -35,7 +35,8 @@ struct RsArgs {
   int quads, stride, rank_stride;      // in LDS: pieces of four a row, floats from one row to the next, and from one row's ranks
   uint32_t low;            // the bits that an index takes, and what they leave of a number's differences
   float lost;
-  bool softmax, normalize, whole;
+  int piece;               // logits that are read at once
+  bool softmax, normalize;
 };
 
 __device__ __forceinline__ int64_t rs_bits(double v) { return __builtin_bit_cast(int64_t, v); }
@@ -197,7 +198,19 @@ struct rs_list {
   }
 };
 
-// 1 / (1 + exp(-l)) by the instructions, within 2^-22.
+// The larger two of the pairs that L lanes have.
+template <int L, int D = 1>
+__device__ __forceinline__ void rs_join_two(float &first, float &second) {
+  if constexpr (D < L) {
+    const float f = hc_other<D>(first), s = hc_other<D>(second);
+    second = __builtin_amdgcn_fmed3f(first, f, fmaxf(second, s));
+    first = fmaxf(first, f);
+    rs_join_two<L, 2 * D>(first, second);
+  }
+}
+
+// exp(x) by the instruction, x <= 0: off by 2^-23 and |x| 2^-23 of itself.  1 / (1 + exp(-l)) by the instructions, within 2^-22.
+__device__ __forceinline__ float rs_near_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 __device__ __forceinline__ float rs_near_sigma(float l) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l * -1.44269504f));
 }
@@ -216,13 +229,13 @@ __device__ __forceinline__ float rs_choice(float l, float bias) {
 }
 
 // Rows r0 .. r0 + rows into LDS: c where the score is a logit's own and there is a bias, l otherwise.
-template <typename T>
+template <typename T, int PIECE>
 __device__ __forceinline__ void rs_stage(const RsArgs &a, int64_t r0, int rows, float *s, const float *bias) {
-  constexpr int PIECE = 16 / (int)sizeof(T), AT_ONCE = 4;
+  constexpr int AT_ONCE = 4;
   const int lane = hc_lane();
   const T *from = static_cast<const T *>(a.logits) + r0 * a.E;
   const bool make = a.bias != nullptr && !a.softmax;
-  if (a.whole) {
+  if constexpr (PIECE > 1) {
     const int pieces = rows * (a.E / PIECE), each = a.E / PIECE, down = HC_WAVE / each, across = HC_WAVE % each;
     int row = lane / each, col = lane % each;
     for (int q0 = lane; q0 < pieces; q0 += AT_ONCE * HC_WAVE) {
@@ -302,9 +315,15 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     for (int e = lane; e < a.E; e += HC_WAVE) bias[e] = rs_plain(a.bias[e]);
     rt_in_order();
   }
-  if (a.dtype == HC_F32) rs_stage<float>(a, r0, rows, s_all, bias);
-  else if (a.dtype == HC_F16) rs_stage<__half>(a, r0, rows, s_all, bias);
-  else rs_stage<__hip_bfloat16>(a, r0, rows, s_all, bias);
+  const auto stage = [&](auto type) {
+    typedef decltype(type) T;
+    if (a.piece == 8) rs_stage<T, sizeof(T) == 2 ? 8 : 4>(a, r0, rows, s_all, bias);
+    else if (a.piece >= 4) rs_stage<T, 4>(a, r0, rows, s_all, bias);
+    else rs_stage<T, 1>(a, r0, rows, s_all, bias);
+  };
+  if (a.dtype == HC_F32) stage(float{});
+  else if (a.dtype == HC_F16) stage(__half{});
+  else stage(__hip_bfloat16{});
   rt_in_order();
   float *row = s_all + (live ? mine : 0) * a.stride;
   float top = RS_SHUT, all = 0.f;
@@ -314,7 +333,8 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     // (a closed expert lies so far below every other that its exponential is 0)
     double sum = 0.0;
     rs_each<L>(row, 0, 4 * a.quads, sub, true, [&](float4 l, int) {
-      sum += ((double)expf(l.x - top) + (double)expf(l.y - top)) + ((double)expf(l.z - top) + (double)expf(l.w - top));
+      sum += ((double)rs_near_exp(l.x - top) + (double)rs_near_exp(l.y - top)) +
+             ((double)rs_near_exp(l.z - top) + (double)rs_near_exp(l.w - top));
     });
     sum = rs_double(hc_join<L>(rs_bits(sum), [](int64_t x, int64_t y) { return rs_bits(rs_double(x) + rs_double(y)); }));
     all = (float)sum;
@@ -345,16 +365,11 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
         more(c.z);
         more(c.w);
       });
-#pragma unroll
-      for (int d = 1; d < L; d *= 2) {
-        const float f = __shfl_xor(first, d, HC_WAVE), s = __shfl_xor(second, d, HC_WAVE);
-        second = fmaxf(second, s);
-        more(f);
-      }
+      rs_join_two<L>(first, second);
       near = near || first >= RS_MOST;               // (infinite, or no number)
       if (exact && !rs_shut(first)) {
-        first = a.softmax ? expf(first - top) : rs_sigma(first);
-        second = rs_shut(second) ? second : a.softmax ? expf(second - top) : rs_sigma(second);
+        first = a.softmax ? rs_near_exp(first - top) : rs_near_sigma(first);
+        second = rs_shut(second) ? second : a.softmax ? rs_near_exp(second - top) : rs_near_sigma(second);
       }
       if (sub == 0) rank[g] = rs_shut(second) ? first : first + second;
     }
@@ -375,7 +390,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     open = (uint64_t)hc_join<L>((int64_t)open, [](int64_t x, int64_t y) { return x | y; });
     least = hc_join<L>(least, [](float x, float y) { return fminf(x, y); });
     most = hc_join<L>(most, [](float x, float y) { return fmaxf(x, y); });
-    const float off = exact ? 0x1p-16f * fabsf(least) : 0x1p-19f * (1.f + fabsf(least));
+    const float off = exact ? 0x1p-15f * fabsf(least) : 0x1p-19f * (1.f + fabsf(least));
     near = near || (!rs_shut(most) && !(least - most > off));
   }
   // f for the row's open elements that this lane takes
@@ -529,21 +544,20 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
   float *own = s_row + threadIdx.x * V, *row = own - lane * V;
 #pragma unroll
   for (int i = 0; i < V; ++i) own[i] = 0.f;
-  // a choice's share of t and of S; what it brings
+  // a choice's share of t and of S, and ds / dl; what it brings
   const auto first = [&](int64_t e, float w, float d, float p, float &t, float &sum) {
-    if (e < 0) return;
+    if (e < 0) return 0.f;
     t += w * d;
-    if (by_logit) sum += rs_sigma(p);
+    if (!by_logit) return 0.f;
+    const float x = expf(-fabsf(p)), q = 1.f / (1.f + x);
+    sum += p < 0.f ? x * q : q;
+    return x * q * q;
   };
-  const auto bring = [&](int64_t e, float w, float d, float p, float t, float sum) {
+  const auto bring = [&](int64_t e, float w, float d, float slope, float t, float sum) {
     if (e < 0 || e >= a.E) return;
     d *= a.scale;
-    if (by_logit) {
-      const float x = expf(-fabsf(p)), slope = x / ((1.f + x) * (1.f + x));
-      row[e] = !a.normalize ? d * slope : sum == 0.f ? 0.f : (d - t) / sum * slope;
-    } else {
-      row[e] = a.normalize ? w / a.scale * (d - t) : d;
-    }
+    if (by_logit) row[e] = !a.normalize ? d * slope : sum == 0.f ? 0.f : (d - t) / sum * slope;
+    else row[e] = a.normalize ? w / a.scale * (d - t) : d;
   };
   // (the first L choices stay in registers)
   int64_t e = -1;
@@ -552,15 +566,18 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
     e = a.expert[at + lane], w = a.weight[at + lane], d = a.g[at + lane];
     if (by_logit) p = a.picked[at + lane];
   }
-  first(e, w, d, p, t, sum);
+  const float slope = first(e, w, d, p, t, sum);
   for (int j = lane + L; j < a.k; j += L)
     first(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, t, sum);
   t = hc_join<L>(t, plus);
   if (by_logit) sum = hc_join<L>(sum, plus);
   rt_in_order();
-  bring(e, w, d, p, t, sum);
-  for (int j = lane + L; j < a.k; j += L)
-    bring(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, t, sum);
+  bring(e, w, d, slope, t, sum);
+  for (int j = lane + L; j < a.k; j += L) {
+    float none = 0.f;
+    const float other = first(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, none, none);
+    bring(a.expert[at + j], a.weight[at + j], a.g[at + j], other, t, sum);
+  }
   rt_in_order();
   float out[V];
 #pragma unroll
@@ -606,12 +623,13 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
   if (dtype < HC_F32 || dtype > HC_BF16) return HC_EDTYPE;
   RsArgs a{logits, bias, expert, weight, picked, n, scale, dtype, (int)E, (int)top_k,
            // (all groups open: as if there were one)
-           top_group == num_group ? 1 : (int)num_group, (int)(E / num_group), (int)top_group, 0, 0, 0, 0, 0.f, score != RS_SIGMOID,
-           normalize != 0, false};
+           top_group == num_group ? 1 : (int)num_group, (int)(E / num_group), (int)top_group, 0, 0, 0, 0, 0.f, 1, score != RS_SIGMOID,
+           normalize != 0};
   a.low = 15;
   while (a.low + 1 < (uint32_t)(E + 3) / 4 * 4) a.low = 2 * a.low + 1;
   a.lost = (float)(a.low + 1) * 0x1p-22f;
-  a.whole = dtype == HC_F32 ? rt_row<float, 4>::whole(logits, E) : rt_row<__half, 8>::whole(logits, E);
+  if (dtype == HC_F32) a.piece = rt_row<float, 4>::whole(logits, E) ? 4 : 1;
+  else a.piece = rt_row<__half, 8>::whole(logits, E) ? 8 : rt_row<__half, 4>::whole(logits, E) ? 4 : 1;
   a.quads = (int)((E + 3) / 4);
   const auto launch = [&](auto places, auto lanes) {
     constexpr int L = decltype(lanes)::value;
