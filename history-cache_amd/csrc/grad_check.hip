@@ -382,39 +382,52 @@ __device__ __forceinline__ void copy_rows_fast(const float *__restrict__ emb, TT
 
 // The same for a table in 8 bits (packed_rows.h): a lane takes eight adjacent columns of a row, L lanes share a group's scale, and
 // the block's lanes lie one after the other over the admitted rows' groups, GC_PACK_AT_ONCE times before the first of them is packed.
-// slot_of (held by lane j): the slot of rank j.
+// A tile has one block and most batches few tiles, so that what a wave has to do one after the other is what bounds them: addresses go
+// by 32-bit steps from the tile's and the ring's own, and rows of whole groups (WHOLE) without a look at their ends.
+// slot0: the slot of rank 0, below capacity.
 constexpr int GC_PACK_AT_ONCE = 4;
-template <int L>
+template <int L, bool WHOLE>
 __device__ __forceinline__ void copy_rows_packed(const float *__restrict__ emb, int8_t *__restrict__ codes,
-                                                 float *__restrict__ scale, int64_t F, int src_lane, int64_t slot_of,
-                                                 int64_t tile0, int first_rank, int n_adm, int wave, int lane) {
+                                                 float *__restrict__ scale, uint32_t F, int src_lane, int64_t slot0,
+                                                 int64_t capacity, int first_rank, int n_adm, int wave, int lane) {
   constexpr int U = GC_PACK_AT_ONCE;
-  const uint32_t groups = (uint32_t)((F + L * PK_EACH - 1) / (L * PK_EACH)), lanes = groups * L;
+  const uint32_t groups = (F + L * PK_EACH - 1) / (L * PK_EACH), lanes = groups * L;
   // one lane after the other: rank and place in the row, and how far on HC_BLOCK lanes are
   const uint32_t down = HC_BLOCK / lanes, across = HC_BLOCK % lanes, start = (uint32_t)(wave * HC_WAVE + lane);
   uint32_t q = (uint32_t)first_rank + start / lanes, in = start % lanes;
+  // (ranks that go round the ring's end; a ring of fewer slots than a tile has rows may be gone round more than once)
+  const int64_t room = capacity - slot0;
   while (__any(q < (uint32_t)n_adm)) {
     float v[U][PK_EACH];
-    int64_t to[U], of_scale[U];
+    uint64_t to[U], of_scale[U];
     int valid[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool live = q < (uint32_t)n_adm;
-      const int from = (int)(live ? q : 0u);
-      const int64_t row = tile0 + __shfl(src_lane, from, HC_WAVE), slot = __shfl(slot_of, from, HC_WAVE);
-      const int64_t col = (int64_t)in * PK_EACH;
-      valid[u] = !live || col >= F ? 0 : F - col >= PK_EACH ? PK_EACH : (int)(F - col);
-      pk_row<float>::load(emb + row * F + col, valid[u], v[u]);
+      const uint32_t from = (uint32_t)__shfl(src_lane, (int)(live ? q : 0u), HC_WAVE), col = in * PK_EACH;
+      valid[u] = !live || (!WHOLE && col >= F) ? 0 : WHOLE || F - col >= PK_EACH ? PK_EACH : (int)(F - col);
+      if constexpr (WHOLE) {
+        const float *p = emb + ((uint64_t)from * F + col);
+        float x[4], y[4];
+        hc_vec<float, 4>::load_nt(p, x);
+        hc_vec<float, 4>::load_nt(p + 4, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] = x[i], v[u][4 + i] = y[i];
+      } else {
+        pk_row<float>::load(emb + ((uint64_t)from * F + col), valid[u], v[u]);
+      }
+      uint64_t slot = (uint64_t)slot0 + q;
+      if ((int64_t)q >= room) slot = capacity >= GC_TILE ? slot - (uint64_t)capacity : slot % (uint64_t)capacity;
       to[u] = slot * F + col;
-      of_scale[u] = live && in % L == 0 ? slot * groups + in / L : -1;
+      of_scale[u] = slot * groups + in / L;
       q += down;
       in += across;
       if (in >= lanes) in -= lanes, ++q;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float s = pk_encode<L>(v[u], codes + to[u], valid[u]);
-      if (of_scale[u] >= 0) scale[of_scale[u]] = s;
+      const float s = pk_encode<L, true>(v[u], codes + to[u], valid[u]);
+      if (valid[u] > 0 && lane % L == 0) __builtin_nontemporal_store(s, scale + of_scale[u]);
     }
   }
 }
@@ -527,8 +540,13 @@ __global__ __launch_bounds__(HC_BLOCK) void gc_pass3_ring(
   const int target = m ? rank : n_adm + (lane - rank);
   const int src_lane = __builtin_amdgcn_ds_permute(target << 2, lane);
   if constexpr (PACKED != 0) {
-    copy_rows_packed<PACKED>(emb, static_cast<int8_t *>(table), scale, F, src_lane, (slot0 + lane) % capacity, tile0, first_rank,
-                             n_adm, wave, lane);
+    const bool whole = F % (PACKED * PK_EACH) == 0 && reinterpret_cast<uintptr_t>(emb) % 16 == 0;
+    const auto copy = [&](auto whole_) {
+      copy_rows_packed<PACKED, decltype(whole_)::value>(emb + tile0 * F, static_cast<int8_t *>(table), scale, (uint32_t)F, src_lane,
+                                                        slot0 % capacity, capacity, first_rank, n_adm, wave, lane);
+    };
+    if (whole) copy(std::true_type{});
+    else copy(std::false_type{});
     return;
   }
   const bool fast = (F % 256 == 0) && (F / 256 <= 4) && (reinterpret_cast<uintptr_t>(emb) % 16 == 0) &&

@@ -143,7 +143,7 @@ __device__ __forceinline__ void pk_load_codes(const int8_t *__restrict__ p, int 
 
 // The scale of the group that L lanes hold, and this lane's codes.  The largest magnitude is found on the bits, where a NaN
 // is above infinity and infinity above every number.
-template <int L>
+template <int L, bool NT = false>
 __device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__restrict__ p, int valid) {
   uint32_t m = 0;
 #pragma unroll
@@ -155,12 +155,22 @@ __device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__
   const float most = __uint_as_float(m);
   const bool zero = most < PK_SMALLEST, bad = m >= 0x7f800000u;
   const float inverse = zero || bad ? 0.f : 1.0f / most * 127.0f;
-  uint32_t w[2] = {};
+  // 1.5 2^23 more has the rounded number in its lowest byte
+  uint32_t w[2], c[PK_EACH];
 #pragma unroll
-  for (int i = 0; i < PK_EACH; ++i) w[i / 4] |= ((uint32_t)(int)rintf(v[i] * inverse) & 0xffu) << (8 * (i % 4));
+  for (int i = 0; i < PK_EACH; ++i) c[i] = __float_as_uint(v[i] * inverse + 0x1.8p23f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u), 0x05040100u);
   if (bad) w[0] = w[1] = 0;
   if (valid >= PK_EACH) {
-    *reinterpret_cast<pk_codes *>(p) = pk_codes{{w[0], w[1]}};
+    if constexpr (NT) {
+      typedef uint32_t two __attribute__((ext_vector_type(2), aligned(1)));
+      __builtin_nontemporal_store(two{w[0], w[1]}, reinterpret_cast<two *>(p));
+    } else {
+      *reinterpret_cast<pk_codes *>(p) = pk_codes{{w[0], w[1]}};
+    }
   } else if (valid > 0) {
     pk_store_tail<1>(reinterpret_cast<char *>(p), valid, w);
   }
