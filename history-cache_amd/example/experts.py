@@ -7,6 +7,7 @@ width is kept in 8 bits.
 
     python experts.py                               # 20 000 nodes, 60 steps
     python experts.py --nodes 200000 --experts 16 --dtype bf16 --full-width
+    python experts.py --score sigmoid --balance 0.01 --state-bits 8    # evenly loaded experts, the optimizer's moments in 8 bits
 """
 import argparse
 import contextlib
@@ -26,12 +27,12 @@ TYPES = 3
 
 
 class Net(torch.nn.Module):
-    def __init__(self, features, hidden, classes, experts, top_k, dtype):
+    def __init__(self, features, hidden, classes, experts, top_k, dtype, score="softmax", balance=False):
         super().__init__()
         self.by_type = torch.nn.Parameter(torch.randn(TYPES, hidden, features) / features ** 0.5)
         self.conv = hiscache.MySageConvHistory(hidden, hidden, need_grad=False)
         self.norm = torch.nn.LayerNorm(hidden)
-        self.experts = hiscache.ExpertMLP(hidden, 2 * hidden, experts, top_k, dtype=dtype)
+        self.experts = hiscache.ExpertMLP(hidden, 2 * hidden, experts, top_k, dtype=dtype, score=score, balance=balance)
         self.out = torch.nn.Linear(hidden, classes)
         self.dtype = dtype
 
@@ -62,8 +63,12 @@ def run(args, say=print):
     device, dtype = "cuda:0", {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}[args.dtype]
     torch.manual_seed(args.seed)
     x, types, ptr, idx, y = make_data(args.nodes, args.features, args.classes, args.seed, device)
-    net = Net(args.features, args.hidden, args.classes, args.experts, args.top_k, dtype).to(device).train()
-    opt = torch.optim.Adam(net.parameters(), lr=args.lr)
+    net = Net(args.features, args.hidden, args.classes, args.experts, args.top_k, dtype, args.score,
+              args.balance > 0).to(device).train()
+    if args.state_bits:
+        opt = hiscache.AdamW(net.parameters(), lr=args.lr, weight_decay=0.0, state_bits=args.state_bits)
+    else:
+        opt = torch.optim.Adam(net.parameters(), lr=args.lr)
     context = contextlib.nullcontext if args.full_width else hiscache.packed_activations
     losses = []
     for step in range(args.steps):
@@ -73,6 +78,8 @@ def run(args, say=print):
         opt.zero_grad()
         loss.backward()
         opt.step()
+        if args.balance > 0:
+            net.experts.balance_step(args.balance)
         losses.append(loss.detach())
         if step % 10 == 0 or step == args.steps - 1:
             say(f"step {step:4d}  loss {float(loss.detach()):.4f}  kept for backward {kept / 2 ** 20:.0f} MiB")
@@ -86,6 +93,9 @@ def parse(argv=None):
         p.add_argument("--" + name, type=int, default=value)
     p.add_argument("--lr", type=float, default=3e-3)
     p.add_argument("--dtype", choices=("fp32", "fp16", "bf16"), default="fp32", help="type of the experts' rows and matrices")
+    p.add_argument("--score", choices=("softmax", "sigmoid"), default="softmax", help="the router's scores")
+    p.add_argument("--balance", type=float, default=0.0, help="step of the bias that loads the experts evenly (0: none)")
+    p.add_argument("--state-bits", type=int, choices=(0, 8, 32), default=0, help="hiscache.AdamW's moments (0: torch's Adam)")
     p.add_argument("--full-width", action="store_true", help="keep activations at full width")
     return p.parse_args(argv)
 

@@ -14,6 +14,7 @@ import os
 import sys
 
 import numpy as np
+import torch
 import yaml
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
@@ -52,7 +53,16 @@ def trainer_options(config):
     """The ``trainer`` group as ``HistoryTrainer`` arguments."""
     t = config.get("trainer") or {}
     mb = float(t.get("cache_megabytes", 0) or 0)
-    return dict(recorded=bool(t.get("recorded", False)), read_ahead=bool(t.get("read_ahead", False)),
+    ring = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16, "int8": torch.int8}
+    dtype = str(t.get("ring_dtype", "fp16") or "fp16")
+    if dtype not in ring:
+        raise ValueError(f"trainer.ring_dtype must be one of {sorted(ring)}, got {dtype}")
+    more = {}                                   # (what is not asked for is the trainer's to choose)
+    if dtype != "fp16":
+        more["ring_dtype"] = ring[dtype]
+    if t.get("state_bits"):
+        more["state_bits"] = int(t["state_bits"])
+    return dict(more, recorded=bool(t.get("recorded", False)), read_ahead=bool(t.get("read_ahead", False)),
                 features_in_device_memory=bool(t.get("features_in_device_memory", False)),
                 hot_rows=int(t.get("hot_rows", 0) or 0), ring_rows=int(t.get("ring_rows", 0) or 0),
                 cache_bytes=int(mb * 2 ** 20) if mb > 0 else None, seed=int(t.get("seed", 0) or 0))

@@ -16,14 +16,28 @@ class ExpertMLP(torch.nn.Module):
     """``sum_j weight[i, j] * expert[i, j](x[i])`` with ``expert_e(x) = (silu(x A_e) * (x B_e)) C_e``.
 
     channels: width of the rows in and out; hidden: width inside an expert; num_expert: E; top_k: experts a row;
-    normalize: a row's weights add up to one.  In training [x A | x B] is kept in 8 bits, a scale for every ``group`` columns."""
+    normalize: a row's weights add up to one.  In training [x A | x B] is kept in 8 bits, a scale for every ``group`` columns.
 
-    def __init__(self, channels, hidden, num_expert, top_k=2, normalize=True, group=64, device=None, dtype=None):
+    score, num_group, top_group, scale: the router's (``hiscache_backend.route_rows``).  ``balance``: experts are chosen by score + bias,
+    where ``balance_bias`` (a buffer, zeros at first, fp32 whatever the module is cast to) rises for experts that had too few rows
+    and falls for those that had too many by every :meth:`balance_step`, as it were a loss on their load that does not
+    disturb the gradients."""
+
+    def __init__(self, channels, hidden, num_expert, top_k=2, normalize=True, group=64, device=None, dtype=None, score="softmax",
+                 num_group=1, top_group=1, scale=1.0, balance=False):
         super().__init__()
         if not 1 <= top_k <= num_expert:
             raise ValueError(f"top_k must be between 1 and the {num_expert} experts, got {top_k}")
+        if score not in ("softmax", "sigmoid") or not scale > 0:
+            raise ValueError(f"score must be softmax or sigmoid and scale positive, got {score!r}, {scale}")
+        if not 1 <= top_group <= num_group or num_expert % num_group or top_k > num_expert // num_group * top_group:
+            raise ValueError(f"{num_group} groups must divide the {num_expert} experts, and {top_group} of them hold {top_k} experts")
         self.channels, self.hidden, self.num_expert = channels, hidden, num_expert
         self.top_k, self.normalize, self.group = top_k, normalize, group
+        self.score, self.num_group, self.top_group, self.scale = score, num_group, top_group, scale
+        bias = torch.zeros(num_expert, device=device, dtype=torch.float32) if balance else None
+        self.register_buffer("balance_bias", bias)
+        self._offset = None                               # of the last training pass: the experts' loads
         # the router's logits are fp32 whatever the rows are, under autocast and in a module cast to half precision as well: near-ties
         # decide where a row goes
         self.router = torch.nn.Parameter(torch.empty(num_expert, channels, device=device, dtype=torch.float32))
@@ -36,6 +50,24 @@ class ExpertMLP(torch.nn.Module):
             for w, fan in ((self.router, self.channels), (self.w_in, self.channels), (self.w_out, self.hidden)):
                 w.uniform_(-1 / math.sqrt(fan), 1 / math.sqrt(fan))
 
+    def _apply(self, fn, recurse=True):
+        bias = self.balance_bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.balance_bias.dtype is not torch.float32:
+            # (a cast to half precision would lose steps of the bias)
+            self.balance_bias = bias.to(self.balance_bias.device)
+        return self
+
+    @torch.no_grad()
+    def balance_step(self, rate=1e-3):
+        """Moves the bias of every expert by ``rate`` towards an even load, by the rows that each had in the last training pass
+        of :meth:`forward` that asked the router; nothing happens before the first.  Once a step, after the backward pass."""
+        if self.balance_bias is None:
+            raise RuntimeError("this layer has no bias for balance: ExpertMLP(..., balance=True)")
+        if self._offset is not None:
+            load = (self._offset[1:] - self._offset[:-1]).float()
+            self.balance_bias.add_(torch.sign(load.mean() - load), alpha=rate)
+
     def route(self, x, allowed=None):
         """The router's choice for the rows of x: (expert int64 [n, top_k], weight fp32 [n, top_k]).  ``allowed`` (bool
         [n, E] or [E], optional): experts that a row may go to; a row that may go nowhere gets -1 and weight 0."""
@@ -46,7 +78,11 @@ class ExpertMLP(torch.nn.Module):
             logits = F.linear(x.float(), self.router.float())
         if allowed is not None:
             logits = logits.masked_fill(~allowed, -math.inf)
-        return hiscache_backend.route_rows(logits, self.top_k, normalize=self.normalize)
+        how = dict(normalize=self.normalize)
+        if self.score != "softmax" or self.num_group != 1 or self.scale != 1 or self.balance_bias is not None:
+            how.update(score=self.score, bias=self.balance_bias, num_group=self.num_group, top_group=self.top_group,
+                       scale=self.scale)
+        return hiscache_backend.route_rows(logits, self.top_k, **how)
 
     def forward(self, x, expert=None, weight=None, allowed=None):
         """x [n, channels] through its experts.  ``expert`` (int64 [n] or [n, k]) and ``weight`` (fp32, default ones) replace
@@ -55,15 +91,19 @@ class ExpertMLP(torch.nn.Module):
         be = hiscache_backend
         if (weight if expert is None else allowed) is not None:
             raise ValueError("weight goes with expert, allowed with the router's choice")
-        if expert is None:
+        routed = expert is None
+        if routed:
             expert, weight = self.route(x, allowed)
         order = be.expert_order(expert, self.num_expert)
+        if routed and self.balance_bias is not None and self.training:
+            self._offset = order.offset
         y = be.gated_experts(be.rows_to_experts(x, order), self.w_in, self.w_out, order.offset, self.group)
         return be.rows_from_experts(y, order, weight)
 
     def extra_repr(self):
         return (f"{self.channels}, hidden={self.hidden}, num_expert={self.num_expert}, top_k={self.top_k}, "
-                f"normalize={self.normalize}, group={self.group}")
+                f"normalize={self.normalize}, group={self.group}, score={self.score}, num_group={self.num_group}, "
+                f"top_group={self.top_group}, scale={self.scale}, balance={self.balance_bias is not None}")
 
 
 # Steps back through the history of a matrix that are looked at: a cast, a slice or a normalised weight is up to six from its

@@ -19,6 +19,7 @@ import torch
 from .dataset import ProcessedDataset
 from .history_cache import HistoryCache
 from .history_model import HistoryRGCN, get_model
+from .optimizer import AdamW
 from .recorded import RecordedIteration
 from .ring_cache import RingHistoryCache
 from .util import backward_on_this_thread, log
@@ -37,13 +38,13 @@ class HistoryTrainer:
 
     def __init__(self, config, dataset=None, fanout=None, batch_size=None, lr=None, num_epochs=None, eval_begin=None,
                  features_in_device_memory=False, hot_rows=0, cache_bytes=None, ring_rows=0, recorded=False,
-                 read_ahead=False, replay_slots=4, seed=0, model_factory=None):
+                 read_ahead=False, replay_slots=4, seed=0, model_factory=None, ring_dtype=torch.float16, state_bits=None):
         """``config``: the tree ``make_config`` builds (``dl.dataset.path`` names the dataset directory).  The
         loader's settings are arguments, with the configuration's own keys as defaults where it has them
         (``dl.sampler.train.batch_size`` / ``num_neighbors``, ``train.optimizer.lr``, ``train.train.num_epochs`` /
         ``eval_begin``).  ``cache_bytes``: size of the cache's buffer (default: what the configuration's
         ``history.limit`` and the free device memory give, as in the reference).  ``ring_rows`` > 0: the embeddings live in a
-        ``RingHistoryCache`` of that many fp16 rows instead (entries age out after ``history.staleness_thres``
+        ``RingHistoryCache`` of that many rows of ``ring_dtype`` (fp32, fp16, bf16, or int8: 8 bits with scales) instead (entries age out after ``history.staleness_thres``
         iterations; no feature cache inside it: use ``hot_rows``).  ``recorded``: train through
         ``RecordedIteration`` (batches of ``batch_size`` seeds; the last, shorter batch of an epoch takes the
         ordinary path).  ``read_ahead``: the feature rows of the next batch are read over the host link beside
@@ -51,7 +52,8 @@ class HistoryTrainer:
         own), for a matrix that is not wholly in device memory.  ``replay_slots``: the sampler's launches for a
         batch are recorded once per slot and replayed (see ``NeighborSampler``; the trainer never holds more than
         three batches, so four slots are safe; 0 switches it off).  ``model_factory(config, table)``: builds
-        the model instead of ``get_model`` (a relational model with its own node-type ranges, say)."""
+        the model instead of ``get_model`` (a relational model with its own node-type ranges, say).  ``state_bits`` 32 or 8:
+        the steps are ``hiscache.AdamW``'s, without decay, its moments in that many bits (default: torch's Adam)."""
         self.config = config
         self.device = torch.device(config.dl.device)
         self.feat_mode = config.dl.loading.feat_mode
@@ -80,15 +82,17 @@ class HistoryTrainer:
         if ring_rows:
             self.table = RingHistoryCache(self.uvm, ds.num_nodes, config.dl.dataset.feature_dim,
                                           config.train.model.hidden_dim, capacity=int(ring_rows),
-                                          num_layers=self.num_layers, table_dtype=torch.float16,
+                                          num_layers=self.num_layers, table_dtype=ring_dtype,
                                           rate=float(config.history.rate), method=config.history.method,
                                           age_limit=int(config.history.staleness_thres), device=self.device)
         else:
             self.table = HistoryCache(uvm=self.uvm, config=config, mode=self.feat_mode, buffer_bytes=cache_bytes)
         self.model = (model_factory or get_model)(config, self.table).to(self.device)
-        self.optimizer = torch.optim.Adam(self.model.parameters(),
-                                          lr=float(lr or _option(config, "train.optimizer.lr", 1e-3)), fused=True,
-                                          capturable=self.recorded)
+        lr = float(lr or _option(config, "train.optimizer.lr", 1e-3))
+        if state_bits is None:
+            self.optimizer = torch.optim.Adam(self.model.parameters(), lr=lr, fused=True, capturable=self.recorded)
+        else:
+            self.optimizer = AdamW(self.model.parameters(), lr=lr, weight_decay=0.0, state_bits=state_bits)
         self.scheduler = None
         self.loss_fn = torch.nn.functional.nll_loss
         # every batch comes with the transposed view of its CSR; the relational layer also reads the view's edge slots

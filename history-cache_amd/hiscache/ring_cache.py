@@ -1,4 +1,4 @@
-"""RingHistoryCache: historical-embedding cache as one ring table in fp32 / fp16 / bf16 with the
+"""RingHistoryCache: historical-embedding cache as one ring table in fp32 / fp16 / bf16 or 8 bits with the
 admission pass fused on the device.
 
 A build extension for the large synthetic configurations (a 111M x 256 fp16 table does not fit the
@@ -17,6 +17,10 @@ absent, so the model recomputes that row from its neighbours and the admission p
 the fresh value (the reference un-maps old slots for the same effect,
 /root/reference/hiscache/history_table.py:189-200).  A row that was served from the table is never
 re-admitted: what it would store is the cached value itself.
+
+``table_dtype=torch.int8`` keeps the rows as codes with an fp32 scale for every ``group`` columns
+(``hiscache_backend.pack_rows``; 1.06 bytes an element at 64): a row is packed as it is admitted and read back in fp32 by the
+lookup, off by half a scale, 1/254 of its group's largest magnitude, at most.
 """
 import torch
 
@@ -29,7 +33,7 @@ class RingHistoryCache:
 
     def __init__(self, uvm, total_num_node, in_channels, hidden_channels, capacity, num_layers,
                  table_dtype=torch.float16, rate=0.5, thres=None, age_limit=1 << 30, method="grad",
-                 device="cuda:0", collect_stats=True):
+                 device="cuda:0", collect_stats=True, group=64):
         self.uvm = uvm
         self.total_num_node = int(total_num_node)
         self.in_channels = in_channels
@@ -39,7 +43,14 @@ class RingHistoryCache:
         self.method = method
         self.rate = rate
         self.age_limit = int(age_limit)
-        self.table = torch.zeros((capacity, hidden_channels), dtype=table_dtype, device=self.device)
+        if table_dtype is torch.int8:
+            if group not in (32, 64, 128):
+                raise ValueError(f"group must be 32, 64 or 128, got {group}")
+            self.table = _be.PackedRows(torch.zeros((capacity, hidden_channels), dtype=torch.int8, device=self.device),
+                                        torch.zeros((capacity, -(-hidden_channels // group)), device=self.device), group,
+                                        torch.float32)
+        else:
+            self.table = torch.zeros((capacity, hidden_channels), dtype=table_dtype, device=self.device)
         self.full2slot = torch.full((self.total_num_node,), -1, dtype=torch.int64, device=self.device)
         self.slot2full = torch.full((capacity,), -1, dtype=torch.int64, device=self.device)
         self.checkin = torch.full((capacity,), -1, dtype=torch.int64, device=self.device)
@@ -184,23 +195,28 @@ class RingHistoryCache:
         self.last_score = score
         self.produced_embedding = None
 
-    _STATE = ("table", "full2slot", "slot2full", "checkin", "_header")
+    def _state(self):
+        """Name -> tensor of what a checkpoint holds."""
+        packed = isinstance(self.table, _be.PackedRows)
+        table = {"table": self.table.codes, "table_scale": self.table.scale} if packed else {"table": self.table}
+        return {**table, "full2slot": self.full2slot, "slot2full": self.slot2full, "checkin": self.checkin,
+                "header": self._header}
 
     def state_dict(self):
         """The table, its maps and write position and the iteration counter, copied, for a checkpoint."""
-        out = {name.lstrip("_"): getattr(self, name).detach().clone() for name in self._STATE}
+        out = {name: t.detach().clone() for name, t in self._state().items()}
         out["glb_iter"] = self.glb_iter
         return out
 
     def load_state_dict(self, state):
         """Restore what ``state_dict`` saved into a cache of the same sizes."""
-        for name in self._STATE:
-            src, dst = state[name.lstrip("_")], getattr(self, name)
-            if tuple(src.shape) != tuple(dst.shape) or src.dtype != dst.dtype:
-                raise ValueError(f"{name.lstrip('_')}: saved {tuple(src.shape)} {src.dtype}, "
-                                 f"this cache has {tuple(dst.shape)} {dst.dtype}")
-        for name in self._STATE:
-            getattr(self, name).copy_(state[name.lstrip("_")])
+        for name, dst in self._state().items():
+            src = state.get(name)
+            if src is None or tuple(src.shape) != tuple(dst.shape) or src.dtype != dst.dtype:
+                what = "nothing" if src is None else f"{tuple(src.shape)} {src.dtype}"
+                raise ValueError(f"{name}: saved {what}, this cache has {tuple(dst.shape)} {dst.dtype}")
+        for name, dst in self._state().items():
+            dst.copy_(state[name])
         self.glb_iter = int(state["glb_iter"])
         self.produced_embedding = self.sub2embed = self.cached_embedding = self.used_masks = None
 
@@ -227,13 +243,16 @@ class RingHistoryCache:
         warm-start helper).  ``rows`` [len, hidden] fills the table rows, else they stay as they are."""
         n = node_ids.numel()
         h = self.header
-        cap = self.table.shape[0]
+        cap = self.slot2full.numel()
         if h + n > cap:
             raise ValueError("preload does not wrap the ring")
         slots = torch.arange(h, h + n, device=self.device)
         self.full2slot[node_ids] = slots
         self.slot2full[h:h + n] = node_ids
         self.checkin[h:h + n] = 0
-        if rows is not None:
+        if rows is not None and isinstance(self.table, _be.PackedRows):
+            kept = _be.pack_rows(rows.to(self.device, torch.float32).contiguous(), self.table.group)
+            self.table.codes[h:h + n], self.table.scale[h:h + n] = kept.codes, kept.scale
+        elif rows is not None:
             self.table[h:h + n] = rows.to(self.table.dtype)
         self._header.fill_((h + n) % cap)
