@@ -41,10 +41,10 @@ struct RsArgs {
 
 __device__ __forceinline__ int64_t rs_bits(double v) { return __builtin_bit_cast(int64_t, v); }
 __device__ __forceinline__ double rs_double(int64_t v) { return __builtin_bit_cast(double, v); }
-// What is compared lies between these as fp32, so that it stays a number when its lowest bits are an index: NaN and infinity as the
-// largest number; a closed expert below the lowest of the others.
+// What is compared lies between these as fp32, so that it stays a number when its ten lowest bits are an index: NaN and infinity as
+// the largest number; a closed expert below the lowest of the others.  (Logits within 2^-12 of fp32's lowest number count as one.)
 constexpr float RS_MOST = 0x1.fffffep+127f, RS_LEAST = -0x1.ffep+127f, RS_SHUT = -0x1.fffffep+127f;
-__device__ __forceinline__ bool rs_shut(float c) { return c < RS_LEAST; }
+__device__ __forceinline__ bool rs_shut(float c) { return c < -0x1.fffp+127f; }
 
 // ---- the exact way: one row by a whole wave
 // fp64 as whole numbers that order like it: NaN above everything, CLOSED below.
@@ -327,6 +327,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
   rt_in_order();
   float *row = s_all + (live ? mine : 0) * a.stride;
   float top = RS_SHUT, all = 0.f;
+  bool near = false, no_number = false;              // too near for fp32; a softmax with an infinity or a NaN in it
   if (a.softmax) {
     rs_each<L>(row, 0, 4 * a.quads, sub, true, [&](float4 l, int) { top = fmaxf(top, fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w))); });
     top = hc_join<L>(top, [](float x, float y) { return fmaxf(x, y); });
@@ -338,6 +339,12 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     });
     sum = rs_double(hc_join<L>(rs_bits(sum), [](int64_t x, int64_t y) { return rs_bits(rs_double(x) + rs_double(y)); }));
     all = (float)sum;
+    if (__ballot(top >= RS_MOST) != 0) {
+      int bad = 0;
+      for (int e = sub; e < a.E; e += L) bad |= rs_logit(a, r * a.E + e) < __builtin_inff() ? 0 : 1;
+      no_number = hc_join<L>(bad, [](int x, int y) { return x | y; }) != 0;
+      near = no_number && !exact;
+    }
     if (!exact) {
       rt_in_order();
       if (live)
@@ -348,7 +355,6 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
       rt_in_order();
     }
   }
-  bool near = false;                                 // too near for fp32
   uint64_t open = ~0ull;
   const bool by_four = a.per_group % 4 == 0;
   if (a.groups > 1) {
@@ -412,21 +418,28 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
 #pragma unroll
     for (int j = 0; j <= K; ++j) t[j] = RS_SHUT;
     const uint32_t low = a.low;
-    const auto more = [&](float c, int e) {
-      const float x = __uint_as_float((__float_as_uint(c) & ~low) | (low - (uint32_t)e));
+    // SIGNED: the lower of two indexes makes a negative number the larger one, too (sums below 0 are left to the look at what is near)
+    const auto fill = [&](auto signed_) {
+      const auto more = [&](float c, int e) {
+        const uint32_t b = __float_as_uint(c), turn = decltype(signed_)::value ? (uint32_t)((int32_t)b >> 31) & low : 0u;
+        const float x = __uint_as_float((b & ~low) | ((low - (uint32_t)e) ^ turn));
 #pragma unroll
-      for (int j = K; j >= 1; --j) t[j] = __builtin_amdgcn_fmed3f(t[j - 1], t[j], x);
-      t[0] = __builtin_amdgcn_fmed3f(t[0], x, __builtin_inff());
+        for (int j = K; j >= 1; --j) t[j] = __builtin_amdgcn_fmed3f(t[j - 1], t[j], x);
+        t[0] = __builtin_amdgcn_fmed3f(t[0], x, __builtin_inff());
+      };
+      each_open([&](float4 c, int e) {
+        more(c.x, e);
+        more(c.y, e + 1);
+        more(c.z, e + 2);
+        more(c.w, e + 3);
+      });
     };
-    each_open([&](float4 c, int e) {
-      more(c.x, e);
-      more(c.y, e + 1);
-      more(c.z, e + 2);
-      more(c.w, e + 3);
-    });
+    if (exact) fill(std::true_type{});
+    else fill(std::false_type{});
     // (indexes behind the row's end are those of shut places, of which the list's first ones are some as well)
     const auto whole = [&](float x) {
-      const int e = (int)(low - (__float_as_uint(x) & low));
+      const uint32_t b = __float_as_uint(x), turn = exact ? (uint32_t)((int32_t)b >> 31) & low : 0u;
+      const int e = (int)(low - ((b & low) ^ turn));
       const float c = row[e < a.stride ? e : 0];
       return rs_shut(x) ? rs_key(RS_SHUT, 0) : rs_key(c, e);
     };
@@ -461,13 +474,18 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     const float c = rs_key_value(last), d = rs_key_value(next), off = exact ? 0.f : 0x1p-20f * (1.f + fabsf(c));
     const bool count = !near && !rs_shut(d) && !(c - d > off + a.lost * fmaxf(fabsf(c), 0x1p-126f));
     if (__ballot(count) != 0) {
+      // with logits the last winner's place in the row, otherwise how many are not clearly behind it
       int there = 0;
-      each_open([&](float4 v, int) {
-        const float from = c - off;
-        there += (v.x >= from ? 1 : 0) + (v.y >= from ? 1 : 0) + (v.z >= from ? 1 : 0) + (v.w >= from ? 1 : 0);
+      const int at = exact ? rs_key_index(last) : a.E;
+      const float from = c - off;
+      each_open([&](float4 v, int e) {
+        there += v.x > from || (v.x == from && e <= at) ? 1 : 0;
+        there += v.y > from || (v.y == from && e + 1 <= at) ? 1 : 0;
+        there += v.z > from || (v.z == from && e + 2 <= at) ? 1 : 0;
+        there += v.w > from || (v.w == from && e + 3 <= at) ? 1 : 0;
       });
       there = hc_join<L>(there, [](int x, int y) { return x + y; });
-      if (count) near = there > a.k && !(there == a.k + 1 && equal(last, next));
+      if (count) near = there > a.k && (exact || !(there == a.k + 1 && equal(last, next)));
     }
   }
   // this lane's winners
@@ -499,15 +517,11 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
 #pragma unroll
   for (int u = 0; u < OWN; ++u) {
     p[u] = won[u] >= 0 ? rs_logit(a, r * a.E + won[u]) : 0.f;
-    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(p[u] - top) : rs_sigma(p[u]);
+    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(rs_plain(p[u]) - top) : rs_sigma(p[u]);
     sum += s[u];
   }
   sum = hc_join<L>(sum, [](float x, float y) { return x + y; });
-  if (a.softmax) {
-    // a NaN or an infinity is the row's first winner
-    const float first = __shfl(p[0], lane - sub, HC_WAVE);
-    if (!(first < __builtin_inff())) all = sum = __builtin_nanf("");
-  }
+  if (no_number) all = sum = __builtin_nanf("");
   const float of = a.normalize ? sum : a.softmax ? all : 1.f;
   if (!live) return;
 #pragma unroll
