@@ -2,9 +2,9 @@
 //
 //   s = sigma(l) or softmax(l);  c = s + bias;  a group's rank: the sum of its two largest c;  the top_group best groups stay open
 //   chosen: the top_k largest c in open groups, ties to the lowest index;  w = scale * s / (normalize ? sum of the chosen s : 1)
-//   S = sum of the chosen s, t = sum_j w[j] g[j]
+//   S = sum of the chosen s, t = scale sum_j s[j] g[j] / S
 //   sigmoid:  dl[chosen j] = (normalize ? (scale g[j] - t) / S : scale g[j]) s[j] (1 - s[j])
-//   softmax:  dl[chosen j] = w[j] / scale * (scale g[j] - t) (normalize);  dl[e] = p[e] ((e chosen ? scale g : 0) - t)
+//   softmax:  dl[chosen j] = s[j] / S (scale g[j] - t) (normalize);  dl[e] = s[e] ((e chosen ? scale g : 0) - t S)
 //
 // The bias keeps experts evenly loaded and is no part of the weights; a logit or a bias of -inf closes an expert.  Which of two sums is
 // larger is decided in fp64: in fp32 one row in some ten thousand would go to another expert than by the formula.  Without a
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
 struct RsGradArgs {
   const void *logits;
   const int64_t *expert;
-  const float *weight, *picked, *g;
+  const float *picked, *g;
   void *grad;
   int64_t n;
   float scale;
@@ -545,6 +545,7 @@ struct RsGradArgs {
   bool softmax, normalize, whole;
 };
 
+// By the chosen logits alone, but for softmax weights as they are, which go by all of a row's.
 template <typename T, int L, int V>
 __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
   // the row in LDS: what its choices bring, each from the lane that has read it; zeros elsewhere
@@ -554,64 +555,101 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
   const bool live = r < a.n;
   const int64_t at = (live ? r : 0) * a.k;
   const auto plus = [](float x, float y) { return x + y; };
-  const bool by_logit = !a.softmax;
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  const bool by_row = a.softmax && !a.normalize;
   float *own = s_row + threadIdx.x * V, *row = own - lane * V;
 #pragma unroll
   for (int i = 0; i < V; ++i) own[i] = 0.f;
-  // a choice's share of t and of S, and ds / dl; what it brings
-  const auto first = [&](int64_t e, float w, float d, float p, float &t, float &sum) {
-    if (e < 0) return 0.f;
-    t += w * d;
-    if (!by_logit) return 0.f;
-    const float x = expf(-fabsf(p)), q = 1.f / (1.f + x);
-    sum += p < 0.f ? x * q : q;
-    return x * q * q;
+  // a choice: its expert, what reaches its weight, its logit (the first L choices stay in registers)
+  struct choice {
+    int64_t e;
+    float d, p;
   };
-  const auto bring = [&](int64_t e, float w, float d, float slope, float t, float sum) {
-    if (e < 0 || e >= a.E) return;
-    d *= a.scale;
-    if (by_logit) row[e] = !a.normalize ? d * slope : sum == 0.f ? 0.f : (d - t) / sum * slope;
-    else row[e] = a.normalize ? w / a.scale * (d - t) : d;
+  const auto read = [&](int j) {
+    choice c{-1, 0.f, 0.f};
+    if (j < a.k) {
+      c.e = a.expert[at + j];
+      c.d = a.scale * a.g[at + j];
+      if (!by_row) c.p = a.picked[at + j];
+    }
+    return c;
   };
-  // (the first L choices stay in registers)
-  int64_t e = -1;
-  float w = 0.f, d = 0.f, p = 0.f, t = 0.f, sum = 0.f;
-  if (lane < a.k) {
-    e = a.expert[at + lane], w = a.weight[at + lane], d = a.g[at + lane];
-    if (by_logit) p = a.picked[at + lane];
+  const choice mine = read(lane);
+  float top = -__builtin_inff();
+  if (a.softmax && a.normalize) {
+    if (mine.e >= 0) top = mine.p;
+    for (int j = lane + L; j < a.k; j += L) {
+      const choice c = read(j);
+      if (c.e >= 0) top = fmaxf(top, c.p);
+    }
+    top = hc_join<L>(top, larger);
   }
-  const float slope = first(e, w, d, p, t, sum);
-  for (int j = lane + L; j < a.k; j += L)
-    first(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, t, sum);
-  t = hc_join<L>(t, plus);
-  if (by_logit) sum = hc_join<L>(sum, plus);
+  // s of a choice and its slope; for a softmax s on the scale of the row's choices
+  const auto score = [&](const choice &c, float &slope) {
+    if (a.softmax) return slope = c.e < 0 ? 0.f : expf(c.p - top);
+    const float x = expf(-fabsf(c.p)), q = 1.f / (1.f + x);
+    slope = x * q * q;
+    return c.e < 0 ? 0.f : c.p < 0.f ? x * q : q;
+  };
+  float sum = 0.f, t = 0.f, slope = 0.f;
+  if (a.normalize) {
+    const float s = score(mine, slope);
+    sum = s;
+    t = s * mine.d;
+    for (int j = lane + L; j < a.k; j += L) {
+      const choice c = read(j);
+      float other;
+      const float s2 = score(c, other);
+      sum += s2;
+      t += s2 * c.d;
+    }
+    sum = hc_join<L>(sum, plus);
+    t = hc_join<L>(t, plus);
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    t *= inverse;
+    sum = inverse;
+  } else {
+    if (!a.softmax) (void)score(mine, slope);
+    sum = 1.f;
+  }
   rt_in_order();
-  bring(e, w, d, slope, t, sum);
+  const auto bring = [&](const choice &c, float ds) {
+    if (c.e >= 0 && c.e < a.E) row[c.e] = by_row ? c.d : (c.d - t) * sum * ds;
+  };
+  bring(mine, slope);
   for (int j = lane + L; j < a.k; j += L) {
-    float none = 0.f;
-    const float other = first(a.expert[at + j], a.weight[at + j], a.g[at + j], by_logit ? a.picked[at + j] : 0.f, none, none);
-    bring(a.expert[at + j], a.weight[at + j], a.g[at + j], other, t, sum);
+    const choice c = read(j);
+    float other = 0.f;
+    if (!by_row) (void)score(c, other);
+    bring(c, other);
   }
   rt_in_order();
   float out[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = own[i];
-  if (a.softmax && !a.normalize) {
+  if (by_row) {
     T v[V];
-    float p[V], top = -__builtin_inff(), all = 0.f;
+    float p[V], most = -__builtin_inff(), all = 0.f;
     rt_row<T, V>::load(static_cast<const T *>(a.logits) + (live ? r : 0) * a.E, lane * V, a.E, a.whole, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = fmaxf(top, hc_to_f32<T>(v[i]));
-    top = hc_join<L>(top, [](float x, float y) { return fmaxf(x, y); });
+    for (int i = 0; i < V; ++i) most = fmaxf(most, hc_to_f32<T>(v[i]));
+    most = hc_join<L>(most, larger);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float f = hc_to_f32<T>(v[i]);
-      p[i] = rt_masked(f) ? 0.f : expf(f - top);
+      p[i] = rt_masked(f) ? 0.f : expf(f - most);
       all += p[i];
     }
     all = hc_join<L>(all, plus);
+    float inner = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = (all == 0.f ? 0.f : p[i] / all) * (out[i] - t);
+    for (int i = 0; i < V; ++i) {
+      p[i] = all == 0.f ? 0.f : p[i] / all;
+      inner += p[i] * out[i];
+    }
+    inner = hc_join<L>(inner, plus);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = p[i] * (out[i] - inner);
   }
   if (live) rt_row<T, V>::store(static_cast<T *>(a.grad) + r * a.E, lane * V, a.E, a.whole, out);
 }
@@ -681,18 +719,18 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
 }
 
 extern "C" int hc_route_scores_grad(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int score, int normalize,
-                                    float scale, const int64_t *expert, const float *weight, const float *picked,
-                                    const float *grad_weight, void *grad_logits, void *stream) {
+                                    float scale, const int64_t *expert, const float *picked, const float *grad_weight,
+                                    void *grad_logits, void *stream) {
   if (const int rc = rs_sizes(n, E, top_k, score, scale)) return rc;
   if (n == 0) return dtype >= HC_F32 && dtype <= HC_BF16 ? HC_OK : HC_EDTYPE;
-  HC_REQUIRE((score == RS_SIGMOID ? picked != nullptr : logits || normalize) && expert && weight && grad_weight && grad_logits);
+  HC_REQUIRE((score != RS_SIGMOID && !normalize ? logits != nullptr : picked != nullptr) && expert && grad_weight && grad_logits);
   return rt_with_type(dtype, [&](auto type) {
     typedef decltype(type) T;
     return rt_with_shape((int)E, [&](auto lanes, auto each) {
       constexpr int L = decltype(lanes)::value, V = decltype(each)::value;
       const int64_t blocks = (n + HC_BLOCK / L - 1) / (HC_BLOCK / L);
       if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
-      const RsGradArgs a{logits, expert, weight, picked, grad_weight, grad_logits, n, scale, (int)E, (int)top_k,
+      const RsGradArgs a{logits, expert, picked, grad_weight, grad_logits, n, scale, (int)E, (int)top_k,
                          score != RS_SIGMOID, normalize != 0,
                          rt_row<T, V>::whole(logits, E) && rt_row<T, V>::whole(grad_logits, E)};
       rs_backward<T, L, V><<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(a);

@@ -172,7 +172,7 @@ _SIGNATURES = {
     "hc_route_scores": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_int, ctypes.c_float, _c_p,
                                  _c_p, _c_p, _c_p]),
     "hc_route_scores_grad": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_int, ctypes.c_float, _c_p, _c_p, _c_p,
-                                      _c_p, _c_p, _c_p]),
+                                      _c_p, _c_p]),
     "hc_grad_check_packed": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, ctypes.c_int32, _c_int,
                                       _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p,
                                       _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_sz, _c_p]),
@@ -1787,14 +1787,17 @@ def _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, s
 class _RouteScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, top_k, normalize, score, num_group, top_group, scale):
-        by_logit = score == _SCORES["sigmoid"]
-        expert, weight, *picked = _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, scale, by_logit)
+        # (the gradient goes by the chosen logits; that of softmax weights as they are by all of a row's)
+        by_row = not normalize and not score
+        if by_row:
+            expert, weight = _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, scale)
+            kept = logits
+        else:
+            expert, weight, kept = _route_scores(logits, bias, top_k, normalize, score, num_group, top_group, scale, True)
         ctx.mark_non_differentiable(expert)
         ctx.set_materialize_grads(False)
-        # (softmax weights that add up to one go by themselves, sigmoid ones by the chosen logits)
-        kept = picked[0] if by_logit else None if normalize else logits
-        ctx.save_for_backward(_bits(kept), expert, _bits(weight))
-        ctx.hc = (top_k, normalize, score, scale, by_logit, logits.shape, logits.dtype)
+        ctx.save_for_backward(kept.view(_WORD[kept.dtype]), expert)
+        ctx.hc = by_row, logits.shape, logits.dtype, top_k, score, normalize, scale
         return expert, weight
 
     @staticmethod
@@ -1802,14 +1805,15 @@ class _RouteScores(torch.autograd.Function):
     def backward(ctx, _g_expert, g):
         if g is None:
             return (None,) * 8
-        kept, expert, weight = ctx.saved_tensors
-        top_k, normalize, score, scale, by_logit, (n, E), dtype = ctx.hc
+        kept, expert = ctx.saved_tensors
+        by_row, (n, E), dtype, top_k, score, normalize, scale = ctx.hc
         g = _arriving(g)
         grad = g.new_empty((n, E), dtype=dtype)
-        _check(load_library().hc_route_scores_grad(None if by_logit else _ptr(kept), _DTYPES[dtype], n, E, top_k, score, normalize,
-                                                   scale, expert.data_ptr(), weight.data_ptr(), _ptr(kept) if by_logit else None,
-                                                   g.data_ptr(), grad.data_ptr(), _stream_for(g)), "hc_route_scores_grad")
-        return (grad,) + (None,) * 7
+        at = kept.data_ptr()
+        _check(load_library().hc_route_scores_grad(at if by_row else None, _DTYPES[dtype], n, E, top_k, score, normalize, scale,
+                                                   expert.data_ptr(), None if by_row else at, g.data_ptr(), grad.data_ptr(),
+                                                   _stream_for(g)), "hc_route_scores_grad")
+        return grad, None, None, None, None, None, None, None
 
 
 _SCORES = {"softmax": 0, "sigmoid": 1}

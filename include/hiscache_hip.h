@@ -816,17 +816,17 @@ int hc_route_rows_grad(const void *logits, int dtype, int64_t n, int64_t E, int6
  * chosen, of equal ones the lowest index first.  c and the sums are compared in fp64.
  * weight = scale * s / (normalize ? sum of the chosen s : 1); 0 where that sum is 0.
  * A logit or a bias of -inf closes an expert (-1, weight 0, where fewer than top_k are open).
- * picked [n, top_k] (NULL: not kept): the chosen logits, which hc_route_scores_grad
- * takes with score 1.  num_group <= 64 divides E, top_k <= E / num_group * top_group, scale > 0;
+ * picked [n, top_k] (NULL: not kept): the chosen logits, 0 where there is none.  num_group <= 64 divides E, top_k <= E / num_group * top_group, scale > 0;
  * the other limits are hc_route_rows'.
- * hc_route_scores_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and the
- * outputs of hc_route_scores (logits: score 0 without normalize; picked: score 1). */
+ * hc_route_scores_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and
+ * hc_route_scores' expert and picked (score 0 without normalize: its logits and expert; the
+ * other may be NULL). */
 int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int score, const float *bias,
                     int64_t num_group, int64_t top_group, int normalize, float scale, int64_t *expert,
                     float *weight, float *picked, void *stream);
 int hc_route_scores_grad(const void *logits, int dtype, int64_t n, int64_t E, int64_t top_k, int score,
-                         int normalize, float scale, const int64_t *expert, const float *weight,
-                         const float *picked, const float *grad_weight, void *grad_logits, void *stream);
+                         int normalize, float scale, const int64_t *expert, const float *picked,
+                         const float *grad_weight, void *grad_logits, void *stream);
 
 /* hc_expert_order: stable sort of the pairs (row, choice) by expert, for
  * expert [pairs]; numbers outside [0, E) name no expert.  offset[E + 1]: the

@@ -34,13 +34,13 @@ def test_route_scores(lib, p):
     assert call(E=130, G=65, top=65) == EUNSUPPORTED and call(n=1 << 40) == EUNSUPPORTED
     assert call(n=0, logits=None, expert=None, weight=None) == OK
 
-    def grad(logits=p, dtype=0, n=4, E=8, k=2, score=1, normalize=1, scale=1.0, expert=p, weight=p, picked=p, g=p, out=p):
-        return lib.hc_route_scores_grad(logits, dtype, n, E, k, score, normalize, scale, expert, weight, picked, g, out, None)
+    def grad(logits=p, dtype=0, n=4, E=8, k=2, score=1, normalize=1, scale=1.0, expert=p, picked=p, g=p, out=p):
+        return lib.hc_route_scores_grad(logits, dtype, n, E, k, score, normalize, scale, expert, picked, g, out, None)
     for bad in (dict(n=-1), dict(k=9), dict(score=3), dict(scale=0.0), dict(picked=None), dict(score=0, normalize=0, logits=None),
                 dict(expert=None), dict(g=None), dict(out=None)):
         assert grad(**bad) == EINVAL, bad
     assert grad(dtype=3) == EDTYPE and grad(E=1025) == EUNSUPPORTED and grad(n=1 << 40) == EUNSUPPORTED
-    assert grad(n=0, expert=None, weight=None, picked=p, g=None, out=None) == OK
+    assert grad(n=0, expert=None, picked=None, g=None, out=None) == OK
 
 
 def test_ring_in_8_bits(lib, p):
