@@ -686,7 +686,7 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
   const auto launch = [&](auto places, auto lanes) {
     constexpr int L = decltype(lanes)::value;
     const int64_t blocks = (n + HC_WAVE / L - 1) / (HC_WAVE / L);
-    if (!hc_grid_ok(blocks)) return (int)HC_EUNSUPPORTED;
+    if (blocks > (int64_t)(0xffffffffu / HC_WAVE)) return (int)HC_EUNSUPPORTED;
     // rows lie so that lanes which read side by side read from other banks
     int from_row = a.quads;
     while (L < 8 && from_row % 8 != L) ++from_row;

@@ -910,9 +910,7 @@ def grad_check(grad, emb, slot, sub_to_full, thres, table, full2slot, slot2full,
     if packed:
         if static_scratch:
             raise ValueError("a table in 8 bits goes with a workspace")
-        for t, n in ((checkin, "checkin"), (full2slot, "full2slot")):
-            if t is not None and t.device != table.codes.device:
-                raise ValueError(f"{n} and the table must lie on one device")
+        _together(emb, table.codes, table.scale, slot, sub_to_full, thres, full2slot, slot2full, header)
         if checkin is not None and checkin.numel() < capacity:
             raise ValueError("checkin is shorter than the table")
         ws = _workspace(lib.hc_grad_check_workspace_bytes(M), dev)
@@ -1294,6 +1292,7 @@ def ring_lookup(full2slot, ids, table, checkin=None, now=0, age_limit=1 << 62, w
     slot = torch.empty(n, dtype=torch.int64, device=ids.device)
     rows = torch.empty((n, F), dtype=torch.float32, device=ids.device) if want_rows else None
     if packed:
+        _together(ids, full2slot, table.codes, table.scale)
         on_device = isinstance(now, torch.Tensor)
         if on_device != (n_valid is not None):
             raise ValueError("now and n_valid go together as one-element int64 device tensors")

@@ -817,7 +817,8 @@ int hc_route_rows_grad(const void *logits, int dtype, int64_t n, int64_t E, int6
  * weight = scale * s / (normalize ? sum of the chosen s : 1); 0 where that sum is 0.
  * A logit or a bias of -inf closes an expert (-1, weight 0, where fewer than top_k are open).
  * picked [n, top_k] (NULL: not kept): the chosen logits, 0 where there is none.  num_group <= 64 divides E, top_k <= E / num_group * top_group, scale > 0;
- * the other limits are hc_route_rows'.
+ * n L <= 2^32 - 64 for L = 2 lanes a row up to 64 experts, 8 up to 256, 32 above, and
+ * hc_route_rows' other limits (the gradient: all of them).
  * hc_route_scores_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and
  * hc_route_scores' expert and picked (score 0 without normalize: its logits and expert; the
  * other may be NULL). */

@@ -447,3 +447,35 @@ def test_refusals_of_the_optimizer():
     with pytest.raises(ValueError):
         hiscache.AdamW([crossed]).step()
     assert hiscache.AdamW([w]).step(lambda: 3.0) == 3.0       # nothing has a gradient
+
+
+def test_tensors_of_more_than_2_31_elements():
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of free device memory")
+    n, tail = (1 << 31) + 5003, 9000
+    p, g = torch.ones(n, device=DEV, dtype=torch.bfloat16), torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    first = n - tail - (n - tail) % 128                      # (from the start of a group on)
+    p[first:], g[first:] = draw(gen, (n - first,), torch.bfloat16), draw(gen, (n - first,), torch.bfloat16)
+    q, h = p[first:].clone(), g[first:].clone()
+    a, b = be.adamw_state(p, 8), be.adamw_state(q, 8)
+    for _ in range(2):
+        be.adamw_step([p], [g], [a], **HOW)
+        be.adamw_step([q], [h], [b], **HOW)
+    assert torch.equal(p[first:], q) and torch.equal(a.exp_avg[first:], b.exp_avg) and torch.equal(a.scale[:, first // 128:], b.scale)
+    assert bool((p[:first] == p[0]).all()) and int(a.exp_avg[:first].max()) == 0 and a.step.tolist() == [2, 0]
+    (m, _), = be.adamw_moments([a], torch.bfloat16)
+    assert torch.equal(m[first:], be.adamw_moments([b], torch.bfloat16)[0][0])
+
+
+@pytest.mark.parametrize("dtype", ("fp32", "bf16"))
+def test_the_example_of_experts_runs_with_all_of_it(dtype):
+    import importlib.util
+    import os
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "history-cache_amd", "example", "experts.py")
+    spec = importlib.util.spec_from_file_location("hiscache_example_experts", at)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    losses = ex.run(ex.parse(["--nodes", "2000", "--steps", "4", "--score", "sigmoid", "--balance", "0.01", "--state-bits", "8",
+                              "--dtype", dtype]), say=lambda *_: None)
+    assert len(losses) == 4 and all(math.isfinite(v) for v in losses)

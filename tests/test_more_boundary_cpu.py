@@ -125,3 +125,17 @@ def test_states_fit_their_tensors():
     assert s.scale.shape == (2, 0)
     with pytest.raises(ValueError):
         be._check_adamw_state(s, torch.Size([1]), -1)
+
+
+def test_the_example_s_options(tmp_path):
+    import importlib.util
+    import os
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "history-cache_amd", "example")
+    spec = importlib.util.spec_from_file_location("hiscache_example_main", os.path.join(here, "main.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    config = ex.load_config(os.path.join(here, "config.yaml"), ["trainer.ring_dtype=int8", "trainer.state_bits=8"])
+    options = ex.trainer_options(config)
+    assert options["ring_dtype"] is torch.int8 and options["state_bits"] == 8
+    with pytest.raises(ValueError):
+        ex.trainer_options(ex.load_config(os.path.join(here, "config.yaml"), ["trainer.ring_dtype=int4"]))
