@@ -699,18 +699,16 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
                                              static_cast<hipStream_t>(stream)>>>(a);
     return hc_launch_status();
   };
+  // Lanes a row: as few as leave a compute unit enough waves beside their rows in LDS (8.7 KB a wave), and twice as many where that makes
+  // fewer waves than there are SIMDs.  Us by 1 / 2 / 4 / 8 lanes: 500 009 rows of 64 50 / 43 / 47, 30 000 15 / 11 / 9.3 / 9.3,
+  // 250 8.7 / 6.0 / 4.5 / 4.2; by 4 / 8 / 16 / 32: 65 537 rows of 256 in groups 51 / 48 / 65, 8 000 23 / 21 / 21 / 27, 250 14.5 / 10.7 /
+  // 10.2 / 9.3; by 16 / 32 / 64: 30 000 rows of 1 024 78 / 79 / 94, 250 14.6 / 10.5 / 8.8.
   const auto with_lanes = [&](auto places) {
-    // as few lanes a row as keep its wave's rows under 18 KB of LDS (nine waves a compute unit), more where rows are few
     const int least = E <= 64 ? 2 : E <= 256 ? 8 : 32;
-    int lanes = least;
-    while (lanes < 64 && lanes < a.quads && n * lanes < 64 * 2048) lanes *= 2;
-    if (lanes == 1) return launch(places, std::integral_constant<int, 1>{});
-    if (lanes == 2) return launch(places, std::integral_constant<int, 2>{});
-    if (lanes == 4) return launch(places, std::integral_constant<int, 4>{});
-    if (lanes == 8) return launch(places, std::integral_constant<int, 8>{});
-    if (lanes == 16) return launch(places, std::integral_constant<int, 16>{});
-    if (lanes == 32) return launch(places, std::integral_constant<int, 32>{});
-    return launch(places, std::integral_constant<int, 64>{});
+    const bool few = n * least < 64 * 1024;
+    if (least == 2) return few ? launch(places, std::integral_constant<int, 4>{}) : launch(places, std::integral_constant<int, 2>{});
+    if (least == 8) return few ? launch(places, std::integral_constant<int, 16>{}) : launch(places, std::integral_constant<int, 8>{});
+    return few ? launch(places, std::integral_constant<int, 64>{}) : launch(places, std::integral_constant<int, 32>{});
   };
   if (top_k <= 2) return with_lanes(std::integral_constant<int, 2>{});
   if (top_k <= 4) return with_lanes(std::integral_constant<int, 4>{});
