@@ -214,10 +214,18 @@ __device__ __forceinline__ float rs_near_exp(float x) { return __builtin_amdgcn_
 __device__ __forceinline__ float rs_near_sigma(float l) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l * -1.44269504f));
 }
-__device__ __forceinline__ float rs_sigma(float l) {
-  const float e = expf(-fabsf(l));
-  return (l < 0.f ? e : 1.f) / (1.f + e);
+
+// s = 1 / (1 + exp(-l)) on the scale exp(-base), base <= 0, l <= base or base = 0; and s (1 - s).  What is divided by its sum is taken on the
+// scale of the largest logit, so that scores which 32 bits do not hold (l < -87) still have their shares.
+__device__ __forceinline__ float rs_sigma(float l, float base, float &slope) {
+  const float x = expf(-fabsf(l)), q = __builtin_amdgcn_rcpf(1.f + x);
+  const float s = l >= 0.f ? q : (base < 0.f ? expf(l - base) : x) * q;
+  slope = l >= 0.f ? s * x * q : s * q;
+  return s;
 }
+__device__ __forceinline__ float rs_base(float largest) { return fminf(largest, 0.f); }
+// Scores of less than exp of this are 0, as they soon are in 64 bits.
+constexpr float RS_NOTHING = -700.f;
 
 // What is compared, as it lies in LDS: of a logit or a bias; of a sum that cannot be too small; of a logit and a bias in LDS.
 __device__ __forceinline__ float rs_plain(float l) {
@@ -396,7 +404,8 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     open = (uint64_t)hc_join<L>((int64_t)open, [](int64_t x, int64_t y) { return x | y; });
     least = hc_join<L>(least, [](float x, float y) { return fminf(x, y); });
     most = hc_join<L>(most, [](float x, float y) { return fmaxf(x, y); });
-    const float off = exact ? 0x1p-15f * fabsf(least) : 0x1p-19f * (1.f + fabsf(least));
+    // (scores below 2^-126 are 0 to the instructions)
+    const float off = exact ? 0x1p-15f * fmaxf(fabsf(least), 0x1p-100f) : 0x1p-19f * (1.f + fabsf(least));
     near = near || (!rs_shut(most) && !(least - most > off));
   }
   // f for the row's open elements that this lane takes
@@ -513,14 +522,24 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
       rt_in_order();
     }
   }
-  float p[OWN], s[OWN], sum = 0.f;
+  // shares on the scale of the largest chosen; where that is nothing beside the row, or by itself, so are the weights
+  float p[OWN], s[OWN], sum = 0.f, largest = -__builtin_inff();
 #pragma unroll
   for (int u = 0; u < OWN; ++u) {
     p[u] = won[u] >= 0 ? rs_logit(a, r * a.E + won[u]) : 0.f;
-    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(rs_plain(p[u]) - top) : rs_sigma(p[u]);
+    if (won[u] >= 0) largest = fmaxf(largest, a.softmax ? rs_plain(p[u]) : p[u]);
+  }
+  if (a.normalize) largest = hc_join<L>(largest, [](float x, float y) { return fmaxf(x, y); });
+  const float base = a.softmax ? (a.normalize ? largest : top) : a.normalize ? rs_base(largest) : 0.f;
+#pragma unroll
+  for (int u = 0; u < OWN; ++u) {
+    float slope;
+    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(rs_plain(p[u]) - base) : rs_sigma(p[u], base, slope);
     sum += s[u];
   }
   sum = hc_join<L>(sum, [](float x, float y) { return x + y; });
+  const bool nothing = a.normalize && (a.softmax ? largest - top : largest) < RS_NOTHING && sum == sum;
+  if (nothing) sum = 0.f;
   if (no_number) all = sum = __builtin_nanf("");
   const float of = a.normalize ? sum : a.softmax ? all : 1.f;
   if (!live) return;
@@ -530,7 +549,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     if (j >= a.k) continue;
     a.expert[r * a.k + j] = won[u];
     a.weight[r * a.k + j] = won[u] < 0 || of == 0.f ? 0.f : a.scale * (s[u] / of);
-    if (a.picked != nullptr) a.picked[r * a.k + j] = p[u];
+    if (a.picked != nullptr) a.picked[r * a.k + j] = won[u] >= 0 && nothing ? -__builtin_inff() : p[u] < RS_LEAST ? RS_LEAST : p[u];
   }
 }
 
@@ -575,23 +594,23 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
     return c;
   };
   const choice mine = read(lane);
-  float top = -__builtin_inff();
-  if (a.softmax && a.normalize) {
-    if (mine.e >= 0) top = mine.p;
+  float top = RS_SHUT;
+  if (a.normalize) {
+    if (mine.e >= 0) top = fmaxf(top, mine.p);
     for (int j = lane + L; j < a.k; j += L) {
       const choice c = read(j);
       if (c.e >= 0) top = fmaxf(top, c.p);
     }
     top = hc_join<L>(top, larger);
   }
-  // s of a choice and its slope; for a softmax s on the scale of the row's choices
+  // s of a choice and its slope, normalised on the scale of the largest
+  const float base = a.normalize ? rs_base(top) : 0.f;
   const auto score = [&](const choice &c, float &slope) {
-    if (a.softmax) return slope = c.e < 0 ? 0.f : expf(c.p - top);
-    const float x = expf(-fabsf(c.p)), q = 1.f / (1.f + x);
-    slope = x * q * q;
-    return c.e < 0 ? 0.f : c.p < 0.f ? x * q : q;
+    const float s = a.softmax ? slope = expf(c.p - top) : rs_sigma(c.p, base, slope);
+    if (c.e < 0) slope = 0.f;
+    return c.e < 0 ? 0.f : s;
   };
-  float sum = 0.f, t = 0.f, slope = 0.f;
+  float sum = 0.f, t = 0.f, slope = 0.f, inverse = 1.f;
   if (a.normalize) {
     const float s = score(mine, slope);
     sum = s;
@@ -605,16 +624,15 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
     }
     sum = hc_join<L>(sum, plus);
     t = hc_join<L>(t, plus);
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    // (the largest's own score is a half at least, and all are 0 where the weights are)
+    inverse = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);
     t *= inverse;
-    sum = inverse;
-  } else {
-    if (!a.softmax) (void)score(mine, slope);
-    sum = 1.f;
+  } else if (!a.softmax) {
+    (void)score(mine, slope);
   }
   rt_in_order();
   const auto bring = [&](const choice &c, float ds) {
-    if (c.e >= 0 && c.e < a.E) row[c.e] = by_row ? c.d : (c.d - t) * sum * ds;
+    if (c.e >= 0 && c.e < a.E) row[c.e] = by_row ? c.d : (c.d - t) * inverse * ds;
   };
   bring(mine, slope);
   for (int j = lane + L; j < a.k; j += L) {

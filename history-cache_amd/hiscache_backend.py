@@ -1826,10 +1826,12 @@ def route_rows(logits, top_k, normalize=True, score="softmax", bias=None, num_gr
     expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
     weights.  The gradient of the weights reaches ``logits``.  top_k <= 32.
 
-    ``score`` "sigmoid": the logistic function of each logit in place of the softmax (a NaN logit is chosen first; weights whose
-    sum is 0 are 0).  ``bias`` (fp32 [E]): experts are chosen by score + bias, the larger in fp64, and weighted by the score alone; it
-    has no gradient, and -inf closes an expert.  ``top_group`` < ``num_group`` <= 64: experts lie in ``num_group`` groups of as many neighbours, of
+    ``score`` "sigmoid": the logistic function of each logit in place of the softmax (a NaN logit is chosen first).  ``bias``
+    (fp32 [E]): experts are chosen by score + bias, the larger in fp64, and weighted by the score alone; it has no gradient, and
+    -inf closes an expert.  ``top_group`` < ``num_group`` <= 64: experts lie in ``num_group`` groups of as many neighbours, of
     which a row may take the ``top_group`` with the largest sum of two (score + bias) in them, of equal ones the lowest.
+    Normalised weights are shares also of scores that fp32 does not hold; they are 0 where all of a row's chosen logits are
+    below -700 (softmax: 700 below the row's largest), as masked ones are.
     ``scale``: a positive factor of the weights."""
     logits = _operand(logits, "logits")
     if logits.dtype not in _DTYPES:

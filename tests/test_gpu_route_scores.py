@@ -145,7 +145,10 @@ def test_masks_of_the_lowest_value_and_saturated_scores(score, dtype):
         wide = (40 * torch.randn(600, 32, generator=gen, device=DEV)).to(dtype)
         check(wide, 4, score=score, normalize=False, bias=torch.linspace(0, 1, 32, device=DEV))
         expert, weight = be.route_rows(torch.full((3, 8), -200.0, device=DEV).to(dtype), 2, score=score)
-        assert expert.tolist() == [[0, 1]] * 3 and weight.tolist() == [[0.0, 0.0]] * 3     # their sum is 0
+        # sigma(-200) is 0 in 32 bits, but not its share: sigma(-200) / (2 sigma(-200)) = 1 / 2
+        assert expert.tolist() == [[0, 1]] * 3 and weight.tolist() == [[0.5, 0.5]] * 3
+        expert, weight = be.route_rows(torch.full((3, 8), -900.0, device=DEV).to(dtype), 2, score=score)
+        assert expert.tolist() == [[0, 1]] * 3 and weight.tolist() == [[0.0, 0.0]] * 3     # exp(-900) is 0 in 64 bits
 
 
 def test_infinities_and_nan():
@@ -352,3 +355,44 @@ def test_a_layer_of_groups():
     y = torch.einsum("neh,edh->ned", h, layer.w_out)
     want = (y.gather(1, expert.unsqueeze(2).expand(-1, -1, 32)) * weight.unsqueeze(2)).sum(1)
     assert torch.allclose(out, want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("k", (1, 4, 11))
+def test_shares_of_scores_that_32_bits_do_not_hold(k):
+    """Normalised sigmoid weights go by the formula down to logits of -700, in the gradient as well."""
+    gen = torch.Generator(device=DEV).manual_seed(k)
+    logits = torch.randn(700, 24, generator=gen, device=DEV) - torch.arange(700, device=DEV).unsqueeze(1) * 0.98
+    logits[650:, 12:] = 3.0                                  # among others that are nothing to them
+    check(logits, k, score="sigmoid", num_group=1, scale=2.0)
+    check(logits, k, score="sigmoid", num_group=4, top_group=2, scale=2.0)
+    g = torch.randn(700, k, generator=gen, device=DEV)
+    leaf = logits.clone().requires_grad_(True)
+    be.route_rows(leaf, k, score="sigmoid", scale=2.0)[1].backward(g)
+    _, w, ref = reference(logits, k, score="sigmoid", scale=2.0)
+    w.backward(g.double().cpu())
+    off = (leaf.grad.double().cpu() - ref.grad).abs()
+    assert bool((off <= 8 * OFF * g.abs().max(1, keepdim=True)[0].double().cpu()).all())
+
+
+def test_shares_of_a_softmax_among_experts_that_are_nothing_to_its_largest():
+    """A bias that sends rows to experts 90 to 690 below the largest logit: their shares, and their gradients."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    logits = torch.randn(600, 16, generator=gen, device=DEV)
+    logits[:, :8] += 90 + torch.arange(600, device=DEV).unsqueeze(1).float()
+    bias = torch.zeros(16, device=DEV)
+    bias[:8] = -2.0
+    expert, weight = check(logits, 3, score="softmax", bias=bias)
+    assert bool((expert >= 8).all()) and bool((weight > 0).all())
+    g = torch.randn(600, 3, generator=gen, device=DEV)
+    leaf = logits.clone().requires_grad_(True)
+    be.route_rows(leaf, 3, bias=bias)[1].backward(g)
+    _, w, ref = reference(logits, 3, bias=bias)
+    w.backward(g.double().cpu())
+    off = (leaf.grad.double().cpu() - ref.grad).abs()
+    assert bool((off <= 8 * OFF * g.abs().max(1, keepdim=True)[0].double().cpu()).all())
+    # masked ones have no shares
+    logits[:, 8:] = torch.finfo(torch.float32).min
+    leaf = logits.clone().requires_grad_(True)
+    expert, weight = be.route_rows(leaf, 3, bias=bias)
+    weight.backward(g)
+    assert bool((expert >= 8).all()) and bool((weight == 0).all()) and bool((leaf.grad == 0).all())
