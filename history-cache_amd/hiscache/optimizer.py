@@ -13,7 +13,7 @@ class AdamW(torch.optim.Optimizer):
     of fewer than ``min_elements`` keep 32 bits: there is little to gain); 3 to 6 % of a moment are rounded off from step to step.
     ``master``: parameters in half precision have a copy in fp32 that takes the steps; one that something else has changed since the
     last step (weights that were loaded, say) is taken as it is, an element that its copy still rounds to keeps the copy.  (A
-    change through ``.data`` is not noticed.)
+    change through ``.data`` is not noticed, nor one between replays of a recorded step.)
 
     Parameters must be contiguous and on a GPU.  States are made by a parameter's first step, which cannot be recorded."""
 

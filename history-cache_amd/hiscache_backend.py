@@ -16,7 +16,8 @@ Beyond the reference's set: ``aggr_forward_source_history`` (per-source substitu
 ``gather_rows`` / ``lookup``, ``typed_csr`` / ``edge_types_by_ranges`` (relational blocks),
 ``sample_layers`` (device sampler), ``bias_bn_relu`` (a hidden layer's epilogue), ``check_csr`` (input
 validation), ``route_rows`` / ``expert_order`` / ``rows_to_experts`` / ``expert_linear`` / ``gated_experts`` /
-``rows_from_experts`` (a layer of experts) and ``pack_rows`` / ``unpack_rows`` (activations in 8 bits).
+``rows_from_experts`` (a layer of experts), ``pack_rows`` / ``unpack_rows`` (activations and ring tables in 8 bits) and
+``adamw_step`` / ``adamw_moments`` (an optimizer's step over many tensors, its states in 32 or 8 bits).
 
 There is no CPU or PyTorch fallback: if the shared library is missing or a
 tensor is not on a GPU, the call raises.
@@ -861,7 +862,8 @@ def grad_check(grad, emb, slot, sub_to_full, thres, table, full2slot, slot2full,
 
     ``grad`` [M,F] fp32 (or None with ``score`` given), ``emb`` [M,F] fp32, ``slot`` [M] int64
     (-1 = not cached), ``thres`` 1-element fp32 device tensor, ``table`` [capacity,F]
-    fp32/fp16/bf16, or :class:`PackedRows` of as many rows (an admitted row is packed as :func:`pack_rows` does), maps int64, ``header`` 1-element int64 device tensor (advanced in place).
+    fp32/fp16/bf16, or :class:`PackedRows` of as many rows (an admitted row is packed as :func:`pack_rows` does), maps int64,
+    ``header`` 1-element int64 device tensor (advanced in place).
     Returns (mask[bool], score[f32]) and the per-row slot when ``want_slots``."""
     lib = load_library()
     _dev(emb, "emb", torch.float32)
@@ -1269,8 +1271,7 @@ def _packed_table(table):
 
 def ring_lookup(full2slot, ids, table, checkin=None, now=0, age_limit=1 << 62, want_rows=True, n_valid=None):
     """Slots of ``ids`` in a ring table (fp32, fp16, bf16 or :class:`PackedRows`) and the table rows of the hits, in one launch.
-    An entry with
-    ``now - checkin[slot] >= age_limit`` counts as absent (-1).  Returns (slot[int64], rows[fp32] or
+    An entry with ``now - checkin[slot] >= age_limit`` counts as absent (-1).  Returns (slot[int64], rows[fp32] or
     None); rows of absent ids are zero.  For recorded iterations ``now`` may be a one-element int64 device
     tensor, together with ``n_valid`` (the same): ids behind the first ``n_valid`` are padding and find nothing."""
     lib = load_library()
@@ -2379,6 +2380,8 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
         of_g = [g.data_ptr() for g in grads]
     if len(set(at)) < len(at) and len({a for a, n in zip(at, numels) if n}) < len([n for n in numels if n]):
         raise ValueError("a parameter is named twice")
+    if len({id(s.step) for s in states}) < len(states):
+        raise ValueError("a state goes with one parameter")
     for state, shape in zip(states, shapes):
         _check_adamw_state(state, shape, index)
     kinds = [(dtype, state.scale is not None, state.master is not None) for dtype, state in zip(dtypes, states)]

@@ -479,3 +479,36 @@ def test_the_example_of_experts_runs_with_all_of_it(dtype):
     losses = ex.run(ex.parse(["--nodes", "2000", "--steps", "4", "--score", "sigmoid", "--balance", "0.01", "--state-bits", "8",
                               "--dtype", dtype]), say=lambda *_: None)
     assert len(losses) == 4 and all(math.isfinite(v) for v in losses)
+
+
+def test_a_state_goes_with_one_parameter():
+    a, b = torch.zeros(300, device=DEV), torch.zeros(300, device=DEV)
+    state, other = be.adamw_state(a), be.adamw_state(a)
+    with pytest.raises(ValueError, match="one parameter"):
+        be.adamw_step([a, b], [a + 1, b + 1], [state, state])
+    with pytest.raises(ValueError, match="one parameter"):
+        be.adamw_step([a, b], [a + 1, b + 1], [state, be.AdamWState(other.exp_avg, other.exp_avg_sq, state.step)])
+    assert not bool(a.any()) and not bool(state.step.any())
+
+
+@pytest.mark.parametrize("bits", (32, 8))
+def test_steps_on_two_streams_at_once(bits):
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    made = [[draw(gen, (700_001,), torch.float32), draw(gen, (33,), torch.float32)] for _ in range(2)]
+    grads = [[draw(gen, p.shape, torch.float32) for p in ps] for ps in made]
+    alone = [[p.clone() for p in ps] for ps in made]
+    for ps, gs in zip(alone, grads):
+        states = [be.adamw_state(p, bits) for p in ps]
+        for _ in range(4):
+            be.adamw_step(ps, gs, states, **HOW)
+    kept = [[be.adamw_state(p, bits) for p in ps] for ps in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for st, ps, gs, states in zip(streams, made, grads, kept):
+            with torch.cuda.stream(st):
+                be.adamw_step(ps, gs, states, **HOW)
+    torch.cuda.synchronize()
+    for ps, want, states in zip(made, alone, kept):
+        assert all(torch.equal(a, b) for a, b in zip(ps, want))
+        assert all(s.step.tolist() == [4, 0] for s in states)
