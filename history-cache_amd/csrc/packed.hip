@@ -15,7 +15,7 @@
 // Groups do not reach over from a to b.
 //
 // A lane owns eight adjacent columns; group / 8 lanes share a group, whose largest magnitude goes round from lane to lane.  Bound by
-// memory, one pass over each operand: 150 001 rows of 602 fp32 91 us kept (5.0 TB/s), 75 to 101 read back (4.5 to 6.0); the gate of
+// memory, one pass over each operand: 150 001 rows of 602 fp32 81 us kept (5.6 TB/s), 75 to 101 read back (4.5 to 6.0); the gate of
 // 65 537 rows of 2 x 1 024 bf16 118 us forward (545 MB, 4.6 TB/s), 116 backward (680 MB, 5.9).
 #include "packed_rows.h"
 

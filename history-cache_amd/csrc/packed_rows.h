@@ -73,7 +73,8 @@ template <int S>
 __device__ __forceinline__ void pk_store_tail(char *p, int valid, const uint32_t (&w)[2 * S]) {
   uint32_t a[S];
 #pragma unroll
-  for (int i = 0; i < S; ++i) a[i] = valid & 4 ? w[S + i] : w[i];
+  // (by bits: a choice between neighbours becomes a search by a computed index)
+  for (int i = 0; i < S; ++i) a[i] = w[i] ^ ((w[i] ^ w[S + i]) & (valid & 4 ? ~0u : 0u));
   if (valid & 4) pk_few<S, 4>::store(p, w);
   if (valid & 2) pk_few<S, 2>::store(p + (valid & 4) * S, a);
   const uint32_t one = valid & 2 ? (S == 1 ? a[0] >> 16 : a[S / 2]) : a[0];
@@ -141,10 +142,25 @@ __device__ __forceinline__ void pk_load_codes(const int8_t *__restrict__ p, int 
   for (int i = 0; i < PK_EACH; ++i) v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * scale;
 }
 
+// NT: with the non-temporal hint
+template <bool NT = false>
+__device__ __forceinline__ void pk_store_codes(int8_t *__restrict__ p, int valid, const uint32_t (&w)[2]) {
+  if (valid >= PK_EACH) {
+    if constexpr (NT) {
+      typedef uint32_t two __attribute__((ext_vector_type(2), aligned(1)));
+      __builtin_nontemporal_store(two{w[0], w[1]}, reinterpret_cast<two *>(p));
+    } else {
+      *reinterpret_cast<pk_codes *>(p) = pk_codes{{w[0], w[1]}};
+    }
+  } else if (valid > 0) {
+    pk_store_tail<1>(reinterpret_cast<char *>(p), valid, w);
+  }
+}
+
 // The scale of the group that L lanes hold, and this lane's codes.  The largest magnitude is found on the bits, where a NaN
 // is above infinity and infinity above every number.
-template <int L, bool NT = false>
-__device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__restrict__ p, int valid) {
+template <int L>
+__device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], uint32_t (&w)[2]) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
@@ -156,7 +172,7 @@ __device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__
   const bool zero = most < PK_SMALLEST, bad = m >= 0x7f800000u;
   const float inverse = zero || bad ? 0.f : 1.0f / most * 127.0f;
   // 1.5 2^23 more has the rounded number in its lowest byte
-  uint32_t w[2], c[PK_EACH];
+  uint32_t c[PK_EACH];
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) c[i] = __float_as_uint(v[i] * inverse + 0x1.8p23f);
 #pragma unroll
@@ -164,18 +180,16 @@ __device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__
     w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0c0c0400u),
                                  __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u), 0x05040100u);
   if (bad) w[0] = w[1] = 0;
-  if (valid >= PK_EACH) {
-    if constexpr (NT) {
-      typedef uint32_t two __attribute__((ext_vector_type(2), aligned(1)));
-      __builtin_nontemporal_store(two{w[0], w[1]}, reinterpret_cast<two *>(p));
-    } else {
-      *reinterpret_cast<pk_codes *>(p) = pk_codes{{w[0], w[1]}};
-    }
-  } else if (valid > 0) {
-    pk_store_tail<1>(reinterpret_cast<char *>(p), valid, w);
-  }
   const float scale = most * (1.0f / 127.0f);
   return zero ? 0.f : !bad && scale > PK_LARGEST_SCALE ? PK_LARGEST_SCALE : scale;
+}
+
+template <int L>
+__device__ __forceinline__ float pk_encode(const float (&v)[PK_EACH], int8_t *__restrict__ p, int valid) {
+  uint32_t w[2];
+  const float scale = pk_encode<L>(v, w);
+  pk_store_codes(p, valid, w);
+  return scale;
 }
 
 #endif  // __HIPCC__
