@@ -9,13 +9,17 @@
 //
 // 8 bits: m and r = sqrt(v) as numbers of four bits of exponent; m has a sign and three bits of mantissa, r, which has none, four.
 // 128 adjacent elements share the exponent E (one byte, as fp32's biased exponent) of their largest magnitude rounded to that
-// mantissa.  Elements differ by orders of magnitude, and an update goes by m / r: equal steps would lose the small
-// ones altogether, a mantissa keeps each within 1/16 (r: 1/32) down to 2^-14 of the largest, and 2^-18 (r: 2^-19) of that above.  r is
+// mantissa.  Elements differ by orders of magnitude, and an update goes by m / r: equal steps would lose the small ones
+// altogether, a mantissa keeps each within 1/16 (r: 1/32) down to 2^-14 of the largest, and 2^-18 (r: 2^-19) of that below.  r is
 // rounded up from zero: an element whose r was lost would move by m / eps.  (Scaled by 2^(15 - E) a number's upper bits are
 // its code, subnormal ones included.)  E = 0: zeros, the largest is below fp32's normal numbers.  E = 255: a group that held an
 // infinity or a NaN, all of which reads back as NaN.
 //
-// A block takes pieces of 2 048 elements of the tensors' concatenation, eight a lane; sixteen lanes share a group.
+// A block takes pieces of 2 048 elements of the tensors' concatenation, eight a lane; sixteen lanes share a group.  Every element is
+// read and written once, which bounds large calls: 50.3 M elements of fp32 (us and TB/s) with 8 bits 166 (4.9), 32 bits 278 (5.1), of
+// bf16 with 8 bits 104 (4.8), with a copy in fp32 168 (4.8), 32 bits 219 (5.0), with a copy 284 (5.0); a copy of memory reaches 4.8.  Eight
+// small tensors take 6.6 us: their counts, the powers of the rates in 64 bits, a memory's latency for the elements and one for
+// the arrival.  Non-temporal stores: no difference.
 #include "packed_rows.h"
 
 namespace {
@@ -153,9 +157,9 @@ __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
   __shared__ AwFactors s_factor[AW_MAX];
   const bool counts = (int)threadIdx.x < a.count;
   const int64_t count = counts ? *a.t[threadIdx.x].step + 1 : 0;
-  // s_factor is worked out while a block's first piece is on its way where that costs nothing: with states in 8 bits, whose pieces are
-  // bound by their operations, the loop without it is faster (50 M elements of bf16 116 us against 130; eight small tensors in 32
-  // bits 6.8 against 6.5).
+  // s_factor is worked out while a block's first piece is on its way where that costs nothing: with states in 8 bits, whose pieces
+  // have more operations, the loop without it is faster (50 M elements of bf16 104 us against 118; eight small tensors in 32 bits
+  // 6.8 against 6.5).
   bool known = false;
   const auto work_out = [&] {
     if (counts) s_factor[threadIdx.x].work_out(a, count);
