@@ -618,13 +618,13 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
   if (a.normalize) {
     const float s = score(mine, slope);
     sum = s;
-    t = s * mine.d;
+    t = mine.e < 0 ? 0.f : s * mine.d;             // (what reaches a weight that stands for nothing may be no number)
     for (int j = lane + L; j < a.k; j += L) {
       const choice c = read(j);
       float other;
       const float s2 = score(c, other);
       sum += s2;
-      t += s2 * c.d;
+      t += c.e < 0 ? 0.f : s2 * c.d;
     }
     sum = hc_join<L>(sum, plus);
     t = hc_join<L>(t, plus);

@@ -396,3 +396,19 @@ def test_shares_of_a_softmax_among_experts_that_are_nothing_to_its_largest():
     expert, weight = be.route_rows(leaf, 3, bias=bias)
     weight.backward(g)
     assert bool((expert >= 8).all()) and bool((weight == 0).all()) and bool((leaf.grad == 0).all())
+
+
+@pytest.mark.parametrize("how", (dict(score="sigmoid"), dict(score="sigmoid", normalize=False), dict(scale=2.0), dict(scale=2.0, normalize=False)))
+def test_what_reaches_the_weights_of_missing_experts_is_left_alone(how):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    logits = torch.randn(300, 20, generator=gen, device=DEV)
+    logits[:, 3:] = -math.inf
+    g = torch.randn(300, 12, generator=gen, device=DEV)
+    grads = []
+    for value in (0.0, math.nan, math.inf):
+        leaf = logits.clone().requires_grad_(True)
+        expert, weight = be.route_rows(leaf, 12, **how)
+        assert bool((expert[:, 3:] == -1).all()) and not bool(weight[:, 3:].any())
+        weight.backward(torch.where(expert < 0, value, g))
+        grads.append(leaf.grad)
+    assert bool(torch.isfinite(grads[0]).all()) and all(torch.equal(x, grads[0]) for x in grads[1:])
