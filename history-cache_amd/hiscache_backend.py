@@ -22,6 +22,7 @@ validation), ``route_rows`` / ``expert_order`` / ``rows_to_experts`` / ``expert_
 There is no CPU or PyTorch fallback: if the shared library is missing or a
 tensor is not on a GPU, the call raises.
 """
+import array
 import ctypes
 import math
 import os
@@ -2418,8 +2419,8 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
             words += [s.scale.data_ptr() for s in ss]
         if copies:
             words += [s.master.data_ptr() for s in ss]
-        host = (_c_i64 * len(words))(*words)              # the arrays of the call one after the other
-        first = ctypes.addressof(host)
+        host = array.array("q", words)                    # the arrays of the call one after the other
+        first = host.buffer_info()[0]
         to = [first + 8 * n * k for k in range(8)]
         _check(lib.hc_adamw_step(n, to[0], to[1], _DTYPES[dtype], to[2], to[3], to[6] if bits8 else None,
                                  to[6 + bits8] if copies else None, to[4], to[5], 8 if bits8 else 32, float(lr), _ptr(lr_dev),
