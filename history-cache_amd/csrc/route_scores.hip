@@ -219,13 +219,11 @@ __device__ __forceinline__ float rs_near_sigma(float l) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l * -1.44269504f));
 }
 
-// s = 1 / (1 + exp(-l)) on the scale exp(-base), base <= 0, l <= base or base = 0; and s (1 - s).  What is divided by its sum is
-// taken on the scale of the largest logit, so that scores which 32 bits do not hold (l < -87) still have their shares.
-__device__ __forceinline__ float rs_sigma(float l, float base, float &slope) {
+// s = 1 / (1 + exp(-l)) on the scale exp(-base), base <= 0, l <= base or base = 0; and 1 - s.  What is divided by its sum is taken on the scale of the largest logit, so that scores which 32 bits do not hold (l < -87) still have their shares.
+__device__ __forceinline__ float rs_sigma(float l, float base, float &rest) {
   const float x = expf(-fabsf(l)), q = __builtin_amdgcn_rcpf(1.f + x);
-  const float s = l >= 0.f ? q : (base < 0.f ? expf(l - base) : x) * q;
-  slope = l >= 0.f ? s * x * q : s * q;
-  return s;
+  rest = l >= 0.f ? x * q : q;
+  return l >= 0.f ? q : (base < 0.f ? expf(l - base) : x) * q;
 }
 __device__ __forceinline__ float rs_base(float largest) { return fminf(largest, 0.f); }
 // Scores of less than exp of this are 0, as they soon are in 64 bits.
@@ -537,8 +535,8 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
   const float base = a.softmax ? (a.normalize ? largest : top) : a.normalize ? rs_base(largest) : 0.f;
 #pragma unroll
   for (int u = 0; u < OWN; ++u) {
-    float slope;
-    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(rs_plain(p[u]) - base) : rs_sigma(p[u], base, slope);
+    float rest;
+    s[u] = won[u] < 0 ? 0.f : a.softmax ? expf(rs_plain(p[u]) - base) : rs_sigma(p[u], base, rest);
     sum += s[u];
   }
   sum = hc_join<L>(sum, [](float x, float y) { return x + y; });
@@ -607,43 +605,46 @@ __global__ __launch_bounds__(HC_BLOCK) void rs_backward(RsGradArgs a) {
     }
     top = hc_join<L>(top, larger);
   }
-  // s of a choice and its slope, normalised on the scale of the largest
+  // s of a choice, normalised on the scale of the largest, and what its slope is more than s
   const float base = a.normalize ? rs_base(top) : 0.f;
-  const auto score = [&](const choice &c, float &slope) {
-    const float s = a.softmax ? slope = expf(c.p - top) : rs_sigma(c.p, base, slope);
-    if (c.e < 0) slope = 0.f;
-    return c.e < 0 ? 0.f : s;
+  const auto score = [&](const choice &c, float &rest) {
+    rest = 1.f;
+    return c.e < 0 ? 0.f : a.softmax ? expf(c.p - top) : rs_sigma(c.p, base, rest);
   };
-  float sum = 0.f, t = 0.f, slope = 0.f, inverse = 1.f;
+  float rest = 1.f, s = by_row ? 1.f : score(mine, rest), sum = s, inverse = 0.f, t = 0.f;
+  // (a reciprocal and one correction: the share of a choice that is its row's only one is 1, and its gradient 0)
+  const auto share = [&](float s) {
+    const float f = s * inverse;
+    return __builtin_fmaf(__builtin_fmaf(-f, sum, s), inverse, f);
+  };
   if (a.normalize) {
-    const float s = score(mine, slope);
-    sum = s;
-    t = mine.e < 0 ? 0.f : s * mine.d;             // (what reaches a weight that stands for nothing may be no number)
+    for (int j = lane + L; j < a.k; j += L) {
+      float other;
+      sum += score(read(j), other);
+    }
+    sum = hc_join<L>(sum, plus);
+    // (the largest's own score is a half at least, and all are 0 where the weights are)
+    inverse = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);
+    s = share(s);
+    // (what reaches a weight that stands for nothing may be no number)
+    t = mine.e < 0 ? 0.f : s * mine.d;
     for (int j = lane + L; j < a.k; j += L) {
       const choice c = read(j);
       float other;
-      const float s2 = score(c, other);
-      sum += s2;
-      t += c.e < 0 ? 0.f : s2 * c.d;
+      t += c.e < 0 ? 0.f : share(score(c, other)) * c.d;
     }
-    sum = hc_join<L>(sum, plus);
     t = hc_join<L>(t, plus);
-    // (the largest's own score is a half at least, and all are 0 where the weights are)
-    inverse = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);
-    t *= inverse;
-  } else if (!a.softmax) {
-    (void)score(mine, slope);
   }
   rt_in_order();
   const auto bring = [&](const choice &c, float ds) {
-    if (c.e >= 0 && c.e < a.E) row[c.e] = by_row ? c.d : (c.d - t) * inverse * ds;
+    if (c.e >= 0 && c.e < a.E) row[c.e] = by_row ? c.d : (c.d - t) * ds;
   };
-  bring(mine, slope);
+  bring(mine, s * rest);
   for (int j = lane + L; j < a.k; j += L) {
     const choice c = read(j);
-    float other = 0.f;
-    if (!by_row) (void)score(c, other);
-    bring(c, other);
+    float other = 1.f, f = 1.f;
+    if (!by_row) f = score(c, other);
+    bring(c, (a.normalize ? share(f) : f) * other);
   }
   rt_in_order();
   float out[V];

@@ -412,3 +412,18 @@ def test_what_reaches_the_weights_of_missing_experts_is_left_alone(how):
         weight.backward(torch.where(expert < 0, value, g))
         grads.append(leaf.grad)
     assert bool(torch.isfinite(grads[0]).all()) and all(torch.equal(x, grads[0]) for x in grads[1:])
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("score", ("sigmoid", "softmax"))
+def test_the_only_choice_of_a_row_has_weight_1_and_no_gradient(score, dtype):
+    """Divided by itself a score is 1 whatever the logit is, to the last bit, in the gradient as well."""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    logits = (9 * torch.randn(4000, 40, generator=gen, device=DEV)).to(dtype)
+    logits[2000:, :39] = -math.inf                           # of four choices three name no expert
+    bias = torch.randn(40, generator=gen, device=DEV)
+    for rows, k in ((logits[:2000], 1), (logits[2000:], 4)):
+        leaf = rows.clone().requires_grad_(True)
+        expert, weight = be.route_rows(leaf, k, score=score, bias=bias)
+        weight.backward(torch.randn(2000, k, generator=gen, device=DEV))
+        assert bool((weight[:, 0] == 1).all()) and not bool(weight[:, 1:].any()) and not bool(leaf.grad.any())
