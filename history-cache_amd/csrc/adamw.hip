@@ -15,9 +15,18 @@
 // its code, subnormal ones included.)  E = 0: zeros, the largest is below fp32's normal numbers.  E = 255: a group that held an
 // infinity or a NaN, all of which reads back as NaN.
 //
+// A code is the nearest one, or (HC_ADAMW_RANDOM) one of the two that a number lies between, the upper one as often as the number lies
+// nearer to it.  The nearest one is right for one step from given moments; over many it stops r, which moves by (1 - b2) / 2 of itself a
+// step, far less than half a code: at b2 = 0.999 and gradients that stay as they are it ends at 0.13 to 0.5 of the right one, and
+// never falls again.  At random a number is kept in the mean: r's mean over elements stays within 1 % of the right one at any b2, an
+// element's own within 10 % (one standard deviation; each step's two thousandths add up over the steps that v remembers).  What
+// is random is a hash of the element's place in its tensor and the tensor's count, so that a step that is made again, in a
+// recording, or in another launch is the same.
+//
 // A block takes pieces of 2 048 elements of the tensors' concatenation, eight a lane; sixteen lanes share a group.  Every element is
 // read and written once, which bounds large calls: 50.3 M elements of fp32 (us and TB/s) with 8 bits 166 (4.9), 32 bits 278 (5.1), of
-// bf16 with 8 bits 104 (4.8), with a copy in fp32 168 (4.8), 32 bits 219 (5.0), with a copy 284 (5.0); a copy of memory reaches 4.8.  Eight
+// bf16 with 8 bits 104 (4.8), with a copy in fp32 168 (4.8), 32 bits 219 (5.0), with a copy 284 (5.0); rounded at random, fifteen operations an
+// element more, 164, 107 and 168.  torch's copy of 4 GiB reaches 4.8 TB/s, of 256 MiB 5.4.  Eight
 // small tensors take 6.6 us: their counts, the powers of the rates in 64 bits, a memory's latency for the elements and one for
 // the arrival.  Non-temporal stores: no difference.
 #include "packed_rows.h"
@@ -58,14 +67,24 @@ __device__ __forceinline__ double aw_power(double b, int64_t t) {
   return r;
 }
 
+// Two rounds of an odd factor (the golden section's, the circle number's digits) and the upper half folded into the lower one: a change of
+// one bit changes every other in about half of all cases.
+__device__ __forceinline__ uint32_t aw_mix(uint32_t x) {
+  x = (x ^ x >> 16) * 0x9e3779b1u;
+  x = (x ^ x >> 15) * 0x85a308d3u;
+  return x ^ x >> 16;
+}
+
 // What a tensor's elements share.
 struct AwFactors {
   float keep, size, lift;
+  uint32_t key;                              // of what is random in this step
   __device__ __forceinline__ void work_out(const AwArgs &a, int64_t count) {
     const double lr = a.lr_dev != nullptr ? (double)*a.lr_dev : a.lr;
     keep = (float)(1.0 - lr * a.decay);
     size = (float)(lr / (1.0 - aw_power(a.b1, count)));
     lift = (float)(1.0 / sqrt(1.0 - aw_power(a.b2, count)));
+    key = aw_mix(aw_mix((uint32_t)count) + (uint32_t)((uint64_t)count >> 32) * 0x9e3779b1u + 0x243f6a88u);
   }
 };
 
@@ -92,35 +111,38 @@ __device__ __forceinline__ void aw_decode(const uint32_t (&w)[2], uint32_t E, fl
   }
 }
 
-// Adds half a unit of MAN bits of mantissa to fp32 bits, a little less where that breaks a tie the even way.
-template <int MAN>
-__device__ __forceinline__ uint32_t aw_round(uint32_t b) {
+// Adds half a unit of MAN bits of mantissa to fp32 bits, a little less where that breaks a tie the even way.  RANDOM: what half of
+// a random word (its lower one for three bits, its upper one for four) is of a unit, 2^-17 more, so that a code's own number stays.
+template <int MAN, bool RANDOM>
+__device__ __forceinline__ uint32_t aw_round(uint32_t b, uint32_t random) {
+  if constexpr (RANDOM) return b + (MAN == 3 ? (random & 0xffffu) << 4 | 8u : (random >> 16) << 3 | 4u);
   return b + (1u << (22 - MAN)) - 1u + (b >> (23 - MAN) & 1u);
 }
 
 // The E of the group that AW_LANES lanes hold, and this lane's codes.
-template <int MAN>
-__device__ __forceinline__ uint32_t aw_encode(const float (&v)[PK_EACH], uint32_t (&w)[2]) {
+template <int MAN, bool RANDOM>
+__device__ __forceinline__ uint32_t aw_encode(const float (&v)[PK_EACH], const uint32_t (&random)[PK_EACH], uint32_t (&w)[2]) {
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    if constexpr (RANDOM) b = aw_round<MAN, true>(b, random[i]);       // (which of them is the largest goes by what they become)
     most = b > most ? b : most;
   }
   most = hc_join<AW_LANES>(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-  const uint32_t top = aw_round<MAN>(most) >> 23, E = top > 255u ? 255u : top;
+  const uint32_t top = (RANDOM ? most : aw_round<MAN, false>(most, 0)) >> 23, E = top > 255u ? 255u : top;
   uint32_t c[PK_EACH];                       // the code in the upper byte
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
     uint32_t b = __float_as_uint(__builtin_amdgcn_ldexpf(v[i], 15 - (int)E));
     if constexpr (MAN == 3) {
-      b = aw_round<3>(b);
+      b = aw_round<3, RANDOM>(b, random[i]);
       c[i] = (b & 0x80000000u) | (b << 4 & 0x7fffffffu);
     } else {
       // (a root that is not 0 is above 2^-75)
       const uint32_t least = __float_as_uint(v[i]) < 1u << 19 ? __float_as_uint(v[i]) : 1u << 19;
       b = b > least ? b : least;
-      c[i] = aw_round<4>(b) << 5;
+      c[i] = aw_round<4, RANDOM>(b, random[i]) << 5;
     }
   }
 #pragma unroll
@@ -151,7 +173,8 @@ __device__ __forceinline__ void aw_store_codes(void *p, int64_t at, int valid, c
   else if (valid > 0) pk_store_tail<1>(q, valid, w);
 }
 
-template <typename T, int BITS, bool MASTER>
+// RANDOM: states in 8 bits are rounded at random.
+template <typename T, int BITS, bool MASTER, bool RANDOM>
 __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
   const float b1 = (float)a.b1, c1 = (float)(1.0 - a.b1), b2 = (float)a.b2, c2 = (float)(1.0 - a.b2);
   __shared__ AwFactors s_factor[AW_MAX];
@@ -226,10 +249,15 @@ __global__ __launch_bounds__(HC_BLOCK) void aw_step(AwArgs a) {
           for (int k = 0; k < PK_EACH; ++k)
             if (k >= valid) m[k] = r[k] = 0.f;               // (what lies behind the end: codes of zero scales, no numbers)
         }
-        uint32_t w[2];
-        const uint32_t Em = aw_encode<3>(m, w);
+        uint32_t random[PK_EACH], w[2];
+        if constexpr (RANDOM) {
+          const uint32_t from = f.key + (uint32_t)at + (uint32_t)((uint64_t)at >> 32) * 0x9e3779b1u;
+#pragma unroll
+          for (int k = 0; k < PK_EACH; ++k) random[k] = aw_mix(from + (uint32_t)k);
+        }
+        const uint32_t Em = aw_encode<3, RANDOM>(m, random, w);
         aw_store_codes(t.m, at, valid, w);
-        const uint32_t Ev = aw_encode<4>(r, w);
+        const uint32_t Ev = aw_encode<4, RANDOM>(r, random, w);
         aw_store_codes(t.v, at, valid, w);
         if (valid > 0 && threadIdx.x % AW_LANES == 0) {
           t.scale[at / AW_GROUP] = (uint8_t)Em;
@@ -310,6 +338,8 @@ extern "C" int hc_adamw_step(int count, void *const *param, const void *const *g
                              void *const *exp_avg_sq, uint8_t *const *scale, float *const *master, int64_t *const *step,
                              const int64_t *numel, int state_bits, double lr, const float *lr_dev, double beta1, double beta2,
                              double eps, double weight_decay, void *stream) {
+  const bool random = state_bits == (8 | HC_ADAMW_RANDOM);
+  if (random) state_bits = 8;
   HC_REQUIRE(count >= 0 && (state_bits == 8 || state_bits == 32));
   HC_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0);
   if (dtype < HC_F32 || dtype > HC_BF16) return HC_EDTYPE;
@@ -338,15 +368,16 @@ extern "C" int hc_adamw_step(int count, void *const *param, const void *const *g
     hipStream_t st = static_cast<hipStream_t>(stream);
     const auto launch = [&](auto type) {
       typedef decltype(type) T;
+      const auto with_copy = [&](auto copy) {
+        constexpr bool MASTER = decltype(copy)::value;
+        if (state_bits == 32) aw_step<T, 32, MASTER, false><<<grid, block, 0, st>>>(a);
+        else if (random) aw_step<T, 8, MASTER, true><<<grid, block, 0, st>>>(a);
+        else aw_step<T, 8, MASTER, false><<<grid, block, 0, st>>>(a);
+      };
       if constexpr (!std::is_same<T, float>::value) {
-        if (master) {
-          if (state_bits == 8) aw_step<T, 8, true><<<grid, block, 0, st>>>(a);
-          else aw_step<T, 32, true><<<grid, block, 0, st>>>(a);
-          return;
-        }
+        if (master) return with_copy(std::true_type{});
       }
-      if (state_bits == 8) aw_step<T, 8, false><<<grid, block, 0, st>>>(a);
-      else aw_step<T, 32, false><<<grid, block, 0, st>>>(a);
+      with_copy(std::false_type{});
     };
     if (dtype == HC_F32) launch(float{});
     else if (dtype == HC_F16) launch(__half{});

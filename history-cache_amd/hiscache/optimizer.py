@@ -10,7 +10,9 @@ import hiscache_backend as _be
 
 class AdamW(torch.optim.Optimizer):
     """lr: a number or one fp32 on the parameters' device.  ``state_bits`` 8: both moments take a byte an element (parameters
-    of fewer than ``min_elements`` keep 32 bits: there is little to gain); 3 to 6 % of a moment are rounded off from step to step.
+    of fewer than ``min_elements`` keep 32 bits: there is little to gain), rounded at random so that they are right in the mean over
+    any number of steps and at any betas: over the elements the root of the second moment is within 1 % of that in 32 bits, for one element
+    within 10 % (one standard deviation; up to 35 % while it falls to a hundredth), the first moment within 10 %.
     ``master``: parameters in half precision have a copy in fp32 that takes the steps; one that something else has changed since the
     last step (weights that were loaded, say) is taken as it is, an element that its copy still rounds to keeps the copy.  (A
     change through ``.data`` is not noticed, nor one between replays of a recorded step.)
@@ -66,7 +68,8 @@ class AdamW(torch.optim.Optimizer):
             if not params:
                 continue
             states = [self._handle(p, group) for p in params]
-            how = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
+            how = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                       rounding="random")
             with torch.cuda.device(params[0].device):
                 _be.adamw_step(params, [p.grad for p in params], states, **how)
             for p, s in zip(params, states):

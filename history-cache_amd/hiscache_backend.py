@@ -2339,7 +2339,10 @@ def _pointers(tensors):
     return (_c_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
-def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+_ADAMW_RANDOM = 256
+
+
+def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, rounding="nearest"):
     """One AdamW step over many tensors, in place and in one launch for every 48 of a kind (element type, bits of the states, with
     or without a copy):
 
@@ -2350,7 +2353,10 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
     :class:`AdamWState` each (:func:`adamw_state`); t is each tensor's own count, on the device, so that a recorded step can be
     replayed.  States in 8 bits: four bits of exponent below the largest of 128 elements, with three bits of mantissa for m and four
     for sqrt(v), which is never rounded down to 0; the step that makes them uses them unrounded.  A group that holds an infinity
-    or a NaN is NaN from the next step on.  ``lr``: a number, or one fp32 on the device.  The tensors must not overlap: one that is
+    or a NaN is NaN from the next step on.  ``rounding`` "random": each is kept as one of the two codes around it, the nearer one more
+    often, so that it is right in the mean over any number of steps: what a training run takes (``hiscache.AdamW`` does).  "nearest": right for
+    one step from given moments, but a moment that changes by less than half a code a step, as sqrt(v) does where b2 is near 1,
+    stays where it is.  (States in 32 bits are rounded as fp32 is.)  ``lr``: a number, or one fp32 on the device.  The tensors must not overlap: one that is
     named twice is refused."""
     params, grads, states = list(params), list(grads), list(states)
     if len(grads) != len(params) or len(states) != len(params):
@@ -2358,6 +2364,9 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
     b1, b2 = float(betas[0]), float(betas[1])
     if not (0 <= b1 < 1 and 0 <= b2 < 1 and eps >= 0):
         raise ValueError(f"betas must lie in [0, 1) and eps must not be negative, got {betas}, {eps}")
+    if rounding not in ("nearest", "random"):
+        raise ValueError(f"rounding must be nearest or random, got {rounding!r}")
+    bits_of_8 = 8 if rounding == "nearest" else 8 | _ADAMW_RANDOM
     if not params:
         return
     index = params[0].get_device()
@@ -2423,7 +2432,7 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
         first = host.buffer_info()[0]
         to = [first + 8 * n * k for k in range(8)]
         _check(lib.hc_adamw_step(n, to[0], to[1], _DTYPES[dtype], to[2], to[3], to[6] if bits8 else None,
-                                 to[6 + bits8] if copies else None, to[4], to[5], 8 if bits8 else 32, float(lr), _ptr(lr_dev),
+                                 to[6 + bits8] if copies else None, to[4], to[5], bits_of_8 if bits8 else 32, float(lr), _ptr(lr_dev),
                                  b1, b2, float(eps), float(weight_decay), stream), "hc_adamw_step")
     # the kernels wrote behind autograd's back: what was saved of a parameter is out of date
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

@@ -932,8 +932,18 @@ int hc_ring_lookup_packed(const int64_t *full2slot, int64_t n_full, const int64_
  * above them) or 4 bits of mantissa (sqrt(v), at least the smallest code where it
  * is not 0): the code.  E = 0: zeros.  E = 255: a group with an infinity or a NaN,
  * all of which reads back as NaN.
+ * state_bits 8 | HC_ADAMW_RANDOM: as 8, but a code is the next one towards zero, or, as
+ * often as the number lies nearer to it, the next one away from zero: with u the lower
+ * (m) or upper (sqrt(v)) half of the word below, away where the part of a code's step that
+ * is left is at least 1 - (u + 1/2) / 2^16; E is the largest exponent that these have.  Moments
+ * are kept in the mean; rounded half to even one that changes by less than half a code a step
+ * stays where it is, sqrt(v) at beta2 = 0.999 from the first dozens of steps on.
+ * The word of element i in step t: mix(i_lo + 0x9e3779b1 i_hi + key), key = mix(mix(t_lo) +
+ * 0x9e3779b1 t_hi + 0x243f6a88), mix(x): x = (x ^ x >> 16) 0x9e3779b1; x = (x ^ x >> 15) 0x85a308d3;
+ * x ^ x >> 16, in 32 bits.
  * No two of the tensors may overlap.  hc_adamw_moments: m and sqrt(v) of states of
  * 8 bits as numbers of dtype. */
+#define HC_ADAMW_RANDOM 256
 int hc_adamw_step(int count, void *const *param, const void *const *grad, int dtype, void *const *exp_avg,
                   void *const *exp_avg_sq, uint8_t *const *scale, float *const *master, int64_t *const *step,
                   const int64_t *numel, int state_bits, double lr, const float *lr_dev, double beta1, double beta2,
