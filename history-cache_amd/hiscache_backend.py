@@ -2310,13 +2310,23 @@ def adamw_state(param, bits=32, master=False):
 
 
 def _check_adamw_state(state, shape, index):
-    """Do the parts of a state fit a tensor of this shape on device ``index``?"""
+    """Do the parts of a state fit a tensor of this shape on device ``index``?  Their addresses (0: there is none) and the number of
+    elements."""
+    m, v, step, scale, master = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
+    # (by what the tensors are now: ``.data = ``, ``set_`` and ``resize_`` change one that stays the same object.  An address names
+    # its device as well; as many bytes in one piece at the same place are read as before whatever a view calls them.)
+    if scale is None and master is None:
+        facts = (m.data_ptr(), v.data_ptr(), step.data_ptr(), m.nbytes, v.nbytes, step.nbytes, m.is_contiguous(), v.is_contiguous(),
+                 step.is_contiguous(), shape, index)
+    else:
+        facts = (m.data_ptr(), v.data_ptr(), step.data_ptr(), m.nbytes, v.nbytes, step.nbytes, m.is_contiguous(), v.is_contiguous(),
+                 step.is_contiguous(), shape, index,
+                 None if scale is None else (scale.data_ptr(), scale.nbytes, scale.is_contiguous()),
+                 None if master is None else (master.data_ptr(), master.nbytes, master.is_contiguous()))
     known = state._checked
-    if (known is not None and known[0] is state.exp_avg and known[1] is state.exp_avg_sq and known[2] is state.step
-            and known[3] is state.scale and known[4] is state.master and known[5] == shape and known[6] == index):
-        return
-    parts = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
-    m, v, step, scale, master = parts
+    if known is not None and known[0] == facts:
+        return known[1]
+    parts = m, v, step, scale, master
     bits8 = scale is not None
     want = torch.uint8 if bits8 else torch.float32
     numel = math.prod(shape)
@@ -2332,7 +2342,11 @@ def _check_adamw_state(state, shape, index):
         if t is not None and (not t.is_cuda or t.get_device() != index or not t.is_contiguous() or t.is_neg()
                               or t._is_zerotensor()):
             raise ValueError("a state's parts must be contiguous and lie on the parameter's device")
-    state._checked = *parts, shape, index
+        if t is not None and t.untyped_storage().nbytes() < t.storage_offset() * t.element_size() + t.nbytes:
+            raise ValueError("a state's parts must lie in memory")
+    at = *[0 if t is None else t.data_ptr() for t in parts], numel
+    state._checked = facts, at
+    return at
 
 
 def _pointers(tensors):
@@ -2372,28 +2386,30 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
     index = params[0].get_device()
     # (a step of a few small tensors is the host's: what can be asked of all tensors is, in lists; a tensor of its own is looked at
     # only where an answer is not the usual one)
+    n = len(params)
     dtypes = [p.dtype for p in params]
     shapes = [p.shape for p in params]
-    if (index < 0 or [g.dtype for g in grads] != dtypes or [g.shape for g in grads] != shapes
-            or [p.get_device() for p in params].count(index) != len(params)
-            or [g.get_device() for g in grads].count(index) != len(params)
-            or False in [p.is_contiguous() for p in params] or True in [p.is_neg() for p in params]
-            or [g.layout for g in grads].count(torch.strided) != len(params)):
-        _adamw_refuse(params, grads)
-    if False in [g.is_contiguous() for g in grads] or True in [g.is_neg() for g in grads]:
-        grads = [_operand(g.contiguous(), "grad") for g in grads]
-    numels, at, of_g = [p.numel() for p in params], [p.data_ptr() for p in params], [g.data_ptr() for g in grads]
+    try:
+        if (index < 0 or [g.dtype for g in grads] != dtypes or [g.shape for g in grads] != shapes
+                or [p.get_device() for p in params].count(index) != n or [g.get_device() for g in grads].count(index) != n
+                or False in [p.is_contiguous() for p in params] or True in [p.is_neg() for p in params]):
+            _adamw_refuse(params, grads)
+        if False in [g.is_contiguous() for g in grads] or True in [g.is_neg() for g in grads]:
+            grads = [_operand(g.contiguous(), "grad") for g in grads]
+        at, of_g = [p.data_ptr() for p in params], [g.data_ptr() for g in grads]
+    except RuntimeError:
+        _adamw_refuse(params, grads)                      # (a tensor that has no such thing)
+        raise
     if 0 in at or 0 in of_g:                              # empty tensors, and zeros that were never written
-        if 0 in [a for a, n in zip(at, numels) if n]:
+        if 0 in [a for a, p in zip(at, params) if p.numel()]:
             raise ValueError("a parameter must lie in memory")
         grads = [g.clone() if g._is_zerotensor() else g for g in grads]
         of_g = [g.data_ptr() for g in grads]
-    if len(set(at)) < len(at) and len({a for a, n in zip(at, numels) if n}) < len([n for n in numels if n]):
+    if len(set(at)) < n and len({a for a in at if a}) < n - at.count(0):
         raise ValueError("a parameter is named twice")
     if len({id(s.step) for s in states}) < len(states):
         raise ValueError("a state goes with one parameter")
-    for state, shape in zip(states, shapes):
-        _check_adamw_state(state, shape, index)
+    of_states = [_check_adamw_state(state, shape, index) for state, shape in zip(states, shapes)]
     kinds = [(dtype, state.scale is not None, state.master is not None) for dtype, state in zip(dtypes, states)]
     _together(params[0])
     if forward_ad._current_level >= 0:
@@ -2408,26 +2424,24 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
         else:
             lr = lr.item()
     lib, stream = load_library(), _stream_of_device(index)
-    for kind in set(kinds):
+    each = set(kinds)
+    for kind in each:
         dtype, bits8, copies = kind
         if copies and dtype is torch.float32:
             raise ValueError("a parameter in fp32 has no other copy in fp32")
         if dtype not in _DTYPES:
             _float_dtype(params[kinds.index(kind)], "param")
-    for kind in set(kinds):
+    for kind in each:
         dtype, bits8, copies = kind
-        mine = range(len(kinds)) if kinds.count(kind) == len(kinds) else [i for i, k in enumerate(kinds) if k == kind]
-        n, ss = len(mine), [states[i] for i in mine]
-        words = [at[i] for i in mine]
-        words += [of_g[i] for i in mine]
-        words += [s.exp_avg.data_ptr() for s in ss]
-        words += [s.exp_avg_sq.data_ptr() for s in ss]
-        words += [s.step.data_ptr() for s in ss]
-        words += [numels[i] for i in mine]
+        words, theirs, mine = at, of_g, of_states
+        if len(each) > 1:
+            words, theirs, mine = zip(*[w for w, k in zip(zip(at, of_g, of_states), kinds) if k == kind])
+        m, v, step, scale, master, numels = zip(*mine)
+        n, words = len(mine), [*words, *theirs, *m, *v, *step, *numels]
         if bits8:
-            words += [s.scale.data_ptr() for s in ss]
+            words += scale
         if copies:
-            words += [s.master.data_ptr() for s in ss]
+            words += master
         host = array.array("q", words)                    # the arrays of the call one after the other
         first = host.buffer_info()[0]
         to = [first + 8 * n * k for k in range(8)]

@@ -1,0 +1,70 @@
+"""What a call looks at of the tensors behind its handles: those that they hold now, not those that an earlier call saw."""
+import pytest
+import torch
+
+import hiscache_backend as be
+
+
+class OnDevice:
+    """A tensor of the host that says it lies on a GPU."""
+    is_cuda = True
+    index = 0
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return self.index
+
+
+def state(shape, bits=32, master=False):
+    made = be.adamw_state(torch.zeros(shape, dtype=torch.bfloat16 if master else torch.float32), bits, master)
+    parts = [getattr(made, k) for k in ("exp_avg", "exp_avg_sq", "step", "scale", "master")]
+    return be.AdamWState(*[None if t is None else OnDevice(t) for t in parts])
+
+
+CHANGES = {
+    "smaller": lambda t: t[:1].clone(), "narrower": lambda t: t.to(torch.int16), "of another type": lambda t: t.to(torch.int32),
+    "expanded": lambda t: t.new_zeros(1).expand(t.shape), "in steps": lambda t: t.new_zeros(*t.shape[:-1], 2 * t.shape[-1])[..., ::2],
+    "reshaped": lambda t: t.new_zeros(t.numel() + 1),
+}
+
+
+@pytest.mark.parametrize("part", ("exp_avg", "exp_avg_sq", "step", "scale", "master"))
+@pytest.mark.parametrize("change", sorted(CHANGES))
+def test_a_state_that_changed_behind_its_object_is_looked_at_again(part, change):
+    shape = torch.Size([256])
+    s = state(shape, 8, True)
+    at = be._check_adamw_state(s, shape, 0)
+    assert be._check_adamw_state(s, shape, 0) == at and at[0] == s.exp_avg.data_ptr()
+    t = getattr(s, part)
+    t.t.data = CHANGES[change](t.t)
+    with pytest.raises(ValueError):
+        be._check_adamw_state(s, shape, 0)
+
+
+def test_a_state_elsewhere_or_without_memory():
+    shape = torch.Size([64])
+    s = state(shape)
+    at = be._check_adamw_state(s, shape, 0)
+    new = torch.ones(64)
+    s.exp_avg.t.data = new                                   # the same kind at another place: its address is taken
+    assert be._check_adamw_state(s, shape, 0) == (new.data_ptr(), *at[1:])
+    s.exp_avg.t.data, s.exp_avg.index = torch.ones(64), -1   # (a device's address is no host's)
+    with pytest.raises(ValueError):
+        be._check_adamw_state(s, shape, 0)
+    s = state(shape)
+    be._check_adamw_state(s, shape, 0)
+    s.exp_avg_sq.t.untyped_storage().resize_(0)
+    with pytest.raises(ValueError):
+        be._check_adamw_state(s, shape, 0)
+    s = state(shape)
+    be._check_adamw_state(s, shape, 0)
+    s.exp_avg.t.resize_(32)
+    with pytest.raises(ValueError):
+        be._check_adamw_state(s, shape, 0)
+    with pytest.raises(ValueError):
+        be._check_adamw_state(state(shape), shape, 1)
