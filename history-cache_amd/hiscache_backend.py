@@ -1716,6 +1716,13 @@ def _operand(t, name, dtype=None):
     return t.clone() if t._is_zerotensor() else t
 
 
+# A handle's tensors are checked once and then only asked where they lie, in how many bytes and whether in one piece: ``.data = ``,
+# ``set_`` and ``resize_`` change a tensor that stays the same object.  (An address names its device as well.)
+def _in_memory(t):
+    """Does all of a contiguous tensor lie in its storage?"""
+    return t.untyped_storage().nbytes() >= t.storage_offset() * t.element_size() + t.nbytes
+
+
 def _arriving(g):
     """A gradient as the kernels read it, packed."""
     if forward_ad._current_level >= 0:
@@ -1968,7 +1975,8 @@ def _keep_places(ctx, places):
 
 def _versions(slot, offset):
     # (a tensor made in inference mode counts none, and may not be changed in place outside it)
-    return None if slot.is_inference() else slot._version, None if offset.is_inference() else offset._version
+    return (None if slot.is_inference() else slot._version, None if offset.is_inference() else offset._version, slot.data_ptr(),
+            offset.data_ptr())
 
 
 def _kept_places(ctx):
@@ -1983,13 +1991,14 @@ def _places(order):
     if not isinstance(order, ExpertOrder):
         raise TypeError("order must be an ExpertOrder")
     known, slot, offset, n, top_k, E = order._checked, order.slot, order.offset, order.rows, order.top_k, order.experts
-    if (known is not None and known[0] is slot and known[1] is offset and known[2] == n and known[3] == top_k and known[4] == E):
-        return known
+    facts = (slot.data_ptr(), slot.nbytes, slot.is_contiguous(), offset.data_ptr(), offset.nbytes, offset.is_contiguous(), n, top_k, E)
+    if known == facts:
+        return slot, offset, n, top_k, E
     if (slot.dtype != torch.int32 or offset.dtype != torch.int64 or slot.numel() != n * top_k or offset.numel() != E + 1
-            or not slot.is_contiguous() or not offset.is_contiguous()):
+            or not slot.is_contiguous() or not offset.is_contiguous() or not _in_memory(slot) or not _in_memory(offset)):
         raise ValueError(f"the order must hold {n * top_k} places (slot, int32) and {E + 1} offsets (int64), both contiguous")
-    order._checked = slot, offset, n, top_k, E
-    return order._checked
+    order._checked = facts
+    return slot, offset, n, top_k, E
 
 
 def _check_order(order):
@@ -2142,9 +2151,9 @@ def _pack_arguments(x, name, group):
 def _check_kept(kept, halves):
     """Rows and columns of what :func:`pack_rows` (``halves`` 1) or :func:`gated_pack` (2) kept, if it is whole."""
     codes, scale, group, dtype, known = kept.codes, kept.scale, kept.group, kept.dtype, kept._checked
-    if (known is not None and known[0] is codes and known[1] is scale and known[2] == group and known[3] is dtype
-            and known[4] == halves):
-        return known[5]
+    facts = _kept_facts(kept, halves)
+    if known is not None and known[0] == facts:
+        return known[1]
     if codes.dim() != 2 or scale.dim() != 2 or group not in (32, 64, 128) or codes.shape[1] < 1 or codes.shape[1] % halves:
         raise ValueError("codes must be [n, columns], scale [n, groups], a group 32, 64 or 128 columns")
     n, F = codes.shape[0], codes.shape[1] // halves
@@ -2152,10 +2161,16 @@ def _check_kept(kept, halves):
         raise ValueError("the scales do not fit the codes" + (": were these rows kept by gated_pack?" if halves == 1 else
                                                               ": rows [n, 2 F] that gated_pack kept"))
     if (codes.dtype != torch.int8 or scale.dtype != torch.float32 or not codes.is_contiguous() or not scale.is_contiguous()
-            or dtype not in _DTYPES):
+            or dtype not in _DTYPES or not _in_memory(codes) or not _in_memory(scale)):
         raise ValueError("codes must be int8 and scale float32, both contiguous, dtype float32, float16 or bfloat16")
-    kept._checked = codes, scale, group, dtype, halves, (n, F)
+    kept._checked = facts, (n, F)
     return n, F
+
+
+def _kept_facts(kept, halves):
+    codes, scale = kept.codes, kept.scale
+    return (codes.data_ptr(), codes.shape, codes.is_contiguous(), scale.data_ptr(), scale.nbytes, scale.is_contiguous(), kept.group,
+            kept.dtype, halves)
 
 
 def pack_rows(x, group=64):
@@ -2174,7 +2189,7 @@ def pack_rows(x, group=64):
 
 def _whole(kept, halves, n, F):
     """``kept``, which has just been made: it need not be checked."""
-    kept._checked = kept.codes, kept.scale, kept.group, kept.dtype, halves, (n, F)
+    kept._checked = _kept_facts(kept, halves), (n, F)
     return kept
 
 
@@ -2313,8 +2328,6 @@ def _check_adamw_state(state, shape, index):
     """Do the parts of a state fit a tensor of this shape on device ``index``?  Their addresses (0: there is none) and the number of
     elements."""
     m, v, step, scale, master = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
-    # (by what the tensors are now: ``.data = ``, ``set_`` and ``resize_`` change one that stays the same object.  An address names
-    # its device as well; as many bytes in one piece at the same place are read as before whatever a view calls them.)
     if scale is None and master is None:
         facts = (m.data_ptr(), v.data_ptr(), step.data_ptr(), m.nbytes, v.nbytes, step.nbytes, m.is_contiguous(), v.is_contiguous(),
                  step.is_contiguous(), shape, index)
@@ -2342,7 +2355,7 @@ def _check_adamw_state(state, shape, index):
         if t is not None and (not t.is_cuda or t.get_device() != index or not t.is_contiguous() or t.is_neg()
                               or t._is_zerotensor()):
             raise ValueError("a state's parts must be contiguous and lie on the parameter's device")
-        if t is not None and t.untyped_storage().nbytes() < t.storage_offset() * t.element_size() + t.nbytes:
+        if t is not None and not _in_memory(t):
             raise ValueError("a state's parts must lie in memory")
     at = *[0 if t is None else t.data_ptr() for t in parts], numel
     state._checked = facts, at

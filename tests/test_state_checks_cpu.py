@@ -68,3 +68,50 @@ def test_a_state_elsewhere_or_without_memory():
         be._check_adamw_state(s, shape, 0)
     with pytest.raises(ValueError):
         be._check_adamw_state(state(shape), shape, 1)
+
+
+@pytest.mark.parametrize("part", ("codes", "scale"))
+@pytest.mark.parametrize("change", sorted(CHANGES))
+def test_packed_rows_that_changed_behind_their_object_are_looked_at_again(part, change):
+    kept = be.PackedRows(torch.zeros(6, 64, dtype=torch.int8), torch.zeros(6, 2), 32, torch.float32)
+    assert be._check_kept(kept, 1) == be._check_kept(kept, 1) == (6, 64)
+    t = getattr(kept, part)
+    t.data = CHANGES[change](t)
+    with pytest.raises(ValueError):
+        be._check_kept(kept, 1)
+    kept = be.PackedRows(torch.zeros(6, 64, dtype=torch.int8), torch.zeros(6, 2), 32, torch.float32)
+    be._check_kept(kept, 1)
+    getattr(kept, part).untyped_storage().resize_(0)
+    with pytest.raises(ValueError):
+        be._check_kept(kept, 1)
+
+
+@pytest.mark.parametrize("part", ("slot", "offset"))
+@pytest.mark.parametrize("change", sorted(CHANGES))
+def test_an_order_that_changed_behind_its_object_is_looked_at_again(part, change):
+    def make():
+        return be.ExpertOrder(torch.zeros(12, dtype=torch.int32), torch.zeros(12, dtype=torch.int32), torch.zeros(5, dtype=torch.int64),
+                              6, 2, 4)
+    order = make()
+    assert be._places(order)[2:] == be._places(order)[2:] == (6, 2, 4)
+    t = getattr(order, part)
+    t.data = t.to(torch.int16) if change == "of another type" else CHANGES[change](t)
+    with pytest.raises(ValueError):
+        be._places(order)
+    order = make()
+    be._places(order)
+    getattr(order, part).untyped_storage().resize_(0)
+    with pytest.raises(ValueError):
+        be._places(order)
+
+
+@pytest.mark.parametrize("part", (0, 1))
+def test_an_order_that_changed_between_forward_and_backward_is_noticed(part):
+    class Node:
+        pass
+    node, places = Node(), (torch.zeros(12, dtype=torch.int32), torch.zeros(5, dtype=torch.int64), 6, 2, 4)
+    be._keep_places(node, places)
+    assert be._kept_places(node) == places
+    places[part].data = places[part][:1].clone()
+    with pytest.raises(RuntimeError, match="modified"):
+        be._kept_places(node)
