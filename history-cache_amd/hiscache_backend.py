@@ -2383,8 +2383,9 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
     or a NaN is NaN from the next step on.  ``rounding`` "random": each is kept as one of the two codes around it, the nearer one more
     often, so that it is right in the mean over any number of steps: what a training run takes (``hiscache.AdamW`` does).  "nearest": right for
     one step from given moments, but a moment that changes by less than half a code a step, as sqrt(v) does where b2 is near 1,
-    stays where it is.  (States in 32 bits are rounded as fp32 is.)  ``lr``: a number, or one fp32 on the device.  The tensors must not overlap: one that is
-    named twice is refused."""
+    stays where it is.  (States in 32 bits are rounded as fp32 is.)  ``lr``: a number, or one fp32 on the
+    device.  The tensors must not overlap: a parameter or a part of a state that is named twice is refused, as any two with one
+    address are."""
     params, grads, states = list(params), list(grads), list(states)
     if len(grads) != len(params) or len(states) != len(params):
         raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(states)} states")
@@ -2418,11 +2419,8 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
             raise ValueError("a parameter must lie in memory")
         grads = [g.clone() if g._is_zerotensor() else g for g in grads]
         of_g = [g.data_ptr() for g in grads]
-    if len(set(at)) < n and len({a for a in at if a}) < n - at.count(0):
-        raise ValueError("a parameter is named twice")
-    if len({id(s.step) for s in states}) < len(states):
-        raise ValueError("a state goes with one parameter")
     of_states = [_check_adamw_state(state, shape, index) for state, shape in zip(states, shapes)]
+    _written_once(at, of_states)
     kinds = [(dtype, state.scale is not None, state.master is not None) for dtype, state in zip(dtypes, states)]
     _together(params[0])
     if forward_ad._current_level >= 0:
@@ -2463,6 +2461,18 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
                                  b1, b2, float(eps), float(weight_decay), stream), "hc_adamw_step")
     # the kernels wrote behind autograd's back: what was saved of a parameter is out of date
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+
+
+def _written_once(at, of_states):
+    """Does every parameter and every part of a state (their addresses; 0: there is none) lie in memory of its own?"""
+    m, v, step, scale, master, _ = zip(*of_states)
+    every = [*at, *m, *v, *step, *scale, *master]
+    seen = set(every)
+    if len(seen) - (0 in seen) < len(every) - every.count(0):
+        params, held = [a for a in at if a], [a for a in every[len(at):] if a]
+        raise ValueError("a parameter is named twice" if len(set(params)) < len(params) else
+                         "a state goes with one parameter, and so does each of its parts" if len(set(held)) < len(held) else
+                         "a parameter is no part of a state")
 
 
 def _adamw_refuse(params, grads):

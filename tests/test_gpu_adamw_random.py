@@ -137,3 +137,22 @@ def test_places_beyond_32_bits():
     for x, bits, got, row in ((g[-tail:].float(), 3, s.exp_avg, 0), (g[-tail:].float().abs(), 4, s.exp_avg_sq, 1)):
         code, E, _ = hold(x, bits, w)
         assert torch.equal(got[-tail:], code) and torch.equal(s.scale[row, -E.numel():], E)
+
+
+def test_a_part_of_a_state_goes_with_one_parameter():
+    """Two states with one moment, one scale, one copy or two views of one count: refused before anything is written."""
+    ps = [torch.zeros(300, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    gs = [torch.ones_like(p) for p in ps]
+    for part in ("exp_avg", "exp_avg_sq", "step", "scale", "master"):
+        a, b = (be.adamw_state(p, 8, True) for p in ps)
+        shared = getattr(a, part)
+        setattr(b, part, shared.view(shared.shape))
+        with pytest.raises(ValueError, match="one parameter"):
+            be.adamw_step(ps, gs, [a, b])
+        assert not bool(a.step.any()) and not bool(b.step.any()) and not bool(a.exp_avg.any())
+    q = torch.zeros(300, device=DEV)
+    s = be.adamw_state(q)
+    with pytest.raises(ValueError, match="part of a state"):
+        be.adamw_step([q], [q + 1], [be.AdamWState(s.exp_avg, q.view(300), s.step)])
+    none = [torch.zeros(0, device=DEV) for _ in range(2)]
+    be.adamw_step(none, none, [be.adamw_state(p) for p in none])

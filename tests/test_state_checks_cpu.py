@@ -115,3 +115,18 @@ def test_an_order_that_changed_between_forward_and_backward_is_noticed(part):
     places[part].data = places[part][:1].clone()
     with pytest.raises(RuntimeError, match="modified"):
         be._kept_places(node)
+
+
+def test_parts_of_states_that_two_parameters_would_share():
+    a, b = (0x1000, 0x2000, 0x3000, 0, 0, 8), (0x4000, 0x5000, 0x6000, 0x7000, 0x8000, 8)
+    be._written_once([0x9000, 0xA000], [a, b])
+    be._written_once([0, 0], [(0, 0, 0x3000, 0, 0, 0), (0, 0, 0x6000, 0, 0, 0)])           # empty tensors lie nowhere
+    for i in range(5):
+        shared = list(b)
+        shared[i] = 0x3000
+        with pytest.raises(ValueError, match="one parameter"):
+            be._written_once([0x9000, 0xA000], [a, tuple(shared)])
+    with pytest.raises(ValueError, match="one parameter"):
+        be._written_once([0x9000], [(0x1000, 0x1000, 0x3000, 0, 0, 8)])
+    with pytest.raises(ValueError, match="part of a state"):
+        be._written_once([0x9000, 0x8000], [a, b])
