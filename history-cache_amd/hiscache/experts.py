@@ -21,7 +21,7 @@ class ExpertMLP(torch.nn.Module):
     score, num_group, top_group, scale: the router's (``hiscache_backend.route_rows``).  ``balance``: experts are chosen by score + bias,
     where ``balance_bias`` (a buffer, zeros at first, fp32 whatever the module is cast to) rises for experts that had too few rows
     and falls for those that had too many by every :meth:`balance_step`, as it were a loss on their load that does not
-    disturb the gradients."""
+    disturb the gradients.  Every row of x counts, one that only pads a batch too unless ``allowed`` closes all experts to it."""
 
     def __init__(self, channels, hidden, num_expert, top_k=2, normalize=True, group=64, device=None, dtype=None, score="softmax",
                  num_group=1, top_group=1, scale=1.0, balance=False):
@@ -37,7 +37,9 @@ class ExpertMLP(torch.nn.Module):
         self.score, self.num_group, self.top_group, self.scale = score, num_group, top_group, scale
         bias = torch.zeros(num_expert, device=device, dtype=torch.float32) if balance else None
         self.register_buffer("balance_bias", bias)
-        self._offset = None                               # of the last training pass: the experts' loads
+        # of the last training pass: the experts' loads, where a pass that is recorded and replayed leaves them as well
+        self.register_buffer("_offset", torch.zeros(num_expert + 1, device=device, dtype=torch.int64) if balance else None,
+                             persistent=False)
         # the router's logits are fp32 whatever the rows are, under autocast and in a module cast to half precision as well: near-ties
         # decide where a row goes
         self.router = torch.nn.Parameter(torch.empty(num_expert, channels, device=device, dtype=torch.float32))
@@ -49,6 +51,9 @@ class ExpertMLP(torch.nn.Module):
         with torch.no_grad():
             for w, fan in ((self.router, self.channels), (self.w_in, self.channels), (self.w_out, self.hidden)):
                 w.uniform_(-1 / math.sqrt(fan), 1 / math.sqrt(fan))
+            if self.balance_bias is not None:
+                self.balance_bias.zero_()
+                self._offset.zero_()
 
     def _apply(self, fn, recurse=True):
         bias = self.balance_bias
@@ -61,12 +66,12 @@ class ExpertMLP(torch.nn.Module):
     @torch.no_grad()
     def balance_step(self, rate=1e-3):
         """Moves the bias of every expert by ``rate`` towards an even load, by the rows that each had in the last training pass
-        of :meth:`forward` that asked the router; nothing happens before the first.  Once a step, after the backward pass."""
+        of :meth:`forward` that asked the router, be it a replayed one; nothing happens before the first.  Once a step, after
+        the backward pass; it may be recorded itself."""
         if self.balance_bias is None:
             raise RuntimeError("this layer has no bias for balance: ExpertMLP(..., balance=True)")
-        if self._offset is not None:
-            load = (self._offset[1:] - self._offset[:-1]).float()
-            self.balance_bias.add_(torch.sign(load.mean() - load), alpha=rate)
+        load = (self._offset[1:] - self._offset[:-1]).float()
+        self.balance_bias.add_(torch.sign(load.mean() - load), alpha=rate)
 
     def route(self, x, allowed=None):
         """The router's choice for the rows of x: (expert int64 [n, top_k], weight fp32 [n, top_k]).  ``allowed`` (bool
@@ -96,7 +101,7 @@ class ExpertMLP(torch.nn.Module):
             expert, weight = self.route(x, allowed)
         order = be.expert_order(expert, self.num_expert)
         if routed and self.balance_bias is not None and self.training:
-            self._offset = order.offset
+            self._offset.copy_(order.offset)
         y = be.gated_experts(be.rows_to_experts(x, order), self.w_in, self.w_out, order.offset, self.group)
         return be.rows_from_experts(y, order, weight)
 

@@ -1,0 +1,87 @@
+"""The bias that loads experts evenly, moved by the loads of the last pass: an eager one, or a recorded one that is replayed."""
+import copy
+
+import pytest
+import torch
+
+import hiscache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def loads(layer, x):
+    expert, _ = layer.route(x)
+    return torch.bincount(expert.view(-1), minlength=layer.num_expert).float()
+
+
+def moved(load, rate):
+    return rate * torch.sign(load.mean() - load)
+
+
+def test_loads_of_the_pass_that_was_replayed_last():
+    """Two recordings of one layer, as for batches of two shapes: each replay is what the next step outside goes by."""
+    torch.manual_seed(0)
+    layer = hiscache.ExpertMLP(32, 32, 8, 2, score="sigmoid", balance=True, device=DEV).train()
+    inputs = [torch.randn(n, 32, device=DEV) for n in (200, 77)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for x in inputs:
+            layer(x).sum().backward()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in inputs]
+    for graph, x in zip(graphs, inputs):
+        layer.zero_grad(set_to_none=True)
+        with torch.cuda.graph(graph):
+            layer(x).sum().backward()
+    for i in (0, 1, 0, 0, 1, 0):
+        graphs[i].replay()
+        load, bias = loads(layer, inputs[i]), layer.balance_bias.clone()
+        assert float(load.sum()) == 2 * inputs[i].shape[0]
+        layer.balance_step(0.01)
+        assert torch.equal(layer.balance_bias, bias + moved(load, 0.01))
+        inputs[i].copy_(torch.randn_like(inputs[i]))
+    # an eager pass comes next, an evaluation and a choice from outside do not count
+    x = torch.randn(50, 32, device=DEV)
+    layer(x).sum().backward()
+    load = loads(layer, x)
+    layer.eval()(inputs[0])
+    layer.train()(inputs[1], expert=torch.zeros(77, dtype=torch.int64, device=DEV))
+    bias = layer.balance_bias.clone()
+    layer.balance_step(0.5)
+    assert torch.equal(layer.balance_bias, bias + moved(load, 0.5))
+
+
+def test_the_loads_go_where_the_layer_goes():
+    torch.manual_seed(0)
+    layer = hiscache.ExpertMLP(32, 32, 8, 2, balance=True, device=DEV).train()
+    x = torch.randn(50, 32, device=DEV)
+    layer(x)
+    load = loads(layer, x)
+    assert sorted(k for k in layer.state_dict() if "w_" not in k) == ["balance_bias", "router"]
+    for other in (copy.deepcopy(layer), copy.deepcopy(layer).half(), copy.deepcopy(layer).cpu()):
+        other.balance_step(0.25)
+        assert other.balance_bias.dtype == torch.float32 and torch.equal(other.balance_bias.to(DEV), moved(load, 0.25))
+    # a layer that is built without memory and then given some starts from zeros
+    late = hiscache.ExpertMLP(32, 32, 8, 2, balance=True, device="meta").to_empty(device=DEV)
+    late.reset_parameters()
+    late.balance_step()
+    assert not bool(late.balance_bias.any())
+    late.train()(x)
+    late.balance_step(1.0)
+    assert bool(late.balance_bias.any())
+
+
+def test_two_passes_before_one_backward():
+    """The loads are a copy: a second pass leaves what the first one's backward pass goes by."""
+    torch.manual_seed(0)
+    layer = hiscache.ExpertMLP(32, 32, 8, 2, score="sigmoid", balance=True, device=DEV).train()
+    x, y = torch.randn(60, 32, device=DEV), torch.randn(33, 32, device=DEV)
+    layer(x).square().sum().backward()
+    layer(y).square().sum().backward()
+    want = [p.grad.clone() for p in layer.parameters()]
+    layer.zero_grad(set_to_none=True)
+    (layer(x).square().sum() + layer(y).square().sum()).backward()
+    for p, g in zip(layer.parameters(), want):
+        assert torch.allclose(p.grad, g, rtol=1e-5, atol=1e-6 * float(g.abs().max()))
