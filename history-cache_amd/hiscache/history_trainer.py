@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from .dataset import ProcessedDataset
+from .experts import ExpertMLP
 from .history_cache import HistoryCache
 from .history_model import HistoryRGCN, get_model
 from .optimizer import AdamW
@@ -38,7 +39,8 @@ class HistoryTrainer:
 
     def __init__(self, config, dataset=None, fanout=None, batch_size=None, lr=None, num_epochs=None, eval_begin=None,
                  features_in_device_memory=False, hot_rows=0, cache_bytes=None, ring_rows=0, recorded=False,
-                 read_ahead=False, replay_slots=4, seed=0, model_factory=None, ring_dtype=torch.float16, state_bits=None):
+                 read_ahead=False, replay_slots=4, seed=0, model_factory=None, ring_dtype=torch.float16, state_bits=None,
+                 balance_rate=None):
         """``config``: the tree ``make_config`` builds (``dl.dataset.path`` names the dataset directory).  The
         loader's settings are arguments, with the configuration's own keys as defaults where it has them
         (``dl.sampler.train.batch_size`` / ``num_neighbors``, ``train.optimizer.lr``, ``train.train.num_epochs`` /
@@ -53,7 +55,8 @@ class HistoryTrainer:
         batch are recorded once per slot and replayed (see ``NeighborSampler``; the trainer never holds more than
         three batches, so four slots are safe; 0 switches it off).  ``model_factory(config, table)``: builds
         the model instead of ``get_model`` (a relational model with its own node-type ranges, say).  ``state_bits`` 32 or 8:
-        the steps are ``hiscache.AdamW``'s, without decay, its moments in that many bits (default: torch's Adam)."""
+        the steps are ``hiscache.AdamW``'s, without decay, its moments in that many bits (default: torch's Adam).  ``balance_rate``: after
+        every step the model's ``ExpertMLP(balance=True)`` layers move their biases by that much (``balance_step``)."""
         self.config = config
         self.device = torch.device(config.dl.device)
         self.feat_mode = config.dl.loading.feat_mode
@@ -93,6 +96,7 @@ class HistoryTrainer:
             self.optimizer = torch.optim.Adam(self.model.parameters(), lr=lr, fused=True, capturable=self.recorded)
         else:
             self.optimizer = AdamW(self.model.parameters(), lr=lr, weight_decay=0.0, state_bits=state_bits)
+        self.balance_rate = balance_rate
         self.scheduler = None
         self.loss_fn = torch.nn.functional.nll_loss
         # every batch comes with the transposed view of its CSR; the relational layer also reads the view's edge slots
@@ -112,7 +116,7 @@ class HistoryTrainer:
                 self.splits[split] = torch.from_numpy(np.array(ds.split_idx(key))).to(self.device)
         self._generator = torch.Generator(device=self.device).manual_seed(seed)
         self._step = RecordedIteration(self.model, self.table, self.optimizer, self.num_layers,
-                                       loss_fn=self.loss_fn) if self.recorded else None
+                                       loss_fn=self.loss_fn, after_step=self._balance) if self.recorded else None
         self.glb_iter = 0
         self.prof = bool(_option(config, "dl.performance.prof", False))     # train() then runs the profiled epoch
         self.times = None
@@ -181,6 +185,12 @@ class HistoryTrainer:
             yield batch
             batch = nxt
 
+    def _balance(self):
+        if self.balance_rate:
+            for m in self.model.modules():
+                if isinstance(m, ExpertMLP) and m.balance_bias is not None:
+                    m.balance_step(self.balance_rate)
+
     @staticmethod
     def evaluator(y_pred, y_true):
         """Accuracy of the arg-max class (the evaluator of the node-classification datasets)."""
@@ -210,6 +220,7 @@ class HistoryTrainer:
                 loss = self.loss_fn(out, batch.y)
                 backward_on_this_thread(loss)
                 self.optimizer.step()
+                self._balance()
                 self.table.update_history(batch, self.glb_iter)
             if self.scheduler is not None:
                 self.scheduler.step()
@@ -256,6 +267,7 @@ class HistoryTrainer:
             backward_on_this_thread(loss)
             mark(row)
             self.optimizer.step()
+            self._balance()
             if self.scheduler is not None:
                 self.scheduler.step()
             mark(row)

@@ -43,10 +43,11 @@ class _Record:
 class RecordedIteration:
 
     def __init__(self, model, cache, optimizer, num_layers, loss_fn=None, step=1.125, round_to=256,
-                 max_records=16, with_view=True, record=True, read_ahead_slots=2):
+                 max_records=16, with_view=True, record=True, read_ahead_slots=2, after_step=None):
         self.model, self.cache, self.optimizer = model, cache, optimizer
         self.L = int(num_layers)
         self.loss_fn = loss_fn or torch.nn.functional.nll_loss
+        self.after_step = after_step or (lambda: None)     # called behind the optimizer's step, and recorded with it
         self.step = float(step)
         self.round_to = int(round_to)
         self.max_records = int(max_records)
@@ -202,6 +203,7 @@ class RecordedIteration:
         self.optimizer.zero_grad(set_to_none=True)
         backward_on_this_thread(loss)
         self.optimizer.step()
+        self.after_step()
         self.cache.update_history(b, None)
         return loss.detach()
 
@@ -246,6 +248,7 @@ class RecordedIteration:
             self.optimizer.zero_grad(set_to_none=True)
             backward_on_this_thread(loss)
             self.optimizer.step()
+            self.after_step()
             self.cache.update_history(b, glb_iter)
             return loss.detach()
         self._stage(r, batch, nnl, n_edges, self.cache.glb_iter, glb_iter, handle)

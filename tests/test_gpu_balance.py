@@ -1,6 +1,7 @@
 """The bias that loads experts evenly, moved by the loads of the last pass: an eager one, or a recorded one that is replayed."""
 import copy
 
+import numpy as np
 import pytest
 import torch
 
@@ -85,3 +86,48 @@ def test_two_passes_before_one_backward():
     (layer(x).square().sum() + layer(y).square().sum()).backward()
     for p, g in zip(layer.parameters(), want):
         assert torch.allclose(p.grad, g, rtol=1e-5, atol=1e-6 * float(g.abs().max()))
+
+
+class Net(torch.nn.Module):
+    def __init__(self, config, table):
+        super().__init__()
+        C = config.dl.dataset.num_classes
+        self.base = hiscache.get_model(config, table)
+        self.experts = hiscache.ExpertMLP(C, 32, 8, 2, score="sigmoid", balance=True)
+        self.fixed = hiscache.ExpertMLP(C, 32, 8, 2)
+
+    @property
+    def convs(self):
+        return self.base.convs
+
+    def forward(self, batch):
+        h = self.base(batch)
+        return (h + self.experts(h) + self.fixed(h)).log_softmax(1)
+
+
+@pytest.mark.parametrize("recorded", (False, True))
+def test_the_trainer_balances(tmp_path, recorded):
+    """After every step, replayed ones too: each moves an expert's bias by the rate, or not where its load is the mean."""
+    from test_gpu_trainer import dataset
+    L = 3
+    dataset(tmp_path, np.random.default_rng(9), Fin=32, C=4)
+    cfg = hiscache.make_config(32, 4, 64, L, method="grad", rate=0.6, staleness_thres=5, device=DEV, path=str(tmp_path))
+
+    def run(rate, epochs=2):
+        torch.manual_seed(7)
+        t = hiscache.HistoryTrainer(cfg, fanout=[4, 3, 2], batch_size=200, lr=1e-2, num_epochs=epochs, eval_begin=9, ring_rows=3000,
+                                    recorded=recorded, model_factory=Net, balance_rate=rate)
+        t.train()
+        return t
+
+    t = run(2.0 ** -10)
+    moves = t.model.experts.balance_bias * 2 ** 10
+    assert bool((moves == moves.round()).all()) and 0 < float(moves.abs().max()) <= t.glb_iter
+    if recorded:
+        assert t._step.replays > 10
+    # a few rows beside the mean or not: what one step would do is seen from the last loads
+    load = (t.model.experts._offset[1:] - t.model.experts._offset[:-1]).float()
+    before = t.model.experts.balance_bias.clone()
+    t._balance()
+    assert torch.equal(t.model.experts.balance_bias, before + moved(load, 2.0 ** -10))
+    assert not bool(run(None, 1).model.experts.balance_bias.any())
