@@ -14,9 +14,9 @@
 // is then gone through by L lanes, which hold the K + 1 largest of their share sorted in registers: a number's lowest bits make way for
 // the expert's index, and a new one moves into the list by one median a place.  What a lane has found gets its lost bits back, is
 // sorted by them and then the index, and put together with what the row's other lanes have.
-// Such a choice is right where nothing near stands against it.  c in fp32 is off by up to 2^-21: where neighbours in the list, or the last
-// open and the first closed group, are nearer than that and do not come from equal numbers, the wave decides the row again in fp64, all
-// lanes on it.  Where the first outside the list is near by the bits that were kept, it is counted how many are that near by all bits.
+// Such a choice is right where nothing near stands against it.  c in fp32 is off by up to 2^-22 and half a unit of |c|: where neighbours in
+// the list, or the last open and the first closed group (by the larger of the numbers that they are sums of), are nearer than twice that and
+// do not come from equal numbers, the wave decides the row again in fp64, all lanes on it.  Where the first outside the list is near by the bits that were kept, it is counted how many are that near by all bits.
 // Bound by those medians, K + 1 a logit, and the exponentials: 500 009 rows of 64 bf16 logits to four experts 46 us for 96 MB, with sorted
 // lists of fp64 keys 50 and with insertion into unsorted ones 106; 65 537 rows of 256 fp32 in groups to eight 49 us for 75 MB; eight such
 // rows 9.3, of which most is the way of some thousand instructions from memory.  A whole fp64 pass over every row: 125 and 173.
@@ -369,6 +369,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
   const bool by_four = a.per_group % 4 == 0;
   if (a.groups > 1) {
     float *rank = s_all + ROWS * a.stride + mine * a.rank_stride;
+    float size = 0.f;                                // of the summands, whose errors a sum has
     for (int g = 0; g < a.groups; ++g) {
       float first = RS_SHUT, second = RS_SHUT;
       const auto more = [&](float c) {
@@ -383,6 +384,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
       });
       rs_join_two<L>(first, second);
       near = near || first >= RS_MOST;               // (infinite, or no number)
+      size = fmaxf(size, fmaxf(rs_shut(first) ? 0.f : fabsf(first), rs_shut(second) ? 0.f : fabsf(second)));
       if (exact && !rs_shut(first)) {
         first = a.softmax ? rs_near_exp(first - top) : rs_near_sigma(first);
         second = rs_shut(second) ? second : a.softmax ? rs_near_exp(second - top) : rs_near_sigma(second);
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     least = hc_join<L>(least, [](float x, float y) { return fminf(x, y); });
     most = hc_join<L>(most, [](float x, float y) { return fmaxf(x, y); });
     // (scores below 2^-126 are 0 to the instructions)
-    const float off = exact ? 0x1p-15f * fmaxf(fabsf(least), 0x1p-100f) : 0x1p-19f * (1.f + fabsf(least));
+    const float off = exact ? 0x1p-15f * fmaxf(fabsf(least), 0x1p-100f) : 0x1p-19f * (1.f + size);
     near = near || (!rs_shut(most) && !(least - most > off));
   }
   // f for the row's open elements that this lane takes
