@@ -553,7 +553,11 @@ __global__ __launch_bounds__(HC_WAVE) void rs_forward(RsArgs a) {
     if (j >= a.k) continue;
     a.expert[r * a.k + j] = won[u];
     a.weight[r * a.k + j] = won[u] < 0 || of == 0.f ? 0.f : a.scale * (s[u] / of);
-    if (a.picked != nullptr) a.picked[r * a.k + j] = won[u] >= 0 && nothing ? -__builtin_inff() : p[u] < RS_LEAST ? RS_LEAST : p[u];
+    if (a.picked != nullptr) {
+      // (a chosen one need not be the infinity or NaN that makes all of its row's scores NaN)
+      const float kept = no_number ? __builtin_nanf("") : nothing ? -__builtin_inff() : p[u] < RS_LEAST ? RS_LEAST : p[u];
+      a.picked[r * a.k + j] = won[u] >= 0 ? kept : 0.f;
+    }
   }
 }
 

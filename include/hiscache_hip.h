@@ -818,7 +818,7 @@ int hc_route_rows_grad(const void *logits, int dtype, int64_t n, int64_t E, int6
  * where all chosen logits are below -700 (score 0: 700 below the row's largest).
  * A logit or a bias of -inf closes an expert (-1, weight 0, where fewer than top_k are open).
  * picked [n, top_k] (NULL: not kept): the chosen logits for the gradient, 0 where there is
- * none, -inf where normalised weights are 0.  num_group <= 64 divides E, top_k <=
+ * none, -inf where normalised weights are 0, NaN where a softmax is.  num_group <= 64 divides E, top_k <=
  * E / num_group * top_group, scale > 0; n L <= 2^32 - 64 for L = 2 lanes a row up to 64
  * experts, 8 up to 256, 32 above, and hc_route_rows' other limits (the gradient: all of them).
  * hc_route_scores_grad: grad_logits [n, E] (dtype) from grad_weight [n, top_k] and

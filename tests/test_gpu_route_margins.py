@@ -26,3 +26,33 @@ def test_groups_by_sums_of_large_numbers_of_both_signs(score, size, E, G):
     check(logits, 2, score=score, bias=bias, num_group=G, top_group=1)
     if G > 2:
         check(logits, 3, score=score, bias=bias, num_group=G, top_group=3)
+
+
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("bias", (False, True))
+@pytest.mark.parametrize("G,top", ((1, 1), (4, 2)))
+def test_gradient_of_a_softmax_that_is_no_number(normalize, bias, G, top):
+    """A row with an infinity or a NaN has no softmax: its weights are NaN, and what reaches its chosen logits is, too, whichever they are."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    logits = torch.randn(40, 32, generator=gen, device=DEV)
+    logits[:, 3] = -math.inf
+    logits[4, 20], logits[5, 21], logits[6, [9, 30]] = math.inf, math.nan, math.inf
+    bad = torch.zeros(40, dtype=torch.bool)
+    bad[4:7] = True
+    b = torch.randn(32, generator=gen, device=DEV) if bias else None
+    leaf = logits.clone().requires_grad_(True)
+    expert, weight = be.route_rows(leaf, 3, normalize=normalize, bias=b, num_group=G, top_group=top, scale=1.5)
+    weight.backward(torch.randn(40, 3, generator=gen, device=DEV))
+    assert torch.equal(torch.isnan(weight).any(1).cpu(), bad) and torch.equal(torch.isnan(weight).all(1).cpu(), bad)
+    at_chosen = leaf.grad.gather(1, expert.clamp(min=0))
+    assert torch.equal(torch.isnan(at_chosen).all(1).cpu(), bad) and torch.equal(torch.isnan(leaf.grad).any(1).cpu(), bad)
+    # the other rows as without those
+    clean = logits.clone()
+    clean[4:7] = 0.0
+    clean.requires_grad_(True)
+    torch.manual_seed(0)
+    g = torch.randn(40, 3, device=DEV)
+    leaf.grad = None
+    be.route_rows(leaf, 3, normalize=normalize, bias=b, num_group=G, top_group=top, scale=1.5)[1].backward(g)
+    be.route_rows(clean, 3, normalize=normalize, bias=b, num_group=G, top_group=top, scale=1.5)[1].backward(g)
+    assert torch.equal(leaf.grad[7:], clean.grad[7:]) and torch.equal(leaf.grad[:4], clean.grad[:4])
