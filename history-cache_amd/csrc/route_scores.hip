@@ -99,7 +99,8 @@ __device__ __forceinline__ void rs_choose_exactly(const RsArgs &a, int64_t r, in
   };
   for (int e = lane; e < a.E; e += HC_WAVE) {
     const float l = rs_logit(a, r * a.E + e);
-    key[e] = rt_masked(l) ? RS_CLOSED : rs_order(score(l) + (a.bias != nullptr ? (double)a.bias[e] : 0.0));
+    const float b = a.bias != nullptr ? a.bias[e] : 0.f;
+    key[e] = rt_masked(l) || rt_masked(b) ? RS_CLOSED : rs_order(score(l) + (double)b);
   }
   rt_in_order();
   uint64_t open = ~0ull;
@@ -235,7 +236,7 @@ __device__ __forceinline__ float rs_plain(float l) {
 }
 __device__ __forceinline__ float rs_choice(float l, float bias) {
   const float c = fminf(rs_near_sigma(l) + bias, RS_MOST);
-  return rt_masked(l) ? RS_SHUT : c;
+  return rt_masked(l) || rs_shut(bias) ? RS_SHUT : c;          // (beside a closed one's NaN, too)
 }
 
 // Rows r0 .. r0 + rows into LDS: c where the score is a logit's own and there is a bias, l otherwise.

@@ -1835,7 +1835,7 @@ def route_rows(logits, top_k, normalize=True, score="softmax", bias=None, num_gr
     expert to the row: where fewer than ``top_k`` are open the rest are -1 with weight 0.  A row with a NaN or +inf has NaN
     weights.  The gradient of the weights reaches ``logits``.  top_k <= 32.
 
-    ``score`` "sigmoid": the logistic function of each logit in place of the softmax (a NaN logit is chosen first).  ``bias``
+    ``score`` "sigmoid": the logistic function of each logit in place of the softmax (a NaN logit that is open is chosen first).  ``bias``
     (fp32 [E]): experts are chosen by score + bias, the larger in fp64, and weighted by the score alone; it has no gradient, and
     -inf closes an expert.  ``top_group`` < ``num_group`` <= 64: experts lie in ``num_group`` groups of as many neighbours, of
     which a row may take the ``top_group`` with the largest sum of two (score + bias) in them, of equal ones the lowest.

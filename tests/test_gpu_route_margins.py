@@ -56,3 +56,26 @@ def test_gradient_of_a_softmax_that_is_no_number(normalize, bias, G, top):
     be.route_rows(leaf, 3, normalize=normalize, bias=b, num_group=G, top_group=top, scale=1.5)[1].backward(g)
     be.route_rows(clean, 3, normalize=normalize, bias=b, num_group=G, top_group=top, scale=1.5)[1].backward(g)
     assert torch.equal(leaf.grad[7:], clean.grad[7:]) and torch.equal(leaf.grad[:4], clean.grad[:4])
+
+
+@pytest.mark.parametrize("score", ("sigmoid", "softmax"))
+@pytest.mark.parametrize("G,top", ((1, 1), (4, 3)))
+@pytest.mark.parametrize("n", (3, 3000))
+def test_a_bias_closes_an_expert_whatever_its_logit_is(score, G, top, n):
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    logits = torch.randn(n, 32, generator=gen, device=DEV)
+    bias = 0.1 * torch.randn(32, generator=gen, device=DEV)
+    closed = [0, 5, 8, 9, 10, 11, 12, 13, 14, 15]            # (of four groups one whole)
+    bias[closed] = -math.inf
+    for value in (math.nan, math.inf, torch.finfo(torch.float32).max, -math.inf, 1.0):
+        for where in ([0], [5], [9], [5, 9], [0, 5, 20], [31]):
+            l = logits.clone()
+            l[1::2, where] = value
+            expert, weight = be.route_rows(l, 6, score=score, bias=bias, num_group=G, top_group=top)
+            assert not bool(torch.isin(expert, torch.tensor(closed, device=DEV)).any()) and bool((expert >= 0).all())
+            still = [e for e in where if e not in closed]
+            if score == "sigmoid" and math.isnan(value):     # an open one comes first, and makes the row's shares NaN
+                assert all(expert[1::2, 0].eq(e).all() for e in still)
+                assert bool(torch.isnan(weight[1::2]).all()) == bool(still)
+            # rows without are as before
+            assert torch.equal(expert[::2], be.route_rows(logits, 6, score=score, bias=bias, num_group=G, top_group=top)[0][::2])
