@@ -25,8 +25,8 @@
 //
 // A block takes pieces of 2 048 elements of the tensors' concatenation, eight a lane; sixteen lanes share a group.  Every element is
 // read and written once, which bounds large calls: 50.3 M elements of fp32 (us and TB/s) with 8 bits 166 (4.9), 32 bits 278 (5.1), of
-// bf16 with 8 bits 104 (4.8), with a copy in fp32 168 (4.8), 32 bits 219 (5.0), with a copy 284 (5.0); rounded at random, fifteen operations an
-// element more, 164, 107 and 168.  torch's copy of 4 GiB reaches 4.8 TB/s, of 256 MiB 5.4.  Eight
+// bf16 with 8 bits 103 to 108 (4.8), with a copy in fp32 168 (4.8), 32 bits 219 (5.0), with a copy 284 (5.0); rounded at random, fifteen
+// operations an element more, the same.  torch's copy of 4 GiB reaches 4.8 TB/s, of 256 MiB 5.4.  Eight
 // small tensors take 6.6 us: their counts, the powers of the rates in 64 bits, a memory's latency for the elements and one for
 // the arrival.  Non-temporal stores: no difference.
 #include "packed_rows.h"
@@ -122,11 +122,12 @@ __device__ __forceinline__ uint32_t aw_round(uint32_t b, uint32_t random) {
 // The E of the group that AW_LANES lanes hold, and this lane's codes.
 template <int MAN, bool RANDOM>
 __device__ __forceinline__ uint32_t aw_encode(const float (&v)[PK_EACH], const uint32_t (&random)[PK_EACH], uint32_t (&w)[2]) {
-  uint32_t most = 0;
+  uint32_t most = 0, least = 0xffffffffu;    // (of magnitudes' bits; the least one's that is not 0, less 1)
 #pragma unroll
   for (int i = 0; i < PK_EACH; ++i) {
     uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
     if constexpr (RANDOM) b = aw_round<MAN, true>(b, random[i]);       // (which of them is the largest goes by what they become)
+    else least = b - 1u < least ? b - 1u : least;
     most = b > most ? b : most;
   }
   most = hc_join<AW_LANES>(most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
@@ -140,9 +141,22 @@ __device__ __forceinline__ uint32_t aw_encode(const float (&v)[PK_EACH], const u
       c[i] = (b & 0x80000000u) | (b << 4 & 0x7fffffffu);
     } else {
       // (a root that is not 0 is above 2^-75)
-      const uint32_t least = __float_as_uint(v[i]) < 1u << 19 ? __float_as_uint(v[i]) : 1u << 19;
-      b = b > least ? b : least;
+      const uint32_t lowest = __float_as_uint(v[i]) < 1u << 19 ? __float_as_uint(v[i]) : 1u << 19;
+      b = b > lowest ? b : lowest;
       c[i] = aw_round<4, RANDOM>(b, random[i]) << 5;
+    }
+  }
+  if constexpr (!RANDOM) {
+    // Scaled down to below fp32's normal numbers one has been rounded before it is rounded to a code, and may have become a tie: those
+    // are taken in units of the smallest code instead, which are exact.
+    if (__any(E > 15u && least < ((E - 14u) << 23) - 1u)) {
+#pragma unroll
+      for (int i = 0; i < PK_EACH; ++i) {
+        const float u = __builtin_amdgcn_ldexpf(fabsf(v[i]), 141 + MAN - (int)E);
+        uint32_t code = (uint32_t)__builtin_rintf(u);
+        if (MAN == 4 && v[i] > 0.f && code == 0) code = 1;
+        if (u < (float)(1 << MAN)) c[i] = MAN == 3 ? (__float_as_uint(v[i]) & 0x80000000u) | code << 24 : code << 24;
+      }
     }
   }
 #pragma unroll

@@ -40,6 +40,12 @@ def hold(x, bits, word):
     if bits == 4:
         s = torch.maximum(s, torch.clamp(b, max=1 << shift))
     code = rounded(s) >> shift
+    if word is None:                                         # rounded once: below the normal codes in units of the smallest one
+        units = x.abs().double() * torch.exp2((141 + bits - E).double())
+        near = torch.round(units).long()
+        if bits == 4:
+            near = torch.where(x > 0, torch.clamp(near, min=1), near)
+        code = torch.where(units < 1 << bits, near, code)
     dead = (E == 0) | (E == 255)
     value = (code << shift).int().view(torch.float32).double() * torch.exp2((E - 15).double())
     value = torch.where(E == 0, 0.0, torch.where(E == 255, torch.nan, torch.where(x < 0, -value, value)))

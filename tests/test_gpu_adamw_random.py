@@ -156,3 +156,24 @@ def test_a_part_of_a_state_goes_with_one_parameter():
         be.adamw_step([q], [q + 1], [be.AdamWState(s.exp_avg, q.view(300), s.step)])
     none = [torch.zeros(0, device=DEV) for _ in range(2)]
     be.adamw_step(none, none, [be.adamw_state(p) for p in none])
+
+
+@pytest.mark.parametrize("most", (1.0, 2.0 ** 40, 2.0 ** -30))
+def test_small_codes_are_rounded_once(most):
+    """Numbers beside the middle between two of the smallest codes, nearer to it than fp32's smallest steps are where the largest of the group has
+    been scaled to the codes' own exponent: the side that they lie on counts, a tie is even."""
+    for bits in (3, 4):
+        unit = most * 2.0 ** (-14 - bits)
+        k = torch.arange(8, device=DEV).double() + 0.5
+        x = torch.cat([k * (1 + s * 2.0 ** -e) for e in (21, 22, 23) for s in (-1, 0, 1)] + [k * 0 + 0.25, k * 0, -k]).float() * unit
+        g = torch.zeros(128, device=DEV)
+        g[0], g[1:1 + x.numel()] = most, x
+        state = be.adamw_state(g, 8)
+        be.adamw_step([torch.zeros_like(g)], [g], [state], betas=(0.0, 0.0))
+        if bits == 3:
+            code = state.exp_avg[1:25].tolist()
+            assert code[:8] == [0, 1, 2, 3, 4, 5, 6, 7]      # just below the middle: down
+            assert code[8:16] == [0, 2, 2, 4, 4, 6, 6, 8] and code[16:] == [1, 2, 3, 4, 5, 6, 7, 8]
+            assert torch.equal(state.exp_avg, hold(g, 3, None)[0])
+        else:                                                # (b2 = 0: the root of the gradient's square)
+            assert torch.equal(state.exp_avg_sq, hold((g * g).double().sqrt().float(), 4, None)[0])
