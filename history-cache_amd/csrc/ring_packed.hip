@@ -1,28 +1,30 @@
 // Lookup in a ring table of embeddings held in 8 bits (packed_rows.h): slots of ids, and the hits' rows in fp32, code * scale.
 //
-// A block takes 16 rows, in large calls 64: its first lanes look a row up each (three reads that wait for one another), then all of its
-// lanes lie one after the other over the rows' columns.
+// A block takes 16 rows: its first lanes look a row up each (three reads that wait for one another), then all of its lanes lie one after
+// the other over the rows' columns.
 // Bound by memory where there are many: 1 000 003 ids, 400 000 of them hits of 256 columns, 264 us for 1.15 GB (4.4 TB/s; an id's map
 // entry, age, scales and codes lie in lines of their own, 0.25 GB more than is asked for; from a table in fp16 501 us), with ordinary
-// stores 291; 16 or 64 rows a block, four or eight pieces at once, or the next pieces read before the last are written: 258 to 264.
+// stores 291; four or eight pieces at once, or the next pieces read before the last are written: no difference.  64 rows a block in place of
+// 16 (with the calls in turn over four sets of ids): 281 against 266; 200 003 ids of 172 columns 36.5 against 35.4, 1 500 of 128 3.8 against 2.8.
 // 150 001 ids, half of them hits of 172 columns: 32 us (118 MB).  Few: 8 661 of 256 columns 5.4, 1 500 of 128 3.9 us, a launch and four
 // reads one after the other.
 #include "packed_rows.h"
 
 namespace {
 
-constexpr int RP_MOST_ROWS = 64;       // rows a block
+constexpr int RP_ROWS = 16;            // rows a block
+constexpr int RP_MOST_BLOCKS = 0xffffffffu / HC_BLOCK;
 constexpr int RP_AT_ONCE = 4;          // pieces that a lane reads before it writes the first
 constexpr int64_t RP_CACHE = 256 << 20;          // bytes of the last-level cache
 
 struct RpArgs {
   const int64_t *full2slot, *ids, *checkin, *now_dev, *n_valid_dev;
-  int64_t n_full, now, age_limit, capacity, n;
+  int64_t n_full, now, age_limit, capacity, n, first;
   const int8_t *codes;
   const float *scale;
   int64_t *slot_out;
   float *rows_out;
-  uint32_t F, groups, group, rows;
+  uint32_t F, groups, group;
 };
 
 __device__ __forceinline__ int64_t rp_find(const RpArgs &a, int64_t i) {
@@ -39,9 +41,9 @@ __device__ __forceinline__ int64_t rp_find(const RpArgs &a, int64_t i) {
 // any alignment.  NT: for rows that the last-level cache cannot hold until they are read.
 template <int V, bool NT>
 __global__ __launch_bounds__(HC_BLOCK) void rp_lookup(RpArgs a) {
-  __shared__ int64_t s_slot[RP_MOST_ROWS];
-  const int64_t row0 = (int64_t)blockIdx.x * a.rows;
-  const uint32_t rows = a.n - row0 < (int64_t)a.rows ? (uint32_t)(a.n - row0) : a.rows;
+  __shared__ int64_t s_slot[RP_ROWS];
+  const int64_t row0 = a.first + (int64_t)blockIdx.x * RP_ROWS;
+  const uint32_t rows = a.n - row0 < RP_ROWS ? (uint32_t)(a.n - row0) : RP_ROWS;
   if (threadIdx.x < rows) {
     const int64_t slot = rp_find(a, row0 + threadIdx.x);
     s_slot[threadIdx.x] = slot;
@@ -106,18 +108,21 @@ extern "C" int hc_ring_lookup_packed(const int64_t *full2slot, int64_t n_full, c
                                      const int8_t *codes, const float *scale, int64_t group, int64_t capacity, int64_t F,
                                      int64_t *slot_out, float *rows_out, int64_t n, void *stream) {
   HC_REQUIRE(n >= 0 && n_full >= 0 && capacity >= 0 && F > 0);
-  if ((group != 32 && group != 64 && group != 128) || F >= (1 << 30)) return HC_EUNSUPPORTED;
+  if ((group != 32 && group != 64 && group != 128) || F >= (1 << 30) || n >= (int64_t)1 << 40) return HC_EUNSUPPORTED;
   if (n == 0) return HC_OK;
   HC_REQUIRE(full2slot && ids && slot_out);
   HC_REQUIRE(rows_out == nullptr || (codes && scale));
-  RpArgs a{full2slot, ids, checkin, now_dev, n_valid_dev, n_full, now, age_limit, capacity, n, codes, scale, slot_out, rows_out,
-           (uint32_t)F, (uint32_t)((F + group - 1) / group), (uint32_t)group, 16};
-  a.rows = n >= 2048 * RP_MOST_ROWS ? RP_MOST_ROWS : 16;
-  const int64_t blocks = (n + a.rows - 1) / a.rows;
-  if (!hc_grid_ok(blocks)) return HC_EUNSUPPORTED;
+  RpArgs a{full2slot, ids, checkin, now_dev, n_valid_dev, n_full, now, age_limit, capacity, n, 0, codes, scale, slot_out, rows_out,
+           (uint32_t)F, (uint32_t)((F + group - 1) / group), (uint32_t)group};
   const bool whole = F % 4 == 0 && reinterpret_cast<uintptr_t>(codes) % 4 == 0 && reinterpret_cast<uintptr_t>(rows_out) % 16 == 0;
   const bool large = n * F * (int64_t)sizeof(float) > RP_CACHE;
   const auto kernel = whole ? (large ? rp_lookup<4, true> : rp_lookup<4, false>) : large ? rp_lookup<8, true> : rp_lookup<8, false>;
-  kernel<<<dim3((unsigned)blocks), dim3(HC_BLOCK), 0, static_cast<hipStream_t>(stream)>>>(a);
-  return hc_launch_status();
+  // (a launch has fewer than 2^32 lanes)
+  for (; a.first < n; a.first += (int64_t)RP_MOST_BLOCKS * RP_ROWS) {
+    const int64_t blocks = (n - a.first + RP_ROWS - 1) / RP_ROWS;
+    kernel<<<dim3((unsigned)(blocks < RP_MOST_BLOCKS ? blocks : RP_MOST_BLOCKS)), dim3(HC_BLOCK), 0,
+             static_cast<hipStream_t>(stream)>>>(a);
+    if (const int rc = hc_launch_status()) return rc;
+  }
+  return HC_OK;
 }
