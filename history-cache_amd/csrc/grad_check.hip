@@ -385,7 +385,8 @@ __device__ __forceinline__ void copy_rows_fast(const float *__restrict__ emb, TT
 // A tile has one block and most batches few tiles, so that what a wave has to do one after the other bounds them, its instructions' way
 // from memory included: addresses go by steps from the tile's and the ring's own, and rows of whole fours of columns (FOURS) are
 // read without a branch.  401 000 of 1 000 003 rows of 256 columns: 123 us (518 MB, 4.2 TB/s; into fp16 139); 60 000 of 200 003 of 172: 21
-// us (53 MB; with the branches 33); 2 300 of 11 000 of 128: 8.8.  One to four at once: no difference.
+// us (53 MB; with the branches 33); 2 300 of 11 000 of 128: 8.8.  The whole admission with one, two or four at once: 135, 136 and 133 us for the
+// first, 28.4, 28.3 and 28.0 for the second, with 200 columns in groups of 128 29.3, 29.1 and 28.4; 8 661 rows 10.0, 9.6 and 10.0.
 // slot0: the slot of rank 0, below capacity.
 constexpr int GC_PACK_AT_ONCE = 4;
 template <int L, bool FOURS>

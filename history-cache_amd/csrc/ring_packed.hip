@@ -3,9 +3,9 @@
 // A block takes 16 rows: its first lanes look a row up each (three reads that wait for one another), then all of its lanes lie one after
 // the other over the rows' columns.
 // Bound by memory where there are many: 1 000 003 ids, 400 000 of them hits of 256 columns, 264 us for 1.15 GB (4.4 TB/s; an id's map
-// entry, age, scales and codes lie in lines of their own, 0.25 GB more than is asked for; from a table in fp16 501 us), with ordinary
-// stores 291; four or eight pieces at once, or the next pieces read before the last are written: no difference.  64 rows a block in place of
-// 16 (with the calls in turn over four sets of ids): 281 against 266; 200 003 ids of 172 columns 36.5 against 35.4, 1 500 of 128 3.8 against 2.8.
+// entry, age, scales and codes lie in lines of their own, 0.25 GB more than is asked for; from a table in fp16 501 us).  With ordinary
+// stores 291; one, two or four pieces at once 379, 268 and 266; eight, or the next pieces read before the last are written, as four;
+// 64 rows a block 281 (200 003 ids of 172 columns 36.5 against 35.4, 1 500 of 128 3.8 against 2.8).
 // 150 001 ids, half of them hits of 172 columns: 32 us (118 MB).  Few: 8 661 of 256 columns 5.4, 1 500 of 128 3.9 us, a launch and four
 // reads one after the other.
 #include "packed_rows.h"
