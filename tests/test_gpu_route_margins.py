@@ -79,3 +79,22 @@ def test_a_bias_closes_an_expert_whatever_its_logit_is(score, G, top, n):
                 assert bool(torch.isnan(weight[1::2]).all()) == bool(still)
             # rows without are as before
             assert torch.equal(expert[::2], be.route_rows(logits, 6, score=score, bias=bias, num_group=G, top_group=top)[0][::2])
+
+
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("n", ((1 << 17) - 1, 1 << 17))
+def test_a_factor_alone_on_both_sides_of_the_size_from_which_it_is_a_call_of_its_own(n, normalize):
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    logits = (2 * torch.randn(n, 64, generator=gen, device=DEV)).to(torch.bfloat16)
+    logits[::9, 5:] = -math.inf
+    logits[100], logits[101, 3], logits[102, 4] = -math.inf, math.nan, math.inf
+    one, w = be.route_rows(logits, 6, normalize=normalize)
+    two, v = be.route_rows(logits, 6, normalize=normalize, scale=2.5)
+    leaf = logits.clone().requires_grad_(True)
+    three, u = be.route_rows(leaf, 6, normalize=normalize, scale=2.5)
+    assert torch.equal(one, two) and torch.equal(one, three)
+    for x in (v, u.detach()):
+        assert torch.equal(torch.isnan(x), torch.isnan(w))
+        # (each within OFF of the definition, test_gpu_route_scores)
+        assert float(torch.nan_to_num((x - 2.5 * w).abs() - 200 * 2.0 ** -23 * 2.5 * w).max()) <= 0
+    check(logits[:100], 6, normalize=normalize, scale=2.5)
