@@ -65,9 +65,9 @@ struct rt_key<float> {
   }
 };
 
-// Sorts V keys, the largest first (Batcher's odd-even merge sort).
-template <int V, typename K>
-__device__ __forceinline__ void rt_sort(K (&a)[V]) {
+// Sorts V keys, the largest first (Batcher's odd-even merge sort); in_order(x, y) leaves the larger one in x.
+template <int V, typename K, typename F>
+__device__ __forceinline__ void rt_sort(K (&a)[V], F &&in_order) {
 #pragma unroll
   for (int p = 1; p < V; p *= 2)
 #pragma unroll
@@ -76,11 +76,16 @@ __device__ __forceinline__ void rt_sort(K (&a)[V]) {
       for (int j = k % p; j + k < V; j += 2 * k)
 #pragma unroll
         for (int i = 0; i < k; ++i)
-          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-            const K x = a[i + j], y = a[i + j + k];
-            a[i + j] = x > y ? x : y;
-            a[i + j + k] = x > y ? y : x;
-          }
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) in_order(a[i + j], a[i + j + k]);
+}
+
+template <int V, typename K>
+__device__ __forceinline__ void rt_sort(K (&a)[V]) {
+  rt_sort(a, [](K &first, K &second) {
+    const K x = first, y = second;
+    first = x > y ? x : y;
+    second = x > y ? y : x;
+  });
 }
 
 __device__ __forceinline__ bool rt_masked(float v) { return v == -__builtin_inff(); }

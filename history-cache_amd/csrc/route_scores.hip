@@ -162,17 +162,8 @@ __device__ __forceinline__ void rs_in_order(double &x, double &y) {
 template <int N>
 struct rs_list {
   double t[N], out;
-  // t sorted (Batcher's odd-even merge sort)
   __device__ __forceinline__ void sort() {
-#pragma unroll
-    for (int p = 1; p < N; p *= 2)
-#pragma unroll
-      for (int k = p; k >= 1; k /= 2)
-#pragma unroll
-        for (int j = k % p; j + k < N; j += 2 * k)
-#pragma unroll
-          for (int i = 0; i < k; ++i)
-            if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) rs_in_order(t[i + j], t[i + j + k]);
+    rt_sort(t, [](double &x, double &y) { rs_in_order(x, y); });
   }
   // `out` to its place among t
   __device__ __forceinline__ void settle() {
