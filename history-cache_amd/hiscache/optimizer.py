@@ -51,8 +51,8 @@ class AdamW(torch.optim.Optimizer):
         if handle is None or any(getattr(handle, k) is not state.get(k) for k in self._PARTS):
             handle = self._handles[p] = _be.AdamWState(*(state.get(k) for k in self._PARTS))
         if handle.master is not None and not p.is_inference():
-            known = self._versions.get(p)
-            if known is not None and known != p._version:
+            # (of a parameter that this object has not stepped yet, one of a copied optimizer, say, nothing is known: it is looked at)
+            if self._versions.get(p) != p._version:
                 same = handle.master.to(p.dtype) == p
                 handle.master.copy_(torch.where(same, handle.master, p.float()))
         return handle

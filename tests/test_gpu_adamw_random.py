@@ -1,5 +1,6 @@
 """Moments in 8 bits, rounded at random: the kernel's codes against the definition, and long runs of the optimizer against one
 in 32 bits (the bounds are derived in ``test_adamw_random_cpu``)."""
+import copy
 import math
 
 import pytest
@@ -177,3 +178,24 @@ def test_small_codes_are_rounded_once(most):
             assert torch.equal(state.exp_avg, hold(g, 3, None)[0])
         else:                                                # (b2 = 0: the root of the gradient's square)
             assert torch.equal(state.exp_avg_sq, hold((g * g).double().sqrt().float(), 4, None)[0])
+
+
+def test_a_copied_optimizer_takes_weights_that_were_loaded_before_its_first_step():
+    """The fp32 copies that came with it are of the weights as they were."""
+    torch.manual_seed(0)
+    model = torch.nn.Linear(64, 64).to(DEV, torch.bfloat16)
+    opt = hiscache.AdamW(model.parameters(), lr=1e-3)
+    for p in model.parameters():
+        p.grad = torch.randn_like(p)
+    opt.step()
+    twin, other = copy.deepcopy((model, opt))
+    kept = other.state[twin.weight]["master"].clone()
+    with torch.no_grad():
+        twin.weight[3] = 2.0
+    for p in twin.parameters():
+        p.grad = torch.zeros_like(p)
+    other.param_groups[0].update(lr=0.0)
+    other.step()
+    master = other.state[twin.weight]["master"]
+    assert bool((master[3] == 2.0).all()) and torch.equal(master[:3], kept[:3]) and torch.equal(master[4:], kept[4:])
+    assert torch.equal(twin.weight, master.to(torch.bfloat16)) and torch.equal(opt.state[model.weight]["master"], kept)
