@@ -1264,10 +1264,11 @@ def lookup(map_tensor, ids, offset=0, n_valid=None):
 
 def _packed_table(table):
     """Rows and columns of a ring table in 8 bits."""
-    capacity, F = _check_kept(table, 1)
-    if not table.codes.is_cuda or table.scale.device != table.codes.device:
+    known, shape = table._checked, _check_kept(table, 1)
+    if table._checked is not known and (not table.codes.is_cuda or table.scale.device != table.codes.device):
+        table._checked = None
         raise RuntimeError("codes and scale of a table must live on one GPU; this module has no CPU path")
-    return capacity, F
+    return shape
 
 
 def ring_lookup(full2slot, ids, table, checkin=None, now=0, age_limit=1 << 62, want_rows=True, n_valid=None):
@@ -2331,8 +2332,8 @@ def adamw_state(param, bits=32, master=False):
 
 
 def _check_adamw_state(state, shape, index):
-    """Do the parts of a state fit a tensor of this shape on device ``index``?  Their addresses (0: there is none) and the number of
-    elements."""
+    """Do the parts of a state fit a tensor of this shape on device ``index``?  Their addresses (0: there is none), the number of
+    elements, whether there is a scale and whether there is a copy."""
     m, v, step, scale, master = state.exp_avg, state.exp_avg_sq, state.step, state.scale, state.master
     if scale is None and master is None:
         facts = (m.data_ptr(), v.data_ptr(), step.data_ptr(), m.nbytes, v.nbytes, step.nbytes, m.is_contiguous(), v.is_contiguous(),
@@ -2363,7 +2364,7 @@ def _check_adamw_state(state, shape, index):
             raise ValueError("a state's parts must be contiguous and lie on the parameter's device")
         if t is not None and not _in_memory(t):
             raise ValueError("a state's parts must lie in memory")
-    at = *[0 if t is None else t.data_ptr() for t in parts], numel
+    at = *[0 if t is None else t.data_ptr() for t in parts], numel, bits8, master is not None
     state._checked = facts, at
     return at
 
@@ -2426,8 +2427,8 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
         grads = [g.clone() if g._is_zerotensor() else g for g in grads]
         of_g = [g.data_ptr() for g in grads]
     of_states = [_check_adamw_state(state, shape, index) for state, shape in zip(states, shapes)]
-    _written_once(at, of_states)
-    kinds = [(dtype, state.scale is not None, state.master is not None) for dtype, state in zip(dtypes, states)]
+    columns = _written_once(at, of_states)
+    kinds = list(zip(dtypes, *columns[6:]))
     _together(params[0])
     if forward_ad._current_level >= 0:
         _no_tangent(*params, *grads)
@@ -2450,28 +2451,29 @@ def adamw_step(params, grads, states, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wei
             _float_dtype(params[kinds.index(kind)], "param")
     for kind in each:
         dtype, bits8, copies = kind
-        words, theirs, mine = at, of_g, of_states
+        words, theirs, mine = at, of_g, columns
         if len(each) > 1:
-            words, theirs, mine = zip(*[w for w, k in zip(zip(at, of_g, of_states), kinds) if k == kind])
-        m, v, step, scale, master, numels = zip(*mine)
-        n, words = len(mine), [*words, *theirs, *m, *v, *step, *numels]
+            words, theirs, *mine = zip(*[w for w, k in zip(zip(at, of_g, *columns), kinds) if k == kind])
+        m, v, step, scale, master, numels = mine[:6]
+        n, words = len(m), [*words, *theirs, *m, *v, *step, *numels]
         if bits8:
             words += scale
         if copies:
             words += master
         host = array.array("q", words)                    # the arrays of the call one after the other
-        first = host.buffer_info()[0]
-        to = [first + 8 * n * k for k in range(8)]
-        _check(lib.hc_adamw_step(n, to[0], to[1], _DTYPES[dtype], to[2], to[3], to[6] if bits8 else None,
-                                 to[6 + bits8] if copies else None, to[4], to[5], bits_of_8 if bits8 else 32, float(lr), _ptr(lr_dev),
-                                 b1, b2, float(eps), float(weight_decay), stream), "hc_adamw_step")
+        to, on = host.buffer_info()[0], 8 * n
+        _check(lib.hc_adamw_step(n, to, to + on, _DTYPES[dtype], to + 2 * on, to + 3 * on, to + 6 * on if bits8 else None,
+                                 to + (6 + bits8) * on if copies else None, to + 4 * on, to + 5 * on, bits_of_8 if bits8 else 32,
+                                 float(lr), _ptr(lr_dev), b1, b2, float(eps), float(weight_decay), stream), "hc_adamw_step")
     # the kernels wrote behind autograd's back: what was saved of a parameter is out of date
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
 
 
 def _written_once(at, of_states):
-    """Does every parameter and every part of a state (their addresses; 0: there is none) lie in memory of its own?"""
-    m, v, step, scale, master, _ = zip(*of_states)
+    """Does every parameter and every part of a state (their addresses; 0: there is none) lie in memory of its own?  What
+    :func:`_check_adamw_state` says of the states, by column."""
+    columns = list(zip(*of_states))
+    m, v, step, scale, master = columns[:5]
     every = [*at, *m, *v, *step, *scale, *master]
     seen = set(every)
     if len(seen) - (0 in seen) < len(every) - every.count(0):
@@ -2479,6 +2481,7 @@ def _written_once(at, of_states):
         raise ValueError("a parameter is named twice" if len(set(params)) < len(params) else
                          "a state goes with one parameter, and so does each of its parts" if len(set(held)) < len(held) else
                          "a parameter is no part of a state")
+    return columns
 
 
 def _adamw_refuse(params, grads):

@@ -130,3 +130,16 @@ def test_parts_of_states_that_two_parameters_would_share():
         be._written_once([0x9000], [(0x1000, 0x1000, 0x3000, 0, 0, 8)])
     with pytest.raises(ValueError, match="part of a state"):
         be._written_once([0x9000, 0x8000], [a, b])
+
+
+def test_a_ring_table_on_the_host_is_refused_every_time():
+    table = be.PackedRows(torch.zeros(6, 64, dtype=torch.int8), torch.zeros(6, 1), 64, torch.float32)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            be._packed_table(table)
+    be._check_kept(table, 1)                                 # (rows that another call has looked at)
+    device = be.PackedRows(OnDevice(table.codes), OnDevice(table.scale), 64, torch.float32)
+    assert be._packed_table(device) == be._packed_table(device) == (6, 64)
+    device.codes.t.data = torch.zeros(7, 64, dtype=torch.int8)
+    with pytest.raises(ValueError):
+        be._packed_table(device)
