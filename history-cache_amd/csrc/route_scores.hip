@@ -17,10 +17,16 @@
 // Such a choice is right where nothing near stands against it.  c in fp32 is off by up to 2^-22 and half a unit of |c|: where neighbours in
 // the list, or the last open and the first closed group (by the larger of the numbers that they are sums of), are nearer than twice that and
 // do not come from equal numbers, the wave decides the row again in fp64, all lanes on it.  Where the first outside the list is near by the bits that were kept, it is counted how many are that near by all bits.
-// Bound by those medians, K + 1 a logit, and the exponentials: 500 009 rows of 64 bf16 logits to four experts 46 us for 96 MB, with sorted
-// lists of fp64 keys 50 and with insertion into unsorted ones 106; 65 537 rows of 256 fp32 in groups to eight 49 us for 75 MB; eight such
-// rows 9.3, of which most is the way of some thousand instructions from memory.  A whole fp64 pass over every row: 125 and 173.
-// Backward: memory, 23 us for 96 MB and 20 for 75 (the logits are not read: what is chosen is handed over).
+// Bound by its vector instructions first: 500 009 rows of 64 bf16 logits to four experts 46 us for 96 MB, 1 255 instructions a wave of 32
+// rows, that is 32 logits a lane: for reading logits and making scores, for the lists (K + 1 medians a logit and the index's bits), for
+// joining them and for the weights of what is chosen; at one a SIMD every four cycles they are 32 of the 46 us.  With sorted lists of fp64
+// keys 50, with insertion into unsorted ones 106.  65 537 rows of 256 fp32 in groups to eight 48 us for 75 MB (2 129 a wave of eight rows,
+// 28 of the 48); 200 003 rows of 60 by softmax, in groups, to six 40 (2 505 a wave of 32, 26 of the 40).  Eight rows of 256 9.2: some 2 000
+// instructions one after the other, which come from memory.  A whole fp64 pass over every row: 125 and 173.
+// Lists have 2, 4, 8 or 32 places, so that from nine choices on a row pays for 32: 500 009 rows of 64 to eight experts 65 us, to nine 160,
+// to 32 245; 65 537 of 256 38, 87 and 128; 30 000 of 1 024 80, 182 and 250.
+// Backward: 23 us for 96 MB and 20 for 75 (the logits are not read: what is chosen is handed over), 139 and 160 vector instructions a wave;
+// the softmax's own, which goes by the weights and needs no exponential, 54 and 16.5 us for the same 96 MB.
 #include "route_row.h"
 
 namespace {
@@ -721,7 +727,8 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
     return hc_launch_status();
   };
   // Lanes a row: as few as leave a compute unit enough waves beside their rows in LDS (9.5 KB a wave), and twice as many where that makes
-  // fewer waves than there are SIMDs.  Us by 1 / 2 / 4 / 8 lanes: 500 009 rows of 64 50 / 43 / 47, 30 000 15 / 11 / 9.3 / 9.3,
+  // fewer waves than there are SIMDs.  (Twice as many again are 0.4 to 1 us faster up to 16 000 rows of 64 and 2 slower at 30 000; with 256
+  // experts 0.6 slower at 64 rows, 1 to 6 faster at 1 000, 3 to 6 slower from 4 000 on: no third set of kernels for that.)  Us by 1 / 2 / 4 / 8 lanes: 500 009 rows of 64 50 / 43 / 47, 30 000 15 / 11 / 9.3 / 9.3,
   // 250 8.7 / 6.0 / 4.5 / 4.2; by 4 / 8 / 16 / 32: 65 537 rows of 256 in groups 51 / 48 / 65, 8 000 23 / 21 / 21 / 27, 250 14.5 / 10.7 /
   // 10.2 / 9.3; by 16 / 32 / 64: 30 000 rows of 1 024 78 / 79 / 94, 250 14.6 / 10.5 / 8.8.
   const auto with_lanes = [&](auto places) {

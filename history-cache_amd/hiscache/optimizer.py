@@ -1,7 +1,8 @@
 """AdamW over all parameters in one launch, with states in 32 or in 8 bits (``hiscache_backend.adamw_step``).
 
-A drop-in for ``torch.optim.AdamW(params, capturable=True)``: the steps are counted on the device, so that a recorded iteration
-(``RecordedIteration``) replays them; with ``weight_decay=0`` it is Adam.
+It makes the steps of ``torch.optim.AdamW(params, capturable=True)``: they are counted on the device, so that a recorded iteration
+(``RecordedIteration``) replays them; with ``weight_decay=0`` it is Adam.  It has arguments of its own: none of ``amsgrad``, ``maximize``,
+``foreach``, ``capturable`` and ``fused``; a group's parameters lie on one device.
 """
 import torch
 
