@@ -11,6 +11,7 @@ NLL on the log-softmax the models return, accuracy).  What the hardware adds is 
 device memory or its hottest rows there, and the iteration recorded per padded batch shape and replayed
 (``RecordedIteration``).
 """
+import functools
 import time
 
 import numpy as np
@@ -33,6 +34,14 @@ def _option(config, dotted, default):
             return default
         node = node[key]
     return node
+
+
+def _balance(model, rate):
+    # (of the model alone: what a recording holds of the trainer would keep both alive)
+    if rate:
+        for m in model.modules():
+            if isinstance(m, ExpertMLP) and m.balance_bias is not None:
+                m.balance_step(rate)
 
 
 class HistoryTrainer:
@@ -116,7 +125,7 @@ class HistoryTrainer:
                 self.splits[split] = torch.from_numpy(np.array(ds.split_idx(key))).to(self.device)
         self._generator = torch.Generator(device=self.device).manual_seed(seed)
         self._step = RecordedIteration(self.model, self.table, self.optimizer, self.num_layers,
-                                       loss_fn=self.loss_fn, after_step=self._balance) if self.recorded else None
+                                       loss_fn=self.loss_fn, after_step=functools.partial(_balance, self.model, balance_rate)) if self.recorded else None
         self.glb_iter = 0
         self.prof = bool(_option(config, "dl.performance.prof", False))     # train() then runs the profiled epoch
         self.times = None
@@ -185,12 +194,6 @@ class HistoryTrainer:
             yield batch
             batch = nxt
 
-    def _balance(self):
-        if self.balance_rate:
-            for m in self.model.modules():
-                if isinstance(m, ExpertMLP) and m.balance_bias is not None:
-                    m.balance_step(self.balance_rate)
-
     @staticmethod
     def evaluator(y_pred, y_true):
         """Accuracy of the arg-max class (the evaluator of the node-classification datasets)."""
@@ -220,7 +223,7 @@ class HistoryTrainer:
                 loss = self.loss_fn(out, batch.y)
                 backward_on_this_thread(loss)
                 self.optimizer.step()
-                self._balance()
+                _balance(self.model, self.balance_rate)
                 self.table.update_history(batch, self.glb_iter)
             if self.scheduler is not None:
                 self.scheduler.step()
@@ -267,7 +270,7 @@ class HistoryTrainer:
             backward_on_this_thread(loss)
             mark(row)
             self.optimizer.step()
-            self._balance()
+            _balance(self.model, self.balance_rate)
             if self.scheduler is not None:
                 self.scheduler.step()
             mark(row)

@@ -1,11 +1,14 @@
 """The bias that loads experts evenly, moved by the loads of the last pass: an eager one, or a recorded one that is replayed."""
 import copy
+import gc
+import weakref
 
 import numpy as np
 import pytest
 import torch
 
 import hiscache
+from hiscache.history_trainer import _balance
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -128,6 +131,15 @@ def test_the_trainer_balances(tmp_path, recorded):
     # a few rows beside the mean or not: what one step would do is seen from the last loads
     load = (t.model.experts._offset[1:] - t.model.experts._offset[:-1]).float()
     before = t.model.experts.balance_bias.clone()
-    t._balance()
+    _balance(t.model, 2.0 ** -10)
     assert torch.equal(t.model.experts.balance_bias, before + moved(load, 2.0 ** -10))
     assert not bool(run(None, 1).model.experts.balance_bias.any())
+    # a trainer that nobody holds is gone with its memory, without the collector's help
+    gc.collect()
+    gc.disable()
+    try:
+        gone = weakref.ref(t)
+        del t
+        assert gone() is None
+    finally:
+        gc.enable()
