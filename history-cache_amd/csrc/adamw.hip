@@ -19,7 +19,7 @@
 // nearer to it.  The nearest one is right for one step from given moments; over many it stops r, which moves by (1 - b2) / 2 of itself a
 // step, far less than half a code: at b2 = 0.999 and gradients that stay as they are it ends at 0.13 to 0.5 of the right one, and
 // never falls again.  At random a number is kept in the mean: r's mean over elements stays within 1 % of the right one at any b2, an
-// element's own within 10 % (one standard deviation; each step's two thousandths add up over the steps that v remembers).  What
+// element's own within 10 % (one standard deviation; a step's is half a percent, and they add up over the steps that v remembers).  What
 // is random is a hash of the element's place in its tensor and the tensor's count, so that a step that is made again, in a
 // recording, or in another launch is the same.
 //

@@ -16,7 +16,8 @@
 // sorted by them and then the index, and put together with what the row's other lanes have.
 // Such a choice is right where nothing near stands against it.  c in fp32 is off by up to 2^-22 and half a unit of |c|: where neighbours in
 // the list, or the last open and the first closed group (by the larger of the numbers that they are sums of), are nearer than twice that and
-// do not come from equal numbers, the wave decides the row again in fp64, all lanes on it.  Where the first outside the list is near by the bits that were kept, it is counted how many are that near by all bits.
+// do not come from equal numbers, the wave decides the row again in fp64, all lanes on it.  Where the first outside the list is near by
+// the bits that were kept, it is counted how many are that near by all bits.
 // Bound by its vector instructions first: 500 009 rows of 64 bf16 logits to four experts 46 us for 96 MB, 1 255 instructions a wave of 32
 // rows, that is 32 logits a lane: for reading logits and making scores, for the lists (K + 1 medians a logit and the index's bits), for
 // joining them and for the weights of what is chosen; at one a SIMD every four cycles they are 32 of the 46 us.  With sorted lists of fp64
@@ -728,9 +729,10 @@ extern "C" int hc_route_scores(const void *logits, int dtype, int64_t n, int64_t
   };
   // Lanes a row: as few as leave a compute unit enough waves beside their rows in LDS (9.5 KB a wave), and twice as many where that makes
   // fewer waves than there are SIMDs.  (Twice as many again are 0.4 to 1 us faster up to 16 000 rows of 64 and 2 slower at 30 000; with 256
-  // experts 0.6 slower at 64 rows, 1 to 6 faster at 1 000, 3 to 6 slower from 4 000 on: no third set of kernels for that.)  Us by 1 / 2 / 4 / 8 lanes: 500 009 rows of 64 50 / 43 / 47, 30 000 15 / 11 / 9.3 / 9.3,
-  // 250 8.7 / 6.0 / 4.5 / 4.2; by 4 / 8 / 16 / 32: 65 537 rows of 256 in groups 51 / 48 / 65, 8 000 23 / 21 / 21 / 27, 250 14.5 / 10.7 /
-  // 10.2 / 9.3; by 16 / 32 / 64: 30 000 rows of 1 024 78 / 79 / 94, 250 14.6 / 10.5 / 8.8.
+  // experts 0.6 slower at 64 rows, 1 to 6 faster at 1 000, 3 to 6 slower from 4 000 on: no third set of kernels for that.)  Us by 1 / 2 / 4 /
+  // 8 lanes: 500 009 rows of 64 50 / 43 / 47, 30 000 15 / 11 / 9.3 / 9.3, 250 8.7 / 6.0 / 4.5 / 4.2; by 4 / 8 / 16 / 32: 65 537 rows of 256 in
+  // groups 51 / 48 / 65, 8 000 23 / 21 / 21 / 27, 250 14.5 / 10.7 / 10.2 / 9.3; by 16 / 32 / 64: 30 000 rows of 1 024 78 / 79 / 94, 250
+  // 14.6 / 10.5 / 8.8.
   const auto with_lanes = [&](auto places) {
     const int least = E <= 64 ? 2 : E <= 256 ? 8 : 32;
     const bool few = n * least < 64 * 1024;

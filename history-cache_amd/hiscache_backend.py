@@ -1866,8 +1866,9 @@ def route_rows(logits, top_k, normalize=True, score="softmax", bias=None, num_gr
             _together(logits)
             # A factor alone: the softmax's own kernel and a product, which take less time on the device and more on the host.  500 009 rows
             # of 64 41.8 us in one call against 29.6 in two, 130 000 of 64 12.8 and 13.6, 65 536 9.3 and 13.1; with the gradient's
-            # calls the host is what counts: 83 against 98 at every size.
-            if score == "softmax" and num_group == top_group and shape[0] * E >= 1 << 23 and not _watched(logits):
+            # calls the host is what counts: 83 against 98 at every size.  (The softmax's own kernel takes up to 64 lanes a row, of 2^32.)
+            if (score == "softmax" and num_group == top_group and shape[0] * E >= 1 << 23 and shape[0] <= 1 << 25
+                    and not _watched(logits)):
                 expert, weight = _route(logits, top_k, int(bool(normalize)))
                 return expert, weight.mul_(scale)
         else:

@@ -79,3 +79,18 @@ def test_a_code_s_own_number_stays_as_it_is():
     for t in range(1, 9):
         word = words(torch.arange(value.numel()), t)
         assert torch.equal(hold(value, 3, word)[2][:112], value[:112]) and torch.equal(hold(value, 4, word)[2][:112], value[:112])
+
+
+def test_the_flag_at_the_c_entry():
+    """8 | 256 is 8 with another rounding and wants what 8 wants; 32 | 256 and the flag alone are refused."""
+    import ctypes
+
+    import hiscache_backend as be
+    lib = be.load_library()
+    word = (ctypes.c_void_p * 1)(ctypes.addressof(ctypes.c_int64(0)))
+    numel = (ctypes.c_int64 * 1)(4)
+
+    def step(bits, scale):
+        return lib.hc_adamw_step(1, word, word, 0, word, word, scale, None, word, numel, bits, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, None)
+    assert [step(b, None) for b in (8 | 256, 256, 32 | 256, 16 | 256)] == [1, 1, 1, 1]
+    assert step(32 | 256, word) == 1 and step(8 | 512, word) == 1

@@ -98,3 +98,13 @@ def test_a_factor_alone_on_both_sides_of_the_size_from_which_it_is_a_call_of_its
         # (each within OFF of the definition, test_gpu_route_scores)
         assert float(torch.nan_to_num((x - 2.5 * w).abs() - 200 * 2.0 ** -23 * 2.5 * w).max()) <= 0
     check(logits[:100], 6, normalize=normalize, scale=2.5)
+
+
+def test_a_factor_alone_for_more_rows_than_the_softmax_s_own_kernel_takes():
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GiB of free device memory")
+    n = (1 << 29) + 3                                        # (eight lanes a row there, two here)
+    logits = torch.zeros(n, 2, dtype=torch.bfloat16, device=DEV)
+    logits[-1, 1] = 1.0
+    expert, weight = be.route_rows(logits, 1, scale=2.0)
+    assert expert[-2:, 0].tolist() == [0, 1] and bool((weight == 2.0).all())
