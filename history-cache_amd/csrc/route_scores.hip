@@ -220,7 +220,8 @@ __device__ __forceinline__ float rs_near_sigma(float l) {
 
 // s = 1 / (1 + exp(-l)) on the scale exp(-base), base <= 0, l <= base or base = 0; and 1 - s.  What is divided by its sum is taken on the scale of the largest logit, so that scores which 32 bits do not hold (l < -87) still have their shares.
 __device__ __forceinline__ float rs_sigma(float l, float base, float &rest) {
-  const float x = expf(-fabsf(l)), q = __builtin_amdgcn_rcpf(1.f + x);
+  const float x = expf(-fabsf(l)), y = 1.f + x, near = __builtin_amdgcn_rcpf(y);
+  const float q = __builtin_fmaf(__builtin_fmaf(-y, near, 1.f), near, near);               // (1 / y, right but for the last bit)
   rest = l >= 0.f ? x * q : q;
   return l >= 0.f ? q : (base < 0.f ? expf(l - base) : x) * q;
 }
